@@ -38,7 +38,9 @@ typedef enum mortar_status {
     MORTAR_ERR_UNSUPPORTED = -10   /* combination not implemented                      */
 } mortar_status;
 
-typedef enum mortar_dtype { MORTAR_F32 = 0, MORTAR_BF16 = 1 } mortar_dtype;
+/* MORTAR_F16 and the two 8-bit types are taken where an entry point says so; MORTAR_E5M2 and
+ * MORTAR_E4M3 are one byte a value, the types `float8_e5m2` and `float8_e4m3fn` of torch. */
+typedef enum mortar_dtype { MORTAR_F32 = 0, MORTAR_BF16 = 1, MORTAR_F16 = 2, MORTAR_E4M3 = 3, MORTAR_E5M2 = 4 } mortar_dtype;
 
 /* ---- canonical matrix format: tile-16 BCSR with 2-bit ternary codes ---------------
  * W[out,in]; R = out/16 tile rows, C = in/16 tile columns.
@@ -598,6 +600,85 @@ int mortar_linear_error(int32_t *code, int32_t reset);
 /* Reads (and optionally clears) the error word the prefill kernel sets when one of its
  * bounded barrier waits expires: 0 = none, 1..4 = the waiting role.  Synchronises. */
 int mortar_prefill_error(int32_t *code, int32_t reset);
+
+/* ---- the dense MLP site: norm, block before carving, 8-bit serving form --------------------- */
+
+/* Layer norm over the last dimension: y = (x - mean) * rstd * weight + bias, rstd =
+ * 1 / sqrt(mean((x - mean)^2) + eps).
+ *   x, y     device [rows][cols], fp32, bf16 or fp16 (dtype), row strides ldx / ldy; y may be x
+ *   weight, bias   device fp32[cols] or NULL (1 and 0)
+ *   stats    device fp32[2][rows], mean and rstd for the backward call, or NULL
+ * Statistics are fp32 whatever the type.  cols up to 2^20.  (The norm of
+ * morph/model/routing.py:159-284.) */
+int mortar_layer_norm(const void *x, int32_t dtype, int64_t ldx, int64_t rows, int32_t cols,
+                      const float *weight, const float *bias, float eps, void *y, int64_t ldy,
+                      float *stats, void *stream);
+
+/* fp32 values the backward call needs as scratch (negative = error). */
+int64_t mortar_layer_norm_scratch_floats(int64_t rows, int32_t cols);
+
+/* Gradients of mortar_layer_norm: dx [rows][cols] of the rows' type, dweight and dbias fp32[cols];
+ * each may be NULL when it is not wanted.  `scratch` is used for dweight / dbias only.  The sums over
+ * rows are fp32 and taken in a fixed order: the same call gives the same bits. */
+int mortar_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int32_t dtype,
+                               int64_t rows, int32_t cols, const float *weight, const float *stats,
+                               void *dx, int64_t lddx, float *dweight, float *dbias, float *scratch,
+                               int64_t scratch_floats, void *stream);
+
+/* The gated feed-forward block before it is carved (morph/model/transformer.py:402-431):
+ *   y = (silu(x Wg^T) * (x Wu^T)) Wd^T,  gate_up = [Wg; Wu] [2 d_ff][d_model], down [d_model][d_ff]
+ * x, weights and results are bf16 or fp16 (dtype, one for all); sums are fp32; the hidden block and y
+ * are rounded once each.  d_model and d_ff are multiples of 16, pointers 16-byte aligned, row strides
+ * multiples of 8.
+ *   hidden        device [rows][d_ff], written: the hidden block (scratch, and an input of the
+ *                 backward call)
+ *   gate_up_sums  device [rows][2 d_ff], written for the backward call, or NULL
+ * Bounded in-kernel waits report through mortar_dense_error. */
+int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64_t rows, const void *gate_up,
+                     int64_t ld_gate_up, const void *down, int64_t ld_down, int32_t d_model, int32_t d_ff,
+                     void *hidden, void *gate_up_sums, void *y, int64_t ldy, void *stream);
+
+/* Gradients of mortar_mlp_dense from dy [rows][d_model], its inputs, `hidden` and `gate_up_sums`:
+ * dx [rows][d_model], dgate_up [2 d_ff][d_model], ddown [d_model][d_ff], contiguous, of the same
+ * type; each may be NULL.  `dgate_up_sums` [rows][2 d_ff] is scratch of that type. */
+int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int32_t dtype,
+                              int64_t rows, const void *gate_up, int64_t ld_gate_up, const void *down,
+                              int64_t ld_down, int32_t d_model, int32_t d_ff, const void *hidden,
+                              const void *gate_up_sums, void *dgate_up_sums, void *dx, void *dgate_up,
+                              void *ddown, void *stream);
+/* First error recorded by the kernels of the two calls above: 0 = none, else the waiting role.
+ * Synchronises. */
+int mortar_dense_error(int32_t *code, int32_t reset);
+
+/* x [rows][cols] (fp32, bf16 or fp16) -> q [rows][cols] (MORTAR_E4M3 or MORTAR_E5M2) with one fp32
+ * scale per block of block_rows x 128, scale [ceil(rows / block_rows)][ceil(cols / 128)];
+ * block_rows is 1 (activations) or 128 (weights).  A block's scale is the smallest power of two that
+ * brings it into the type's range, and q the value nearest to x / scale, ties to even; zeros have
+ * scale 1, a block with an infinity or a NaN scale NaN.  cols a multiple of 16, pointers and row
+ * strides 16-byte aligned. */
+int mortar_quantize_fp8(const void *x, int32_t dtype, int64_t ldx, int64_t rows, int32_t cols,
+                        int32_t block_rows, void *q, int32_t q_dtype, int64_t ldq, float *scale,
+                        void *stream);
+/* out = q * scale, rounded once. */
+int mortar_dequantize_fp8(const void *q, int32_t q_dtype, int64_t ldq, const float *scale, int64_t rows,
+                          int32_t cols, int32_t block_rows, void *out, int32_t out_dtype,
+                          int64_t ld_out, void *stream);
+
+/* y[m][n] = sum_b x_scale[m][b] * w_scale[n / 128][b] * sum_{k in block b} x[m][k] w[n][k], b over
+ * blocks of 128 columns (the last one may be short).
+ *   x, w       device [rows][in_features] / [out_features][in_features], MORTAR_E4M3 or MORTAR_E5M2
+ *              each, 16-byte aligned, row strides multiples of 16
+ *   x_scale, w_scale   device fp32, row strides ld_x_scale / ld_w_scale; any finite values whose
+ *              products are finite
+ *   flags      0 or MORTAR_FLAG_SWIGLU: y = silu(first half) * second half of the output columns;
+ *              out_features a multiple of 256 then
+ *   out        fp32, bf16 or fp16, sums in fp32, rounded once
+ * in_features is a multiple of 16.  Bounded in-kernel waits report through mortar_linear_fp8_error. */
+int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, const float *x_scale, int64_t ld_x_scale,
+                      int64_t rows, const void *w, int32_t w_type, int64_t ldw, const float *w_scale,
+                      int64_t ld_w_scale, int32_t out_features, int32_t in_features, int32_t flags,
+                      void *out, int32_t out_dtype, int64_t ld_out, void *stream);
+int mortar_linear_fp8_error(int32_t *code, int32_t reset);
 
 #ifdef __cplusplus
 }

@@ -7,10 +7,10 @@ torch-facing operators, ``torch_ops.py`` the same as registered custom ops plus 
 seeded synthetic layers for tests and benchmarks, ``build.py`` the nvcc build.
 """
 from . import _lib  # noqa: F401
-from .format import MortarMatrix, StreamMatrix, ternary_quantize  # noqa: F401
+from .format import Fp8Matrix, MortarMatrix, StreamMatrix, ternary_quantize  # noqa: F401
 from . import ops, synth  # noqa: F401
 from . import torch_ops  # noqa: F401  (registers the mortar_b200:: custom ops)
-from .modules import MortarLinear, SwiGLUMortar  # noqa: F401
+from .modules import MortarLinear, SwiGLUDense, SwiGLUFp8, SwiGLUMortar  # noqa: F401
 
-__all__ = ["MortarMatrix", "StreamMatrix", "MortarLinear", "SwiGLUMortar", "ops", "synth",
-           "ternary_quantize"]
+__all__ = ["Fp8Matrix", "MortarMatrix", "StreamMatrix", "MortarLinear", "SwiGLUDense", "SwiGLUFp8",
+           "SwiGLUMortar", "ops", "synth", "ternary_quantize"]

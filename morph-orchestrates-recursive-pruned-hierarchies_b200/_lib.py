@@ -12,7 +12,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libmortar_b200.so")
 
 OK = 0
-F32, BF16 = 0, 1
+F32, BF16, F16, E4M3, E5M2 = 0, 1, 2, 3, 4
 OUT_F32, OUT_BF16, OUT_PLANES = 0, 1, 2
 FLAG_SWIGLU, FLAG_ROUND_BF16, FLAG_GATES_ON_INPUT, FLAG_ACCUMULATE = 1, 2, 4, 8
 PATH_FLAGS = {"auto": 0, "plain": 16, "staged": 32, "persistent": 48}
@@ -123,6 +123,20 @@ _SIGNATURES = {
     "mortar_linear_error": (C.c_int, [_vp, _i32]),
     "mortar_router_gates": (C.c_int, [_vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _i32, _vp,
                                       _i32, _i32, _vp, _vp, _i64, _vp]),
+    "mortar_layer_norm": (C.c_int, [_vp, _i32, _i64, _i64, _i32, _vp, _vp, _f32, _vp, _i64, _vp, _vp]),
+    "mortar_layer_norm_scratch_floats": (_i64, [_i64, _i32]),
+    "mortar_layer_norm_backward": (C.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _i64, _vp, _vp,
+                                             _vp, _i64, _vp]),
+    "mortar_mlp_dense": (C.c_int, [_vp, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i64,
+                                   _vp]),
+    "mortar_mlp_dense_backward": (C.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp,
+                                            _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mortar_dense_error": (C.c_int, [_vp, _i32]),
+    "mortar_quantize_fp8": (C.c_int, [_vp, _i32, _i64, _i64, _i32, _i32, _vp, _i32, _i64, _vp, _vp]),
+    "mortar_dequantize_fp8": (C.c_int, [_vp, _i32, _i64, _vp, _i64, _i32, _i32, _vp, _i32, _i64, _vp]),
+    "mortar_linear_fp8": (C.c_int, [_vp, _i32, _i64, _vp, _i64, _i64, _vp, _i32, _i64, _vp, _i64, _i32, _i32, _i32,
+                                    _vp, _i32, _i64, _vp]),
+    "mortar_linear_fp8_error": (C.c_int, [_vp, _i32]),
 }
 
 # entry points added by later translation units; bound when present in the header list

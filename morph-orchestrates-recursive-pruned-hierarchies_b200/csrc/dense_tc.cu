@@ -1,0 +1,427 @@
+// The dense gated feed-forward block, forward and backward, on the 5th-generation tensor cores.
+//
+//   gu = x Wgu^T (gate columns first), h = silu(g) * u, y = h Wd^T
+//   dh = dy Wd,  dg = dh u (s + a (1 - s)),  du = dh a   with s = sigmoid(g), a = g s
+//   dx = [dg, du] Wgu,  dWgu = [dg, du]^T x,  dWd = dy^T h
+//
+// (`_SwiGLUMortar.forward` before it is carved, morph/model/transformer.py:402-431, and its
+// gradient).  All six products run in one kernel, C[M][N] = sum_k A[m][k] B[n][k], whose operands lie
+// in memory with either index contiguous: the tile copies and the matrix descriptors take both, so
+// nothing is transposed.  Gate and up products of the same hidden columns are the two halves of one
+// accumulator tile, so the gate is applied where the sums are read, and the backward of the gate is
+// the epilogue of dh.
+//
+// One cluster of two CTAs computes a 256 x kBN tile (each CTA 128 rows; the B operand is split between
+// their shared memories): per SM and 64-wide step 16 KB of A and kBN * 64 bytes of B cross from L2,
+// half of what two single CTAs would read, which is what keeps the copies ahead of the MMAs.  Warp 0
+// issues the copies of its CTA, one thread of CTA 0 issues the MMAs of both, warps 2..9 read the
+// accumulators (two sets, so that a tile's epilogue runs under the next tile's MMAs).
+// Every wait is bounded.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+#include <mutex>
+#include "common.h"
+#include "tc_pair.cuh"
+
+namespace {
+
+constexpr int kBN = 256;                         // accumulator columns of a tile
+constexpr int kStages = 6;
+constexpr int kStageA = 128 * 128;               // this CTA's 128 rows, 64 elements of 2 bytes each
+constexpr int kStageB = kBN / 2 * 128;
+constexpr int kStage = kStageA + kStageB;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kTmemCols = 2 * kBN;
+constexpr int kSmem = kStages * kStage + (2 * kStages + 4) * 8 + 1024;
+constexpr int kMaxProblems = 3;
+static_assert(kSmem <= 227 * 1024, "shared memory budget");
+
+__device__ int g_dense_error;
+
+enum Epilogue { kStore = 0, kSwiglu = 1, kSwigluBackward = 2 };
+
+struct Problem {
+    void *out;               // 16-bit [m][n]
+    long long ld_out;
+    long long m;             // rows of C
+    int n;                   // columns of C (hidden columns for kSwiglu)
+    int tiles_m, tiles_n;
+    int k_steps;             // 64-wide steps of the reduction
+    int a_mn, b_mn;          // 1: the operand's row index is the contiguous one in memory
+    int first_item;
+};
+
+struct DenseParams {
+    CUtensorMap map_a[kMaxProblems], map_b[kMaxProblems];
+    Problem prob[kMaxProblems];
+    int n_problems, n_items;
+    int half;                // 1: fp16, 0: bf16
+    int d_ff;                // kSwiglu / kSwigluBackward: rows between a gate row and its up row
+    void *gu;                // kSwiglu: where gate and up sums are kept ([m][2 d_ff], or NULL); kSwigluBackward: read
+    void *hidden;            // unused by kStore
+    long long ld_gu;
+};
+
+__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + __expf(-g)); }
+
+// 32 accumulator columns -> 32 16-bit values of one row; n_left = columns of the row from col on
+__device__ __forceinline__ void store32(void *base, long long idx, const float (&v)[32], int n_left, bool half) {
+    uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(base) + idx);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (8 * j < n_left)
+            dst[j] = make_uint4(tc::pack16(v[8 * j], v[8 * j + 1], half), tc::pack16(v[8 * j + 2], v[8 * j + 3], half),
+                                tc::pack16(v[8 * j + 4], v[8 * j + 5], half), tc::pack16(v[8 * j + 6], v[8 * j + 7], half));
+}
+
+__device__ __forceinline__ void load32(const void *base, long long idx, float (&v)[32], int n_left, bool half) {
+    const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(base) + idx);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint4 w = 8 * j < n_left ? __ldg(src + j) : make_uint4(0, 0, 0, 0);
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = tc::unpack16(ws[i], half);
+            v[8 * j + 2 * i] = f.x;
+            v[8 * j + 2 * i + 1] = f.y;
+        }
+    }
+}
+
+__device__ __forceinline__ void acc32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    tc::ld32(taddr, r);
+    tc::wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+struct TileId { int p, tm, tn; };
+
+// Items walk a problem's tiles in bands of 8 tile rows, column by column, so that the clusters at work
+// share few A and B panels.
+__device__ __forceinline__ TileId tile_of(const DenseParams &p, int item) {
+    TileId t;
+    t.p = 0;
+    while (t.p + 1 < p.n_problems && item >= p.prob[t.p + 1].first_item) ++t.p;
+    const Problem &q = p.prob[t.p];
+    const int i = item - q.first_item;
+    const int band = i / (8 * q.tiles_n), r = i - band * 8 * q.tiles_n;
+    const int h = min(8, q.tiles_m - band * 8);
+    t.tn = r / h;
+    t.tm = band * 8 + r - t.tn * h;
+    return t;
+}
+
+template <int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+dense_pair_kernel(const __grid_constant__ DenseParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t *>(stages + kStages * kStage), *empty = full + kStages;
+    uint64_t *acc_full = empty + kStages, *acc_empty = acc_full + 2;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int abort_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = tc::cluster_rank();
+    const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        abort_s = 0;
+        for (int s = 0; s < kStages; ++s) { tc::mbar_init(tc::smem_u32(&full[s]), 1); tc::mbar_init(tc::smem_u32(&empty[s]), 1); }
+        for (int s = 0; s < 2; ++s) { tc::mbar_init(tc::smem_u32(&acc_full[s]), 1); tc::mbar_init(tc::smem_u32(&acc_empty[s]), 2 * kEpiWarps); }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                     ::"r"(tc::smem_u32(&tmem_base_s)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();                                   // barriers of both CTAs are initialised
+    tc::fence_after();
+    const uint32_t tmem = tmem_base_s;
+    volatile int *abort_flag = &abort_s;
+
+    if (warp == 0) {
+        // ---------------- copies: one thread in each CTA, completing on CTA 0's barriers ----------------
+        if (lane == 0) {
+            const uint32_t full_lead = tc::cluster_addr(tc::smem_u32(full), 0);
+            const uint32_t empty0 = tc::smem_u32(empty), stage0 = tc::smem_u32(stages);
+            uint32_t s = 0, parity = 1;
+            bool ok = true;
+            for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
+                const TileId t = tile_of(p, item);
+                const Problem &q = p.prob[t.p];
+                const CUtensorMap *ma = &p.map_a[t.p], *mb = &p.map_b[t.p];
+                const int row0 = t.tm * 256 + (int)rank * 128;
+                const int col0 = EPI == kSwiglu ? t.tn * (kBN / 2) + (rank ? p.d_ff : 0) : t.tn * kBN + (int)rank * (kBN / 2);
+                for (int k = 0; k < q.k_steps; ++k) {
+                    if (!tc::mbar_wait(empty0 + 8 * s, parity, abort_flag, &g_dense_error, 1)) { ok = false; break; }
+                    const uint32_t bar = full_lead + 8 * s, dst = stage0 + s * kStage;
+                    if (rank == 0) tc::mbar_arrive_expect_tx(tc::smem_u32(&full[s]), 2 * kStage);
+                    if (q.a_mn) {
+                        tc::load_pair(dst, ma, row0, k * 64, bar);
+                        tc::load_pair(dst + 8192, ma, row0 + 64, k * 64, bar);
+                    } else {
+                        tc::load_pair(dst, ma, k * 64, row0, bar);
+                    }
+                    if (q.b_mn) {
+#pragma unroll
+                        for (int i = 0; i < kBN / 128; ++i)
+                            tc::load_pair(dst + kStageA + i * 8192, mb, col0 + i * 64, k * 64, bar);
+                    } else {
+                        tc::load_pair(dst + kStageA, mb, k * 64, col0, bar);
+                    }
+                    if (++s == kStages) { s = 0; parity ^= 1; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issue: one thread of CTA 0 for the pair ----------------
+        if (rank == 0 && lane == 0) {
+            // D fp32 (bit 4); A and B type at bits 7 and 10 (0 fp16, 1 bf16); M/N-major at bits 15 and 16;
+            // N >> 3 at bit 17, M >> 4 at bit 24 (M = 256 over the pair)
+            const uint32_t type = p.half ? 0u : (1u << 7) | (1u << 10);
+            const uint32_t idesc0 = (1u << 4) | type | ((uint32_t)(kBN >> 3) << 17) | ((256u >> 4) << 24);
+            const uint32_t full0 = tc::smem_u32(full), empty0 = tc::smem_u32(empty);
+            const uint32_t empty0_peer = tc::cluster_addr(empty0, 1);
+            const uint32_t stage0 = tc::smem_u32(stages);
+            uint32_t s = 0, parity = 0;
+            int it = 0;
+            bool ok = true;
+            for (int item = cluster_id; item < p.n_items && ok; item += n_clusters, ++it) {
+                const Problem &q = p.prob[tile_of(p, item).p];
+                const int buf = it & 1;
+                if (!tc::mbar_wait(tc::smem_u32(&acc_empty[buf]), ((it >> 1) & 1) ^ 1u, abort_flag, &g_dense_error, 2)) break;
+                tc::fence_after();
+                const uint32_t acc = tmem + buf * kBN;
+                const uint32_t idesc = idesc0 | ((uint32_t)q.a_mn << 15) | ((uint32_t)q.b_mn << 16);
+                // row-contiguous operand: 64 elements of k are one 128-byte row, 16 of them 32 bytes further;
+                // k-contiguous... the other order: one k is a 128-byte row of 64 rows, 16 of them 2048 bytes,
+                // the next 64 rows one 8 KB box further
+                const uint64_t da = tc::make_smem_desc(stage0, q.a_mn ? 8192 : 16, 1024, 2);
+                const uint64_t db = tc::make_smem_desc(stage0 + kStageA, q.b_mn ? 8192 : 16, 1024, 2);
+                const uint64_t step_a = q.a_mn ? 2048 >> 4 : 32 >> 4, step_b = q.b_mn ? 2048 >> 4 : 32 >> 4;
+                for (int k = 0; k < q.k_steps; ++k) {
+                    if (!tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_dense_error, 3)) { ok = false; break; }
+                    tc::fence_after();
+                    const uint64_t a = da + (uint64_t)(s * kStage >> 4), b = db + (uint64_t)(s * kStage >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        tc::mma_pair_f16(acc, a + kk * step_a, b + kk * step_b, idesc, (k | kk) ? 1u : 0u);
+                    tc::commit_pair(empty0 + 8 * s);
+                    tc::commit_pair(empty0_peer + 8 * s);
+                    if (++s == kStages) { s = 0; parity ^= 1; }
+                }
+                if (!ok) break;
+                tc::commit_pair(tc::smem_u32(&acc_full[buf]));
+                tc::commit_pair(tc::cluster_addr(tc::smem_u32(&acc_full[buf]), 1));
+            }
+        }
+    } else {
+        // ---------------- epilogue: warp w reads tensor-memory lanes 32 (w % 4) .. +31 ----------------
+        const int quarter = warp & 3, side = (warp - 2) >> 2;
+        const bool half = p.half != 0;
+        int it = 0;
+        for (int item = cluster_id; item < p.n_items; item += n_clusters, ++it) {
+            const TileId t = tile_of(p, item);
+            const Problem &q = p.prob[t.p];
+            const int buf = it & 1;
+            const long long row = (long long)t.tm * 256 + (long long)rank * 128 + quarter * 32 + lane;
+            if (!tc::mbar_wait(tc::smem_u32(&acc_full[buf]), (it >> 1) & 1, abort_flag, &g_dense_error, 4)) break;
+            tc::fence_after();
+            const uint32_t taddr = tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16);
+            if (EPI == kStore) {
+                for (int c = side * (kBN / 2); c < (side + 1) * (kBN / 2); c += 32) {
+                    float v[32];
+                    acc32(taddr + c, v);
+                    const int col = t.tn * kBN + c;
+                    if (row < q.m) store32(q.out, row * q.ld_out + col, v, q.n - col, half);
+                }
+            } else if (EPI == kSwiglu) {
+                for (int c = side * (kBN / 4); c < (side + 1) * (kBN / 4); c += 32) {
+                    float g[32], u[32];
+                    acc32(taddr + c, g);
+                    acc32(taddr + kBN / 2 + c, u);
+                    const int col = t.tn * (kBN / 2) + c;
+                    if (row < q.m) {
+                        if (p.gu) {
+                            store32(p.gu, row * p.ld_gu + col, g, q.n - col, half);
+                            store32(p.gu, row * p.ld_gu + p.d_ff + col, u, q.n - col, half);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid(g[i]) * u[i];
+                        store32(q.out, row * q.ld_out + col, g, q.n - col, half);
+                    }
+                }
+            } else {
+                for (int c = side * (kBN / 2); c < (side + 1) * (kBN / 2); c += 32) {
+                    float dh[32];
+                    acc32(taddr + c, dh);
+                    const int col = t.tn * kBN + c;
+                    if (row < q.m) {
+                        float g[32], u[32];
+                        load32(p.gu, row * p.ld_gu + col, g, q.n - col, half);
+                        load32(p.gu, row * p.ld_gu + p.d_ff + col, u, q.n - col, half);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float s = sigmoid(g[i]), a = g[i] * s, d = dh[i];
+                            g[i] = d * u[i] * (s + a * (1.f - s));
+                            u[i] = d * a;
+                        }
+                        store32(q.out, row * q.ld_out + col, g, q.n - col, half);
+                        store32(q.out, row * q.ld_out + p.d_ff + col, u, q.n - col, half);
+                    }
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::arrive_cluster(tc::cluster_addr(tc::smem_u32(&acc_empty[buf]), 0));
+        }
+    }
+
+    // neither CTA may leave (or free tensor memory) while its peer can still read its shared memory or
+    // signal its barriers
+    __syncwarp();
+    if (*abort_flag) tc::drain_after_abort();
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+bool misaligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+
+// Adds C[m][n] = sum_k A[m][k] B[n][k] to a launch.  `a` is [m][k] (row stride lda) or, with a_mn, [k][m];
+// `b` is [n][k] or, with b_mn, [k][n].  For kSwiglu n counts hidden columns and b has 2 n rows.
+int add_problem(DenseParams &p, int epi, const void *a, int64_t lda, bool a_mn, const void *b, int64_t ldb, bool b_mn,
+                int64_t m, int64_t n, int64_t k, void *out, int64_t ld_out) {
+    const int i = p.n_problems;
+    Problem &q = p.prob[i];
+    const int64_t b_rows = epi == kSwiglu ? 2 * n : n, tile_n = epi == kSwiglu ? kBN / 2 : kBN;
+    int rc = a_mn ? tc::encode_bf16_2d(&p.map_a[i], a, m, k, lda, 64, 64)
+                  : tc::encode_bf16_2d(&p.map_a[i], a, k, m, lda, 64, 128);
+    if (rc != MORTAR_OK) return rc;
+    rc = b_mn ? tc::encode_bf16_2d(&p.map_b[i], b, b_rows, k, ldb, 64, 64)
+              : tc::encode_bf16_2d(&p.map_b[i], b, k, b_rows, ldb, 64, kBN / 2);
+    if (rc != MORTAR_OK) return rc;
+    const int64_t tm = (m + 255) / 256, tn = (n + tile_n - 1) / tile_n;
+    if (tm * tn + p.n_items > 0x3fffffff) return MORTAR_ERR_CAPACITY;
+    q.out = out; q.ld_out = ld_out; q.m = m; q.n = (int)n;
+    q.tiles_m = (int)tm; q.tiles_n = (int)tn; q.k_steps = (int)((k + 63) / 64);
+    q.a_mn = a_mn; q.b_mn = b_mn; q.first_item = p.n_items;
+    p.n_items += (int)(tm * tn);
+    ++p.n_problems;
+    return MORTAR_OK;
+}
+
+std::mutex g_dense_mutex;
+
+template <int EPI>
+int launch(const DenseParams &p, cudaStream_t st) {
+    static bool ready[64] = {false};
+    int sms = 0;
+    int rc = tc::allow_smem(dense_pair_kernel<EPI>, kSmem, ready, g_dense_mutex, nullptr);
+    if (rc != MORTAR_OK) return rc;
+    rc = tc::sm_count(&sms);
+    if (rc != MORTAR_OK) return rc;
+    const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
+    dense_pair_kernel<EPI><<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
+    MORTAR_CUDA_CHECK(cudaGetLastError());
+    return MORTAR_OK;
+}
+
+int check_shape(int32_t dtype, int64_t rows, int32_t d_model, int32_t d_ff) {
+    if (rows < 0 || d_model <= 0 || d_ff <= 0 || d_model % 16 || d_ff % 16) return MORTAR_ERR_SHAPE;
+    if (rows > 0x7fffff00LL || d_ff > (1 << 29) || d_model > (1 << 29)) return MORTAR_ERR_CAPACITY;
+    if (dtype != MORTAR_BF16 && dtype != MORTAR_F16) return MORTAR_ERR_DTYPE;
+    return MORTAR_OK;
+}
+
+}  // namespace
+
+extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64_t rows, const void *gate_up,
+                                int64_t ld_gate_up, const void *down, int64_t ld_down, int32_t d_model, int32_t d_ff,
+                                void *hidden, void *gate_up_sums, void *y, int64_t ldy, void *stream) {
+    if (!x || !gate_up || !down || !hidden || !y) return MORTAR_ERR_NULL;
+    int rc = check_shape(dtype, rows, d_model, d_ff);
+    if (rc != MORTAR_OK) return rc;
+    if (ldx < d_model || ld_gate_up < d_model || ld_down < d_ff || ldy < d_model) return MORTAR_ERR_SHAPE;
+    if (misaligned(x) || misaligned(gate_up) || misaligned(down) || misaligned(hidden) || misaligned(gate_up_sums) ||
+        misaligned(y) || ldx % 8 || ld_gate_up % 8 || ld_down % 8 || ldy % 8)
+        return MORTAR_ERR_ALIGN;
+    if (rows == 0) return MORTAR_OK;
+    cudaStream_t st = (cudaStream_t)stream;
+    alignas(64) DenseParams p = {};
+    p.half = dtype == MORTAR_F16;
+    p.d_ff = d_ff;
+    p.gu = gate_up_sums;
+    p.ld_gu = 2LL * d_ff;
+    rc = add_problem(p, kSwiglu, x, ldx, false, gate_up, ld_gate_up, false, rows, d_ff, d_model, hidden, d_ff);
+    if (rc == MORTAR_OK) rc = launch<kSwiglu>(p, st);
+    if (rc != MORTAR_OK) return rc;
+    alignas(64) DenseParams p2 = {};
+    p2.half = p.half;
+    rc = add_problem(p2, kStore, hidden, d_ff, false, down, ld_down, false, rows, d_model, d_ff, y, ldy);
+    return rc == MORTAR_OK ? launch<kStore>(p2, st) : rc;
+}
+
+extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int32_t dtype,
+                                         int64_t rows, const void *gate_up, int64_t ld_gate_up, const void *down,
+                                         int64_t ld_down, int32_t d_model, int32_t d_ff, const void *hidden,
+                                         const void *gate_up_sums, void *dgate_up_sums, void *dx, void *dgate_up,
+                                         void *ddown, void *stream) {
+    if (!dy || !x || !gate_up || !down || !hidden || !gate_up_sums || !dgate_up_sums) return MORTAR_ERR_NULL;
+    int rc = check_shape(dtype, rows, d_model, d_ff);
+    if (rc != MORTAR_OK) return rc;
+    if (lddy < d_model || ldx < d_model || ld_gate_up < d_model || ld_down < d_ff) return MORTAR_ERR_SHAPE;
+    if (misaligned(dy) || misaligned(x) || misaligned(gate_up) || misaligned(down) || misaligned(hidden) ||
+        misaligned(gate_up_sums) || misaligned(dgate_up_sums) || misaligned(dx) || misaligned(dgate_up) ||
+        misaligned(ddown) || lddy % 8 || ldx % 8 || ld_gate_up % 8 || ld_down % 8)
+        return MORTAR_ERR_ALIGN;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (rows == 0) {
+        if (dgate_up) MORTAR_CUDA_CHECK(cudaMemsetAsync(dgate_up, 0, (size_t)4 * d_ff * d_model, st));
+        if (ddown) MORTAR_CUDA_CHECK(cudaMemsetAsync(ddown, 0, (size_t)2 * d_ff * d_model, st));
+        return MORTAR_OK;
+    }
+    const int64_t f2 = 2LL * d_ff;
+    if (dx || dgate_up) {
+        alignas(64) DenseParams p = {};
+        p.half = dtype == MORTAR_F16;
+        p.d_ff = d_ff;
+        p.gu = const_cast<void *>(gate_up_sums);
+        p.ld_gu = f2;
+        rc = add_problem(p, kSwigluBackward, dy, lddy, false, down, ld_down, true, rows, d_ff, d_model, dgate_up_sums, f2);
+        if (rc == MORTAR_OK) rc = launch<kSwigluBackward>(p, st);
+        if (rc != MORTAR_OK) return rc;
+    }
+    alignas(64) DenseParams p = {};
+    p.half = dtype == MORTAR_F16;
+    if (dgate_up)
+        rc = add_problem(p, kStore, dgate_up_sums, f2, true, x, ldx, true, f2, d_model, rows, dgate_up, d_model);
+    if (rc == MORTAR_OK && dx)
+        rc = add_problem(p, kStore, dgate_up_sums, f2, false, gate_up, ld_gate_up, true, rows, d_model, f2, dx, d_model);
+    if (rc == MORTAR_OK && ddown)
+        rc = add_problem(p, kStore, dy, lddy, true, hidden, d_ff, true, d_model, d_ff, rows, ddown, d_ff);
+    if (rc != MORTAR_OK || p.n_problems == 0) return rc;
+    return launch<kStore>(p, st);
+}
+
+extern "C" int mortar_dense_error(int32_t *code, int32_t reset) {
+    if (!code) return MORTAR_ERR_NULL;
+    int v = 0;
+    MORTAR_CUDA_CHECK(cudaMemcpyFromSymbol(&v, g_dense_error, sizeof(int)));
+    *code = v;
+    if (reset && v != 0) {
+        const int zero = 0;
+        MORTAR_CUDA_CHECK(cudaMemcpyToSymbol(g_dense_error, &zero, sizeof(int)));
+    }
+    return MORTAR_OK;
+}

@@ -1,0 +1,305 @@
+// Matrix product of two 8-bit floating-point operands with one scale per block of 128, on the
+// 5th-generation tensor cores:
+//
+//   y[m][n] = sum over blocks b of sx[m][b] * sw[n / 128][b] * sum_{k in block b} qx[m][k] qw[n][k]
+//
+// (activations scaled per 1 x 128, weights per 128 x 128), and with the gate applied,
+// y = silu(y[:, :n/2]) * y[:, n/2:].
+//
+// The scales are any fp32 numbers, so a block's sum has to leave the accumulator before the next
+// block's begins: one pipeline stage is one block (128 bytes of k, a swizzle row), its four MMAs
+// (kind::f8f6f4, K = 32) write one of two accumulator sets, and the epilogue warps read the set,
+// multiply by sx * sw (one factor per thread and 128 columns) and add it to fp32 sums in registers
+// while the MMAs fill the other set.  A cluster of two CTAs computes 256 x 256: per SM and block the
+// MMAs take 512 cycles, the tensor-memory reads of 128 x 256 sums about 256 and their multiply-adds
+// 256 issue slots of each scheduler, so the sums keep up with the MMAs.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+#include <mutex>
+#include "common.h"
+#include "tc_pair.cuh"
+
+namespace {
+
+constexpr int kStages = 6;
+constexpr int kStageA = 128 * 128;               // this CTA's 128 rows, one block of 128 bytes each
+constexpr int kStageB = 128 * 128;               // this CTA's half of the 256 output columns
+constexpr int kStage = kStageA + kStageB;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kTmemCols = 512;
+constexpr int kSmem = kStages * kStage + (2 * kStages + 4) * 8 + 1024;
+
+__device__ int g_fp8_error;
+
+struct Fp8Params {
+    CUtensorMap map_x, map_w;
+    const float *xs, *ws;
+    long long ld_xs, ld_ws;
+    long long rows;
+    int n;                   // output columns (hidden columns with the gate)
+    int tiles_m, tiles_n, n_items;
+    int k_blocks;
+    int up_row;              // 0, or the first up row of w (gate applied)
+    int w_blocks;            // rows of ws
+    uint32_t types;          // operand type bits of the instruction descriptor
+    void *out;
+    long long ld_out;
+    int out_dtype;
+    int vec;                 // 1: rows of out start on 16 bytes
+};
+
+__device__ __forceinline__ float silu(float g) { return g / (1.f + expf(-g)); }
+
+// 32 values of one row from column `col` on
+__device__ __forceinline__ void store_row32(const Fp8Params &p, long long row, int col, const float (&v)[32]) {
+    const int left = p.n - col;
+    if (row >= p.rows || left <= 0) return;
+    const long long idx = row * p.ld_out + col;
+    if (p.out_dtype == MORTAR_F32) {
+        float *o = reinterpret_cast<float *>(p.out) + idx;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (p.vec && 4 * j + 4 <= left) reinterpret_cast<float4 *>(o)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (4 * j + i < left) o[4 * j + i] = v[4 * j + i];
+        }
+        return;
+    }
+    const bool half = p.out_dtype == MORTAR_F16;
+    uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + idx;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = tc::pack16(v[8 * j + 2 * i], v[8 * j + 2 * i + 1], half);
+        if (p.vec && 8 * j + 8 <= left) reinterpret_cast<uint4 *>(o)[j] = make_uint4(w[0], w[1], w[2], w[3]);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (8 * j + i < left) o[8 * j + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
+}
+
+__device__ __forceinline__ void tile_of(const Fp8Params &p, int item, int &tm, int &tn) {
+    const int band = item / (8 * p.tiles_n), r = item - band * 8 * p.tiles_n;
+    const int h = min(8, p.tiles_m - band * 8);
+    tn = r / h;
+    tm = band * 8 + r - tn * h;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t *>(stages + kStages * kStage), *empty = full + kStages;
+    uint64_t *acc_full = empty + kStages, *acc_empty = acc_full + 2;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int abort_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = tc::cluster_rank();
+    const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        abort_s = 0;
+        for (int s = 0; s < kStages; ++s) { tc::mbar_init(tc::smem_u32(&full[s]), 1); tc::mbar_init(tc::smem_u32(&empty[s]), 1); }
+        for (int s = 0; s < 2; ++s) { tc::mbar_init(tc::smem_u32(&acc_full[s]), 1); tc::mbar_init(tc::smem_u32(&acc_empty[s]), 2 * kEpiWarps); }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                     ::"r"(tc::smem_u32(&tmem_base_s)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();
+    tc::fence_after();
+    const uint32_t tmem = tmem_base_s;
+    volatile int *abort_flag = &abort_s;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint32_t full_lead = tc::cluster_addr(tc::smem_u32(full), 0);
+            const uint32_t empty0 = tc::smem_u32(empty), stage0 = tc::smem_u32(stages);
+            uint32_t s = 0, parity = 1;
+            bool ok = true;
+            for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
+                int tm, tn;
+                tile_of(p, item, tm, tn);
+                const int row0 = tm * 256 + (int)rank * 128;
+                const int col0 = p.up_row ? tn * 128 + (rank ? p.up_row : 0) : tn * 256 + (int)rank * 128;
+                for (int k = 0; k < p.k_blocks; ++k) {
+                    if (!tc::mbar_wait(empty0 + 8 * s, parity, abort_flag, &g_fp8_error, 1)) { ok = false; break; }
+                    const uint32_t bar = full_lead + 8 * s, dst = stage0 + s * kStage;
+                    if (rank == 0) tc::mbar_arrive_expect_tx(tc::smem_u32(&full[s]), 2 * kStage);
+                    tc::load_pair(dst, &p.map_x, k * 128, row0, bar);
+                    tc::load_pair(dst + kStageA, &p.map_w, k * 128, col0, bar);
+                    if (++s == kStages) { s = 0; parity ^= 1; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && lane == 0) {
+            const uint32_t idesc = (1u << 4) | p.types | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+            const uint32_t full0 = tc::smem_u32(full), empty0 = tc::smem_u32(empty);
+            const uint32_t empty0_peer = tc::cluster_addr(empty0, 1);
+            const uint32_t acc0 = tc::smem_u32(acc_full), acc0_peer = tc::cluster_addr(acc0, 1);
+            const uint64_t da = tc::make_smem_desc(tc::smem_u32(stages), 16, 1024, 2);
+            const uint64_t db = tc::make_smem_desc(tc::smem_u32(stages) + kStageA, 16, 1024, 2);
+            uint32_t s = 0, parity = 0, g = 0;
+            bool ok = true;
+            for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
+                for (int k = 0; k < p.k_blocks; ++k, ++g) {
+                    const uint32_t buf = g & 1;
+                    if (!tc::mbar_wait(tc::smem_u32(&acc_empty[buf]), ((g >> 1) & 1) ^ 1u, abort_flag, &g_fp8_error, 2) ||
+                        !tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_fp8_error, 3)) { ok = false; break; }
+                    tc::fence_after();
+                    const uint64_t a = da + (uint64_t)(s * kStage >> 4), b = db + (uint64_t)(s * kStage >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        tc::mma_pair_f8(tmem + buf * 256, a + 2 * kk, b + 2 * kk, idesc, kk ? 1u : 0u);
+                    tc::commit_pair(empty0 + 8 * s);
+                    tc::commit_pair(empty0_peer + 8 * s);
+                    tc::commit_pair(acc0 + 8 * buf);
+                    tc::commit_pair(acc0_peer + 8 * buf);
+                    if (++s == kStages) { s = 0; parity ^= 1; }
+                }
+            }
+        }
+    } else {
+        // warp w: accumulator lanes 32 (w % 4) .. +31, columns 64 side .. +63 of either 128-column half, so
+        // that a thread holds the gate and the up sum of its hidden columns
+        const int quarter = warp & 3, side = (warp - 2) >> 2;
+        const uint32_t lead_empty = tc::cluster_addr(tc::smem_u32(acc_empty), 0);
+        uint32_t g = 0;
+        bool ok = true;
+        for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
+            int tm, tn;
+            tile_of(p, item, tm, tn);
+            const long long row = (long long)tm * 256 + (long long)rank * 128 + quarter * 32 + lane;
+            const int wb0 = p.up_row ? tn : 2 * tn, wb1 = p.up_row ? p.up_row / 128 + tn : 2 * tn + 1;
+            const float *xs = p.xs + (row < p.rows ? row : p.rows - 1) * p.ld_xs;
+            const float *ws0 = p.ws + (long long)wb0 * p.ld_ws, *ws1 = p.ws + (long long)min(wb1, p.w_blocks - 1) * p.ld_ws;
+            float sum[4][32];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sum[j][i] = 0.f;
+            for (int k = 0; k < p.k_blocks; ++k, ++g) {
+                const uint32_t buf = g & 1;
+                const float sx = __ldg(xs + k), f0 = sx * __ldg(ws0 + k), f1 = sx * __ldg(ws1 + k);
+                if (!tc::mbar_wait(tc::smem_u32(&acc_full[buf]), (g >> 1) & 1, abort_flag, &g_fp8_error, 4)) { ok = false; break; }
+                tc::fence_after();
+                const uint32_t taddr = tmem + buf * 256 + ((uint32_t)(quarter * 32) << 16) + side * 64;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t r[32];
+                    tc::ld32(taddr + (j >> 1) * 128 + (j & 1) * 32, r);
+                    tc::wait_ld();
+                    const float f = j < 2 ? f0 : f1;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[j][i] = fmaf(__uint_as_float(r[i]), f, sum[j][i]);
+                }
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::arrive_cluster(lead_empty + 8 * buf);
+            }
+            if (!ok) break;
+            if (p.up_row) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[j][i] = silu(sum[j][i]) * sum[j + 2][i];
+                    store_row32(p, row, tn * 128 + side * 64 + j * 32, sum[j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) store_row32(p, row, tn * 256 + (j >> 1) * 128 + side * 64 + (j & 1) * 32, sum[j]);
+            }
+        }
+    }
+
+    __syncwarp();
+    if (*abort_flag) tc::drain_after_abort();
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+bool misaligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
+
+std::mutex g_fp8_mutex;
+
+}  // namespace
+
+extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, const float *x_scale, int64_t ld_x_scale,
+                                 int64_t rows, const void *w, int32_t w_type, int64_t ldw, const float *w_scale,
+                                 int64_t ld_w_scale, int32_t out_features, int32_t in_features, int32_t flags, void *out,
+                                 int32_t out_dtype, int64_t ld_out, void *stream) {
+    if (!x || !x_scale || !w || !w_scale || !out) return MORTAR_ERR_NULL;
+    const bool gated = (flags & MORTAR_FLAG_SWIGLU) != 0;
+    const int64_t k_blocks = ((int64_t)in_features + 127) / 128;
+    if (rows < 0 || out_features <= 0 || in_features <= 0 || in_features % 16 || ldx < in_features ||
+        ldw < in_features || ld_x_scale < k_blocks || ld_w_scale < k_blocks || (gated && out_features % 256) ||
+        ld_out < (gated ? out_features / 2 : out_features))
+        return MORTAR_ERR_SHAPE;
+    if ((x_type != MORTAR_E4M3 && x_type != MORTAR_E5M2) || (w_type != MORTAR_E4M3 && w_type != MORTAR_E5M2) ||
+        (out_dtype != MORTAR_F32 && out_dtype != MORTAR_BF16 && out_dtype != MORTAR_F16) || (flags & ~MORTAR_FLAG_SWIGLU))
+        return MORTAR_ERR_DTYPE;
+    const size_t e = out_dtype == MORTAR_F32 ? 4 : 2;
+    if (misaligned(x, 16) || misaligned(w, 16) || ldx % 16 || ldw % 16 || misaligned(out, e) || misaligned(x_scale, 4) ||
+        misaligned(w_scale, 4))
+        return MORTAR_ERR_ALIGN;
+    if (rows > 0x7fffff00LL || out_features > 0x7fffff00) return MORTAR_ERR_CAPACITY;
+    if (rows == 0) return MORTAR_OK;
+    cudaStream_t st = (cudaStream_t)stream;
+
+    alignas(64) Fp8Params p = {};
+    int rc = tc::encode_u8_2d(&p.map_x, x, in_features, rows, ldx, 128);
+    if (rc != MORTAR_OK) return rc;
+    rc = tc::encode_u8_2d(&p.map_w, w, in_features, out_features, ldw, 128);
+    if (rc != MORTAR_OK) return rc;
+    p.xs = x_scale; p.ws = w_scale; p.ld_xs = ld_x_scale; p.ld_ws = ld_w_scale;
+    p.rows = rows;
+    p.n = gated ? out_features / 2 : out_features;
+    p.up_row = gated ? out_features / 2 : 0;
+    const int tile_n = gated ? 128 : 256;
+    p.tiles_m = (int)((rows + 255) / 256);
+    p.tiles_n = (p.n + tile_n - 1) / tile_n;
+    if ((int64_t)p.tiles_m * p.tiles_n > 0x3fffffff) return MORTAR_ERR_CAPACITY;
+    p.n_items = p.tiles_m * p.tiles_n;
+    p.k_blocks = (int)k_blocks;
+    p.w_blocks = (out_features + 127) / 128;
+    p.types = (x_type == MORTAR_E5M2 ? 1u << 7 : 0u) | (w_type == MORTAR_E5M2 ? 1u << 10 : 0u);
+    p.out = out; p.ld_out = ld_out; p.out_dtype = out_dtype;
+    p.vec = !misaligned(out, 16) && (ld_out * e) % 16 == 0;
+
+    static bool ready[64] = {false};
+    int sms = 0;
+    rc = tc::allow_smem(fp8_pair_kernel, kSmem, ready, g_fp8_mutex, nullptr);
+    if (rc != MORTAR_OK) return rc;
+    rc = tc::sm_count(&sms);
+    if (rc != MORTAR_OK) return rc;
+    const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
+    fp8_pair_kernel<<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
+    MORTAR_CUDA_CHECK(cudaGetLastError());
+    return MORTAR_OK;
+}
+
+extern "C" int mortar_linear_fp8_error(int32_t *code, int32_t reset) {
+    if (!code) return MORTAR_ERR_NULL;
+    int v = 0;
+    MORTAR_CUDA_CHECK(cudaMemcpyFromSymbol(&v, g_fp8_error, sizeof(int)));
+    *code = v;
+    if (reset && v != 0) {
+        const int zero = 0;
+        MORTAR_CUDA_CHECK(cudaMemcpyToSymbol(g_fp8_error, &zero, sizeof(int)));
+    }
+    return MORTAR_OK;
+}

@@ -1,0 +1,140 @@
+// Device helpers of the kernels that run one tcgen05 product on two CTAs (cta_group::2): cluster
+// addressing, loads and commits that complete on a barrier of either CTA, paired MMAs of both operand
+// kinds, wide tensor-memory reads, and the reduced-precision conversions of their epilogues.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "tc_common.cuh"
+
+namespace tc {
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+    return r;
+}
+// shared::cluster address of the same shared-memory offset in CTA `rank` of this cluster
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+
+// TMA tile load into this CTA's shared memory that completes on a barrier of either CTA of the pair
+__device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t cluster_bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];\n"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t cluster_bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+                 ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void mma_pair_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_pair_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// 32 accumulator columns of this thread's tensor-memory lane; `wait_ld` before the registers are read
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+
+// two fp32 values as one word of bf16 (or fp16) values, `lo` in the low half, round to nearest even
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool half) {
+    if (half) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ float2 unpack16(uint32_t w, bool half) {
+    if (half) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w));
+}
+
+// A role that gave up leaves copies and MMAs of its CTA in flight; they end within microseconds of
+// the last issue, so an aborted CTA waits about a millisecond before it frees anything.
+__device__ __forceinline__ void drain_after_abort() {
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+}
+
+// [rows][cols] 8-bit row-major with row stride ld as a 2-D map with a [box_rows][128] box and the
+// 128-byte swizzle.
+inline int encode_u8_2d(CUtensorMap *map, const void *base, int64_t cols, int64_t rows, int64_t ld,
+                        uint32_t box_rows) {
+    EncodeTiledFn encode;
+    const int rc = get_encode_fn(&encode);
+    if (rc != MORTAR_OK) return rc;
+    const cuuint64_t gdim[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t gstride[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {128, box_rows};
+    const cuuint32_t estride[2] = {1, 1};
+    const CUresult cr = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), gdim, gstride, box,
+                               estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) {
+        mortar_set_cuda_error("cuTensorMapEncodeTiled", "failed to encode a tensor map");
+        return MORTAR_ERR_CUDA;
+    }
+    return MORTAR_OK;
+}
+
+// First use of a kernel on the current device: its dynamic shared memory limit.  `done` holds one
+// flag per device.
+template <class Kernel>
+inline int allow_smem(Kernel kernel, int bytes, bool (&done)[64], std::mutex &m, int *device) {
+    int dev = 0;
+    MORTAR_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return MORTAR_ERR_CAPACITY;
+    std::lock_guard<std::mutex> lock(m);
+    if (!done[dev]) {
+        MORTAR_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done[dev] = true;
+    }
+    if (device) *device = dev;
+    return MORTAR_OK;
+}
+
+// SMs of the current device (queried once per device)
+inline int sm_count(int *out) {
+    static int cached[64] = {0};
+    static std::mutex m;
+    int dev = 0;
+    MORTAR_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return MORTAR_ERR_CAPACITY;
+    std::lock_guard<std::mutex> lock(m);
+    if (!cached[dev])
+        MORTAR_CUDA_CHECK(cudaDeviceGetAttribute(&cached[dev], cudaDevAttrMultiProcessorCount, dev));
+    *out = cached[dev];
+    return MORTAR_OK;
+}
+
+}  // namespace tc

@@ -654,3 +654,47 @@ class StreamMatrix:
                                   self.out_features // TILE, self.in_features // TILE, self.scale,
                                   None if self.row_scale is None else self.row_scale.data_ptr())
         return self._c
+
+
+class Fp8Matrix:
+    """A dense matrix [out_features, in_features] in 8-bit floating point with one fp32 scale per
+    128 x 128 block (``scale`` [ceil(out/128), ceil(in/128)]): the weights of ``ops.linear_fp8``.
+    ``from_dense`` quantises a matrix; the constructor takes the parts another program made, with
+    any finite scales."""
+
+    BLOCK = 128
+
+    def __init__(self, data: torch.Tensor, scale: torch.Tensor):
+        if data.dim() != 2 or data.dtype not in (torch.float8_e4m3fn, torch.float8_e5m2):
+            raise ValueError("data must be a float8_e4m3fn or float8_e5m2 matrix [out_features, in_features]")
+        out_features, in_features = data.shape
+        if out_features < 1 or in_features < 1 or in_features % TILE:
+            raise ValueError(f"in_features must be a positive multiple of {TILE} and out_features positive, "
+                             f"got [{out_features}, {in_features}]")
+        want = (-(-out_features // self.BLOCK), -(-in_features // self.BLOCK))
+        if tuple(scale.shape) != want or scale.dtype != torch.float32:
+            raise ValueError(f"scale must be float32 {list(want)}, got {scale.dtype} {list(scale.shape)}")
+        if scale.device != data.device:
+            raise ValueError(f"data is on {data.device} but scale on {scale.device}")
+        if data.stride(1) != 1 or data.stride(0) % 16 or data.stride(0) < in_features or data.data_ptr() % 16:
+            data = data.contiguous()
+        self.data, self.scale = data, scale.contiguous()
+        self.out_features, self.in_features = int(out_features), int(in_features)
+
+    @classmethod
+    def from_dense(cls, weight: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> "Fp8Matrix":
+        """Quantises a CUDA matrix (fp32, bf16 or fp16) with ``ops.quantize_fp8``."""
+        from . import ops
+        return cls(*ops.quantize_fp8(weight.detach(), block_rows=cls.BLOCK, dtype=dtype))
+
+    def to_dense(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """data * scale, rounded once to ``dtype``."""
+        from . import ops
+        return ops.dequantize_fp8(self.data, self.scale, out_dtype=dtype)
+
+    def to(self, device) -> "Fp8Matrix":
+        return Fp8Matrix(self.data.to(device), self.scale.to(device))
+
+    @property
+    def device(self):
+        return self.data.device

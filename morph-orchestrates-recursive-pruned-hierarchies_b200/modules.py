@@ -4,8 +4,9 @@
 Same constructor signatures, attribute names, ``state_dict`` keys, argument meaning and error
 behaviour; the forward runs the sm_100a kernels of this package.
 
-Only the carved (post-``carve()``) phase is served: the dense pre-carve phase, saliency
-scoring and pruning belong to training.  A layer built with the reference constructor holds
+The mirrors serve the carved (post-``carve()``) phase; ``SwiGLUDense`` is the block before it
+(trainable) and ``SwiGLUFp8`` its 8-bit serving form.  Saliency scoring and pruning are not part of
+this package.  A mirror built with the reference constructor holds
 no weights until a carved ``state_dict`` is loaded into it (the reference's own
 ``mortar_*`` keys, unpacked or 2-bit packed) or it is filled with ``from_matrix`` /
 ``from_reference``.
@@ -23,7 +24,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from .format import TILE, BlockSched, MortarMatrix, SchedMatrix, StreamMatrix, wants_block_path
+from .format import TILE, BlockSched, Fp8Matrix, MortarMatrix, SchedMatrix, StreamMatrix, wants_block_path
 
 # bf16 token blocks with at least this many rows take the tensor-memory kernel.  Measured on
 # B200 at the 768/2048 and 2048/5632 shapes: the streaming kernel wins below 128 rows, the
@@ -363,6 +364,63 @@ class SwiGLUMortar(nn.Module):
             return ops.mlp_prefill(x, gu.stream(), dn.stream(), gates=gates, n_clusters=self.n_clusters)
         return ops.mlp_decode(x, gu.stream(), dn.stream(), gates=gates, n_clusters=self.n_clusters,
                               n_planes=3)
+
+
+class SwiGLUDense(nn.Module):
+    """The MLP site before it is carved (morph/model/transformer.py:319-431 with dense weights),
+    trainable: [layer norm ->] gate_up -> silu(gate) * up -> down through ``ops.layer_norm`` and
+    ``ops.mlp_dense``.  ``gate_up.weight`` [2 d_ff, d_model] (gate rows first) and ``down.weight``
+    [d_model, d_ff] are what a carve quantises; ``norm=True`` puts a layer norm with weight and
+    bias in front.  bf16 and fp16 inputs run with weights of their type (fp32 weights are cast, their
+    gradients come back in fp32); fp32 inputs need autocast, whose type they are cast to after
+    the norm."""
+
+    def __init__(self, d_model: int, d_ff: int, norm: bool = False, eps: float = 1e-5, device=None, dtype=None):
+        super().__init__()
+        if d_model < 1 or d_ff < 1 or d_model % TILE or d_ff % TILE:
+            raise ValueError(f"d_model and d_ff must be positive multiples of {TILE}, got {d_model} and {d_ff}")
+        self.gate_up = nn.Linear(d_model, 2 * d_ff, bias=False, device=device, dtype=dtype)
+        self.down = nn.Linear(d_ff, d_model, bias=False, device=device, dtype=dtype)
+        self.norm = nn.LayerNorm(d_model, eps=eps, device=device, dtype=dtype) if norm else None
+        self.d_model, self.d_ff = d_model, d_ff
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.norm is not None:
+            x = ops.layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps)
+        if torch.is_autocast_enabled() and x.is_cuda and x.dtype == torch.float32:
+            x = x.to(torch.get_autocast_dtype("cuda"))
+        return ops.mlp_dense(x, self.gate_up.weight.to(x.dtype), self.down.weight.to(x.dtype))
+
+    def to_fp8(self, dtype: torch.dtype = torch.float8_e4m3fn) -> "SwiGLUFp8":
+        """The same site with its weights in 8-bit floating point, for serving."""
+        n = self.norm
+        return SwiGLUFp8(Fp8Matrix.from_dense(self.gate_up.weight, dtype), Fp8Matrix.from_dense(self.down.weight, dtype),
+                         None if n is None else (n.weight.detach().clone(), n.bias.detach().clone(), n.eps))
+
+
+class SwiGLUFp8(nn.Module):
+    """The MLP site served in 8-bit floating point (``ops.mlp_fp8``), with the layer norm of the
+    ``SwiGLUDense`` it was made from: ``norm`` = (weight, bias, eps) or None."""
+
+    def __init__(self, gate_up: Fp8Matrix, down: Fp8Matrix, norm=None):
+        super().__init__()
+        if gate_up.out_features != 2 * down.in_features or gate_up.in_features != down.out_features:
+            raise ValueError("gate_up must be [2*d_ff, d_model] and down [d_model, d_ff]")
+        if gate_up.out_features % 256:
+            raise ValueError(f"d_ff must be a multiple of 128, got {down.in_features}")
+        for name, m in (("gate_up", gate_up), ("down", down)):
+            self.register_buffer(name + "_data", m.data)
+            self.register_buffer(name + "_scale", m.scale)
+        self.register_buffer("norm_weight", None if norm is None else norm[0])
+        self.register_buffer("norm_bias", None if norm is None else norm[1])
+        self.eps = None if norm is None else float(norm[2])
+        self.d_model, self.d_ff = down.out_features, down.in_features
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.eps is not None:
+            x = ops.layer_norm(x, self.norm_weight, self.norm_bias, self.eps)
+        return ops.mlp_fp8(x, Fp8Matrix(self.gate_up_data, self.gate_up_scale), Fp8Matrix(self.down_data, self.down_scale))
 
 
 def decode_stack(mlps: Sequence[SwiGLUMortar], norm_weights: Sequence[Optional[torch.Tensor]],

@@ -5,13 +5,14 @@ morph/sparse/stk/backend/custom_ops.py:35).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .format import TILE, BlockSched, GemvBlocks, MortarMatrix, SchedMatrix, StreamMatrix, TopologyDev
+from .format import TILE, BlockSched, Fp8Matrix, GemvBlocks, MortarMatrix, SchedMatrix, StreamMatrix, TopologyDev
 
 _launches = 0      # kernels launched by this module (bench.py reports it)
 _kernel_counts: dict = {}   # the same, per kernel family
@@ -953,6 +954,370 @@ def rmsnorm_rows(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Ten
     activation-prep kernel and re-assembled from its three exact planes."""
     planes = act_prep(x, 3, rms_weight=weight, eps=eps)
     return planes.float().sum(0).reshape(x.shape)
+
+
+# ---- the dense MLP site: norm, block before carving, 8-bit serving form -----------------
+
+_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16,
+         torch.float8_e4m3fn: _lib.E4M3, torch.float8_e5m2: _lib.E5M2}
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
+
+
+def _on_device(t: torch.Tensor):
+    """The launch goes to the device of ``t`` and to that device's current stream."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _same_device(t: torch.Tensor, **others) -> None:
+    for name, o in others.items():
+        if o is not None and o.device != t.device:
+            raise ValueError(f"{name} is on {o.device}, expected {t.device}")
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [rows, cols] itself when its rows are contiguous and start on 16 bytes, else a copy."""
+    per16 = 16 // t.element_size()
+    if t.stride(1) != 1 or t.stride(0) % per16 or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _rows_any(t: torch.Tensor) -> torch.Tensor:
+    """[..., cols] -> [rows, cols] with contiguous rows that do not overlap."""
+    t2 = t.reshape(-1, t.shape[-1])
+    if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:
+        t2 = t2.contiguous()
+    return t2
+
+
+def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
+                       want_stats: bool):
+    """``layer_norm`` without its gradient: (y, stats) with stats fp32 [2, rows] = mean and 1/std
+    (None unless ``want_stats``)."""
+    _require_cuda(x, "x")
+    if x.dim() < 1 or x.dtype not in _FLOATS:
+        raise ValueError(f"x must be a float32, bfloat16 or float16 tensor [..., cols], got {x.dtype}")
+    cols = x.shape[-1]
+    if cols < 1:
+        raise ValueError("the last dimension is empty: a mean of nothing is not defined")
+    _same_device(x, weight=weight, bias=bias)
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (tuple(t.shape) != (cols,) or t.dtype not in _FLOATS):
+            raise ValueError(f"{name} must be a float tensor [{cols}], got {t.dtype} {list(t.shape)}")
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    x2 = _rows_any(x)
+    rows = x2.shape[0]
+    stats = torch.empty(2, rows, device=x.device, dtype=torch.float32) if want_stats else None
+    if rows == 0:
+        return y, stats
+    w = None if weight is None else weight.detach().float().contiguous()
+    b = None if bias is None else bias.detach().float().contiguous()
+    with _on_device(x):
+        _lib.check(_lib.lib().mortar_layer_norm(_ptr(x2), _CODE[x.dtype], x2.stride(0), rows, cols, _ptr(w), _ptr(b),
+                                                float(eps), _ptr(y), cols, _ptr(stats), _stream_ptr()),
+                   "mortar_layer_norm")
+    _count("layer_norm")
+    return y, stats
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor,
+                        want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
+    """(dx, dweight, dbias) of ``layer_norm`` from the stats its forward kept; dweight and dbias are
+    fp32 [cols]; what is not wanted is None."""
+    _require_cuda(dy, "dy")
+    if dy.shape != x.shape:
+        raise ValueError(f"dy has shape {list(dy.shape)}, x {list(x.shape)}")
+    _same_device(x, dy=dy, weight=weight, stats=stats)
+    cols = x.shape[-1]
+    d2, x2 = _rows_any(dy.to(x.dtype)), _rows_any(x)
+    rows = x2.shape[0]
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
+        raise ValueError(f"stats must be contiguous float32 [2, {rows}]")
+    dev = x.device
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if want_dx else None
+    dw = torch.empty(cols, device=dev, dtype=torch.float32) if want_dweight else None
+    db = torch.empty(cols, device=dev, dtype=torch.float32) if want_dbias else None
+    if not (want_dx or want_dweight or want_dbias) or (rows == 0 and dw is None and db is None):
+        return dx, dw, db
+    w = None if weight is None else weight.detach().float().contiguous()
+    L = _lib.lib()
+    n = L.mortar_layer_norm_scratch_floats(rows, cols) if want_dweight or want_dbias else 0
+    scratch = torch.empty(n, device=dev, dtype=torch.float32) if n else None
+    with _on_device(x):
+        _lib.check(L.mortar_layer_norm_backward(
+            _ptr(d2), d2.stride(0), _ptr(x2), x2.stride(0), _CODE[x.dtype], rows, cols, _ptr(w), _ptr(stats),
+            _ptr(dx), cols, _ptr(dw), _ptr(db), _ptr(scratch), n, _stream_ptr()), "mortar_layer_norm_backward")
+    _count("layer_norm_backward")
+    return dx, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = layer_norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = layer_norm_backward(dy, x, weight, stats, need[0], need[1], need[2])
+        return (dx, None if dw is None else dw.to(weight.dtype), None if db is None else db.to(ctx.bias_dtype), None)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last dimension of x [..., cols] (fp32, bf16 or fp16), differentiable in x,
+    ``weight`` and ``bias`` ([cols], fp32 or the type of x; None = 1 and 0): the norm of the
+    reference's router query (morph/model/routing.py:159-284) as an operator beside
+    ``rmsnorm_rows``.  Statistics and the gradients of weight and bias are summed in fp32, in a fixed
+    order (the same call gives the same bits); y and dx are rounded once, to the type of x.  Like
+    every operator here it can be captured into a CUDA graph.  When a backward pass is captured,
+    no eager autograd graph over the same leaves may be alive (a rule of torch's autograd, whose
+    gradient accumulators remember the stream they were made on)."""
+    if _wants_grad(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return layer_norm_forward(x, weight, bias, eps, False)[0]
+
+
+def dense_error(reset: bool = True) -> int:
+    """Error word of the dense block's kernels (0 = none; synchronises the device)."""
+    code = C.c_int32(0)
+    _lib.check(_lib.lib().mortar_dense_error(C.byref(code), int(reset)), "mortar_dense_error")
+    return code.value
+
+
+def _mlp_dense_args(x, gate_up, down):
+    _require_cuda(x, "x")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"mlp_dense takes bfloat16 or float16 activations, got {x.dtype}")
+    if x.dim() < 1 or gate_up.dim() != 2 or down.dim() != 2:
+        raise ValueError("x [..., d_model], gate_up [2 d_ff, d_model] and down [d_model, d_ff] expected")
+    d_model, d_ff = down.shape
+    if tuple(gate_up.shape) != (2 * d_ff, d_model) or x.shape[-1] != d_model:
+        raise ValueError(f"x {list(x.shape)}, gate_up {list(gate_up.shape)} and down {list(down.shape)} do not fit: "
+                         f"x [..., d_model], gate_up [2 d_ff, d_model] and down [d_model, d_ff] expected")
+    if d_model < 1 or d_ff < 1 or d_model % TILE or d_ff % TILE:
+        raise ValueError(f"d_model and d_ff must be positive multiples of {TILE}, got {d_model} and {d_ff}")
+    for name, t in (("gate_up", gate_up), ("down", down)):
+        if t.dtype != x.dtype:
+            raise ValueError(f"{name} is {t.dtype}, x is {x.dtype}: one type for all")
+    _same_device(x, gate_up=gate_up, down=down)
+    return d_model, d_ff
+
+
+def mlp_dense_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, want_saved: bool):
+    """``mlp_dense`` without its gradient: (y, hidden, sums) with hidden [rows, d_ff] and, when
+    ``want_saved``, sums [rows, 2 d_ff] = x gate_up^T for ``mlp_dense_backward`` (else None)."""
+    d_model, d_ff = _mlp_dense_args(x, gate_up, down)
+    x2 = _rows16(x.reshape(-1, d_model))
+    gu, dn = _rows16(gate_up), _rows16(down)
+    rows, dev = x2.shape[0], x.device
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    hidden = torch.empty(rows, d_ff, device=dev, dtype=x.dtype)
+    sums = torch.empty(rows, 2 * d_ff, device=dev, dtype=x.dtype) if want_saved else None
+    if rows == 0:
+        return y, hidden, sums
+    with _on_device(x):
+        _lib.check(_lib.lib().mortar_mlp_dense(
+            _ptr(x2), x2.stride(0), _CODE[x.dtype], rows, _ptr(gu), gu.stride(0), _ptr(dn), dn.stride(0), d_model,
+            d_ff, _ptr(hidden), _ptr(sums), _ptr(y), d_model, _stream_ptr()), "mortar_mlp_dense")
+    _count("dense", 2)
+    return y, hidden, sums
+
+
+def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor,
+                       hidden: torch.Tensor, sums: torch.Tensor, want_dx: bool = True, want_dgate_up: bool = True,
+                       want_ddown: bool = True):
+    """(dx, dgate_up, ddown) of ``mlp_dense`` from what its forward kept; all in the type of x."""
+    d_model, d_ff = _mlp_dense_args(x, gate_up, down)
+    if dy.shape != x.shape:
+        raise ValueError(f"dy has shape {list(dy.shape)}, x {list(x.shape)}")
+    _same_device(x, dy=dy, hidden=hidden, sums=sums)
+    d2, x2 = _rows16(dy.to(x.dtype).reshape(-1, d_model)), _rows16(x.reshape(-1, d_model))
+    gu, dn = _rows16(gate_up), _rows16(down)
+    rows, dev, dt = x2.shape[0], x.device, x.dtype
+    for name, t, n in (("hidden", hidden, d_ff), ("sums", sums, 2 * d_ff)):
+        if tuple(t.shape) != (rows, n) or t.dtype != dt or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {dt} [{rows}, {n}]")
+    dx = torch.empty(x.shape, device=dev, dtype=dt) if want_dx else None
+    dgu = torch.empty(2 * d_ff, d_model, device=dev, dtype=dt) if want_dgate_up else None
+    ddn = torch.empty(d_model, d_ff, device=dev, dtype=dt) if want_ddown else None
+    if not (want_dx or want_dgate_up or want_ddown):
+        return dx, dgu, ddn
+    dsums = torch.empty_like(sums)
+    with _on_device(x):
+        _lib.check(_lib.lib().mortar_mlp_dense_backward(
+            _ptr(d2), d2.stride(0), _ptr(x2), x2.stride(0), _CODE[dt], rows, _ptr(gu), gu.stride(0), _ptr(dn),
+            dn.stride(0), d_model, d_ff, _ptr(hidden), _ptr(sums), _ptr(dsums), _ptr(dx), _ptr(dgu), _ptr(ddn),
+            _stream_ptr()), "mortar_mlp_dense_backward")
+    _count("dense_backward", (1 if want_dx or want_dgate_up else 0) + 1)
+    return dx, dgu, ddn
+
+
+class _MlpDense(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_up, down):
+        y, hidden, sums = mlp_dense_forward(x, gate_up, down, True)
+        ctx.save_for_backward(x, gate_up, down, hidden, sums)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return mlp_dense_backward(dy, *ctx.saved_tensors, *ctx.needs_input_grad)
+
+
+def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor) -> torch.Tensor:
+    """The gated feed-forward block before it is carved: y = (silu(x Wg^T) * (x Wu^T)) Wd^T for
+    x [..., d_model], ``gate_up`` = [Wg; Wu] [2 d_ff, d_model] and ``down`` [d_model, d_ff], all
+    bfloat16 or all float16; the dense counterpart of ``mlp_prefill_blocks``
+    (morph/model/transformer.py:402-431), differentiable in all three.  d_model and d_ff are
+    multiples of 16.  Sums are fp32; the hidden block and the result are rounded once each, and
+    for the backward pass so are the gate and up sums that it keeps and their gradients.  The note on
+    captured backward passes in ``layer_norm`` holds here too."""
+    if _wants_grad(x, gate_up, down):
+        return _MlpDense.apply(x, gate_up, down)
+    return mlp_dense_forward(x, gate_up, down, False)[0]
+
+
+def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1, dtype: torch.dtype = torch.float8_e4m3fn):
+    """8-bit values and block scales of x [rows, cols] (fp32, bf16 or fp16): (q [rows, cols], scale fp32
+    [ceil(rows / block_rows), ceil(cols / 128)]), one scale per ``block_rows`` x 128 block: 1 for
+    activations, 128 for weights.  The 8-bit floating-point counterpart of ``quantize_rows``.  A
+    scale is the smallest power of two that brings its block into the type's range, so q is the
+    value nearest to x / scale, ties to even, for every input type.  A block of zeros has scale 1;
+    one that holds an infinity or a NaN has scale NaN and reads back as NaN.  cols is a multiple
+    of 16."""
+    _require_cuda(x, "x")
+    if x.dim() != 2 or x.dtype not in _FLOATS:
+        raise ValueError(f"quantize_fp8 takes a 2-D float32, bfloat16 or float16 tensor, got {x.dtype} {list(x.shape)}")
+    if dtype not in _FP8:
+        raise ValueError(f"dtype must be float8_e4m3fn or float8_e5m2, got {dtype}")
+    if block_rows not in (1, 128):
+        raise ValueError(f"block_rows must be 1 or 128, got {block_rows}")
+    rows, cols = x.shape
+    if cols < 1 or cols % TILE:
+        raise ValueError(f"cols must be a positive multiple of {TILE}, got {cols}")
+    x2 = _rows16(x)
+    q = torch.empty(rows, cols, device=x.device, dtype=dtype)
+    scale = torch.empty(-(-rows // block_rows), -(-cols // 128), device=x.device, dtype=torch.float32)
+    if rows == 0:
+        return q, scale
+    with _on_device(x):
+        _lib.check(_lib.lib().mortar_quantize_fp8(_ptr(x2), _CODE[x.dtype], x2.stride(0), rows, cols, block_rows,
+                                                  _ptr(q), _CODE[dtype], cols, _ptr(scale), _stream_ptr()),
+                   "mortar_quantize_fp8")
+    _count("quantize_fp8")
+    return q, scale
+
+
+def dequantize_fp8(q: torch.Tensor, scale: torch.Tensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """q * scale, rounded once to ``out_dtype``, for what ``quantize_fp8`` gives (or another program
+    made, with any scales).  One scale row per row of q, or one per 128 rows."""
+    _require_cuda(q, "q")
+    if q.dim() != 2 or q.dtype not in _FP8:
+        raise ValueError(f"q must be a 2-D float8_e4m3fn or float8_e5m2 tensor, got {q.dtype} {list(q.shape)}")
+    if out_dtype not in _FLOATS:
+        raise ValueError(f"unsupported out_dtype {out_dtype}")
+    rows, cols = q.shape
+    if cols < 1 or cols % TILE:
+        raise ValueError(f"cols must be a positive multiple of {TILE}, got {cols}")
+    nb = -(-cols // 128)
+    if scale.dtype != torch.float32 or tuple(scale.shape) not in ((rows, nb), (-(-rows // 128), nb)):
+        raise ValueError(f"scale must be float32 [{rows}, {nb}] or [{-(-rows // 128)}, {nb}], got {scale.dtype} "
+                         f"{list(scale.shape)}")
+    _same_device(q, scale=scale)
+    block_rows = 1 if scale.shape[0] == rows else 128
+    out = torch.empty(rows, cols, device=q.device, dtype=out_dtype)
+    if rows == 0:
+        return out
+    q2, s2 = _rows16(q), scale.contiguous()
+    with _on_device(q):
+        _lib.check(_lib.lib().mortar_dequantize_fp8(_ptr(q2), _CODE[q.dtype], q2.stride(0), _ptr(s2), rows, cols,
+                                                    block_rows, _ptr(out), _CODE[out_dtype], cols, _stream_ptr()),
+                   "mortar_dequantize_fp8")
+    _count("dequantize_fp8")
+    return out
+
+
+def linear_fp8_error(reset: bool = True) -> int:
+    """Error word of the 8-bit floating-point product (0 = none; synchronises the device)."""
+    code = C.c_int32(0)
+    _lib.check(_lib.lib().mortar_linear_fp8_error(C.byref(code), int(reset)), "mortar_linear_fp8_error")
+    return code.value
+
+
+def linear_fp8(x: torch.Tensor, w: Fp8Matrix, *, x_scale: Optional[torch.Tensor] = None, swiglu: bool = False,
+               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y = x @ W^T for an 8-bit weight with a scale per 128 x 128 block and activations with a scale
+    per 1 x 128 block: [..., out], or [..., out/2] = silu(first half) * second half with ``swiglu``
+    (out a multiple of 256 then).  x is either 8-bit already, with ``x_scale``
+    [..., ceil(in / 128)] as ``quantize_fp8`` gives, or fp32 / bf16 / fp16 and then quantised to e4m3
+    first.  Every block's sum is scaled in fp32 and added in fp32; the result is rounded once to
+    ``out_dtype`` (default: the type of x, bfloat16 for 8-bit x).  The 8-bit floating-point
+    counterpart of ``linear_tc_i8``; for serving, not differentiable (inputs that require a
+    gradient are refused while gradients are enabled)."""
+    _require_cuda(x, "x")
+    if x.dtype not in _FLOATS + _FP8 or x.dim() < 1:
+        raise ValueError(f"x must be a float or float8 tensor [..., in], got {x.dtype}")
+    if (x_scale is None) != (x.dtype in _FLOATS):
+        raise ValueError("x_scale goes with an 8-bit x, and only with one")
+    if x.shape[-1] != w.in_features:
+        raise ValueError(f"x has last dim {x.shape[-1]}, expected {w.in_features}")
+    if _wants_grad(x, x_scale):
+        raise ValueError("linear_fp8 is not differentiable: detach x or call it under torch.no_grad()")
+    if swiglu and w.out_features % 256:
+        raise ValueError(f"swiglu needs out_features to be a multiple of 256, got {w.out_features}")
+    if out_dtype is None:
+        out_dtype = x.dtype if x.dtype in _FLOATS else torch.bfloat16
+    if out_dtype not in _FLOATS:
+        raise ValueError(f"unsupported out_dtype {out_dtype}")
+    _same_device(x, w=w.data, x_scale=x_scale)
+    lead, nb = x.shape[:-1], -(-w.in_features // 128)
+    x2 = x.reshape(-1, w.in_features)
+    rows = x2.shape[0]
+    if x_scale is None:
+        x2, s2 = quantize_fp8(x2)
+    else:
+        if x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (*lead, nb):
+            raise ValueError(f"x_scale must be float32 {[*lead, nb]}, got {x_scale.dtype} {list(x_scale.shape)}")
+        x2, s2 = _rows16(x2), _rows_any(x_scale)
+    n_out = w.out_features // 2 if swiglu else w.out_features
+    out = torch.empty(*lead, n_out, device=x.device, dtype=out_dtype)
+    if rows == 0:
+        return out
+    with _on_device(x):
+        _lib.check(_lib.lib().mortar_linear_fp8(
+            _ptr(x2), _CODE[x2.dtype], x2.stride(0), _ptr(s2), s2.stride(0), rows, _ptr(w.data), _CODE[w.data.dtype],
+            w.data.stride(0), _ptr(w.scale), w.scale.stride(0), w.out_features, w.in_features,
+            _lib.FLAG_SWIGLU if swiglu else 0, _ptr(out), _CODE[out_dtype], n_out, _stream_ptr()),
+            "mortar_linear_fp8")
+    _count("linear_fp8")
+    return out
+
+
+def mlp_fp8(x: torch.Tensor, gate_up: Fp8Matrix, down: Fp8Matrix, *,
+            out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The gated feed-forward block in 8-bit floating point, the form ``mlp_prefill_tc_i8`` has in
+    int8: quantise x, gate/up product with the gate applied (hidden block bfloat16, or the type of a
+    16-bit x), quantise the hidden block, down product.  Four launches; for serving."""
+    if gate_up.out_features != 2 * down.in_features or gate_up.in_features != down.out_features:
+        raise ValueError("gate_up must be [2 d_ff, d_model] and down [d_model, d_ff]")
+    if x.dtype not in _FLOATS:
+        raise ValueError(f"mlp_fp8 takes float32, bfloat16 or float16 activations, got {x.dtype}")
+    h = linear_fp8(x, gate_up, swiglu=True, out_dtype=torch.float16 if x.dtype == torch.float16 else torch.bfloat16)
+    return linear_fp8(h, down, out_dtype=x.dtype if out_dtype is None else out_dtype)
 
 
 # ---- reference-signature shims ---------------------------------------------------------
