@@ -1044,8 +1044,10 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if want_dx else None
     dw = torch.empty(cols, device=dev, dtype=torch.float32) if want_dweight else None
     db = torch.empty(cols, device=dev, dtype=torch.float32) if want_dbias else None
-    if not (want_dx or want_dweight or want_dbias) or (rows == 0 and dw is None and db is None):
+    if not (want_dx or want_dweight or want_dbias):
         return dx, dw, db
+    if rows == 0:
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
     w = None if weight is None else weight.detach().float().contiguous()
     L = _lib.lib()
     n = L.mortar_layer_norm_scratch_floats(rows, cols) if want_dweight or want_dbias else 0
@@ -1155,6 +1157,8 @@ def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor,
     ddn = torch.empty(d_model, d_ff, device=dev, dtype=dt) if want_ddown else None
     if not (want_dx or want_dgate_up or want_ddown):
         return dx, dgu, ddn
+    if rows == 0:
+        return dx, None if dgu is None else dgu.zero_(), None if ddn is None else ddn.zero_()
     dsums = torch.empty_like(sums)
     with _on_device(x):
         _lib.check(_lib.lib().mortar_mlp_dense_backward(

@@ -14,6 +14,10 @@ shape and dtype.  There is no CPU implementation: calling an op with CPU tensors
     mortar_b200::linear_tc(x, <sched>, gates?, cluster_size) -> y            (tcgen05 kernel)
     mortar_b200::mlp_prefill_tc(x, <gate_up sched>, <down sched>, gates?, n_clusters) -> y
     mortar_b200::stack_decode(x!, blobs, table, app_layer, status!, ...) -> ()   (in place)
+    mortar_b200::layer_norm(x, weight?, bias?, eps) -> (y, stats)            (differentiable in y)
+    mortar_b200::mlp_dense(x, gate_up, down) -> (y, hidden, sums)            (differentiable in y)
+    mortar_b200::quantize_fp8(x, block_rows, e5m2) -> (q, scale);  dequantize_fp8(q, scale, out_dtype) -> x
+    mortar_b200::linear_fp8(x, x_scale?, w, w_scale, swiglu, out_dtype) -> y
     <stream> = grp_ptr, grp_cols, grp_codes, scale, out_features, in_features, n_groups
     <sched>  = step_data, step_off, step_meta, panel_step_ptr, panel_mask, n_tiles, n_runs, n_steps,
                data_units, n_panels, out_features, in_features, swiglu, scale
@@ -31,13 +35,13 @@ reference op (block_sparse.py:909-919, 951-956).
 from __future__ import annotations
 
 from collections import OrderedDict
-from typing import Optional
+from typing import Optional, Tuple
 
 import numpy as np
 import torch
 
 from . import ops
-from .format import (BlockSched, MortarMatrix, SchedMatrix, StreamMatrix, TopologyDev, matrix_from_stream, pack_codes_2bit,
+from .format import (BlockSched, Fp8Matrix, MortarMatrix, SchedMatrix, StreamMatrix, TopologyDev, matrix_from_stream, pack_codes_2bit,
                      wants_block_path)
 
 _LIB = "mortar_b200"
@@ -242,6 +246,121 @@ def stack_decode(x: torch.Tensor, blobs: torch.Tensor, blob_table: torch.Tensor,
 def _(x, blobs, blob_table, app_layer, rms_weights, status, n_layers, d_model, d_ff, max_gate_up_bytes,
       max_down_bytes, cluster_size, eps, n_planes):
     return None
+
+
+# ---- the dense MLP site -----------------------------------------------------------------
+
+@torch.library.custom_op(f"{_LIB}::layer_norm", mutates_args=(), device_types="cuda")
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+               eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``ops.layer_norm`` and the statistics that its gradient needs (fp32 [2, rows]); differentiable
+    in the first result."""
+    return ops.layer_norm_forward(x, weight, bias, eps, True)
+
+
+@layer_norm.register_fake
+def _(x, weight, bias, eps):
+    return x.new_empty(x.shape), x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_LIB}::layer_norm_backward", mutates_args=(), device_types="cuda")
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor],
+                        stats: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return ops.layer_norm_backward(dy, x, weight, stats)
+
+
+@layer_norm_backward.register_fake
+def _(dy, x, weight, stats):
+    col = x.new_empty((x.shape[-1],), dtype=torch.float32)
+    return x.new_empty(x.shape), col, torch.empty_like(col)
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    x, weight, bias, _ = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.mark_non_differentiable(output[1])
+    ctx.bias_dtype = None if bias is None else bias.dtype
+
+
+def _layer_norm_grad(ctx, dy, _dstats):
+    x, weight, stats = ctx.saved_tensors
+    dx, dw, db = torch.ops.mortar_b200.layer_norm_backward(dy, x, weight, stats)
+    return (dx, None if weight is None else dw.to(weight.dtype),
+            None if ctx.bias_dtype is None else db.to(ctx.bias_dtype), None)
+
+
+layer_norm.register_autograd(_layer_norm_grad, setup_context=_layer_norm_setup)
+
+
+@torch.library.custom_op(f"{_LIB}::mlp_dense", mutates_args=(), device_types="cuda")
+def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor,
+              down: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``ops.mlp_dense`` and what its gradient needs (hidden block, gate and up sums); differentiable
+    in the first result."""
+    return ops.mlp_dense_forward(x, gate_up, down, True)
+
+
+@mlp_dense.register_fake
+def _(x, gate_up, down):
+    rows, d_ff = x.numel() // x.shape[-1], down.shape[1]
+    return x.new_empty(x.shape), x.new_empty((rows, d_ff)), x.new_empty((rows, 2 * d_ff))
+
+
+@torch.library.custom_op(f"{_LIB}::mlp_dense_backward", mutates_args=(), device_types="cuda")
+def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor,
+                       hidden: torch.Tensor,
+                       sums: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return ops.mlp_dense_backward(dy, x, gate_up, down, hidden, sums)
+
+
+@mlp_dense_backward.register_fake
+def _(dy, x, gate_up, down, hidden, sums):
+    return x.new_empty(x.shape), x.new_empty(gate_up.shape), x.new_empty(down.shape)
+
+
+def _mlp_dense_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs, output[1], output[2])
+    ctx.mark_non_differentiable(output[1], output[2])
+
+
+def _mlp_dense_grad(ctx, dy, _dhidden, _dsums):
+    return torch.ops.mortar_b200.mlp_dense_backward(dy, *ctx.saved_tensors)
+
+
+mlp_dense.register_autograd(_mlp_dense_grad, setup_context=_mlp_dense_setup)
+
+
+@torch.library.custom_op(f"{_LIB}::quantize_fp8", mutates_args=(), device_types="cuda")
+def quantize_fp8(x: torch.Tensor, block_rows: int, e5m2: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    return ops.quantize_fp8(x, block_rows=block_rows, dtype=torch.float8_e5m2 if e5m2 else torch.float8_e4m3fn)
+
+
+@quantize_fp8.register_fake
+def _(x, block_rows, e5m2):
+    rows, cols = x.shape
+    return (x.new_empty((rows, cols), dtype=torch.float8_e5m2 if e5m2 else torch.float8_e4m3fn),
+            x.new_empty((-(-rows // block_rows), -(-cols // 128)), dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_LIB}::dequantize_fp8", mutates_args=(), device_types="cuda")
+def dequantize_fp8(q: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
+    return ops.dequantize_fp8(q, scale, out_dtype=out_dtype)
+
+
+@dequantize_fp8.register_fake
+def _(q, scale, out_dtype):
+    return q.new_empty(q.shape, dtype=out_dtype)
+
+
+@torch.library.custom_op(f"{_LIB}::linear_fp8", mutates_args=(), device_types="cuda")
+def linear_fp8(x: torch.Tensor, x_scale: Optional[torch.Tensor], w: torch.Tensor, w_scale: torch.Tensor,
+               swiglu: bool, out_dtype: torch.dtype) -> torch.Tensor:
+    return ops.linear_fp8(x, Fp8Matrix(w, w_scale), x_scale=x_scale, swiglu=swiglu, out_dtype=out_dtype)
+
+
+@linear_fp8.register_fake
+def _(x, x_scale, w, w_scale, swiglu, out_dtype):
+    return x.new_empty((*x.shape[:-1], w.shape[0] // 2 if swiglu else w.shape[0]), dtype=out_dtype)
 
 
 # ---------------------------------------------------------------------------------------

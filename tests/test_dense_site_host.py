@@ -1,0 +1,205 @@
+"""The dense MLP site without a GPU: what the entry points refuse, the shapes and types the
+registered operators promise, and that CPU tensors are turned away."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import mortar_b200 as mb
+
+L = mb._lib.lib()
+NULL, SHAPE, ALIGN, DTYPE, CAP = -1, -2, -6, -7, -8
+F32, BF16, F16, E4M3, E5M2 = 0, 1, 2, 3, 4
+
+
+def _buf(nbytes=4096):
+    a = np.zeros(nbytes + 256, dtype=np.uint8)
+    return a, C.c_void_p((a.ctypes.data + 255) & ~255)
+
+
+def _off(p, n):
+    return C.c_void_p(p.value + n)
+
+
+def test_layer_norm_entry_points_validate():
+    keep, p = _buf()
+    f = L.mortar_layer_norm
+    assert f(None, F32, 64, 4, 64, p, p, 1e-5, p, 64, p, None) == NULL
+    assert f(p, F32, 64, 4, 64, p, p, 1e-5, None, 64, p, None) == NULL
+    assert f(p, F32, 63, 4, 64, p, p, 1e-5, p, 64, p, None) == SHAPE
+    assert f(p, F32, 64, 4, 64, p, p, 1e-5, p, 63, p, None) == SHAPE
+    assert f(p, F32, 64, -1, 64, p, p, 1e-5, p, 64, p, None) == SHAPE
+    assert f(p, F32, 64, 4, 0, p, p, 1e-5, p, 64, p, None) == SHAPE
+    assert f(p, E4M3, 64, 4, 64, p, p, 1e-5, p, 64, p, None) == DTYPE
+    assert f(_off(p, 2), F32, 64, 4, 64, p, p, 1e-5, p, 64, p, None) == ALIGN
+    assert f(p, F32, (1 << 20) + 1, 4, (1 << 20) + 1, p, p, 1e-5, p, (1 << 20) + 1, p, None) == CAP
+    assert f(p, F32, 64, 0, 64, p, p, 1e-5, p, 64, p, None) == 0
+    b = L.mortar_layer_norm_backward
+    assert b(None, 64, p, 64, F32, 4, 64, p, p, p, 64, p, p, p, 1 << 20, None) == NULL
+    assert b(p, 64, p, 64, F32, 4, 64, p, None, p, 64, p, p, p, 1 << 20, None) == NULL
+    assert b(p, 64, p, 64, F32, 4, 64, p, p, p, 60, p, p, p, 1 << 20, None) == SHAPE
+    assert b(p, 64, p, 64, 9, 4, 64, p, p, p, 64, p, p, p, 1 << 20, None) == DTYPE
+    assert b(p, 64, p, 64, F32, 4, 64, p, p, p, 64, p, p, None, 0, None) == CAP
+    assert b(p, 64, p, 64, F32, 4, 64, p, p, p, 64, p, p, p, 1, None) == CAP
+    assert L.mortar_layer_norm_scratch_floats(4, 0) == SHAPE
+    assert L.mortar_layer_norm_scratch_floats(0, 64) >= 0
+
+
+def test_mlp_dense_entry_points_validate():
+    keep, p = _buf()
+    f = L.mortar_mlp_dense
+    ok = [p, 64, BF16, 4, p, 64, p, 128, 64, 128, p, p, p, 64, None]
+
+    def call(fn, base, **at):
+        args = list(base)
+        for i, v in at.items():
+            args[int(i[1:])] = v
+        return fn(*args)
+
+    for i in (0, 4, 6, 10, 12):
+        assert call(f, ok, **{f"a{i}": None}) == NULL
+    assert call(f, ok, a3=-1) == SHAPE
+    assert call(f, ok, a8=60) == SHAPE and call(f, ok, a9=120) == SHAPE
+    assert call(f, ok, a1=32) == SHAPE and call(f, ok, a5=32) == SHAPE and call(f, ok, a7=64) == SHAPE
+    assert call(f, ok, a13=32) == SHAPE
+    assert call(f, ok, a2=F32) == DTYPE
+    assert call(f, ok, a0=_off(p, 2)) == ALIGN and call(f, ok, a1=68) == ALIGN
+    assert call(f, ok, a3=1 << 31) == CAP
+    assert call(f, ok, a3=0) == 0
+    b = L.mortar_mlp_dense_backward
+    okb = [p, 64, p, 64, BF16, 4, p, 64, p, 128, 64, 128, p, p, p, p, p, p, None]
+    for i in (0, 2, 6, 8, 12, 13, 14):
+        assert call(b, okb, **{f"a{i}": None}) == NULL
+    assert call(b, okb, a10=60) == SHAPE and call(b, okb, a1=32) == SHAPE
+    assert call(b, okb, a4=F32) == DTYPE
+    assert call(b, okb, a15=_off(p, 8)) == ALIGN
+
+
+def test_fp8_entry_points_validate():
+    keep, p = _buf()
+    f = L.mortar_quantize_fp8
+    assert f(None, BF16, 256, 8, 256, 1, p, E4M3, 256, p, None) == NULL
+    assert f(p, BF16, 256, 8, 250, 1, p, E4M3, 256, p, None) == SHAPE
+    assert f(p, BF16, 256, 8, 256, 64, p, E4M3, 256, p, None) == SHAPE
+    assert f(p, BF16, 128, 8, 256, 1, p, E4M3, 256, p, None) == SHAPE
+    assert f(p, E4M3, 256, 8, 256, 1, p, E4M3, 256, p, None) == DTYPE
+    assert f(p, BF16, 256, 8, 256, 1, p, BF16, 256, p, None) == DTYPE
+    assert f(_off(p, 2), BF16, 256, 8, 256, 1, p, E4M3, 256, p, None) == ALIGN
+    assert f(p, BF16, 256, 8, 256, 1, p, E4M3, 264, p, None) == ALIGN
+    assert f(p, BF16, 256, 0, 256, 1, p, E4M3, 256, p, None) == 0
+    d = L.mortar_dequantize_fp8
+    assert d(None, E4M3, 256, p, 8, 256, 1, p, BF16, 256, None) == NULL
+    assert d(p, E4M3, 256, p, 8, 256, 2, p, BF16, 256, None) == SHAPE
+    assert d(p, F32, 256, p, 8, 256, 1, p, BF16, 256, None) == DTYPE
+    g = L.mortar_linear_fp8
+    assert g(None, E4M3, 256, p, 2, 8, p, E4M3, 256, p, 2, 256, 256, 0, p, BF16, 256, None) == NULL
+    assert g(p, E4M3, 256, None, 2, 8, p, E4M3, 256, p, 2, 256, 256, 0, p, BF16, 256, None) == NULL
+    assert g(p, E4M3, 256, p, 1, 8, p, E4M3, 256, p, 2, 256, 256, 0, p, BF16, 256, None) == SHAPE    # scales of 1 block
+    assert g(p, E4M3, 256, p, 2, 8, p, E4M3, 256, p, 2, 384, 256, mb._lib.FLAG_SWIGLU, p, BF16, 256, None) == SHAPE
+    assert g(p, E4M3, 256, p, 2, 8, p, E4M3, 256, p, 2, 256, 250, 0, p, BF16, 256, None) == SHAPE
+    assert g(p, E4M3, 256, p, 2, 8, p, E4M3, 256, p, 2, 256, 256, 0, p, BF16, 128, None) == SHAPE
+    assert g(p, BF16, 256, p, 2, 8, p, E4M3, 256, p, 2, 256, 256, 0, p, BF16, 256, None) == DTYPE
+    assert g(p, E4M3, 256, p, 2, 8, p, E4M3, 256, p, 2, 256, 256, 4, p, BF16, 256, None) == DTYPE     # unknown flag
+    assert g(p, E4M3, 256, p, 2, 8, p, E4M3, 256, p, 2, 256, 256, 0, p, E4M3, 256, None) == DTYPE
+    assert g(_off(p, 8), E4M3, 256, p, 2, 8, p, E4M3, 256, p, 2, 256, 256, 0, p, BF16, 256, None) == ALIGN
+    assert g(p, E4M3, 264, p, 2, 8, p, E4M3, 256, p, 2, 256, 256, 0, p, BF16, 256, None) == ALIGN
+    assert g(p, E4M3, 256, p, 2, 0, p, E4M3, 256, p, 2, 256, 256, 0, p, BF16, 256, None) == 0
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    with pytest.raises(NotImplementedError, match="CUDA-only"):
+        mb.ops.layer_norm(x)
+    with pytest.raises(NotImplementedError, match="CUDA-only"):
+        mb.ops.mlp_dense(x, torch.zeros(64, 64, dtype=x.dtype), torch.zeros(64, 32, dtype=x.dtype))
+    with pytest.raises(NotImplementedError, match="CUDA-only"):
+        mb.ops.quantize_fp8(x)
+    q = torch.zeros(4, 64, dtype=torch.float8_e4m3fn)
+    with pytest.raises(NotImplementedError, match="CUDA-only"):
+        mb.ops.dequantize_fp8(q, torch.ones(4, 1))
+    with pytest.raises(NotImplementedError, match="CUDA-only"):
+        mb.ops.linear_fp8(q, mb.Fp8Matrix(q, torch.ones(1, 1)), x_scale=torch.ones(4, 1))
+
+
+def test_wrong_arguments_are_refused():
+    """On fake CUDA tensors: every refusal comes before a pointer is taken."""
+    with FakeTensorMode():
+        def z(*shape, dt=torch.bfloat16, dev="cuda"):
+            return torch.empty(*shape, device=dev, dtype=dt)
+        bad = [
+            lambda: mb.ops.layer_norm(z(4, 64, dt=torch.int32)),
+            lambda: mb.ops.layer_norm(z(4, 0)),
+            lambda: mb.ops.layer_norm(z(4, 64), weight=z(63)),
+            lambda: mb.ops.layer_norm(z(4, 64), bias=z(64, dt=torch.int64)),
+            lambda: mb.ops.layer_norm(z(4, 64), weight=z(64, dev="cpu")),
+            lambda: mb.ops.layer_norm_backward(z(4, 32), z(4, 64), None, z(2, 4, dt=torch.float32)),
+            lambda: mb.ops.layer_norm_backward(z(4, 64), z(4, 64), None, z(2, 5, dt=torch.float32)),
+            lambda: mb.ops.mlp_dense(z(4, 64, dt=torch.float32), z(64, 64), z(64, 32)),
+            lambda: mb.ops.mlp_dense(z(4, 64), z(64, 64), z(64, 48)),
+            lambda: mb.ops.mlp_dense(z(4, 48), z(64, 64), z(64, 32)),
+            lambda: mb.ops.mlp_dense(z(4, 40), z(64, 40), z(40, 32)),
+            lambda: mb.ops.mlp_dense(z(4, 64), z(64, 64, dt=torch.float16), z(64, 32)),
+            lambda: mb.ops.mlp_dense(z(4, 64), z(64, 64, dev="cpu"), z(64, 32)),
+            lambda: mb.ops.quantize_fp8(z(4, 64, 2)),
+            lambda: mb.ops.quantize_fp8(z(4, 60)),
+            lambda: mb.ops.quantize_fp8(z(4, 64), block_rows=32),
+            lambda: mb.ops.quantize_fp8(z(4, 64), dtype=torch.float16),
+            lambda: mb.ops.quantize_fp8(z(4, 64, dt=torch.int8)),
+            lambda: mb.ops.dequantize_fp8(z(4, 64), z(4, 1, dt=torch.float32)),
+            lambda: mb.ops.dequantize_fp8(z(4, 64, dt=torch.float8_e4m3fn), z(3, 1, dt=torch.float32)),
+            lambda: mb.ops.dequantize_fp8(z(4, 64, dt=torch.float8_e4m3fn), z(4, 1)),
+            lambda: mb.Fp8Matrix(z(64, 64), z(1, 1, dt=torch.float32)),
+            lambda: mb.Fp8Matrix(z(64, 60, dt=torch.float8_e4m3fn), z(1, 1, dt=torch.float32)),
+            lambda: mb.Fp8Matrix(z(64, 64, dt=torch.float8_e4m3fn), z(2, 1, dt=torch.float32)),
+            lambda: mb.Fp8Matrix(z(64, 64, dt=torch.float8_e4m3fn), z(1, 1, dt=torch.float32, dev="cpu")),
+        ]
+        for i, f in enumerate(bad):
+            with pytest.raises(ValueError):
+                f()
+                pytest.fail(f"call {i} was not refused")
+        w = mb.Fp8Matrix.__new__(mb.Fp8Matrix)                       # fake tensors have no address to check
+        w.data, w.scale = z(384, 64, dt=torch.float8_e4m3fn), z(3, 1, dt=torch.float32)
+        w.out_features, w.in_features = 384, 64
+        q = z(4, 64, dt=torch.float8_e4m3fn)
+        xs = z(4, 1, dt=torch.float32)
+        for f in (lambda: mb.ops.linear_fp8(q, w),                                         # no scale
+                  lambda: mb.ops.linear_fp8(z(4, 64), w, x_scale=xs),                       # a scale too many
+                  lambda: mb.ops.linear_fp8(z(4, 128), w),
+                  lambda: mb.ops.linear_fp8(q, w, x_scale=xs, swiglu=True),                 # 384 is no multiple of 256
+                  lambda: mb.ops.linear_fp8(q, w, x_scale=z(4, 2, dt=torch.float32)),
+                  lambda: mb.ops.linear_fp8(q, w, x_scale=xs, out_dtype=torch.int32),
+                  lambda: mb.ops.linear_fp8(z(4, 64).requires_grad_(), w)):
+            with pytest.raises(ValueError):
+                f()
+
+
+def test_registered_operators_trace():
+    ns = torch.ops.mortar_b200
+    with FakeTensorMode():
+        x = torch.empty(6, 5, 64, device="cuda", dtype=torch.bfloat16)
+        y, stats = ns.layer_norm(x, None, None, 1e-5)
+        assert y.shape == x.shape and stats.shape == (2, 30) and stats.dtype == torch.float32
+        y, hidden, sums = ns.mlp_dense(x, x.new_empty(64, 64), x.new_empty(64, 32))
+        assert y.shape == x.shape and hidden.shape == (30, 32) and sums.shape == (30, 64)
+        q, s = ns.quantize_fp8(x.reshape(30, 64), 128, True)
+        assert q.dtype == torch.float8_e5m2 and s.shape == (1, 1)
+        assert ns.dequantize_fp8(q, s, torch.float16).dtype == torch.float16
+        y = ns.linear_fp8(q, s.new_empty(30, 1), q.new_empty(256, 64), s.new_empty(2, 1), True, torch.float32)
+        assert y.shape == (30, 128) and y.dtype == torch.float32
+
+
+def test_modules_hold_their_parameters():
+    m = mb.SwiGLUDense(64, 128, norm=True)
+    assert {k: tuple(v.shape) for k, v in m.state_dict().items()} == {
+        "gate_up.weight": (256, 64), "down.weight": (64, 128), "norm.weight": (64,), "norm.bias": (64,)}
+    with pytest.raises(ValueError):
+        mb.SwiGLUDense(60, 128)
+    q = lambda o, i: mb.Fp8Matrix(torch.zeros(o, i, dtype=torch.float8_e4m3fn), torch.ones(-(-o // 128), -(-i // 128)))
+    s = mb.SwiGLUFp8(q(256, 64), q(64, 128))
+    assert set(s.state_dict()) == {"gate_up_data", "gate_up_scale", "down_data", "down_scale"}
+    with pytest.raises(ValueError):
+        mb.SwiGLUFp8(q(192, 64), q(64, 96))                          # 96 hidden columns: no multiple of 128
+    with pytest.raises(ValueError):
+        mb.SwiGLUFp8(q(256, 64), q(128, 128))

@@ -1,0 +1,602 @@
+"""The dense MLP site on the GPU against plain 64-bit implementations.
+
+Tolerances are bounds, derived from the roundings the kernels make.  u = eps / 2 of the result's type is
+the error of one rounding relative to the value; f = 2^-24 is that of one fp32 operation, and a sum of n
+fp32 terms taken in parts of at most p terms and then over the parts is off by at most
+(p + n / p + 1) f times the sum of the terms' magnitudes."""
+import pytest
+import torch
+
+import mortar_b200 as mb
+
+pytestmark = pytest.mark.gpu
+ops = mb.ops
+F = 2.0 ** -24
+DEV = "cuda"
+FLOATS = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def half_step(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def rand(*shape, seed=0, scale=1.0, dt=torch.float32):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, generator=gen, device=DEV) * scale).to(dt)
+
+
+def within(got, ref, bound, what=""):
+    got, ref = got.double(), ref.double()
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    over = (got - ref).abs() - bound
+    assert not torch.isnan(got).any() and bool((over <= 0).all()), \
+        f"{what}: off by {float((got - ref).abs().max()):.3e}, {float(over.max()):.3e} over its bound"
+
+
+def errors_are_clear():
+    assert ops.dense_error() == 0 and ops.linear_fp8_error() == 0
+
+
+# ---- layer norm -------------------------------------------------------------------------------
+
+def ln_ref(x, w, b, eps, dy=None):
+    x = x.double()
+    w = torch.ones(x.shape[-1], device=DEV, dtype=torch.float64) if w is None else w.double()
+    b = torch.zeros_like(w) if b is None else b.double()
+    mean = x.mean(-1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(-1, keepdim=True) + eps)
+    xh = (x - mean) * rstd
+    y = xh * w + b
+    if dy is None:
+        return y, xh, rstd, mean
+    dy = dy.double()
+    g = dy * w
+    dx = rstd * (g - g.mean(-1, keepdim=True) - xh * (g * xh).mean(-1, keepdim=True))
+    return y, xh, rstd, mean, dx, dy * xh, dy
+
+
+def ln_bounds(x, w, b, y, xh, rstd, dx, dy, dt):
+    """Bounds on y and dx.  With c = log-depth and per-thread terms of a row's sums (<= cols / 16 + 32
+    additions whatever the split), the mean is off by c f mean|x|, so xh by rstd times that, plus a few f of
+    |xh|, plus what rstd is off relatively ((c + 8) f of the variance, half of it)."""
+    cols = x.shape[-1]
+    c = cols / 16 + 32
+    x, wa = x.double(), (torch.ones(cols, device=DEV, dtype=torch.float64) if w is None else w.double().abs())
+    dxh = F * (c * rstd * x.abs().mean(-1, keepdim=True) + (c + 16) * xh.abs() + 4 * rstd * x.abs())
+    u = half_step(dt) * 1.01
+    by = u * y.abs() + dxh * wa + 4 * F * ((xh * wa).abs() + y.abs())
+    if dt == torch.float16:
+        by = by + 2.0 ** -25                                   # half the smallest subnormal step
+    if dy is None:
+        return by, None
+    g = (dy.double() * wa).abs()
+    m1, m2 = g.mean(-1, keepdim=True), (g * xh.abs()).mean(-1, keepdim=True)
+    bdx = u * dx.abs() + rstd * (F * (c + 16) * (g + m1 + xh.abs() * m2) + dxh * m2 +
+                                 xh.abs() * (g * dxh).mean(-1, keepdim=True)) * 1.01
+    if dt == torch.float16:
+        bdx = bdx + 2.0 ** -25
+    return by, bdx
+
+
+LN_SHAPES = [(1, 1), (1, 768), (3, 5), (7, 64), (130, 768), (257, 1000), (33, 2047), (64, 2048), (5, 4096), (9, 8191),
+             (3, 20011), (700, 16), (2049, 33)]
+
+
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("rows,cols", LN_SHAPES)
+def test_layer_norm_and_its_gradients(rows, cols, dt):
+    x = (rand(rows, cols, seed=1, scale=2.0) + 0.5).to(dt).requires_grad_()
+    w = (1 + rand(cols, seed=2, scale=0.2)).requires_grad_()
+    b = rand(cols, seed=3, scale=0.2).requires_grad_()
+    dy = rand(rows, cols, seed=4, dt=dt)
+    y = ops.layer_norm(x, w, b, 1e-5)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    ry, xh, rstd, _, rdx, tw, tb = ln_ref(x.detach(), w.detach(), b.detach(), 1e-5, dy)
+    by, bdx = ln_bounds(x.detach(), w.detach(), b.detach(), ry, xh, rstd, rdx, dy, dt)
+    assert y.dtype == dt and dx.dtype == dt and dw.dtype == torch.float32
+    within(y.detach(), ry, by, "y")
+    within(dx, rdx, bdx, "dx")
+    # sums over the rows: terms off by (cols / 16 + 48) f like xh, added in parts
+    n = rows / 8 + 320
+    xerr = F * ((cols / 16 + 48) * (xh.abs() + rstd * x.detach().double().abs().mean(-1, keepdim=True)))
+    within(dw, tw.sum(0), F * n * tw.abs().sum(0) + (dy.double().abs() * xerr).sum(0) + 1e-30, "dw")
+    within(db, tb.sum(0), F * n * tb.abs().sum(0) + 1e-30, "db")
+    with torch.no_grad():
+        assert torch.equal(ops.layer_norm(x, w, b, 1e-5), y)
+    again = torch.autograd.grad(ops.layer_norm(x, w, b, 1e-5), (x, w, b), dy)
+    assert all(torch.equal(p, q) for p, q in zip(again, (dx, dw, db)))
+
+
+def test_layer_norm_gradient_against_differences():
+    """<dx, v> from the kernel against (loss(x + h v) - loss(x - h v)) / 2h of the 64-bit formula, whose own
+    error at h = 1e-4 is below 1e-6 of the terms."""
+    x, w, b = rand(11, 96, seed=5).requires_grad_(), (1 + rand(96, seed=6, scale=0.3)).requires_grad_(), rand(96, seed=7).requires_grad_()
+    dy = rand(11, 96, seed=8)
+    grads = torch.autograd.grad(ops.layer_norm(x, w, b), (x, w, b), dy)
+    loss = lambda *a: float((ln_ref(*a, 1e-5)[0] * dy.double()).sum())
+    args = [t.detach().double() for t in (x, w, b)]
+    for i, gr in enumerate(grads):
+        v = rand(*args[i].shape, seed=20 + i).double()
+        hi, lo = list(args), list(args)
+        hi[i], lo[i] = args[i] + 1e-4 * v, args[i] - 1e-4 * v
+        num = (loss(*hi) - loss(*lo)) / 2e-4
+        assert abs(float((gr.double() * v).sum()) - num) <= 1e-5 * float((gr.double() * v).abs().sum())
+
+
+@pytest.mark.parametrize("dt", FLOATS)
+def test_layer_norm_strided_offset_and_typed_inputs(dt):
+    """Rows of a wider tensor, starting off 16 bytes; weight of the rows' type; no weight, no bias; a
+    gradient that is broadcast (stride 0)."""
+    base = rand(40, 300, seed=9, dt=dt)
+    for off in (0, 1, 3, 8):
+        x = base[:, off:off + 200]
+        ry, xh, rstd, _ = ln_ref(x, None, None, 1e-5)
+        by, _ = ln_bounds(x, None, None, ry, xh, rstd, None, None, dt)
+        within(ops.layer_norm(x), ry, by, f"offset {off}")
+    x = rand(2, 3, 64, seed=10, dt=dt).transpose(0, 1)
+    ry, xh, rstd, _ = ln_ref(x, None, None, 1e-5)
+    within(ops.layer_norm(x), ry, ln_bounds(x, None, None, ry, xh, rstd, None, None, dt)[0], "transposed")
+    x = rand(6, 64, seed=11, dt=dt).requires_grad_()
+    w = rand(64, seed=12, dt=dt).requires_grad_()
+    dx, dw = torch.autograd.grad(ops.layer_norm(x, w).sum(), (x, w))
+    assert dw.dtype == dt
+    dy = torch.ones(6, 64, device=DEV, dtype=dt)
+    ry, xh, rstd, _, rdx, tw, _ = ln_ref(x.detach(), w.detach(), None, 1e-5, dy)
+    within(dx, rdx, ln_bounds(x.detach(), w.detach(), None, ry, xh, rstd, rdx, dy, dt)[1], "dx")
+    assert ops.layer_norm(rand(0, 64, dt=dt)).shape == (0, 64)
+
+
+def test_layer_norm_edges():
+    # no rows: gradients of weight and bias are zeros
+    x = rand(0, 64).requires_grad_()
+    w, b = rand(64).requires_grad_(), rand(64).requires_grad_()
+    dx, dw, db = torch.autograd.grad(ops.layer_norm(x, w, b).sum(), (x, w, b))
+    assert dx.shape == (0, 64) and not dw.any() and not db.any()
+    # a constant row has variance 0: y = bias; a far offset keeps the variance (two passes over the row)
+    y = ops.layer_norm(torch.full((2, 48), 7.0, device=DEV), None, w.detach()[:48].contiguous())
+    within(y, w.detach()[:48].expand(2, 48), 1e-6, "constant row")
+    x = rand(4, 512, seed=13) + 4096.0
+    ry, xh, rstd, _ = ln_ref(x, None, None, 1e-5)
+    within(ops.layer_norm(x), ry, ln_bounds(x, None, None, ry, xh, rstd, None, None, torch.float32)[0], "offset row")
+    # a NaN or an infinity stays in its row
+    x = rand(3, 64, seed=14)
+    clean = ops.layer_norm(x)
+    x[1, 5] = float("inf")
+    y = ops.layer_norm(x)
+    assert torch.isnan(y[1]).any() and torch.equal(y[0], clean[0]) and torch.equal(y[2], clean[2])
+
+
+# ---- the dense block ------------------------------------------------------------------------
+
+def mlp_ref(x, gu, dn):
+    x, gu, dn = x.double(), gu.double(), dn.double()
+    f = dn.shape[1]
+    s = x @ gu.t()
+    g, u = s[:, :f], s[:, f:]
+    sig = torch.sigmoid(g)
+    return g, u, sig, g * sig * u, (g * sig * u) @ dn.t()
+
+
+def mlp_grads_ref(dy, x, gu, dn):
+    g, u, sig, h, y = mlp_ref(x, gu, dn)
+    dy, x, gu, dn = dy.double(), x.double(), gu.double(), dn.double()
+    dh = dy @ dn
+    dg, du = dh * u * (sig + g * sig * (1 - sig)), dh * g * sig
+    ds = torch.cat([dg, du], 1)
+    return y, ds @ gu, ds.t() @ x, dy.t() @ h, (g, u, sig, h, dh, dg, du)
+
+
+def mlp_bounds(dy, x, gu, dn, parts, dt):
+    """Elementwise bounds.  The tensor cores add n products in fp32: at most n f of the magnitudes' sum.
+    g and u are off by e_g, e_u from that (kept sums: one rounding more); h = g sig(g) u moves by at most
+    1.1 |u| e_g + |silu(g)| e_u (|silu'| <= 1.1) plus a rounding; dg by |dh| (|silu''| <= 0.5) etc."""
+    g, u, sig, h, dh, dg, du = parts
+    xa, gua, dna, dya = x.double().abs(), gu.double().abs(), dn.double().abs(), dy.double().abs()
+    d, f, m = x.shape[1], dn.shape[1], x.shape[0]
+    us = half_step(dt) * 1.01
+    tiny = 2.0 ** -25 if dt == torch.float16 else 0.0
+    es = F * (d + 2) * (xa @ gua.t())
+    eg, eu = es[:, :f], es[:, f:]
+    a, da = (g * sig).abs(), 1.1
+    eh = us * h.abs() + 1.02 * (da * u.abs() * eg + a * eu) + 64 * F * h.abs() + tiny
+    y = h @ dn.double().t()
+    by = us * y.abs() + 1.01 * (eh @ dna.t()) + F * (f + 2) * (h.abs() @ dna.t()) + tiny
+    # backward: kept sums are rounded
+    kg, ku = eg + us * g.abs() + tiny, eu + us * u.abs() + tiny
+    edh = F * (d + 2) * (dya @ dna)
+    edg = us * dg.abs() + 1.02 * (edh * u.abs() * da + dh.abs() * (da * ku + 0.51 * u.abs() * kg)) + 64 * F * (dh * u).abs() + tiny
+    edu = us * du.abs() + 1.02 * (edh * a + dh.abs() * da * kg) + 64 * F * du.abs() + tiny
+    eds, ds = torch.cat([edg, edu], 1), torch.cat([dg, du], 1)
+    dx, dgu, ddn = ds @ gu.double(), ds.t() @ x.double(), dy.double().t() @ h
+    bdx = us * dx.abs() + 1.01 * (eds @ gua) + F * (2 * f + 2) * (ds.abs() @ gua) + tiny
+    bdgu = us * dgu.abs() + 1.01 * (eds.t() @ xa) + F * (m + 2) * (ds.abs().t() @ xa) + tiny
+    bddn = us * ddn.abs() + 1.01 * (dya.t() @ eh) + F * (m + 2) * (dya.t() @ h.abs()) + tiny
+    return by, bdx, bdgu, bddn
+
+
+def close_in_norm(got, ref, dt, roundings, what):
+    """Independent roundings of relative size u each add up in squares: the whole result is off by at most
+    u sqrt(roundings) of its norm (the elementwise bounds above allow every error the same sign)."""
+    err = float((got.double() - ref).norm() / ref.norm().clamp(min=1e-300))
+    assert err <= half_step(dt) * roundings ** 0.5, f"{what}: {err:.2e} of the norm"
+
+
+MLP_SHAPES = [(1, 16, 16), (1, 768, 2048), (2, 64, 48), (5, 256, 512), (16, 80, 144), (17, 112, 272), (33, 144, 400),
+              (64, 768, 2048), (127, 256, 512), (128, 256, 512), (129, 336, 528), (300, 528, 784), (1000, 272, 1040),
+              (2049, 128, 256)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,d,f", MLP_SHAPES)
+def test_mlp_dense_and_its_gradients(rows, d, f, dt):
+    x = rand(rows, d, seed=1, dt=dt).requires_grad_()
+    gu = rand(2 * f, d, seed=2, scale=d ** -0.5, dt=dt).requires_grad_()
+    dn = rand(d, f, seed=3, scale=f ** -0.5, dt=dt).requires_grad_()
+    dy = rand(rows, d, seed=4, dt=dt)
+    y = ops.mlp_dense(x, gu, dn)
+    grads = torch.autograd.grad(y, (x, gu, dn), dy)
+    errors_are_clear()
+    X, G, D = x.detach(), gu.detach(), dn.detach()
+    *refs, parts = mlp_grads_ref(dy, X, G, D)
+    bounds = mlp_bounds(dy, X, G, D, parts, dt)
+    for name, got, ref, bound, n in zip(("y", "dx", "dgate_up", "ddown"), (y.detach(), *grads), refs, bounds,
+                                        (2, 4, 4, 2)):
+        assert got.dtype == dt
+        within(got, ref, bound, name)
+        if ref.numel() > 200:
+            close_in_norm(got, ref, dt, n, name)
+    with torch.no_grad():
+        within(ops.mlp_dense(x, gu, dn), refs[0], bounds[0], "y without gradients")
+    again = torch.autograd.grad(ops.mlp_dense(x, gu, dn), (x, gu, dn), dy)
+    assert all(torch.equal(p, q) for p, q in zip(again, grads))
+    # one gradient at a time gives the same values
+    for i, t in enumerate((x, gu, dn)):
+        only = torch.autograd.grad(ops.mlp_dense(*(s if j == i else s.detach() for j, s in enumerate((x, gu, dn)))), t, dy)
+        within(only[0], refs[1 + i], bounds[1 + i], "alone")
+
+
+@pytest.mark.parametrize("rows", [1, 2, 8, 9, 15, 16, 24, 31, 32, 40, 63, 65])
+def test_mlp_dense_every_small_batch(rows):
+    dt, d, f = torch.bfloat16, 208, 336
+    x, gu, dn = rand(rows, d, seed=1, dt=dt), rand(2 * f, d, seed=2, scale=d ** -0.5, dt=dt), rand(d, f, seed=3, scale=f ** -0.5, dt=dt)
+    dy = rand(rows, d, seed=4, dt=dt)
+    *refs, parts = mlp_grads_ref(dy, x, gu, dn)
+    within(ops.mlp_dense(x, gu, dn), refs[0], mlp_bounds(dy, x, gu, dn, parts, dt)[0], "y")
+    errors_are_clear()
+
+
+def test_mlp_dense_gradient_against_differences():
+    """<grad, v> against central differences of the 64-bit formula (h = 1e-4: error below 1e-6 of the terms);
+    the gradient itself is off by at most its norm bound, 2 u of the norm, which bounds <grad - ref, v>."""
+    dt, rows, d, f = torch.float16, 24, 64, 96
+    ts = [rand(rows, d, seed=1, dt=dt), rand(2 * f, d, seed=2, scale=0.2, dt=dt), rand(d, f, seed=3, scale=0.2, dt=dt)]
+    dy = rand(rows, d, seed=4, dt=dt)
+    leaves = [t.clone().requires_grad_() for t in ts]
+    grads = torch.autograd.grad(ops.mlp_dense(*leaves), leaves, dy)
+    loss = lambda a: float((mlp_ref(*a)[-1] * dy.double()).sum())
+    for i, gr in enumerate(grads):
+        v = rand(*ts[i].shape, seed=30 + i).double()
+        hi, lo = [t.double() for t in ts], [t.double() for t in ts]
+        hi[i], lo[i] = hi[i] + 1e-4 * v, lo[i] - 1e-4 * v
+        num = (loss(hi) - loss(lo)) / 2e-4
+        tol = 2 * half_step(dt) * float(gr.double().norm() * v.norm()) + 1e-6 * float((gr.double() * v).abs().sum())
+        assert abs(float((gr.double() * v).sum()) - num) <= tol
+
+
+def test_mlp_dense_strides_empty_and_3d():
+    dt, d, f = torch.bfloat16, 96, 160
+    big = rand(40, 2 * d + 8, seed=1, dt=dt)
+    gu_big, dn = rand(2 * f, d + 16, seed=2, scale=d ** -0.5, dt=dt), rand(f, d, seed=3, scale=f ** -0.5, dt=dt).t()
+    for off in (0, 8, 3):
+        x, gu = big[:, off:off + d], gu_big[:, off:off + d]
+        refs = mlp_ref(x, gu, dn)
+        *_, parts = mlp_grads_ref(x, x, gu, dn)
+        by = mlp_bounds(x, x, gu, dn, parts, dt)[0]
+        within(ops.mlp_dense(x, gu, dn), refs[-1], by, f"offset {off}")
+        within(ops.mlp_dense(x.reshape(2, 20, d), gu, dn).reshape(40, d), refs[-1], by, "3d")
+    x = torch.empty(0, d, device=DEV, dtype=dt).requires_grad_()
+    gu, dn = gu_big[:, :d].contiguous().requires_grad_(), dn.contiguous().requires_grad_()
+    dx, dgu, ddn = torch.autograd.grad(ops.mlp_dense(x, gu, dn).sum(), (x, gu, dn))
+    assert dx.shape == (0, d) and not dgu.any() and not ddn.any()
+
+
+@pytest.mark.parametrize("rows", [1, 40, 200])
+def test_mlp_dense_keeps_a_bad_row_to_itself(rows):
+    """A NaN or infinity in one token reaches that token's output only; extreme gates saturate."""
+    dt, d, f = torch.bfloat16, 64, 128
+    x, gu, dn = rand(rows + 1, d, seed=1, dt=dt), rand(2 * f, d, seed=2, scale=0.2, dt=dt), rand(d, f, seed=3, scale=0.2, dt=dt)
+    clean = ops.mlp_dense(x, gu, dn)
+    x[rows, 3] = float("nan")
+    y = ops.mlp_dense(x, gu, dn)
+    assert torch.isnan(y[rows]).all() and torch.equal(y[:rows], clean[:rows])
+    x = torch.full((rows, d), 30.0, device=DEV, dtype=dt)
+    ref = mlp_ref(x, gu, dn)
+    y = ops.mlp_dense(x, gu, dn).double()
+    assert not torch.isnan(y).any()
+    assert float((y - ref[-1]).norm() / ref[-1].norm()) <= 2 * half_step(dt)
+
+
+# ---- 8-bit floating point ---------------------------------------------------------------------
+
+def fp8_ref(x, block_rows, dtype):
+    """Scales and dequantised values by definition, in 64 bits."""
+    top = torch.finfo(dtype).max
+    rows, cols = x.shape
+    rb, nb = -(-rows // block_rows), -(-cols // 128)
+    pad = torch.zeros(rb * block_rows, nb * 128, device=x.device, dtype=torch.float64)
+    pad[:rows, :cols] = x.double()
+    t = pad.reshape(rb, block_rows, nb, 128)
+    amax = t.abs().amax((1, 3))
+    e = torch.arange(-126, 128, device=x.device, dtype=torch.float64)
+    scales = torch.exp2(e)                                                   # every candidate, smallest first
+    fits = amax[..., None] <= scales * top
+    scale = scales[fits.int().argmax(-1)]
+    scale = torch.where(amax == 0, torch.ones_like(scale), scale)
+    scale = torch.where(torch.isfinite(amax), scale, torch.full_like(scale, float("nan")))
+    q = (t / scale[:, None, :, None]).float().to(dtype)                      # exact quotient, one rounding
+    return scale, q.reshape(rb * block_rows, nb * 128)[:rows, :cols]
+
+
+def same(a, b):
+    """Equal values, NaN where the other has NaN."""
+    a, b = a.double(), b.double()
+    return a.shape == b.shape and bool(((a == b) | (torch.isnan(a) & torch.isnan(b))).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("rows,cols,block_rows", [(1, 16, 1), (3, 144, 1), (129, 768, 1), (1000, 2000, 1), (1, 16, 128),
+                                                  (128, 128, 128), (129, 144, 128), (333, 2000, 128)])
+def test_quantize_fp8_is_exact(rows, cols, block_rows, dt, dtype):
+    x = rand(rows, cols, seed=1) * torch.exp2(rand(rows, cols, seed=2).mul(3).round())
+    x[:, : cols // 3] *= 448.0
+    x = x.to(dt)
+    q, s = ops.quantize_fp8(x, block_rows=block_rows, dtype=dtype)
+    rs, rq = fp8_ref(x, block_rows, dtype)
+    assert same(s, rs) and same(q, rq)                                       # fp16 inputs overflow to infinities: NaN blocks
+    back = ops.dequantize_fp8(q, s, out_dtype=torch.float32)
+    per = rs.repeat_interleave(block_rows, 0)[:rows].repeat_interleave(128, 1)[:, :cols]
+    assert same(back, rq.double() * per)
+    for out in (torch.bfloat16, torch.float16):
+        assert same(ops.dequantize_fp8(q, s, out_dtype=out), (rq.double() * per).float().to(out))
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_fp8_borders(block_rows, dtype):
+    """Largest value exactly at a power of two times the type's largest, one step above it, ties, zeros,
+    subnormal blocks, infinities and NaN."""
+    top = torch.finfo(dtype).max
+    n = 9 * block_rows
+    x = rand(n, 256, seed=3, scale=0.01)
+    rows = torch.arange(0, n, block_rows)
+    x[:] = 0
+    x[rows[0], 0] = top * 4
+    x[rows[1], 0] = torch.nextafter(torch.tensor(top * 4), torch.tensor(float("inf")))
+    x[rows[2], :16] = torch.tensor([top] + [1.0 + i / 32 for i in range(15)])            # ties of e4m3 and e5m2 at scale 1
+    x[rows[3], 0] = 1e-42                                                                # a subnormal number
+    x[rows[4], 3] = float("inf")
+    x[rows[5], 130] = float("nan")
+    x[rows[6], 7] = -top * 2.0 ** -100
+    x[rows[7], 7] = 3.0e38
+    q, s = ops.quantize_fp8(x, block_rows=block_rows, dtype=dtype)
+    assert torch.isnan(s[4, 0]) and torch.isnan(s[5, 1]) and not torch.isnan(s[4, 1]) and not torch.isnan(s[5, 0])
+    ok = torch.ones(9, dtype=torch.bool)
+    ok[4] = ok[5] = False
+    rs, rq = fp8_ref(x, block_rows, dtype)
+    assert torch.equal(s.double()[ok], rs[ok])
+    keep = ok.repeat_interleave(block_rows)
+    assert torch.equal(q.float()[keep], rq.float()[keep])
+    back = ops.dequantize_fp8(q, s, out_dtype=torch.float32)
+    assert torch.isnan(back[4 * block_rows:5 * block_rows, :128]).all()
+
+
+def test_quantize_fp8_strided_and_empty():
+    base = rand(37, 400, seed=4, dt=torch.bfloat16)
+    for off in (0, 1, 8):
+        x = base[:, off:off + 272]
+        q, s = ops.quantize_fp8(x)
+        rs, rq = fp8_ref(x, 1, torch.float8_e4m3fn)
+        assert torch.equal(s.double(), rs) and torch.equal(q.float(), rq.float())
+    q, s = ops.quantize_fp8(base[:0, :272], block_rows=128)
+    assert q.shape == (0, 272) and s.shape == (0, 3)
+    assert ops.dequantize_fp8(q, s).shape == (0, 272)
+
+
+def fp8_operands(rows, out, cols, xt, wt, seed=0):
+    nb = -(-cols // 128)
+    x = rand(rows, cols, seed=seed + 1, scale=20).to(xt)
+    w = rand(out, cols, seed=seed + 2, scale=20).to(wt)
+    xs = torch.exp(rand(rows, nb, seed=seed + 3)) / 20
+    ws = torch.exp(rand(-(-out // 128), nb, seed=seed + 4)) / 20 * cols ** -0.5
+    return x, xs, w, ws
+
+
+def fp8_linear_ref(x, xs, w, ws):
+    cols, out = x.shape[1], w.shape[0]
+    xd = x.double() * xs.double().repeat_interleave(128, 1)[:, :cols]
+    wd = w.double() * ws.double().repeat_interleave(128, 0)[:out].repeat_interleave(128, 1)[:, :cols]
+    return xd @ wd.t(), xd.abs() @ wd.abs().t()
+
+
+def fp8_bound(ref, mag, cols, out_dtype):
+    """128 products a block added in fp32 (128 f), scaled (3 f) and added over the blocks."""
+    return half_step(out_dtype) * 1.01 * ref.abs() + F * (128 + 3 + -(-cols // 128)) * mag + \
+        (2.0 ** -25 if out_dtype == torch.float16 else 0.0)
+
+
+FP8_SHAPES = [(1, 16, 16), (1, 3333, 2000), (3, 256, 128), (4, 512, 768), (8, 300, 144), (16, 1000, 400), (17, 128, 2000),
+              (33, 129, 80), (64, 384, 272), (130, 640, 1024), (257, 515, 656), (1001, 1111, 2000)]
+
+
+@pytest.mark.parametrize("xt,wt", [(torch.float8_e4m3fn, torch.float8_e4m3fn), (torch.float8_e5m2, torch.float8_e4m3fn),
+                                   (torch.float8_e4m3fn, torch.float8_e5m2), (torch.float8_e5m2, torch.float8_e5m2)])
+@pytest.mark.parametrize("rows,out,cols", FP8_SHAPES)
+def test_linear_fp8(rows, out, cols, xt, wt):
+    x, xs, w, ws = fp8_operands(rows, out, cols, xt, wt)
+    m = mb.Fp8Matrix(w, ws)
+    ref, mag = fp8_linear_ref(x, xs, w, ws)
+    for od in FLOATS:
+        y = ops.linear_fp8(x, m, x_scale=xs, out_dtype=od)
+        assert y.dtype == od
+        within(y, ref, fp8_bound(ref, mag, cols, od), str(od))
+    assert torch.equal(ops.linear_fp8(x, m, x_scale=xs, out_dtype=od), y)
+    errors_are_clear()
+
+
+@pytest.mark.parametrize("rows,d_ff,cols", [(1, 128, 16), (1, 2048, 768), (2, 128, 768), (5, 384, 144), (16, 256, 2000),
+                                            (40, 640, 400), (129, 256, 272), (515, 896, 1024)])
+@pytest.mark.parametrize("xt", [torch.float8_e4m3fn, torch.float8_e5m2])
+def test_linear_fp8_with_the_gate(rows, d_ff, cols, xt):
+    x, xs, w, ws = fp8_operands(rows, 2 * d_ff, cols, xt, torch.float8_e4m3fn, seed=9)
+    m = mb.Fp8Matrix(w, ws)
+    ref, mag = fp8_linear_ref(x, xs, w, ws)
+    e = fp8_bound(ref, mag, cols, torch.float32) + F * ref.abs()
+    g, u = ref[:, :d_ff], ref[:, d_ff:]
+    h = g * torch.sigmoid(g) * u
+    for od in FLOATS:
+        y = ops.linear_fp8(x, m, x_scale=xs, swiglu=True, out_dtype=od)
+        # silu moves by at most 1.1 of its argument's error; its own evaluation costs a few f of 1 + |g|
+        bound = half_step(od) * 1.01 * h.abs() + 1.02 * (1.1 * u.abs() * e[:, :d_ff] + (g * torch.sigmoid(g)).abs() * e[:, d_ff:]) + \
+            F * (16 + 4 * g.abs()) * h.abs() + (2.0 ** -25 if od == torch.float16 else 1e-37)
+        within(y, h, bound, str(od))
+    errors_are_clear()
+
+
+def test_linear_fp8_quantises_and_takes_strides():
+    dt = torch.bfloat16
+    x = rand(6, 11, 272, seed=1, dt=dt)
+    w = rand(200, 272, seed=2, dt=dt)
+    m = mb.Fp8Matrix.from_dense(w)
+    q, s = ops.quantize_fp8(x.reshape(66, 272))
+    y = ops.linear_fp8(x, m)
+    assert y.shape == (6, 11, 200) and y.dtype == dt
+    assert torch.equal(y.reshape(66, 200), ops.linear_fp8(q, m, x_scale=s))
+    assert torch.equal(m.to_dense(torch.float32).double(), fp8_linear_ref(torch.eye(272, device=DEV).to(q.dtype), torch.ones(272, 3, device=DEV), m.data, m.scale)[0].t())
+    # rows of wider tensors
+    wide = torch.zeros(66, 400, device=DEV, dtype=torch.uint8).view(q.dtype)
+    wide[:, 16:288] = q
+    swide = torch.zeros(66, 7, device=DEV)
+    swide[:, 2:5] = s
+    assert torch.equal(ops.linear_fp8(wide[:, 16:288], m, x_scale=swide[:, 2:5]), y.reshape(66, 200))
+    wwide = torch.zeros(200, 304, device=DEV, dtype=torch.uint8).view(q.dtype)
+    wwide[:, 16:288] = m.data
+    assert torch.equal(ops.linear_fp8(q, mb.Fp8Matrix(wwide[:, 16:288], m.scale), x_scale=s), y.reshape(66, 200))
+    assert ops.linear_fp8(q[:0], m, x_scale=s[:0]).shape == (0, 200)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 200])
+def test_linear_fp8_bad_values_stay_in_their_row(rows):
+    x, xs, w, ws = fp8_operands(rows + 1, 256, 272, torch.float8_e4m3fn, torch.float8_e4m3fn, seed=3)
+    m = mb.Fp8Matrix(w, ws)
+    clean = ops.linear_fp8(x, m, x_scale=xs)
+    xs[rows, 2] = float("nan")                                       # the short last block of one token
+    y = ops.linear_fp8(x, m, x_scale=xs)
+    assert torch.isnan(y[rows]).all() and torch.equal(y[:rows], clean[:rows])
+
+
+# ---- together -------------------------------------------------------------------------------
+
+def test_registered_operators_match_and_differentiate():
+    ns = torch.ops.mortar_b200
+    dt = torch.bfloat16
+    x = rand(70, 128, seed=1, dt=dt).requires_grad_()
+    w, b = rand(128, seed=2).requires_grad_(), rand(128, seed=3).requires_grad_()
+    gu, dn = rand(512, 128, seed=4, scale=0.1, dt=dt).requires_grad_(), rand(128, 256, seed=5, scale=0.1, dt=dt).requires_grad_()
+    dy = rand(70, 128, seed=6, dt=dt)
+    leaves = (x, w, b, gu, dn)
+    a = torch.autograd.grad(ops.mlp_dense(ops.layer_norm(x, w, b), gu, dn), leaves, dy)
+    n, stats = ns.layer_norm(x, w, b, 1e-5)
+    assert not stats.requires_grad
+    y, hidden, sums = ns.mlp_dense(n, gu, dn)
+    c = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.equal(p, q) for p, q in zip(a, c))
+    q, s = ns.quantize_fp8(x.detach(), 1, False)
+    m = mb.Fp8Matrix.from_dense(gu)
+    assert torch.equal(ns.linear_fp8(q, s, m.data, m.scale, True, dt), ops.linear_fp8(x.detach(), m, swiglu=True))
+    assert torch.equal(ns.dequantize_fp8(q, s, dt), ops.dequantize_fp8(q, s))
+
+
+def test_site_trains_and_is_served_in_8_bits():
+    """Norm, block and 8-bit form as a user runs them: a training step by the module against the 64-bit
+    composition, then the same weights served in 8 bits."""
+    torch.manual_seed(0)
+    site = mb.SwiGLUDense(256, 512, norm=True, device=DEV)
+    x = rand(3, 50, 256, seed=1).requires_grad_()
+    dy = rand(3, 50, 256, seed=2, dt=torch.bfloat16)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = site(x)
+    y.backward(dy)
+    assert all(p.grad is not None and p.grad.dtype == torch.float32 for p in site.parameters())
+    xd = x.detach().double().requires_grad_()
+    ws = [p.detach().double().requires_grad_() for p in (site.norm.weight, site.norm.bias, site.gate_up.weight, site.down.weight)]
+    s = ln_ref_graph(xd, ws[0], ws[1], site.norm.eps) @ ws[2].t()
+    yd = (torch.nn.functional.silu(s[..., :512]) * s[..., 512:]) @ ws[3].t()
+    grads = torch.autograd.grad(yd, (xd, *ws), dy.double())
+    # weights and the norm's output are rounded to bf16 too: 8 roundings at most meet in a gradient
+    close_in_norm(y.detach(), yd.detach(), torch.bfloat16, 8, "y")
+    for name, got, ref in zip(("x", "norm.weight", "norm.bias", "gate_up", "down"),
+                              (x.grad, site.norm.weight.grad, site.norm.bias.grad, site.gate_up.weight.grad, site.down.weight.grad), grads):
+        close_in_norm(got, ref, torch.bfloat16, 8, name)
+    served = site.to_fp8()
+    xb = x.detach().bfloat16()
+    got = served(xb)
+    # the same composition from the parts
+    n = ops.layer_norm(xb, site.norm.weight, site.norm.bias, site.norm.eps).detach()
+    gu, dn = mb.Fp8Matrix.from_dense(site.gate_up.weight), mb.Fp8Matrix.from_dense(site.down.weight)
+    h = ops.linear_fp8(n, gu, swiglu=True)
+    assert torch.equal(got, ops.linear_fp8(h, dn))
+    # four tensors rounded to e4m3 on the way (2^-4 each at most, in squares)
+    assert float((got.double() - yd.detach()).norm() / yd.detach().norm()) <= 2.0 ** -4 * 4 ** 0.5
+    errors_are_clear()
+
+
+def ln_ref_graph(x, w, b, eps):
+    mean = x.mean(-1, keepdim=True)
+    return (x - mean) / torch.sqrt(((x - mean) ** 2).mean(-1, keepdim=True) + eps) * w + b
+
+
+def test_streams_and_graphs():
+    """A training step and a served step on a side stream, captured twice and replayed with new inputs, the
+    two graphs' replays running at the same time on two streams."""
+    dt = torch.bfloat16
+    gu, dn = rand(512, 128, seed=1, scale=0.1, dt=dt), rand(128, 256, seed=2, scale=0.1, dt=dt)
+    w, b = rand(128, seed=3), rand(128, seed=4)
+    m8 = mb.Fp8Matrix.from_dense(gu)
+    dy = rand(300, 128, seed=5, dt=dt)
+
+    def step(x):
+        x = x.detach().requires_grad_()
+        ws = [t.detach().requires_grad_() for t in (w, b, gu, dn)]
+        n = ops.layer_norm(x, ws[0], ws[1])
+        y = ops.mlp_dense(n, ws[2], ws[3])
+        return [y.detach(), ops.linear_fp8(n.detach(), m8, swiglu=True), *torch.autograd.grad(y, (x, *ws), dy)]
+
+    xs = [rand(300, 128, seed=10 + i, dt=dt) for i in range(2)]
+    want = [step(x) for x in xs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(xs[0])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(got, want[0]))
+    static = [torch.zeros_like(x) for x in xs]
+    graphs, outs = [], []
+    for st in static:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(st))
+        graphs.append(g)
+    for order in ((0, 1), (1, 0)):
+        for st, i in zip(static, order):
+            st.copy_(xs[i])
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for _ in range(3):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for o, i in zip(outs, order):
+            assert all(torch.equal(p, q) for p, q in zip(o, want[i]))
+    errors_are_clear()
