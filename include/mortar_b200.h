@@ -605,7 +605,7 @@ int mortar_prefill_error(int32_t *code, int32_t reset);
 
 /* Layer norm over the last dimension: y = (x - mean) * rstd * weight + bias, rstd =
  * 1 / sqrt(mean((x - mean)^2) + eps).
- *   x, y     device [rows][cols], fp32, bf16 or fp16 (dtype), row strides ldx / ldy; y may be x
+ *   x, y     device [rows][cols], fp32, bf16 or fp16 (dtype), row strides ldx / ldy
  *   weight, bias   device fp32[cols] or NULL (1 and 0)
  *   stats    device fp32[2][rows], mean and rstd for the backward call, or NULL
  * Statistics are fp32 whatever the type.  cols up to 2^20.  (The norm of

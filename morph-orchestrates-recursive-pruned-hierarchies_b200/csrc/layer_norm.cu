@@ -38,9 +38,379 @@ __device__ __forceinline__ float cta_sum(float v, float *red) {
     return s;
 }
 
+// ---- rows in registers: up to 16384 columns ---------------------------------------------------
+//
+// A group of warps owns a row, thread t of its G columns 8 (t + G i) .. + 7 for i < NE: one pass over
+// memory, the row stays in registers (packed as it was read) for mean, variance and result, the next
+// row is on its way meanwhile, and a thread keeps its columns' weights, and in the backward pass their
+// gradients' sums, from row to row.
+//
+// Rows may start anywhere (odd widths, slices): the 16 bytes at an unaligned address are cut out of
+// the two aligned vectors that hold them (the second is the next thread's, so it comes from L1), and a
+// result row that starts off 16 bytes is put together from a lane's words and its neighbour's.
+
+constexpr int kUnit = 8;                                 // columns a thread holds side by side
+constexpr int kFar = 16384;                              // most columns that stay in registers
+
+struct Span { const char *lo, *hi; };                    // bytes of a tensor, first to last row
+
+// words[0..3] = the 16 bytes at p.  `n` bytes of them are wanted; the rest may hold anything.
+__device__ __forceinline__ void load16(const char *p, int n, const Span &span, uint32_t (&w)[4]) {
+    const uint32_t sh = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+    if (sh == 0 && n >= 16) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        return;
+    }
+    const char *a = p - sh;
+    if (a >= span.lo && a + 32 <= span.hi) {
+        const uint4 v0 = __ldg(reinterpret_cast<const uint4 *>(a)), v1 = __ldg(reinterpret_cast<const uint4 *>(a) + 1);
+        const uint32_t c[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+        uint32_t d[6], e[5];
+#pragma unroll
+        for (int i = 0; i < 6; ++i) d[i] = (sh & 8u) ? c[i + 2] : c[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) e[i] = (sh & 4u) ? d[i + 1] : d[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(e[i], e[i + 1], (sh & 3u) * 8u);
+        return;
+    }
+    // first or last bytes of the tensor: two at a time, nothing outside it
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = 4 * i < n ? *reinterpret_cast<const uint16_t *>(p + 4 * i) : 0u;
+        const uint32_t hi = 4 * i + 2 < n ? *reinterpret_cast<const uint16_t *>(p + 4 * i + 2) : 0u;
+        w[i] = lo | hi << 16;
+    }
+}
+
+// Eight columns of a thread as they lie in memory.
+template <class T> struct Unit {
+    static constexpr int kVecs = sizeof(T) * kUnit / 16;
+    uint32_t w[kVecs][4];
+    // `n` columns (0..8) exist
+    __device__ __forceinline__ void load(const T *p, int n, const Span &span) {
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            const int left = n * (int)sizeof(T) - 16 * v;
+            if (left > 0) load16(reinterpret_cast<const char *>(p) + 16 * v, left, span, w[v]);
+            else w[v][0] = w[v][1] = w[v][2] = w[v][3] = 0u;
+        }
+    }
+    __device__ __forceinline__ float get(int j) const;
+    __device__ __forceinline__ void put(int j, float even, float odd);           // columns j, j + 1
+};
+template <> __device__ __forceinline__ float Unit<float>::get(int j) const { return __uint_as_float(w[j >> 2][j & 3]); }
+template <> __device__ __forceinline__ void Unit<float>::put(int j, float a, float b) {
+    w[j >> 2][j & 3] = __float_as_uint(a);
+    w[j >> 2][(j & 3) + 1] = __float_as_uint(b);
+}
+template <> __device__ __forceinline__ float Unit<__nv_bfloat16>::get(int j) const {
+    const uint32_t v = w[0][j >> 1];
+    return __uint_as_float((j & 1) ? v & 0xffff0000u : v << 16);
+}
+template <> __device__ __forceinline__ void Unit<__nv_bfloat16>::put(int j, float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    w[0][j >> 1] = *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ float Unit<__half>::get(int j) const {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[0][j >> 1]));
+    return (j & 1) ? f.y : f.x;
+}
+template <> __device__ __forceinline__ void Unit<__half>::put(int j, float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    w[0][j >> 1] = *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Stores the units of a warp, lane after lane in memory, `n` columns each.  Where the row starts off 16
+// bytes, every aligned vector between two full neighbours is put together from both; the ends of the
+// warp's stretch go out column by column.
+template <class T>
+__device__ __forceinline__ void store_unit(T *p, int n, const Unit<T> &u) {
+    constexpr int kVecs = Unit<T>::kVecs;
+    const uint32_t sh = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;             // the same in all lanes
+    if (sh == 0) {
+        if (n == kUnit) {
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v)
+                reinterpret_cast<uint4 *>(p)[v] = make_uint4(u.w[v][0], u.w[v][1], u.w[v][2], u.w[v][3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j)
+                if (j < n) p[j] = from_f32<T>(u.get(j));
+        }
+        return;
+    }
+    const int lane = threadIdx.x & 31;
+    const bool full_above = __shfl_down_sync(0xffffffffu, n, 1) == kUnit && lane < 31;
+    const bool joined_below = __shfl_up_sync(0xffffffffu, n, 1) == kUnit && lane > 0 && n == kUnit;
+    {
+        // last 16 bytes of the lane below
+        uint32_t below[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) below[i] = __shfl_up_sync(0xffffffffu, u.w[kVecs - 1][i], 1);
+        if (n == kUnit) {
+            // aligned vector v covers the last `sh` bytes of what precedes vector v and the first 16 - sh of it
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) {
+                if (v == 0 && !joined_below) continue;
+                const uint32_t c[8] = {v ? u.w[v - (v > 0)][0] : below[0], v ? u.w[v - (v > 0)][1] : below[1],
+                                       v ? u.w[v - (v > 0)][2] : below[2], v ? u.w[v - (v > 0)][3] : below[3],
+                                       u.w[v][0], u.w[v][1], u.w[v][2], u.w[v][3]};
+                const uint32_t k = 16u - sh;                                          // bytes of c that are skipped
+                uint32_t d[6], e[5], r[4];
+#pragma unroll
+                for (int i = 0; i < 6; ++i) d[i] = (k & 8u) ? c[i + 2] : c[i];
+#pragma unroll
+                for (int i = 0; i < 5; ++i) e[i] = (k & 4u) ? d[i + 1] : d[i];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = __funnelshift_r(e[i], e[i + 1], (k & 3u) * 8u);
+                *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p) - sh + 16 * v) = make_uint4(r[0], r[1], r[2], r[3]);
+            }
+        }
+    }
+    // what no aligned vector took: the head of a lane that is not joined to the one below, the tail of one that is
+    // not joined to the one above
+    const int head = n == kUnit ? (joined_below ? 0 : (16 - (int)sh) / (int)sizeof(T)) : n;
+    const int tail = n == kUnit && !full_above ? kUnit - (int)sh / (int)sizeof(T) : kUnit;
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j)
+        if (j < n && (j < head || j >= tail)) p[j] = from_f32<T>(u.get(j));
+}
+
+// The warps of a CTA form groups of `warps`, one row each at a time.  A group meets at its own named
+// barrier, so the groups run apart; two sets of sums take turns, so one barrier a sum is enough.
+struct Group {
+    int warps, id, warp, thread;
+    float2 *red;                                         // [2][16]
+    uint32_t turn;
+};
+
+__device__ __forceinline__ Group make_group(int warps, float2 (*red)[2][16]) {
+    Group g;
+    g.warps = warps;
+    g.id = (int)(threadIdx.x >> 5) / warps;
+    g.warp = (int)(threadIdx.x >> 5) - g.id * warps;
+    g.thread = (int)threadIdx.x - g.id * warps * 32;
+    g.red = &red[g.id][0][0];
+    g.turn = 0;
+    return g;
+}
+
+// Sums of a and b over the threads of a row, the same in all of them.
+__device__ __forceinline__ float2 group_sum(float a, float b, Group &g) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    if (g.warps == 1) return make_float2(a, b);
+    float2 *red = g.red + 16 * (g.turn & 1u);
+    ++g.turn;
+    if ((threadIdx.x & 31) == 0) red[g.warp] = make_float2(a, b);
+    asm volatile("bar.sync %0, %1;\n" ::"r"(g.id + 1), "r"(g.warps * 32) : "memory");
+    float2 s = red[0];
+    for (int w = 1; w < g.warps; ++w) {
+        s.x += red[w].x;
+        s.y += red[w].y;
+    }
+    return s;
+}
+
+template <class T>
+__device__ __forceinline__ Span span_of(const T *p, long long ld, long long rows, int cols) {
+    return Span{reinterpret_cast<const char *>(p), reinterpret_cast<const char *>(p + (rows - 1) * ld + cols)};
+}
+
+constexpr int kForwardWarps = 32, kBackwardWarps = 24, kMaxGroups = 15, kWideWarps = 16;
+template <int NE> constexpr int kForwardThreads = 32 * (NE == 1 ? kForwardWarps : kWideWarps);
+template <int NE> constexpr int kBackwardThreads = 32 * (NE == 1 ? kBackwardWarps : kWideWarps);
+
+template <class T, int NE>
+struct Row {
+    Unit<T> u[NE];
+    __device__ __forceinline__ void load(const T *p, long long row, long long ld, int cols, const Group &g, const Span &span) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            const int c = kUnit * (g.thread + 32 * g.warps * i);
+            u[i].load(p + row * ld + c, max(0, min(kUnit, cols - c)), span);
+        }
+    }
+};
+
+template <class T, int NE>
+__global__ void __launch_bounds__(kForwardThreads<NE>, 1)
+layer_norm_kernel(const T *__restrict__ x, long long ldx, long long rows, int cols, const float *__restrict__ w,
+                  const float *__restrict__ b, float eps, T *__restrict__ y, long long ldy, float *__restrict__ stats,
+                  int warps) {
+    __shared__ float2 red[kForwardWarps][2][16];
+    Group g = make_group(warps, red);
+    const int groups = (int)(blockDim.x >> 5) / warps;
+    const Span span = span_of(x, ldx, rows, cols);
+    const float inv = 1.f / cols;
+    const long long stride = (long long)gridDim.x * groups;
+    long long row = (long long)blockIdx.x * groups + g.id;
+    float wv[NE][kUnit], bv[NE][kUnit];
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) {
+            const int c = kUnit * (g.thread + 32 * warps * i) + j;
+            wv[i][j] = w && c < cols ? __ldg(w + c) : 1.f;
+            bv[i][j] = b && c < cols ? __ldg(b + c) : 0.f;
+        }
+    Row<T, NE> next;
+    if (row < rows) next.load(x, row, ldx, cols, g, span);
+    for (; row < rows; row += stride) {
+        const Row<T, NE> cur = next;
+        if (row + stride < rows) next.load(x, row + stride, ldx, cols, g, span);      // under this row's sums
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j)
+                s += kUnit * (g.thread + 32 * warps * i) + j < cols ? cur.u[i].get(j) : 0.f;
+        const float mean = group_sum(s, 0.f, g).x * inv;
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) {
+                const float d = kUnit * (g.thread + 32 * warps * i) + j < cols ? cur.u[i].get(j) - mean : 0.f;
+                v = fmaf(d, d, v);
+            }
+        const float rstd = rsqrtf(group_sum(v, 0.f, g).x * inv + eps);
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            const int c = kUnit * (g.thread + 32 * warps * i);
+            Unit<T> r;
+#pragma unroll
+            for (int j = 0; j < kUnit; j += 2)
+                r.put(j, fmaf((cur.u[i].get(j) - mean) * rstd, wv[i][j], bv[i][j]),
+                      fmaf((cur.u[i].get(j + 1) - mean) * rstd, wv[i][j + 1], bv[i][j + 1]));
+            store_unit(y + row * ldy + c, max(0, min(kUnit, cols - c)), r);
+        }
+        if (stats && g.thread == 0) {
+            stats[row] = mean;
+            stats[rows + row] = rstd;
+        }
+    }
+}
+
+// dx, and partial[cta][0 / 1][col] = the sums of dy xh and dy over the CTA's rows.
+template <class T, int NE>
+__global__ void __launch_bounds__(kBackwardThreads<NE>, 1)
+layer_norm_backward_kernel(const T *__restrict__ dy, long long lddy, const T *__restrict__ x, long long ldx, long long rows,
+                           int cols, const float *__restrict__ w, const float *__restrict__ stats, T *__restrict__ dx,
+                           long long lddx, float *__restrict__ partial, int warps) {
+    __shared__ float2 red[kBackwardWarps][2][16];
+    extern __shared__ float fold[];                      // [groups][columns, rounded up to the group's]
+    Group g = make_group(warps, red);
+    const int groups = (int)(blockDim.x >> 5) / warps;
+    const Span sx = span_of(x, ldx, rows, cols), sd = span_of(dy, lddy, rows, cols);
+    const float inv = 1.f / cols;
+    const long long stride = (long long)gridDim.x * groups;
+    long long row = (long long)blockIdx.x * groups + g.id;
+    float dw[NE][kUnit], db[NE][kUnit], wv[NE][kUnit];
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) {
+            const int c = kUnit * (g.thread + 32 * warps * i) + j;
+            dw[i][j] = db[i][j] = 0.f;
+            wv[i][j] = w && c < cols ? __ldg(w + c) : 1.f;
+        }
+    Row<T, NE> nx, nd;
+    float next_mean = 0.f, next_rstd = 0.f;
+    if (row < rows) {
+        nx.load(x, row, ldx, cols, g, sx);
+        nd.load(dy, row, lddy, cols, g, sd);
+        next_mean = __ldg(stats + row);
+        next_rstd = __ldg(stats + rows + row);
+    }
+    for (; row < rows; row += stride) {
+        const Row<T, NE> cx = nx, cd = nd;
+        const float mean = next_mean, rstd = next_rstd;
+        if (row + stride < rows) {                                                    // under this row's sums
+            nx.load(x, row + stride, ldx, cols, g, sx);
+            nd.load(dy, row + stride, lddy, cols, g, sd);
+            next_mean = __ldg(stats + row + stride);
+            next_rstd = __ldg(stats + rows + row + stride);
+        }
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) {
+                const bool in = kUnit * (g.thread + 32 * warps * i) + j < cols;
+                const float d = in ? cd.u[i].get(j) : 0.f, xh = in ? (cx.u[i].get(j) - mean) * rstd : 0.f, t = d * wv[i][j];
+                s1 += t;
+                s2 = fmaf(t, xh, s2);
+                dw[i][j] = fmaf(d, xh, dw[i][j]);
+                db[i][j] += d;
+            }
+        if (dx) {
+            const float2 c = group_sum(s1, s2, g);
+            const float c1 = c.x * inv, c2 = c.y * inv;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const int col = kUnit * (g.thread + 32 * warps * i);
+                Unit<T> r;
+#pragma unroll
+                for (int j = 0; j < kUnit; j += 2) {
+                    float o[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float xh = (cx.u[i].get(j + k) - mean) * rstd;
+                        o[k] = (cd.u[i].get(j + k) * wv[i][j + k] - c1 - xh * c2) * rstd;
+                    }
+                    r.put(j, o[0], o[1]);
+                }
+                store_unit(dx + row * lddx + col, max(0, min(kUnit, cols - col)), r);
+            }
+        }
+    }
+    if (!partial) return;
+    float *dst = partial + (long long)blockIdx.x * 2 * cols;
+    if (groups == 1) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) {
+                const int c = kUnit * (g.thread + 32 * warps * i) + j;
+                if (c < cols) {
+                    dst[c] = dw[i][j];
+                    dst[cols + c] = db[i][j];
+                }
+            }
+        return;
+    }
+    // several groups: add their sums in group order, dw first, then db
+    const int width = 32 * kUnit * NE * warps;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            float4 *f = reinterpret_cast<float4 *>(fold + g.id * width + kUnit * (g.thread + 32 * warps * i));
+            const float (&v)[kUnit] = which ? db[i] : dw[i];
+            f[0] = make_float4(v[0], v[1], v[2], v[3]);
+            f[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+            float s = 0.f;
+            for (int r = 0; r < groups; ++r) s += fold[r * width + c];
+            dst[which * cols + c] = s;
+        }
+    }
+}
+
+// ---- any number of columns: the row is read again for each step -------------------------------
+
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-layer_norm_kernel(const T *x, long long ldx, long long rows, int cols, const float *w, const float *b, float eps,
+layer_norm_far_kernel(const T *x, long long ldx, long long rows, int cols, const float *w, const float *b, float eps,
                   T *y, long long ldy, float *stats) {
     __shared__ float red[kThreads / 32];
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -68,7 +438,7 @@ layer_norm_kernel(const T *x, long long ldx, long long rows, int cols, const flo
 
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-layer_norm_dx_kernel(const T *dy, long long lddy, const T *x, long long ldx, long long rows, int cols, const float *w,
+layer_norm_far_dx_kernel(const T *dy, long long lddy, const T *x, long long ldx, long long rows, int cols, const float *w,
                      const float *stats, T *dx, long long lddx) {
     __shared__ float red[kThreads / 32];
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -91,7 +461,7 @@ layer_norm_dx_kernel(const T *dy, long long lddy, const T *x, long long ldx, lon
 // partial[split][0][col] = sum over the split's rows of dy xh, partial[split][1][col] = sum of dy
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-layer_norm_dw_kernel(const T *dy, long long lddy, const T *x, long long ldx, long long rows, int cols,
+layer_norm_far_dw_kernel(const T *dy, long long lddy, const T *x, long long ldx, long long rows, int cols,
                      const float *stats, float *partial, long long rows_per_split) {
     const int c = blockIdx.x * kThreads + threadIdx.x;
     if (c >= cols) return;
@@ -106,30 +476,83 @@ layer_norm_dw_kernel(const T *dy, long long lddy, const T *x, long long ldx, lon
     partial[(long long)blockIdx.y * 2 * cols + cols + c] = db;
 }
 
-// dw / db [col] = sum of the partials in split order
+// dw / db [col] = sum of the partials: eight interleaved chains a column, added in a fixed order.
 __global__ void __launch_bounds__(kThreads)
-layer_norm_reduce_kernel(const float *partial, int splits, int cols, float *dw, float *db) {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
-    if (c >= 2 * cols) return;
+layer_norm_reduce_kernel(const float *__restrict__ partial, int splits, int cols, float *dw, float *db) {
+    __shared__ float part[8][33];
+    const int lane = threadIdx.x & 31, chain = threadIdx.x >> 5;
+    const long long c = (long long)blockIdx.x * 32 + lane;
     float s = 0.f;
-    for (int i = 0; i < splits; ++i) s += partial[(long long)i * 2 * cols + c];
-    float *dst = c < cols ? dw : db;
-    if (dst) dst[c < cols ? c : c - cols] = s;
+    if (c < 2LL * cols)
+        for (int i = chain; i < splits; i += 8) s += partial[(long long)i * 2 * cols + c];
+    part[chain][lane] = s;
+    __syncthreads();
+    if (chain == 0 && c < 2LL * cols) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) s += part[k][lane];
+        float *dst = c < cols ? dw : db;
+        if (dst) dst[c < cols ? c : c - cols] = s;
+    }
 }
 
 bool misaligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
 
 size_t elem_bytes(int dtype) { return dtype == MORTAR_F32 ? 4 : 2; }
 
-constexpr int64_t kMaxSplits = 296;
+// How a row of `cols` columns is laid over a CTA: units of 8 columns a thread, warps a row, and rows at a time (at most
+// `most` warps; fewer rows at a time when there are too few rows for every SM).
+struct Layout { int units, warps, groups; };
 
-int64_t splits_for(int64_t rows) { return rows < 1 ? 1 : (rows < kMaxSplits * 4 ? (rows + 3) / 4 : kMaxSplits); }
+Layout layout_of(int64_t rows, int32_t cols, int most) {
+    Layout l;
+    l.units = cols <= 4096 ? 1 : cols <= 8192 ? 2 : 4;
+    l.warps = (cols + 32 * kUnit * l.units - 1) / (32 * kUnit * l.units);
+    int g = l.units > 1 ? 1 : most / l.warps;
+    if (l.warps > 1 && g > kMaxGroups) g = kMaxGroups;
+    const int64_t share = (rows + 147) / 148;
+    l.groups = g < 1 ? 1 : (share < g ? (int)(share < 1 ? 1 : share) : g);
+    return l;
+}
+
+// CTAs of the backward pass, one partial sum each: one per SM at most
+int64_t splits_for(int64_t rows, int32_t cols) {
+    if (cols > kFar) return rows < 4 * 148 ? (rows + 3) / 4 + (rows == 0) : 148;
+    const int64_t need = (rows + layout_of(rows, cols, kBackwardWarps).groups - 1) / layout_of(rows, cols, kBackwardWarps).groups;
+    return need < 1 ? 1 : (need < 148 ? need : 148);
+}
+
+template <class T, int NE>
+int run_forward(const Layout &l, const void *x, int64_t ldx, int64_t rows, int32_t cols, const float *w, const float *b,
+                float eps, void *y, int64_t ldy, float *stats, cudaStream_t st) {
+    const int64_t need = (rows + l.groups - 1) / l.groups;
+    layer_norm_kernel<T, NE><<<(unsigned)(need < 148 ? need : 148), 32 * l.warps * l.groups, 0, st>>>(
+        (const T *)x, ldx, rows, cols, w, b, eps, (T *)y, ldy, stats, l.warps);
+    MORTAR_CUDA_CHECK(cudaGetLastError());
+    return MORTAR_OK;
+}
+
+template <class T, int NE>
+int run_backward(const Layout &l, const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t rows, int32_t cols,
+                 const float *w, const float *stats, void *dx, int64_t lddx, float *partial, cudaStream_t st) {
+    // at most 24 warps' columns: 24 KB
+    const int smem = partial && l.groups > 1 ? l.groups * l.warps * 32 * kUnit * NE * (int)sizeof(float) : 0;
+    layer_norm_backward_kernel<T, NE><<<(unsigned)splits_for(rows, cols), 32 * l.warps * l.groups, smem, st>>>(
+        (const T *)dy, lddy, (const T *)x, ldx, rows, cols, w, stats, (T *)dx, lddx, partial, l.warps);
+    MORTAR_CUDA_CHECK(cudaGetLastError());
+    return MORTAR_OK;
+}
 
 template <class T>
 int forward(const void *x, int64_t ldx, int64_t rows, int32_t cols, const float *w, const float *b, float eps, void *y,
             int64_t ldy, float *stats, cudaStream_t st) {
+    if (cols <= kFar) {
+        const Layout l = layout_of(rows, cols, kForwardWarps);
+        if (l.units == 1) return run_forward<T, 1>(l, x, ldx, rows, cols, w, b, eps, y, ldy, stats, st);
+        if (l.units == 2) return run_forward<T, 2>(l, x, ldx, rows, cols, w, b, eps, y, ldy, stats, st);
+        return run_forward<T, 4>(l, x, ldx, rows, cols, w, b, eps, y, ldy, stats, st);
+    }
     const unsigned grid = (unsigned)(rows < 1184 ? rows : 1184);
-    layer_norm_kernel<T><<<grid, kThreads, 0, st>>>((const T *)x, ldx, rows, cols, w, b, eps, (T *)y, ldy, stats);
+    layer_norm_far_kernel<T><<<grid, kThreads, 0, st>>>((const T *)x, ldx, rows, cols, w, b, eps, (T *)y, ldy, stats);
     MORTAR_CUDA_CHECK(cudaGetLastError());
     return MORTAR_OK;
 }
@@ -137,20 +560,30 @@ int forward(const void *x, int64_t ldx, int64_t rows, int32_t cols, const float 
 template <class T>
 int backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t rows, int32_t cols, const float *w,
              const float *stats, void *dx, int64_t lddx, float *dw, float *db, float *scratch, cudaStream_t st) {
-    const unsigned grid = (unsigned)(rows < 1184 ? rows : 1184);
-    if (dx) {
-        layer_norm_dx_kernel<T><<<grid, kThreads, 0, st>>>((const T *)dy, lddy, (const T *)x, ldx, rows, cols, w, stats,
-                                                          (T *)dx, lddx);
-        MORTAR_CUDA_CHECK(cudaGetLastError());
+    const int64_t splits = splits_for(rows, cols);
+    float *partial = dw || db ? scratch : nullptr;
+    if (cols <= kFar) {
+        const Layout l = layout_of(rows, cols, kBackwardWarps);
+        const int rc = l.units == 1   ? run_backward<T, 1>(l, dy, lddy, x, ldx, rows, cols, w, stats, dx, lddx, partial, st)
+                       : l.units == 2 ? run_backward<T, 2>(l, dy, lddy, x, ldx, rows, cols, w, stats, dx, lddx, partial, st)
+                                      : run_backward<T, 4>(l, dy, lddy, x, ldx, rows, cols, w, stats, dx, lddx, partial, st);
+        if (rc != MORTAR_OK) return rc;
+    } else {
+        if (dx) {
+            const unsigned grid = (unsigned)(rows < 1184 ? rows : 1184);
+            layer_norm_far_dx_kernel<T><<<grid, kThreads, 0, st>>>((const T *)dy, lddy, (const T *)x, ldx, rows, cols, w,
+                                                                  stats, (T *)dx, lddx);
+            MORTAR_CUDA_CHECK(cudaGetLastError());
+        }
+        if (partial) {
+            const unsigned cb = (unsigned)((cols + kThreads - 1) / kThreads);
+            layer_norm_far_dw_kernel<T><<<dim3(cb, (unsigned)splits), kThreads, 0, st>>>(
+                (const T *)dy, lddy, (const T *)x, ldx, rows, cols, stats, partial, (rows + splits - 1) / splits);
+            MORTAR_CUDA_CHECK(cudaGetLastError());
+        }
     }
-    if (dw || db) {
-        const int64_t splits = splits_for(rows), rps = (rows + splits - 1) / splits;
-        const unsigned cb = (unsigned)((cols + kThreads - 1) / kThreads);
-        layer_norm_dw_kernel<T><<<dim3(cb, (unsigned)splits), kThreads, 0, st>>>((const T *)dy, lddy, (const T *)x, ldx,
-                                                                                 rows, cols, stats, scratch, rps);
-        MORTAR_CUDA_CHECK(cudaGetLastError());
-        layer_norm_reduce_kernel<<<(unsigned)((2LL * cols + kThreads - 1) / kThreads), kThreads, 0, st>>>(
-            scratch, (int)splits, cols, dw, db);
+    if (partial) {
+        layer_norm_reduce_kernel<<<(unsigned)((2LL * cols + 31) / 32), kThreads, 0, st>>>(partial, (int)splits, cols, dw, db);
         MORTAR_CUDA_CHECK(cudaGetLastError());
     }
     return MORTAR_OK;
@@ -179,7 +612,7 @@ extern "C" int mortar_layer_norm(const void *x, int32_t dtype, int64_t ldx, int6
 
 extern "C" int64_t mortar_layer_norm_scratch_floats(int64_t rows, int32_t cols) {
     if (rows < 0 || cols <= 0) return MORTAR_ERR_SHAPE;
-    return splits_for(rows) * 2 * cols;
+    return splits_for(rows, cols) * 2 * cols;
 }
 
 extern "C" int mortar_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int32_t dtype,
@@ -200,7 +633,7 @@ extern "C" int mortar_layer_norm_backward(const void *dy, int64_t lddy, const vo
         if (dbias) MORTAR_CUDA_CHECK(cudaMemsetAsync(dbias, 0, (size_t)cols * 4, st));
         return MORTAR_OK;
     }
-    if ((dweight || dbias) && (!scratch || scratch_floats < splits_for(rows) * 2 * cols)) return MORTAR_ERR_CAPACITY;
+    if ((dweight || dbias) && (!scratch || scratch_floats < splits_for(rows, cols) * 2 * cols)) return MORTAR_ERR_CAPACITY;
     if (dtype == MORTAR_F32)
         return backward<float>(dy, lddy, x, ldx, rows, cols, weight, stats, dx, lddx, dweight, dbias, scratch, st);
     if (dtype == MORTAR_BF16)

@@ -5,7 +5,6 @@ morph/sparse/stk/backend/custom_ops.py:35).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 from typing import Optional
 
@@ -964,17 +963,41 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
 
 
-def _on_device(t: torch.Tensor):
-    """The launch goes to the device of ``t`` and to that device's current stream."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch(where: str, t: torch.Tensor, *args) -> None:
+    """Calls the library's ``where`` with ``args`` and the current stream of the device of ``t``, on that
+    device.  Tensors go in as their addresses: building pointer objects and a Stream object costs
+    more than a small kernel runs."""
+    fn = getattr(_lib.lib(), where)
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, where)
 
 
-def _same_device(t: torch.Tensor, **others) -> None:
-    for name, o in others.items():
-        if o is not None and o.device != t.device:
-            raise ValueError(f"{name} is on {o.device}, expected {t.device}")
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _same_device(t: torch.Tensor, name: str, o: Optional[torch.Tensor]) -> None:
+    if o is not None and o.device != t.device:
+        raise ValueError(f"{name} is on {o.device}, expected {t.device}")
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of the shape and type of ``t``."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _f32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().float().contiguous()
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -986,14 +1009,27 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def _once(name: str) -> None:
+    """Called in a backward pass: with ``create_graph`` it would have to be differentiable itself."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} has no second derivative: call backward without create_graph")
 
 
 def _rows_any(t: torch.Tensor) -> torch.Tensor:
     """[..., cols] -> [rows, cols] with contiguous rows that do not overlap."""
-    t2 = t.reshape(-1, t.shape[-1])
+    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:
         t2 = t2.contiguous()
+        if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:          # one row or one column: strides are free
+            t2 = t2.clone(memory_format=torch.contiguous_format).view(t2.shape)
     return t2
 
 
@@ -1001,28 +1037,28 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Op
                        want_stats: bool):
     """``layer_norm`` without its gradient: (y, stats) with stats fp32 [2, rows] = mean and 1/std
     (None unless ``want_stats``)."""
-    _require_cuda(x, "x")
-    if x.dim() < 1 or x.dtype not in _FLOATS:
+    if not x.is_cuda:
+        _require_cuda(x, "x")
+    code = _CODE.get(x.dtype)
+    if code is None or code > _lib.F16 or x.dim() < 1:
         raise ValueError(f"x must be a float32, bfloat16 or float16 tensor [..., cols], got {x.dtype}")
     cols = x.shape[-1]
     if cols < 1:
         raise ValueError("the last dimension is empty: a mean of nothing is not defined")
-    _same_device(x, weight=weight, bias=bias)
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (tuple(t.shape) != (cols,) or t.dtype not in _FLOATS):
-            raise ValueError(f"{name} must be a float tensor [{cols}], got {t.dtype} {list(t.shape)}")
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        if t is not None:
+            if t.dim() != 1 or t.shape[0] != cols or t.dtype not in _FLOATS:
+                raise ValueError(f"{name} must be a float tensor [{cols}], got {t.dtype} {list(t.shape)}")
+            _same_device(x, name, t)
+    y = _like(x)
     x2 = _rows_any(x)
     rows = x2.shape[0]
-    stats = torch.empty(2, rows, device=x.device, dtype=torch.float32) if want_stats else None
+    stats = x.new_empty((2, rows), dtype=torch.float32) if want_stats else None
     if rows == 0:
         return y, stats
-    w = None if weight is None else weight.detach().float().contiguous()
-    b = None if bias is None else bias.detach().float().contiguous()
-    with _on_device(x):
-        _lib.check(_lib.lib().mortar_layer_norm(_ptr(x2), _CODE[x.dtype], x2.stride(0), rows, cols, _ptr(w), _ptr(b),
-                                                float(eps), _ptr(y), cols, _ptr(stats), _stream_ptr()),
-                   "mortar_layer_norm")
+    w, b = _f32(weight), _f32(bias)
+    _launch("mortar_layer_norm", x, x2.data_ptr(), code, x2.stride(0), rows, cols, _at(w), _at(b), eps, y.data_ptr(),
+            cols, _at(stats))
     _count("layer_norm")
     return y, stats
 
@@ -1031,32 +1067,35 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
                         want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
     """(dx, dweight, dbias) of ``layer_norm`` from the stats its forward kept; dweight and dbias are
     fp32 [cols]; what is not wanted is None."""
-    _require_cuda(dy, "dy")
-    if dy.shape != x.shape:
-        raise ValueError(f"dy has shape {list(dy.shape)}, x {list(x.shape)}")
-    _same_device(x, dy=dy, weight=weight, stats=stats)
+    if not x.is_cuda:
+        _require_cuda(x, "x")
+    code = _CODE.get(x.dtype)
+    if code is None or code > _lib.F16 or dy.shape != x.shape:
+        raise ValueError(f"dy has shape {list(dy.shape)}, x {list(x.shape)} ({x.dtype})")
+    for name, t in (("dy", dy), ("weight", weight), ("stats", stats)):
+        _same_device(x, name, t)
     cols = x.shape[-1]
-    d2, x2 = _rows_any(dy.to(x.dtype)), _rows_any(x)
+    if weight is not None and tuple(weight.shape) != (cols,):
+        raise ValueError(f"weight must be [{cols}], got {list(weight.shape)}")
+    d2, x2 = _rows_any(dy if dy.dtype == x.dtype else dy.to(x.dtype)), _rows_any(x)
     rows = x2.shape[0]
     if stats.dtype != torch.float32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
         raise ValueError(f"stats must be contiguous float32 [2, {rows}]")
-    dev = x.device
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if want_dx else None
-    dw = torch.empty(cols, device=dev, dtype=torch.float32) if want_dweight else None
-    db = torch.empty(cols, device=dev, dtype=torch.float32) if want_dbias else None
-    if not (want_dx or want_dweight or want_dbias):
-        return dx, dw, db
+    dx = _like(x) if want_dx else None
+    dw = x.new_empty((cols,), dtype=torch.float32) if want_dweight else None
+    db = x.new_empty((cols,), dtype=torch.float32) if want_dbias else None
     if rows == 0:
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-    w = None if weight is None else weight.detach().float().contiguous()
-    L = _lib.lib()
-    n = L.mortar_layer_norm_scratch_floats(rows, cols) if want_dweight or want_dbias else 0
-    scratch = torch.empty(n, device=dev, dtype=torch.float32) if n else None
-    with _on_device(x):
-        _lib.check(L.mortar_layer_norm_backward(
-            _ptr(d2), d2.stride(0), _ptr(x2), x2.stride(0), _CODE[x.dtype], rows, cols, _ptr(w), _ptr(stats),
-            _ptr(dx), cols, _ptr(dw), _ptr(db), _ptr(scratch), n, _stream_ptr()), "mortar_layer_norm_backward")
-    _count("layer_norm_backward")
+    if not (want_dx or want_dweight or want_dbias):
+        return dx, dw, db
+    w = _f32(weight)
+    scratch, n = None, 0
+    if want_dweight or want_dbias:
+        n = _lib.lib().mortar_layer_norm_scratch_floats(rows, cols)
+        scratch = x.new_empty((n,), dtype=torch.float32)
+    _launch("mortar_layer_norm_backward", x, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), code, rows, cols,
+            _at(w), stats.data_ptr(), _at(dx), cols, _at(dw), _at(db), _at(scratch), n)
+    _count("layer_norm_backward", 2 if n else 1)
     return dx, dw, db
 
 
@@ -1069,18 +1108,21 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once("layer_norm")
         x, weight, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = layer_norm_backward(dy, x, weight, stats, need[0], need[1], need[2])
-        return (dx, None if dw is None else dw.to(weight.dtype), None if db is None else db.to(ctx.bias_dtype), None)
+        dx, dw, db = layer_norm_backward(dy, x, weight, stats, *ctx.needs_input_grad[:3])
+        if dw is not None and weight.dtype != torch.float32:
+            dw = dw.to(weight.dtype)
+        if db is not None and ctx.bias_dtype != torch.float32:
+            db = db.to(ctx.bias_dtype)
+        return dx, dw, db, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last dimension of x [..., cols] (fp32, bf16 or fp16), differentiable in x,
-    ``weight`` and ``bias`` ([cols], fp32 or the type of x; None = 1 and 0): the norm of the
+    ``weight`` and ``bias`` ([cols], any of the three types; None = 1 and 0): the norm of the
     reference's router query (morph/model/routing.py:159-284) as an operator beside
     ``rmsnorm_rows``.  Statistics and the gradients of weight and bias are summed in fp32, in a fixed
     order (the same call gives the same bits); y and dx are rounded once, to the type of x.  Like
@@ -1114,7 +1156,7 @@ def _mlp_dense_args(x, gate_up, down):
     for name, t in (("gate_up", gate_up), ("down", down)):
         if t.dtype != x.dtype:
             raise ValueError(f"{name} is {t.dtype}, x is {x.dtype}: one type for all")
-    _same_device(x, gate_up=gate_up, down=down)
+        _same_device(x, name, t)
     return d_model, d_ff
 
 
@@ -1122,18 +1164,16 @@ def mlp_dense_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor
     """``mlp_dense`` without its gradient: (y, hidden, sums) with hidden [rows, d_ff] and, when
     ``want_saved``, sums [rows, 2 d_ff] = x gate_up^T for ``mlp_dense_backward`` (else None)."""
     d_model, d_ff = _mlp_dense_args(x, gate_up, down)
-    x2 = _rows16(x.reshape(-1, d_model))
+    x2 = _rows16(x if x.dim() == 2 else x.reshape(-1, d_model))
     gu, dn = _rows16(gate_up), _rows16(down)
-    rows, dev = x2.shape[0], x.device
-    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    hidden = torch.empty(rows, d_ff, device=dev, dtype=x.dtype)
-    sums = torch.empty(rows, 2 * d_ff, device=dev, dtype=x.dtype) if want_saved else None
+    rows = x2.shape[0]
+    y = _like(x)
+    hidden = x.new_empty((rows, d_ff))
+    sums = x.new_empty((rows, 2 * d_ff)) if want_saved else None
     if rows == 0:
         return y, hidden, sums
-    with _on_device(x):
-        _lib.check(_lib.lib().mortar_mlp_dense(
-            _ptr(x2), x2.stride(0), _CODE[x.dtype], rows, _ptr(gu), gu.stride(0), _ptr(dn), dn.stride(0), d_model,
-            d_ff, _ptr(hidden), _ptr(sums), _ptr(y), d_model, _stream_ptr()), "mortar_mlp_dense")
+    _launch("mortar_mlp_dense", x, x2.data_ptr(), x2.stride(0), _CODE[x.dtype], rows, gu.data_ptr(), gu.stride(0),
+            dn.data_ptr(), dn.stride(0), d_model, d_ff, hidden.data_ptr(), _at(sums), y.data_ptr(), d_model)
     _count("dense", 2)
     return y, hidden, sums
 
@@ -1145,26 +1185,26 @@ def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor,
     d_model, d_ff = _mlp_dense_args(x, gate_up, down)
     if dy.shape != x.shape:
         raise ValueError(f"dy has shape {list(dy.shape)}, x {list(x.shape)}")
-    _same_device(x, dy=dy, hidden=hidden, sums=sums)
-    d2, x2 = _rows16(dy.to(x.dtype).reshape(-1, d_model)), _rows16(x.reshape(-1, d_model))
+    for name, t in (("dy", dy), ("hidden", hidden), ("sums", sums)):
+        _same_device(x, name, t)
+    dt = x.dtype
+    d2, x2 = _rows16((dy if dy.dtype == dt else dy.to(dt)).reshape(-1, d_model)), _rows16(x.reshape(-1, d_model))
     gu, dn = _rows16(gate_up), _rows16(down)
-    rows, dev, dt = x2.shape[0], x.device, x.dtype
+    rows = x2.shape[0]
     for name, t, n in (("hidden", hidden, d_ff), ("sums", sums, 2 * d_ff)):
         if tuple(t.shape) != (rows, n) or t.dtype != dt or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous {dt} [{rows}, {n}]")
-    dx = torch.empty(x.shape, device=dev, dtype=dt) if want_dx else None
-    dgu = torch.empty(2 * d_ff, d_model, device=dev, dtype=dt) if want_dgate_up else None
-    ddn = torch.empty(d_model, d_ff, device=dev, dtype=dt) if want_ddown else None
+    dx = _like(x) if want_dx else None
+    dgu = x.new_empty((2 * d_ff, d_model)) if want_dgate_up else None
+    ddn = x.new_empty((d_model, d_ff)) if want_ddown else None
     if not (want_dx or want_dgate_up or want_ddown):
         return dx, dgu, ddn
     if rows == 0:
         return dx, None if dgu is None else dgu.zero_(), None if ddn is None else ddn.zero_()
     dsums = torch.empty_like(sums)
-    with _on_device(x):
-        _lib.check(_lib.lib().mortar_mlp_dense_backward(
-            _ptr(d2), d2.stride(0), _ptr(x2), x2.stride(0), _CODE[dt], rows, _ptr(gu), gu.stride(0), _ptr(dn),
-            dn.stride(0), d_model, d_ff, _ptr(hidden), _ptr(sums), _ptr(dsums), _ptr(dx), _ptr(dgu), _ptr(ddn),
-            _stream_ptr()), "mortar_mlp_dense_backward")
+    _launch("mortar_mlp_dense_backward", x, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), _CODE[dt], rows,
+            gu.data_ptr(), gu.stride(0), dn.data_ptr(), dn.stride(0), d_model, d_ff, hidden.data_ptr(), sums.data_ptr(),
+            dsums.data_ptr(), _at(dx), _at(dgu), _at(ddn))
     _count("dense_backward", (1 if want_dx or want_dgate_up else 0) + 1)
     return dx, dgu, ddn
 
@@ -1177,8 +1217,8 @@ class _MlpDense(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once("mlp_dense")
         return mlp_dense_backward(dy, *ctx.saved_tensors, *ctx.needs_input_grad)
 
 
@@ -1214,14 +1254,12 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1, dtype: torch.dtype = t
     if cols < 1 or cols % TILE:
         raise ValueError(f"cols must be a positive multiple of {TILE}, got {cols}")
     x2 = _rows16(x)
-    q = torch.empty(rows, cols, device=x.device, dtype=dtype)
-    scale = torch.empty(-(-rows // block_rows), -(-cols // 128), device=x.device, dtype=torch.float32)
+    q = x.new_empty((rows, cols), dtype=dtype)
+    scale = x.new_empty((-(-rows // block_rows), -(-cols // 128)), dtype=torch.float32)
     if rows == 0:
         return q, scale
-    with _on_device(x):
-        _lib.check(_lib.lib().mortar_quantize_fp8(_ptr(x2), _CODE[x.dtype], x2.stride(0), rows, cols, block_rows,
-                                                  _ptr(q), _CODE[dtype], cols, _ptr(scale), _stream_ptr()),
-                   "mortar_quantize_fp8")
+    _launch("mortar_quantize_fp8", x, x2.data_ptr(), _CODE[x.dtype], x2.stride(0), rows, cols, block_rows, q.data_ptr(),
+            _CODE[dtype], cols, scale.data_ptr())
     _count("quantize_fp8")
     return q, scale
 
@@ -1241,16 +1279,14 @@ def dequantize_fp8(q: torch.Tensor, scale: torch.Tensor, *, out_dtype: torch.dty
     if scale.dtype != torch.float32 or tuple(scale.shape) not in ((rows, nb), (-(-rows // 128), nb)):
         raise ValueError(f"scale must be float32 [{rows}, {nb}] or [{-(-rows // 128)}, {nb}], got {scale.dtype} "
                          f"{list(scale.shape)}")
-    _same_device(q, scale=scale)
+    _same_device(q, "scale", scale)
     block_rows = 1 if scale.shape[0] == rows else 128
-    out = torch.empty(rows, cols, device=q.device, dtype=out_dtype)
+    out = q.new_empty((rows, cols), dtype=out_dtype)
     if rows == 0:
         return out
     q2, s2 = _rows16(q), scale.contiguous()
-    with _on_device(q):
-        _lib.check(_lib.lib().mortar_dequantize_fp8(_ptr(q2), _CODE[q.dtype], q2.stride(0), _ptr(s2), rows, cols,
-                                                    block_rows, _ptr(out), _CODE[out_dtype], cols, _stream_ptr()),
-                   "mortar_dequantize_fp8")
+    _launch("mortar_dequantize_fp8", q, q2.data_ptr(), _CODE[q.dtype], q2.stride(0), s2.data_ptr(), rows, cols, block_rows,
+            out.data_ptr(), _CODE[out_dtype], cols)
     _count("dequantize_fp8")
     return out
 
@@ -1287,9 +1323,10 @@ def linear_fp8(x: torch.Tensor, w: Fp8Matrix, *, x_scale: Optional[torch.Tensor]
         out_dtype = x.dtype if x.dtype in _FLOATS else torch.bfloat16
     if out_dtype not in _FLOATS:
         raise ValueError(f"unsupported out_dtype {out_dtype}")
-    _same_device(x, w=w.data, x_scale=x_scale)
+    _same_device(x, "w", w.data)
+    _same_device(x, "x_scale", x_scale)
     lead, nb = x.shape[:-1], -(-w.in_features // 128)
-    x2 = x.reshape(-1, w.in_features)
+    x2 = x if x.dim() == 2 else x.reshape(-1, w.in_features)
     rows = x2.shape[0]
     if x_scale is None:
         x2, s2 = quantize_fp8(x2)
@@ -1298,15 +1335,12 @@ def linear_fp8(x: torch.Tensor, w: Fp8Matrix, *, x_scale: Optional[torch.Tensor]
             raise ValueError(f"x_scale must be float32 {[*lead, nb]}, got {x_scale.dtype} {list(x_scale.shape)}")
         x2, s2 = _rows16(x2), _rows_any(x_scale)
     n_out = w.out_features // 2 if swiglu else w.out_features
-    out = torch.empty(*lead, n_out, device=x.device, dtype=out_dtype)
+    out = x.new_empty((*lead, n_out), dtype=out_dtype)
     if rows == 0:
         return out
-    with _on_device(x):
-        _lib.check(_lib.lib().mortar_linear_fp8(
-            _ptr(x2), _CODE[x2.dtype], x2.stride(0), _ptr(s2), s2.stride(0), rows, _ptr(w.data), _CODE[w.data.dtype],
-            w.data.stride(0), _ptr(w.scale), w.scale.stride(0), w.out_features, w.in_features,
-            _lib.FLAG_SWIGLU if swiglu else 0, _ptr(out), _CODE[out_dtype], n_out, _stream_ptr()),
-            "mortar_linear_fp8")
+    _launch("mortar_linear_fp8", x, x2.data_ptr(), _CODE[x2.dtype], x2.stride(0), s2.data_ptr(), s2.stride(0), rows,
+            w.data.data_ptr(), _CODE[w.data.dtype], w.data.stride(0), w.scale.data_ptr(), w.scale.stride(0),
+            w.out_features, w.in_features, _lib.FLAG_SWIGLU if swiglu else 0, out.data_ptr(), _CODE[out_dtype], n_out)
     _count("linear_fp8")
     return out
 
