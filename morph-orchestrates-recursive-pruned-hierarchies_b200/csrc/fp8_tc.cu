@@ -27,9 +27,9 @@ constexpr int kStageA = 128 * 128;               // this CTA's 128 rows, one blo
 constexpr int kStageB = 128 * 128;               // this CTA's half of the 256 output columns
 constexpr int kStage = kStageA + kStageB;
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kThreads = 128 + 32 * kEpiWarps;   // warps 0..3: copies, MMAs, two that only lend their registers
 constexpr int kTmemCols = 512;
-constexpr int kSmem = kStages * kStage + (2 * kStages + 4) * 8 + 1024;
+constexpr int kSmem = kStages * kStage + (2 * kStages + 2) * 8 + 1024;
 
 __device__ int g_fp8_error;
 
@@ -47,12 +47,14 @@ struct Fp8Params {
     void *out;
     long long ld_out;
     int out_dtype;
-    int vec;                 // 1: rows of out start on 16 bytes
+    int vec;                 // 1: rows of out start on 32 bytes
 };
 
-__device__ __forceinline__ float silu(float g) { return g / (1.f + expf(-g)); }
+// exp2-based exponential and an approximate quotient, 2^-22 (1 + |g|) at worst: the exact forms cost the
+// epilogue of a 256 x 256 tile three times what its 16 blocks of MMAs take (631 against 420 us at 8192 x 2048 -> 11264)
+__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
-// 32 values of one row from column `col` on
+// 32 values of one row from column `col` on; 32 bytes at a time where the row is aligned
 __device__ __forceinline__ void store_row32(const Fp8Params &p, long long row, int col, const float (&v)[32]) {
     const int left = p.n - col;
     if (row >= p.rows || left <= 0) return;
@@ -60,27 +62,32 @@ __device__ __forceinline__ void store_row32(const Fp8Params &p, long long row, i
     if (p.out_dtype == MORTAR_F32) {
         float *o = reinterpret_cast<float *>(p.out) + idx;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (p.vec && 4 * j + 4 <= left) reinterpret_cast<float4 *>(o)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            else
+        for (int j = 0; j < 4; ++j) {
+            if (p.vec && 8 * j + 8 <= left) {
+                uint32_t w[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (4 * j + i < left) o[4 * j + i] = v[4 * j + i];
+                for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * j + i]);
+                tc::store_v8(o + 8 * j, w);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (8 * j + i < left) o[8 * j + i] = v[8 * j + i];
+            }
         }
         return;
     }
     const bool half = p.out_dtype == MORTAR_F16;
     uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + idx;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t w[4];
+    for (int j = 0; j < 2; ++j) {
+        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = tc::pack16(v[8 * j + 2 * i], v[8 * j + 2 * i + 1], half);
-        if (p.vec && 8 * j + 8 <= left) reinterpret_cast<uint4 *>(o)[j] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < 8; ++i) w[i] = tc::pack16(v[16 * j + 2 * i], v[16 * j + 2 * i + 1], half);
+        if (p.vec && 16 * j + 16 <= left) tc::store_v8(o + 16 * j, w);
         else
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (8 * j + i < left) o[8 * j + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+            for (int i = 0; i < 16; ++i)
+                if (16 * j + i < left) o[16 * j + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
     }
 }
 
@@ -95,8 +102,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t *full = reinterpret_cast<uint64_t *>(stages + kStages * kStage), *empty = full + kStages;
-    uint64_t *acc_full = empty + kStages, *acc_empty = acc_full + 2;
+    // full: a stage's copies have landed (CTA 0's count for both); done: its MMAs have ended, so the stage is free and
+    // its sums are there; acc_empty (CTA 0's): the warps of both have read the sums
+    uint64_t *full = reinterpret_cast<uint64_t *>(stages + kStages * kStage), *done = full + kStages;
+    uint64_t *acc_empty = done + kStages;
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -105,8 +114,8 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
 
     if (threadIdx.x == 0) {
         abort_s = 0;
-        for (int s = 0; s < kStages; ++s) { tc::mbar_init(tc::smem_u32(&full[s]), 1); tc::mbar_init(tc::smem_u32(&empty[s]), 1); }
-        for (int s = 0; s < 2; ++s) { tc::mbar_init(tc::smem_u32(&acc_full[s]), 1); tc::mbar_init(tc::smem_u32(&acc_empty[s]), 2 * kEpiWarps); }
+        for (int s = 0; s < kStages; ++s) { tc::mbar_init(tc::smem_u32(&full[s]), 1); tc::mbar_init(tc::smem_u32(&done[s]), 1); }
+        for (int s = 0; s < 2; ++s) tc::mbar_init(tc::smem_u32(&acc_empty[s]), 2 * kEpiWarps);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
@@ -121,10 +130,13 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
     const uint32_t tmem = tmem_base_s;
     volatile int *abort_flag = &abort_s;
 
-    if (warp == 0) {
-        if (lane == 0) {
+    // 384 threads start with 168 registers each; before any of them waits for another they are dealt
+    // out anew: 128 * 64 + 256 * 216 <= 384 * 168
+    if (warp < 4) {
+        tc::registers_down<64>();
+        if (warp == 0 && lane == 0) {
             const uint32_t full_lead = tc::cluster_addr(tc::smem_u32(full), 0);
-            const uint32_t empty0 = tc::smem_u32(empty), stage0 = tc::smem_u32(stages);
+            const uint32_t done0 = tc::smem_u32(done), stage0 = tc::smem_u32(stages);
             uint32_t s = 0, parity = 1;
             bool ok = true;
             for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
@@ -133,7 +145,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                 const int row0 = tm * 256 + (int)rank * 128;
                 const int col0 = p.up_row ? tn * 128 + (rank ? p.up_row : 0) : tn * 256 + (int)rank * 128;
                 for (int k = 0; k < p.k_blocks; ++k) {
-                    if (!tc::mbar_wait(empty0 + 8 * s, parity, abort_flag, &g_fp8_error, 1)) { ok = false; break; }
+                    if (!tc::mbar_wait(done0 + 8 * s, parity, abort_flag, &g_fp8_error, 1)) { ok = false; break; }
                     const uint32_t bar = full_lead + 8 * s, dst = stage0 + s * kStage;
                     if (rank == 0) tc::mbar_arrive_expect_tx(tc::smem_u32(&full[s]), 2 * kStage);
                     tc::load_pair(dst, &p.map_x, k * 128, row0, bar);
@@ -141,13 +153,9 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                     if (++s == kStages) { s = 0; parity ^= 1; }
                 }
             }
-        }
-    } else if (warp == 1) {
-        if (rank == 0 && lane == 0) {
+        } else if (warp == 1 && rank == 0 && lane == 0) {
             const uint32_t idesc = (1u << 4) | p.types | ((256u >> 3) << 17) | ((256u >> 4) << 24);
-            const uint32_t full0 = tc::smem_u32(full), empty0 = tc::smem_u32(empty);
-            const uint32_t empty0_peer = tc::cluster_addr(empty0, 1);
-            const uint32_t acc0 = tc::smem_u32(acc_full), acc0_peer = tc::cluster_addr(acc0, 1);
+            const uint32_t full0 = tc::smem_u32(full), done0 = tc::smem_u32(done), acc_empty0 = tc::smem_u32(acc_empty);
             const uint64_t da = tc::make_smem_desc(tc::smem_u32(stages), 16, 1024, 2);
             const uint64_t db = tc::make_smem_desc(tc::smem_u32(stages) + kStageA, 16, 1024, 2);
             uint32_t s = 0, parity = 0, g = 0;
@@ -155,27 +163,26 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
             for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
                 for (int k = 0; k < p.k_blocks; ++k, ++g) {
                     const uint32_t buf = g & 1;
-                    if (!tc::mbar_wait(tc::smem_u32(&acc_empty[buf]), ((g >> 1) & 1) ^ 1u, abort_flag, &g_fp8_error, 2) ||
-                        !tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_fp8_error, 3)) { ok = false; break; }
+                    if (!tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_fp8_error, 3) ||
+                        !tc::mbar_wait(acc_empty0 + 8 * buf, ((g >> 1) & 1) ^ 1u, abort_flag, &g_fp8_error, 2)) { ok = false; break; }
                     tc::fence_after();
                     const uint64_t a = da + (uint64_t)(s * kStage >> 4), b = db + (uint64_t)(s * kStage >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
                         tc::mma_pair_f8(tmem + buf * 256, a + 2 * kk, b + 2 * kk, idesc, kk ? 1u : 0u);
-                    tc::commit_pair(empty0 + 8 * s);
-                    tc::commit_pair(empty0_peer + 8 * s);
-                    tc::commit_pair(acc0 + 8 * buf);
-                    tc::commit_pair(acc0_peer + 8 * buf);
+                    tc::commit_both(done0 + 8 * s);
                     if (++s == kStages) { s = 0; parity ^= 1; }
                 }
             }
         }
     } else {
+        tc::registers_up<216>();
         // warp w: accumulator lanes 32 (w % 4) .. +31, columns 64 side .. +63 of either 128-column half, so
         // that a thread holds the gate and the up sum of its hidden columns
-        const int quarter = warp & 3, side = (warp - 2) >> 2;
-        const uint32_t lead_empty = tc::cluster_addr(tc::smem_u32(acc_empty), 0);
-        uint32_t g = 0;
+        const int quarter = warp & 3, side = (warp - 4) >> 2;
+        const uint32_t done0 = tc::smem_u32(done), lead_empty = tc::cluster_addr(tc::smem_u32(acc_empty), 0);
+        const uint32_t taddr0 = tmem + ((uint32_t)(quarter * 32) << 16) + side * 64;
+        uint32_t g = 0, s = 0, parity = 0;
         bool ok = true;
         for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
             int tm, tn;
@@ -184,41 +191,52 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
             const int wb0 = p.up_row ? tn : 2 * tn, wb1 = p.up_row ? p.up_row / 128 + tn : 2 * tn + 1;
             const float *xs = p.xs + (row < p.rows ? row : p.rows - 1) * p.ld_xs;
             const float *ws0 = p.ws + (long long)wb0 * p.ld_ws, *ws1 = p.ws + (long long)min(wb1, p.w_blocks - 1) * p.ld_ws;
-            float sum[4][32];
+            uint64_t sum[4][16];                                  // columns 32 j + 2 i, + 1
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int i = 0; i < 32; ++i) sum[j][i] = 0.f;
+                for (int i = 0; i < 16; ++i) sum[j][i] = 0ull;
+            float sx = __ldg(xs), s0 = __ldg(ws0), s1 = __ldg(ws1);
             for (int k = 0; k < p.k_blocks; ++k, ++g) {
-                const uint32_t buf = g & 1;
-                const float sx = __ldg(xs + k), f0 = sx * __ldg(ws0 + k), f1 = sx * __ldg(ws1 + k);
-                if (!tc::mbar_wait(tc::smem_u32(&acc_full[buf]), (g >> 1) & 1, abort_flag, &g_fp8_error, 4)) { ok = false; break; }
+                const uint32_t buf = g & 1, taddr = taddr0 + buf * 256;
+                const uint32_t f0 = __float_as_uint(sx * s0), f1 = __float_as_uint(sx * s1);
+                const uint64_t ff[2] = {tc::pair_of(f0, f0), tc::pair_of(f1, f1)};
+                if (k + 1 < p.k_blocks) { sx = __ldg(xs + k + 1); s0 = __ldg(ws0 + k + 1); s1 = __ldg(ws1 + k + 1); }
+                if (!tc::mbar_wait(done0 + 8 * s, parity, abort_flag, &g_fp8_error, 4)) { ok = false; break; }
                 tc::fence_after();
-                const uint32_t taddr = tmem + buf * 256 + ((uint32_t)(quarter * 32) << 16) + side * 64;
+                uint32_t r[2][32];
+                tc::ld32(taddr, r[0]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t r[32];
-                    tc::ld32(taddr + (j >> 1) * 128 + (j & 1) * 32, r);
                     tc::wait_ld();
-                    const float f = j < 2 ? f0 : f1;
+                    if (j < 3) tc::ld32(taddr + ((j + 1) >> 1) * 128 + ((j + 1) & 1) * 32, r[(j + 1) & 1]);
+                    else {
+                        tc::fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::arrive_relaxed(lead_empty + 8 * buf);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[j][i] = fmaf(__uint_as_float(r[i]), f, sum[j][i]);
+                    for (int i = 0; i < 16; ++i)
+                        sum[j][i] = tc::fma2(tc::pair_of(r[j & 1][2 * i], r[j & 1][2 * i + 1]), ff[j >> 1], sum[j][i]);
                 }
-                tc::fence_before();
-                __syncwarp();
-                if (lane == 0) tc::arrive_cluster(lead_empty + 8 * buf);
+                if (++s == kStages) { s = 0; parity ^= 1; }
             }
             if (!ok) break;
-            if (p.up_row) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < 4; ++j) {
+                if (j >= 2 && p.up_row) break;
+                float v[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[j][i] = silu(sum[j][i]) * sum[j + 2][i];
-                    store_row32(p, row, tn * 128 + side * 64 + j * 32, sum[j]);
+                for (int i = 0; i < 16; ++i) {
+                    v[2 * i] = tc::low_of(sum[j][i]);
+                    v[2 * i + 1] = tc::high_of(sum[j][i]);
+                    if (p.up_row) {
+                        v[2 * i] = silu(v[2 * i]) * tc::low_of(sum[(j + 2) & 3][i]);
+                        v[2 * i + 1] = silu(v[2 * i + 1]) * tc::high_of(sum[(j + 2) & 3][i]);
+                    }
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) store_row32(p, row, tn * 256 + (j >> 1) * 128 + side * 64 + (j & 1) * 32, sum[j]);
+                const int col = p.up_row ? tn * 128 + side * 64 + j * 32 : tn * 256 + (j >> 1) * 128 + side * 64 + (j & 1) * 32;
+                store_row32(p, row, col, v);
             }
         }
     }
@@ -278,7 +296,7 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     p.w_blocks = (out_features + 127) / 128;
     p.types = (x_type == MORTAR_E5M2 ? 1u << 7 : 0u) | (w_type == MORTAR_E5M2 ? 1u << 10 : 0u);
     p.out = out; p.ld_out = ld_out; p.out_dtype = out_dtype;
-    p.vec = !misaligned(out, 16) && (ld_out * e) % 16 == 0;
+    p.vec = !misaligned(out, 32) && (ld_out * e) % 32 == 0;
 
     static bool ready[64] = {false};
     int sms = 0;
