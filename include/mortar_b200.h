@@ -628,8 +628,8 @@ int mortar_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int6
 /* The gated feed-forward block before it is carved (morph/model/transformer.py:402-431):
  *   y = (silu(x Wg^T) * (x Wu^T)) Wd^T,  gate_up = [Wg; Wu] [2 d_ff][d_model], down [d_model][d_ff]
  * x, weights and results are bf16 or fp16 (dtype, one for all); sums are fp32; the hidden block and y
- * are rounded once each.  d_model and d_ff are multiples of 16, pointers 16-byte aligned, row strides
- * multiples of 8.
+ * are rounded once each.  d_model and d_ff are multiples of 16; x and the weights 16-byte aligned with row
+ * strides that are multiples of 8; what is written or kept 32-byte aligned, ldy a multiple of 16.
  *   hidden        device [rows][d_ff], written: the hidden block (scratch, and an input of the
  *                 backward call)
  *   gate_up_sums  device [rows][2 d_ff], written for the backward call, or NULL
@@ -639,8 +639,8 @@ int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64_t rows, co
                      void *hidden, void *gate_up_sums, void *y, int64_t ldy, void *stream);
 
 /* Gradients of mortar_mlp_dense from dy [rows][d_model], its inputs, `hidden` and `gate_up_sums`:
- * dx [rows][d_model], dgate_up [2 d_ff][d_model], ddown [d_model][d_ff], contiguous, of the same
- * type; each may be NULL.  `dgate_up_sums` [rows][2 d_ff] is scratch of that type. */
+ * dx [rows][d_model], dgate_up [2 d_ff][d_model], ddown [d_model][d_ff], contiguous, 32-byte aligned, of
+ * the same type; each may be NULL.  `dgate_up_sums` [rows][2 d_ff] is scratch of that type. */
 int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int32_t dtype,
                               int64_t rows, const void *gate_up, int64_t ld_gate_up, const void *down,
                               int64_t ld_down, int32_t d_model, int32_t d_ff, const void *hidden,

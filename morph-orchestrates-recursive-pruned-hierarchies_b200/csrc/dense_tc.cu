@@ -64,30 +64,31 @@ struct DenseParams {
     long long ld_gu;
 };
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + __expf(-g)); }
+// exp2-based exponential and an approximate quotient, off by 2^-22 (1 + |g|) at worst; the result is rounded to 16 bits
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
-// 32 accumulator columns -> 32 16-bit values of one row; n_left = columns of the row from col on
+// 32 accumulator columns -> 32 16-bit values of one row; n_left = columns of the row from there on (a multiple
+// of 16, as every width is), and 32 bytes at a time since every row starts on 32 bytes
 __device__ __forceinline__ void store32(void *base, long long idx, const float (&v)[32], int n_left, bool half) {
-    uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(base) + idx);
+    uint16_t *dst = reinterpret_cast<uint16_t *>(base) + idx;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (8 * j < n_left)
-            dst[j] = make_uint4(tc::pack16(v[8 * j], v[8 * j + 1], half), tc::pack16(v[8 * j + 2], v[8 * j + 3], half),
-                                tc::pack16(v[8 * j + 4], v[8 * j + 5], half), tc::pack16(v[8 * j + 6], v[8 * j + 7], half));
+    for (int j = 0; j < 2; ++j) {
+        if (16 * j >= n_left) break;
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = tc::pack16(v[16 * j + 2 * i], v[16 * j + 2 * i + 1], half);
+        tc::store_v8(dst + 16 * j, w);
+    }
 }
 
-__device__ __forceinline__ void load32(const void *base, long long idx, float (&v)[32], int n_left, bool half) {
-    const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(base) + idx);
+__device__ __forceinline__ void load32(const void *base, long long idx, uint32_t (&w)[16], int n_left) {
+    const uint16_t *src = reinterpret_cast<const uint16_t *>(base) + idx;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint4 w = 8 * j < n_left ? __ldg(src + j) : make_uint4(0, 0, 0, 0);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    for (int j = 0; j < 2; ++j) {
+        if (16 * j < n_left) tc::load_v8(src + 16 * j, &w[8 * j]);
+        else
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = tc::unpack16(ws[i], half);
-            v[8 * j + 2 * i] = f.x;
-            v[8 * j + 2 * i + 1] = f.y;
-        }
+            for (int i = 0; i < 8; ++i) w[8 * j + i] = 0u;
     }
 }
 
@@ -189,7 +190,6 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
             const uint32_t type = p.half ? 0u : (1u << 7) | (1u << 10);
             const uint32_t idesc0 = (1u << 4) | type | ((uint32_t)(kBN >> 3) << 17) | ((256u >> 4) << 24);
             const uint32_t full0 = tc::smem_u32(full), empty0 = tc::smem_u32(empty);
-            const uint32_t empty0_peer = tc::cluster_addr(empty0, 1);
             const uint32_t stage0 = tc::smem_u32(stages);
             uint32_t s = 0, parity = 0;
             int it = 0;
@@ -201,9 +201,8 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
                 tc::fence_after();
                 const uint32_t acc = tmem + buf * kBN;
                 const uint32_t idesc = idesc0 | ((uint32_t)q.a_mn << 15) | ((uint32_t)q.b_mn << 16);
-                // row-contiguous operand: 64 elements of k are one 128-byte row, 16 of them 32 bytes further;
-                // k-contiguous... the other order: one k is a 128-byte row of 64 rows, 16 of them 2048 bytes,
-                // the next 64 rows one 8 KB box further
+                // k contiguous: a row's 64 k are 128 bytes, 16 of them 32 bytes further.  Rows contiguous: one k is 128
+                // bytes (64 rows), 16 of them 2048 bytes, and the next 64 rows lie one 8 KB box further
                 const uint64_t da = tc::make_smem_desc(stage0, q.a_mn ? 8192 : 16, 1024, 2);
                 const uint64_t db = tc::make_smem_desc(stage0 + kStageA, q.b_mn ? 8192 : 16, 1024, 2);
                 const uint64_t step_a = q.a_mn ? 2048 >> 4 : 32 >> 4, step_b = q.b_mn ? 2048 >> 4 : 32 >> 4;
@@ -214,13 +213,11 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
                         tc::mma_pair_f16(acc, a + kk * step_a, b + kk * step_b, idesc, (k | kk) ? 1u : 0u);
-                    tc::commit_pair(empty0 + 8 * s);
-                    tc::commit_pair(empty0_peer + 8 * s);
+                    tc::commit_both(empty0 + 8 * s);
                     if (++s == kStages) { s = 0; parity ^= 1; }
                 }
                 if (!ok) break;
-                tc::commit_pair(tc::smem_u32(&acc_full[buf]));
-                tc::commit_pair(tc::cluster_addr(tc::smem_u32(&acc_full[buf]), 1));
+                tc::commit_both(tc::smem_u32(&acc_full[buf]));
             }
         }
     } else {
@@ -261,17 +258,22 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
                 }
             } else {
                 for (int c = side * (kBN / 2); c < (side + 1) * (kBN / 2); c += 32) {
+                    const int col = t.tn * kBN + c;
+                    uint32_t gw[16], uw[16];
+                    if (row < q.m) {
+                        load32(p.gu, row * p.ld_gu + col, gw, q.n - col);
+                        load32(p.gu, row * p.ld_gu + p.d_ff + col, uw, q.n - col);
+                    }
                     float dh[32];
                     acc32(taddr + c, dh);
-                    const int col = t.tn * kBN + c;
                     if (row < q.m) {
                         float g[32], u[32];
-                        load32(p.gu, row * p.ld_gu + col, g, q.n - col, half);
-                        load32(p.gu, row * p.ld_gu + p.d_ff + col, u, q.n - col, half);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            const float s = sigmoid(g[i]), a = g[i] * s, d = dh[i];
-                            g[i] = d * u[i] * (s + a * (1.f - s));
+                            const float2 g2 = tc::unpack16(gw[i >> 1], half), u2 = tc::unpack16(uw[i >> 1], half);
+                            const float gv = (i & 1) ? g2.y : g2.x, uv = (i & 1) ? u2.y : u2.x;
+                            const float s = sigmoid(gv), a = gv * s, d = dh[i];
+                            g[i] = d * uv * (s + a * (1.f - s));
                             u[i] = d * a;
                         }
                         store32(q.out, row * q.ld_out + col, g, q.n - col, half);
@@ -281,7 +283,7 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
             }
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) tc::arrive_cluster(tc::cluster_addr(tc::smem_u32(&acc_empty[buf]), 0));
+            if (lane == 0) tc::arrive_relaxed(tc::cluster_addr(tc::smem_u32(&acc_empty[buf]), 0));
         }
     }
 
@@ -296,7 +298,7 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-bool misaligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+bool misaligned(const void *p, size_t a = 16) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
 
 // Adds C[m][n] = sum_k A[m][k] B[n][k] to a launch.  `a` is [m][k] (row stride lda) or, with a_mn, [k][m];
 // `b` is [n][k] or, with b_mn, [k][n].  For kSwiglu n counts hidden columns and b has 2 n rows.
@@ -353,8 +355,8 @@ extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64
     int rc = check_shape(dtype, rows, d_model, d_ff);
     if (rc != MORTAR_OK) return rc;
     if (ldx < d_model || ld_gate_up < d_model || ld_down < d_ff || ldy < d_model) return MORTAR_ERR_SHAPE;
-    if (misaligned(x) || misaligned(gate_up) || misaligned(down) || misaligned(hidden) || misaligned(gate_up_sums) ||
-        misaligned(y) || ldx % 8 || ld_gate_up % 8 || ld_down % 8 || ldy % 8)
+    if (misaligned(x) || misaligned(gate_up) || misaligned(down) || misaligned(hidden, 32) || misaligned(gate_up_sums, 32) ||
+        misaligned(y, 32) || ldx % 8 || ld_gate_up % 8 || ld_down % 8 || ldy % 16)
         return MORTAR_ERR_ALIGN;
     if (rows == 0) return MORTAR_OK;
     cudaStream_t st = (cudaStream_t)stream;
@@ -381,9 +383,9 @@ extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const voi
     int rc = check_shape(dtype, rows, d_model, d_ff);
     if (rc != MORTAR_OK) return rc;
     if (lddy < d_model || ldx < d_model || ld_gate_up < d_model || ld_down < d_ff) return MORTAR_ERR_SHAPE;
-    if (misaligned(dy) || misaligned(x) || misaligned(gate_up) || misaligned(down) || misaligned(hidden) ||
-        misaligned(gate_up_sums) || misaligned(dgate_up_sums) || misaligned(dx) || misaligned(dgate_up) ||
-        misaligned(ddown) || lddy % 8 || ldx % 8 || ld_gate_up % 8 || ld_down % 8)
+    if (misaligned(dy) || misaligned(x) || misaligned(gate_up) || misaligned(down) || misaligned(hidden, 32) ||
+        misaligned(gate_up_sums, 32) || misaligned(dgate_up_sums, 32) || misaligned(dx, 32) || misaligned(dgate_up, 32) ||
+        misaligned(ddown, 32) || lddy % 8 || ldx % 8 || ld_gate_up % 8 || ld_down % 8)
         return MORTAR_ERR_ALIGN;
     cudaStream_t st = (cudaStream_t)stream;
     if (rows == 0) {
