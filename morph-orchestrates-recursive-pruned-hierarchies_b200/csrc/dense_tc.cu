@@ -27,9 +27,9 @@
 namespace {
 
 constexpr int kBN = 256;                         // accumulator columns of a tile
-constexpr int kStages = 6;
-constexpr int kStageA = 128 * 128;               // this CTA's 128 rows, 64 elements of 2 bytes each
-constexpr int kStageB = kBN / 2 * 128;
+constexpr int kStages = 3;
+constexpr int kStageA = 128 * 256;               // this CTA's 128 rows, 128 elements of 2 bytes each
+constexpr int kStageB = kBN / 2 * 256;
 constexpr int kStage = kStageA + kStageB;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
@@ -48,7 +48,7 @@ struct Problem {
     long long m;             // rows of C
     int n;                   // columns of C (hidden columns for kSwiglu)
     int tiles_m, tiles_n;
-    int k_steps;             // 64-wide steps of the reduction
+    int k_steps;             // 128-wide steps of the reduction
     int a_mn, b_mn;          // 1: the operand's row index is the contiguous one in memory
     int first_item;
 };
@@ -165,18 +165,21 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
                     if (!tc::mbar_wait(empty0 + 8 * s, parity, abort_flag, &g_dense_error, 1)) { ok = false; break; }
                     const uint32_t bar = full_lead + 8 * s, dst = stage0 + s * kStage;
                     if (rank == 0) tc::mbar_arrive_expect_tx(tc::smem_u32(&full[s]), 2 * kStage);
+                    // rows contiguous in memory: boxes of 64 rows x 128 k; k contiguous: 128 rows x 64 k
                     if (q.a_mn) {
-                        tc::load_pair(dst, ma, row0, k * 64, bar);
-                        tc::load_pair(dst + 8192, ma, row0 + 64, k * 64, bar);
+                        tc::load_pair(dst, ma, row0, k * 128, bar);
+                        tc::load_pair(dst + 16384, ma, row0 + 64, k * 128, bar);
                     } else {
-                        tc::load_pair(dst, ma, k * 64, row0, bar);
+                        tc::load_pair(dst, ma, k * 128, row0, bar);
+                        tc::load_pair(dst + 16384, ma, k * 128 + 64, row0, bar);
                     }
                     if (q.b_mn) {
 #pragma unroll
                         for (int i = 0; i < kBN / 128; ++i)
-                            tc::load_pair(dst + kStageA + i * 8192, mb, col0 + i * 64, k * 64, bar);
+                            tc::load_pair(dst + kStageA + i * 16384, mb, col0 + i * 64, k * 128, bar);
                     } else {
-                        tc::load_pair(dst + kStageA, mb, k * 64, col0, bar);
+                        tc::load_pair(dst + kStageA, mb, k * 128, col0, bar);
+                        tc::load_pair(dst + kStageA + kStageB / 2, mb, k * 128 + 64, col0, bar);
                     }
                     if (++s == kStages) { s = 0; parity ^= 1; }
                 }
@@ -193,28 +196,27 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
             const uint32_t stage0 = tc::smem_u32(stages);
             uint32_t s = 0, parity = 0;
             int it = 0;
-            bool ok = true;
+            bool ok = true, ready = tc::mbar_try_wait(full0, 0);
             for (int item = cluster_id; item < p.n_items && ok; item += n_clusters, ++it) {
                 const Problem &q = p.prob[tile_of(p, item).p];
-                const int buf = it & 1;
-                if (!tc::mbar_wait(tc::smem_u32(&acc_empty[buf]), ((it >> 1) & 1) ^ 1u, abort_flag, &g_dense_error, 2)) break;
-                tc::fence_after();
+                const int buf = it & 1, k_steps = q.k_steps;
                 const uint32_t acc = tmem + buf * kBN;
                 const uint32_t idesc = idesc0 | ((uint32_t)q.a_mn << 15) | ((uint32_t)q.b_mn << 16);
-                // k contiguous: a row's 64 k are 128 bytes, 16 of them 32 bytes further.  Rows contiguous: one k is 128
-                // bytes (64 rows), 16 of them 2048 bytes, and the next 64 rows lie one 8 KB box further
-                const uint64_t da = tc::make_smem_desc(stage0, q.a_mn ? 8192 : 16, 1024, 2);
-                const uint64_t db = tc::make_smem_desc(stage0 + kStageA, q.b_mn ? 8192 : 16, 1024, 2);
+                // k contiguous: a row's 64 k are 128 bytes, 16 of them 32 bytes further, the next 64 k one box further.
+                // Rows contiguous: one k is 128 bytes (64 rows), 16 of them 2048 bytes, the next 64 rows one box further
+                const uint64_t da = tc::make_smem_desc(stage0, q.a_mn ? 16384 : 16, 1024, 2);
+                const uint64_t db = tc::make_smem_desc(stage0 + kStageA, q.b_mn ? 16384 : 16, 1024, 2);
                 const uint64_t step_a = q.a_mn ? 2048 >> 4 : 32 >> 4, step_b = q.b_mn ? 2048 >> 4 : 32 >> 4;
-                for (int k = 0; k < q.k_steps; ++k) {
-                    if (!tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_dense_error, 3)) { ok = false; break; }
-                    tc::fence_after();
-                    const uint64_t a = da + (uint64_t)(s * kStage >> 4), b = db + (uint64_t)(s * kStage >> 4);
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        tc::mma_pair_f16(acc, a + kk * step_a, b + kk * step_b, idesc, (k | kk) ? 1u : 0u);
-                    tc::commit_both(empty0 + 8 * s);
+                const uint64_t half_a = q.a_mn ? 8192 >> 4 : 16384 >> 4, half_b = q.b_mn ? 8192 >> 4 : (uint64_t)(kStageB / 2) >> 4;
+                if (!tc::mbar_wait(tc::smem_u32(&acc_empty[buf]), ((it >> 1) & 1) ^ 1u, abort_flag, &g_dense_error, 2)) break;
+                tc::fence_after();
+                for (int k = 0; k < k_steps; ++k) {
+                    if (!ready && !tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_dense_error, 3)) { ok = false; break; }
+                    const uint64_t at = (uint64_t)(s * (kStage >> 4));
+                    const uint32_t bar = empty0 + 8 * s;
                     if (++s == kStages) { s = 0; parity ^= 1; }
+                    ready = tc::poll_mma8_f16(full0 + 8 * s, parity, acc, da + at, db + at, step_a, step_b, half_a, half_b, idesc, k);
+                    tc::commit_both(bar);
                 }
                 if (!ok) break;
                 tc::commit_both(tc::smem_u32(&acc_full[buf]));
@@ -307,16 +309,16 @@ int add_problem(DenseParams &p, int epi, const void *a, int64_t lda, bool a_mn, 
     const int i = p.n_problems;
     Problem &q = p.prob[i];
     const int64_t b_rows = epi == kSwiglu ? 2 * n : n, tile_n = epi == kSwiglu ? kBN / 2 : kBN;
-    int rc = a_mn ? tc::encode_bf16_2d(&p.map_a[i], a, m, k, lda, 64, 64)
+    int rc = a_mn ? tc::encode_bf16_2d(&p.map_a[i], a, m, k, lda, 64, 128)
                   : tc::encode_bf16_2d(&p.map_a[i], a, k, m, lda, 64, 128);
     if (rc != MORTAR_OK) return rc;
-    rc = b_mn ? tc::encode_bf16_2d(&p.map_b[i], b, b_rows, k, ldb, 64, 64)
+    rc = b_mn ? tc::encode_bf16_2d(&p.map_b[i], b, b_rows, k, ldb, 64, 128)
               : tc::encode_bf16_2d(&p.map_b[i], b, k, b_rows, ldb, 64, kBN / 2);
     if (rc != MORTAR_OK) return rc;
     const int64_t tm = (m + 255) / 256, tn = (n + tile_n - 1) / tile_n;
     if (tm * tn + p.n_items > 0x3fffffff) return MORTAR_ERR_CAPACITY;
     q.out = out; q.ld_out = ld_out; q.m = m; q.n = (int)n;
-    q.tiles_m = (int)tm; q.tiles_n = (int)tn; q.k_steps = (int)((k + 63) / 64);
+    q.tiles_m = (int)tm; q.tiles_n = (int)tn; q.k_steps = (int)((k + 127) / 128);
     q.a_mn = a_mn; q.b_mn = b_mn; q.first_item = p.n_items;
     p.n_items += (int)(tm * tn);
     ++p.n_problems;
@@ -360,6 +362,8 @@ extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64
         return MORTAR_ERR_ALIGN;
     if (rows == 0) return MORTAR_OK;
     cudaStream_t st = (cudaStream_t)stream;
+    rc = tc::bind_context();
+    if (rc != MORTAR_OK) return rc;
     alignas(64) DenseParams p = {};
     p.half = dtype == MORTAR_F16;
     p.d_ff = d_ff;
@@ -393,6 +397,8 @@ extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const voi
         if (ddown) MORTAR_CUDA_CHECK(cudaMemsetAsync(ddown, 0, (size_t)2 * d_ff * d_model, st));
         return MORTAR_OK;
     }
+    rc = tc::bind_context();
+    if (rc != MORTAR_OK) return rc;
     const int64_t f2 = 2LL * d_ff;
     if (dx || dgate_up) {
         alignas(64) DenseParams p = {};

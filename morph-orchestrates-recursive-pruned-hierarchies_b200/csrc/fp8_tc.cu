@@ -159,19 +159,18 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
             const uint64_t da = tc::make_smem_desc(tc::smem_u32(stages), 16, 1024, 2);
             const uint64_t db = tc::make_smem_desc(tc::smem_u32(stages) + kStageA, 16, 1024, 2);
             uint32_t s = 0, parity = 0, g = 0;
-            bool ok = true;
+            bool ok = true, ready = tc::mbar_try_wait(full0, 0);
             for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
                 for (int k = 0; k < p.k_blocks; ++k, ++g) {
                     const uint32_t buf = g & 1;
-                    if (!tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_fp8_error, 3) ||
+                    if ((!ready && !tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_fp8_error, 3)) ||
                         !tc::mbar_wait(acc_empty0 + 8 * buf, ((g >> 1) & 1) ^ 1u, abort_flag, &g_fp8_error, 2)) { ok = false; break; }
                     tc::fence_after();
-                    const uint64_t a = da + (uint64_t)(s * kStage >> 4), b = db + (uint64_t)(s * kStage >> 4);
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        tc::mma_pair_f8(tmem + buf * 256, a + 2 * kk, b + 2 * kk, idesc, kk ? 1u : 0u);
-                    tc::commit_both(done0 + 8 * s);
+                    const uint64_t at = (uint64_t)(s * (kStage >> 4));
+                    const uint32_t bar = done0 + 8 * s;
                     if (++s == kStages) { s = 0; parity ^= 1; }
+                    ready = tc::poll_mma4_f8(full0 + 8 * s, parity, tmem + buf * 256, da + at, db + at, idesc);
+                    tc::commit_both(bar);
                 }
             }
         }
@@ -278,8 +277,10 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     if (rows == 0) return MORTAR_OK;
     cudaStream_t st = (cudaStream_t)stream;
 
+    int rc = tc::bind_context();
+    if (rc != MORTAR_OK) return rc;
     alignas(64) Fp8Params p = {};
-    int rc = tc::encode_u8_2d(&p.map_x, x, in_features, rows, ldx, 128);
+    rc = tc::encode_u8_2d(&p.map_x, x, in_features, rows, ldx, 128);
     if (rc != MORTAR_OK) return rc;
     rc = tc::encode_u8_2d(&p.map_w, w, in_features, out_features, ldw, 128);
     if (rc != MORTAR_OK) return rc;

@@ -19,9 +19,6 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void arrive_cluster(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
-}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
@@ -35,11 +32,7 @@ __device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap *map, 
         "[%0], [%1, {%2, %3}], [%4];\n"
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
 }
-__device__ __forceinline__ void commit_pair(uint32_t cluster_bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
-                 ::"r"(cluster_bar) : "memory");
-}
-// the same on the barrier at this offset in both CTAs of the pair
+// one arrival, when the MMAs issued so far have ended, at the barrier of this offset in both CTAs of the pair
 __device__ __forceinline__ void commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
                  ::"r"(bar), "h"((uint16_t)3) : "memory");
@@ -74,17 +67,60 @@ __device__ __forceinline__ void load_v8(const void *p, uint32_t *w) {
 }
 template <int REGS> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS)); }
 template <int REGS> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS)); }
-__device__ __forceinline__ void mma_pair_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// A poll of the barrier that the issuing thread needs next, and the eight (or four) MMAs of a stage as
+// one instruction sequence: the poll's result is read after the MMAs have been issued, so its latency
+// runs under them.  Descriptors advance by step_a / step_b from MMA to MMA, and from the fourth to the
+// fifth so that the fifth starts half_a / half_b after the first.  `acc`: whether the first MMA adds
+// to what the accumulator holds.  Returns whether the polled phase had completed.
+__device__ __forceinline__ bool poll_mma8_f16(uint32_t bar, uint32_t parity, uint32_t d, uint64_t a, uint64_t b,
+                                              uint64_t step_a, uint64_t step_b, uint64_t half_a, uint64_t half_b,
+                                              uint32_t idesc, uint32_t acc) {
+    uint32_t ready;
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+        "{\n.reg .pred q, p0, p1;\n.reg .b64 x, y, x2, y2;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n"
+        "setp.ne.b32 p0, %11, 0;\nsetp.eq.u32 p1, 1, 1;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%3], %4, %5, %10, p0;\n"
+        "add.s64 x, %4, %6;\nadd.s64 y, %5, %7;\nadd.s64 x2, %4, %8;\nadd.s64 y2, %5, %9;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%3], x, y, %10, p1;\n"
+        "add.s64 x, x, %6;\nadd.s64 y, y, %7;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%3], x, y, %10, p1;\n"
+        "add.s64 x, x, %6;\nadd.s64 y, y, %7;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%3], x, y, %10, p1;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%3], x2, y2, %10, p1;\n"
+        "add.s64 x2, x2, %6;\nadd.s64 y2, y2, %7;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%3], x2, y2, %10, p1;\n"
+        "add.s64 x2, x2, %6;\nadd.s64 y2, y2, %7;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%3], x2, y2, %10, p1;\n"
+        "add.s64 x2, x2, %6;\nadd.s64 y2, y2, %7;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%3], x2, y2, %10, p1;\n"
+        "selp.b32 %0, 1, 0, q;\n}\n"
+        : "=r"(ready)
+        : "r"(bar), "r"(parity), "r"(d), "l"(a), "l"(b), "l"(step_a), "l"(step_b), "l"(half_a), "l"(half_b), "r"(idesc),
+          "r"(acc)
+        : "memory");
+    return ready != 0;
 }
-__device__ __forceinline__ void mma_pair_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Four 8-bit MMAs (K = 32 each, 32 bytes apart) into a fresh accumulator.
+__device__ __forceinline__ bool poll_mma4_f8(uint32_t bar, uint32_t parity, uint32_t d, uint64_t a, uint64_t b,
+                                             uint32_t idesc) {
+    uint32_t ready;
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+        "{\n.reg .pred q, p0, p1;\n.reg .b64 x, y;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n"
+        "setp.ne.u32 p0, 1, 1;\nsetp.eq.u32 p1, 1, 1;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%3], %4, %5, %6, p0;\n"
+        "add.s64 x, %4, 2;\nadd.s64 y, %5, 2;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%3], x, y, %6, p1;\n"
+        "add.s64 x, x, 2;\nadd.s64 y, y, 2;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%3], x, y, %6, p1;\n"
+        "add.s64 x, x, 2;\nadd.s64 y, y, 2;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%3], x, y, %6, p1;\n"
+        "selp.b32 %0, 1, 0, q;\n}\n"
+        : "=r"(ready)
+        : "r"(bar), "r"(parity), "r"(d), "l"(a), "l"(b), "r"(idesc)
+        : "memory");
+    return ready != 0;
 }
 
 // 32 accumulator columns of this thread's tensor-memory lane; `wait_ld` before the registers are read
@@ -139,6 +175,16 @@ inline int encode_u8_2d(CUtensorMap *map, const void *base, int64_t cols, int64_
         mortar_set_cuda_error("cuTensorMapEncodeTiled", "failed to encode a tensor map");
         return MORTAR_ERR_CUDA;
     }
+    return MORTAR_OK;
+}
+
+// Makes the current device's context current to the calling thread.  Encoding a tensor map is a driver
+// call and fails in a thread that has made no runtime call that needs a context yet, as an autograd
+// thread whose allocations all come from a cache.
+inline int bind_context() {
+    int dev = 0;
+    MORTAR_CUDA_CHECK(cudaGetDevice(&dev));
+    MORTAR_CUDA_CHECK(cudaSetDevice(dev));
     return MORTAR_OK;
 }
 
