@@ -202,23 +202,25 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                 const uint64_t ff[2] = {tc::pair_of(f0, f0), tc::pair_of(f1, f1)};
                 if (k + 1 < p.k_blocks) { sx = __ldg(xs + k + 1); s0 = __ldg(ws0 + k + 1); s1 = __ldg(ws1 + k + 1); }
                 if (!tc::mbar_wait(done0 + 8 * s, parity, abort_flag, &g_fp8_error, 4)) { ok = false; break; }
+                if (++s == kStages) { s = 0; parity ^= 1; }
                 tc::fence_after();
-                uint32_t r[2][32];
-                tc::ld32(taddr, r[0]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t r[2][32];
+                    tc::ld32(taddr + h * 128, r[0]);
+                    tc::ld32(taddr + h * 128 + 32, r[1]);
                     tc::wait_ld();
-                    if (j < 3) tc::ld32(taddr + ((j + 1) >> 1) * 128 + ((j + 1) & 1) * 32, r[(j + 1) & 1]);
-                    else {
+                    if (h == 1) {
                         tc::fence_before();
                         __syncwarp();
                         if (lane == 0) tc::arrive_relaxed(lead_empty + 8 * buf);
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        sum[j][i] = tc::fma2(tc::pair_of(r[j & 1][2 * i], r[j & 1][2 * i + 1]), ff[j >> 1], sum[j][i]);
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            sum[2 * h + j][i] = tc::fma2(tc::pair_of(r[j][2 * i], r[j][2 * i + 1]), ff[h], sum[2 * h + j][i]);
                 }
-                if (++s == kStages) { s = 0; parity ^= 1; }
             }
             if (!ok) break;
 #pragma unroll
