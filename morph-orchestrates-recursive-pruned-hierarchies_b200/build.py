@@ -14,7 +14,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libmortar_b200.so")
 SOURCES = ["host_pack.cpp", "prefill_sched.cpp", "stream_kernels.cu", "prefill_tc.cu", "stack_decode.cu",
            "router.cu", "backward.cu", "backward_tc.cu", "gemv_tc.cu", "layer_norm.cu", "dense_tc.cu", "fp8_quant.cu",
-           "fp8_tc.cu"]
+           "fp8_tc.cu", "dense_small.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,30 @@
+// Entry of the kernels for a few tokens (dense_small.cu): C[m][n] = sum_k A[m][k] W[n][k], plain or with the
+// gate of the two halves of n applied, for 16-bit operands and for 8-bit ones with block scales.
+#pragma once
+#include <cuda_runtime.h>
+#include <cstdint>
+
+namespace small {
+
+constexpr int kMaxRows = 32;
+
+struct Params {
+    const uint8_t *x, *w;            // rows of bytes
+    long long ldx, ldw;              // bytes
+    int rows;
+    int n;                           // output columns (hidden columns with the gate)
+    int up_row;                      // 0, or the first up row of w
+    int k_bytes;
+    const float *xs, *ws;            // 8-bit: block scales
+    long long ld_xs, ld_ws;
+    void *out;
+    long long ld_out;                // elements
+    int out_dtype;
+    int after_previous;              // x comes from the kernel before in the stream: weights are fetched first
+    int x_dtype, w_dtype;
+};
+
+// Enqueues one product; `sms` = SMs of the device.
+int launch(const Params &p, int sms, cudaStream_t st);
+
+}  // namespace small

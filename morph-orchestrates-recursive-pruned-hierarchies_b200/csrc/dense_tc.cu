@@ -22,6 +22,7 @@
 #include <cstdint>
 #include <mutex>
 #include "common.h"
+#include "dense_small.cuh"
 #include "tc_pair.cuh"
 
 namespace {
@@ -362,6 +363,21 @@ extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64
         return MORTAR_ERR_ALIGN;
     if (rows == 0) return MORTAR_OK;
     cudaStream_t st = (cudaStream_t)stream;
+    if (rows <= small::kMaxRows && !gate_up_sums) {
+        int sms = 0;
+        rc = tc::sm_count(&sms);
+        if (rc != MORTAR_OK) return rc;
+        small::Params q = {};
+        q.x = (const uint8_t *)x; q.ldx = 2 * ldx; q.w = (const uint8_t *)gate_up; q.ldw = 2 * ld_gate_up;
+        q.rows = (int)rows; q.n = d_ff; q.up_row = d_ff; q.k_bytes = 2 * d_model;
+        q.out = hidden; q.ld_out = d_ff; q.out_dtype = q.x_dtype = q.w_dtype = dtype;
+        rc = small::launch(q, sms, st);
+        if (rc != MORTAR_OK) return rc;
+        q.x = (const uint8_t *)hidden; q.ldx = 2LL * d_ff; q.w = (const uint8_t *)down; q.ldw = 2 * ld_down;
+        q.n = d_model; q.up_row = 0; q.k_bytes = 2 * d_ff;
+        q.out = y; q.ld_out = ldy; q.after_previous = 1;
+        return small::launch(q, sms, st);
+    }
     rc = tc::bind_context();
     if (rc != MORTAR_OK) return rc;
     alignas(64) DenseParams p = {};

@@ -18,6 +18,7 @@
 #include <cstdint>
 #include <mutex>
 #include "common.h"
+#include "dense_small.cuh"
 #include "tc_pair.cuh"
 
 namespace {
@@ -279,7 +280,19 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     if (rows == 0) return MORTAR_OK;
     cudaStream_t st = (cudaStream_t)stream;
 
-    int rc = tc::bind_context();
+    int sms = 0;
+    int rc = tc::sm_count(&sms);
+    if (rc != MORTAR_OK) return rc;
+    if (rows <= small::kMaxRows) {
+        small::Params q = {};
+        q.x = (const uint8_t *)x; q.ldx = ldx; q.w = (const uint8_t *)w; q.ldw = ldw;
+        q.rows = (int)rows; q.n = gated ? out_features / 2 : out_features; q.up_row = gated ? out_features / 2 : 0;
+        q.k_bytes = in_features;
+        q.xs = x_scale; q.ws = w_scale; q.ld_xs = ld_x_scale; q.ld_ws = ld_w_scale;
+        q.out = out; q.ld_out = ld_out; q.out_dtype = out_dtype; q.x_dtype = x_type; q.w_dtype = w_type;
+        return small::launch(q, sms, st);
+    }
+    rc = tc::bind_context();
     if (rc != MORTAR_OK) return rc;
     alignas(64) Fp8Params p = {};
     rc = tc::encode_u8_2d(&p.map_x, x, in_features, rows, ldx, 128);
@@ -302,10 +315,7 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     p.vec = !misaligned(out, 32) && (ld_out * e) % 32 == 0;
 
     static bool ready[64] = {false};
-    int sms = 0;
     rc = tc::allow_smem(fp8_pair_kernel, kSmem, ready, g_fp8_mutex, nullptr);
-    if (rc != MORTAR_OK) return rc;
-    rc = tc::sm_count(&sms);
     if (rc != MORTAR_OK) return rc;
     const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
     fp8_pair_kernel<<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
