@@ -636,7 +636,12 @@ int mortar_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int6
  * Bounded in-kernel waits report through mortar_dense_error. */
 int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64_t rows, const void *gate_up,
                      int64_t ld_gate_up, const void *down, int64_t ld_down, int32_t d_model, int32_t d_ff,
-                     void *hidden, void *gate_up_sums, void *y, int64_t ldy, void *stream);
+                     void *hidden, void *gate_up_sums, void *y, int64_t ldy, float *scratch,
+                     int64_t scratch_floats, void *stream);
+/* fp32 values the call needs as scratch (32-byte aligned; 0 = none, negative = error): the parts of
+ * reductions that are cut where there are few tiles, added in order by a launch of their own.
+ * keep_sums: whether gate_up_sums is given. */
+int64_t mortar_mlp_dense_scratch_floats(int64_t rows, int32_t d_model, int32_t d_ff, int32_t keep_sums);
 
 /* Gradients of mortar_mlp_dense from dy [rows][d_model], its inputs, `hidden` and `gate_up_sums`:
  * dx [rows][d_model], dgate_up [2 d_ff][d_model], ddown [d_model][d_ff], contiguous, 32-byte aligned, of
@@ -645,7 +650,10 @@ int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const void *x, int64
                               int64_t rows, const void *gate_up, int64_t ld_gate_up, const void *down,
                               int64_t ld_down, int32_t d_model, int32_t d_ff, const void *hidden,
                               const void *gate_up_sums, void *dgate_up_sums, void *dx, void *dgate_up,
-                              void *ddown, void *stream);
+                              void *ddown, float *scratch, int64_t scratch_floats, void *stream);
+int64_t mortar_mlp_dense_backward_scratch_floats(int64_t rows, int32_t d_model, int32_t d_ff,
+                                                 int32_t want_dx, int32_t want_dgate_up,
+                                                 int32_t want_ddown);
 /* First error recorded by the kernels of the two calls above: 0 = none, else the waiting role.
  * Synchronises. */
 int mortar_dense_error(int32_t *code, int32_t reset);

@@ -128,9 +128,11 @@ _SIGNATURES = {
     "mortar_layer_norm_backward": (C.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _i64, _vp, _vp,
                                              _vp, _i64, _vp]),
     "mortar_mlp_dense": (C.c_int, [_vp, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i64,
-                                   _vp]),
+                                   _vp, _i64, _vp]),
+    "mortar_mlp_dense_scratch_floats": (_i64, [_i64, _i32, _i32, _i32]),
     "mortar_mlp_dense_backward": (C.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp,
-                                            _vp, _vp, _vp, _vp, _vp, _vp]),
+                                            _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mortar_mlp_dense_backward_scratch_floats": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "mortar_dense_error": (C.c_int, [_vp, _i32]),
     "mortar_quantize_fp8": (C.c_int, [_vp, _i32, _i64, _i64, _i32, _i32, _vp, _i32, _i64, _vp, _vp]),
     "mortar_dequantize_fp8": (C.c_int, [_vp, _i32, _i64, _vp, _i64, _i32, _i32, _vp, _i32, _i64, _vp]),

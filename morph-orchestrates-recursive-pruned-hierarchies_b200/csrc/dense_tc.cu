@@ -52,6 +52,8 @@ struct Problem {
     int k_steps;             // 128-wide steps of the reduction
     int a_mn, b_mn;          // 1: the operand's row index is the contiguous one in memory
     int first_item;
+    int splits;              // parts of the reduction, an item each (kStore only)
+    float *partial;          // splits > 1: fp32 [splits][m][n] instead of `out`
 };
 
 struct DenseParams {
@@ -82,6 +84,17 @@ __device__ __forceinline__ void store32(void *base, long long idx, const float (
     }
 }
 
+__device__ __forceinline__ void store32_f32(float *dst, const float (&v)[32], int n_left) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (8 * j >= n_left) break;
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * j + i]);
+        tc::store_v8(dst + 8 * j, w);
+    }
+}
+
 __device__ __forceinline__ void load32(const void *base, long long idx, uint32_t (&w)[16], int n_left) {
     const uint16_t *src = reinterpret_cast<const uint16_t *>(base) + idx;
 #pragma unroll
@@ -101,7 +114,7 @@ __device__ __forceinline__ void acc32(uint32_t taddr, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-struct TileId { int p, tm, tn; };
+struct TileId { int p, tm, tn, split, k_begin, k_end; };
 
 // Items walk a problem's tiles in bands of 8 tile rows, column by column, so that the clusters at work
 // share few A and B panels.
@@ -110,7 +123,15 @@ __device__ __forceinline__ TileId tile_of(const DenseParams &p, int item) {
     t.p = 0;
     while (t.p + 1 < p.n_problems && item >= p.prob[t.p + 1].first_item) ++t.p;
     const Problem &q = p.prob[t.p];
-    const int i = item - q.first_item;
+    int i = item - q.first_item;
+    t.split = q.splits > 1 ? i % q.splits : 0;
+    t.k_begin = 0;
+    t.k_end = q.k_steps;
+    if (q.splits > 1) {
+        i /= q.splits;
+        t.k_begin = (int)((long long)q.k_steps * t.split / q.splits);
+        t.k_end = (int)((long long)q.k_steps * (t.split + 1) / q.splits);
+    }
     const int band = i / (8 * q.tiles_n), r = i - band * 8 * q.tiles_n;
     const int h = min(8, q.tiles_m - band * 8);
     t.tn = r / h;
@@ -162,7 +183,7 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
                 const CUtensorMap *ma = &p.map_a[t.p], *mb = &p.map_b[t.p];
                 const int row0 = t.tm * 256 + (int)rank * 128;
                 const int col0 = EPI == kSwiglu ? t.tn * (kBN / 2) + (rank ? p.d_ff : 0) : t.tn * kBN + (int)rank * (kBN / 2);
-                for (int k = 0; k < q.k_steps; ++k) {
+                for (int k = t.k_begin; k < t.k_end; ++k) {
                     if (!tc::mbar_wait(empty0 + 8 * s, parity, abort_flag, &g_dense_error, 1)) { ok = false; break; }
                     const uint32_t bar = full_lead + 8 * s, dst = stage0 + s * kStage;
                     if (rank == 0) tc::mbar_arrive_expect_tx(tc::smem_u32(&full[s]), 2 * kStage);
@@ -199,8 +220,9 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
             int it = 0;
             bool ok = true, ready = tc::mbar_try_wait(full0, 0);
             for (int item = cluster_id; item < p.n_items && ok; item += n_clusters, ++it) {
-                const Problem &q = p.prob[tile_of(p, item).p];
-                const int buf = it & 1, k_steps = q.k_steps;
+                const TileId t = tile_of(p, item);
+                const Problem &q = p.prob[t.p];
+                const int buf = it & 1, k_steps = t.k_end - t.k_begin;
                 const uint32_t acc = tmem + buf * kBN;
                 const uint32_t idesc = idesc0 | ((uint32_t)q.a_mn << 15) | ((uint32_t)q.b_mn << 16);
                 // k contiguous: a row's 64 k are 128 bytes, 16 of them 32 bytes further, the next 64 k one box further.
@@ -241,7 +263,9 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
                     float v[32];
                     acc32(taddr + c, v);
                     const int col = t.tn * kBN + c;
-                    if (row < q.m) store32(q.out, row * q.ld_out + col, v, q.n - col, half);
+                    if (row >= q.m) continue;
+                    if (q.splits == 1) store32(q.out, row * q.ld_out + col, v, q.n - col, half);
+                    else store32_f32(q.partial + ((long long)t.split * q.m + row) * q.n + col, v, q.n - col);
                 }
             } else if (EPI == kSwiglu) {
                 for (int c = side * (kBN / 4); c < (side + 1) * (kBN / 4); c += 32) {
@@ -301,6 +325,24 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
+// out[m][n] = the parts of its reduction added in order, 8 columns a thread
+__global__ void __launch_bounds__(256)
+dense_reduce_kernel(const float *__restrict__ partial, int splits, long long m, int n, void *out, long long ld_out, int half) {
+    const long long total = m * (n / 8), at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= total) return;
+    const long long row = at / (n / 8);
+    const int col = (int)(at - row * (n / 8)) * 8;
+    const float4 *src = reinterpret_cast<const float4 *>(partial + row * n + col);
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s, src += m * n / 4) {
+        const float4 a = __ldg(src), b = __ldg(src + 1);
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+    *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(out) + row * ld_out + col) =
+        make_uint4(tc::pack16(v[0], v[1], half), tc::pack16(v[2], v[3], half), tc::pack16(v[4], v[5], half), tc::pack16(v[6], v[7], half));
+}
+
 bool misaligned(const void *p, size_t a = 16) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
 
 // Adds C[m][n] = sum_k A[m][k] B[n][k] to a launch.  `a` is [m][k] (row stride lda) or, with a_mn, [k][m];
@@ -320,13 +362,59 @@ int add_problem(DenseParams &p, int epi, const void *a, int64_t lda, bool a_mn, 
     if (tm * tn + p.n_items > 0x3fffffff) return MORTAR_ERR_CAPACITY;
     q.out = out; q.ld_out = ld_out; q.m = m; q.n = (int)n;
     q.tiles_m = (int)tm; q.tiles_n = (int)tn; q.k_steps = (int)((k + 127) / 128);
-    q.a_mn = a_mn; q.b_mn = b_mn; q.first_item = p.n_items;
+    q.a_mn = a_mn; q.b_mn = b_mn; q.first_item = p.n_items; q.splits = 1;
     p.n_items += (int)(tm * tn);
     ++p.n_problems;
     return MORTAR_OK;
 }
 
 std::mutex g_dense_mutex;
+
+// 128-wide steps that each of the 74 clusters would take if a launch's work were spread evenly, and the parts that a
+// product's reduction is cut into: more than one only where its tiles would run twice as long as that or longer (few
+// rows, or few columns of a weight gradient)
+int64_t even_share(int64_t total_steps) { return total_steps < 74 ? 1 : total_steps / 74; }
+int64_t parts_of(int64_t k_steps, int64_t share) { return k_steps >= 2 * share ? k_steps / share : 1; }
+int64_t steps_of(int64_t k) { return (k + 127) / 128; }
+int64_t tiles_of(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256); }
+
+struct Plan { int64_t parts[kMaxProblems], floats; };
+
+// of up to three products m x n over k in one launch
+Plan plan(const int64_t (*mnk)[3], int count) {
+    Plan r = {};
+    int64_t total = 0;
+    for (int i = 0; i < count; ++i) total += tiles_of(mnk[i][0], mnk[i][1]) * steps_of(mnk[i][2]);
+    for (int i = 0; i < count; ++i) {
+        r.parts[i] = parts_of(steps_of(mnk[i][2]), even_share(total));
+        if (r.parts[i] > 1) r.floats += r.parts[i] * mnk[i][0] * mnk[i][1];
+    }
+    return r;
+}
+
+// Deals the scratch out to the products that are cut, and renumbers the items.
+void cut(DenseParams &p, const Plan &plan, float *scratch) {
+    p.n_items = 0;
+    for (int i = 0; i < p.n_problems; ++i) {
+        Problem &q = p.prob[i];
+        q.splits = (int)plan.parts[i];
+        q.partial = scratch;
+        if (q.splits > 1) scratch += plan.parts[i] * q.m * q.n;
+        q.first_item = p.n_items;
+        p.n_items += q.tiles_m * q.tiles_n * q.splits;
+    }
+}
+
+int join(const DenseParams &p, cudaStream_t st) {
+    for (int i = 0; i < p.n_problems; ++i) {
+        const Problem &q = p.prob[i];
+        if (q.splits == 1) continue;
+        dense_reduce_kernel<<<(unsigned)((q.m * (q.n / 8) + 255) / 256), 256, 0, st>>>(q.partial, q.splits, q.m, q.n, q.out,
+                                                                                      q.ld_out, p.half);
+        MORTAR_CUDA_CHECK(cudaGetLastError());
+    }
+    return MORTAR_OK;
+}
 
 template <int EPI>
 int launch(const DenseParams &p, cudaStream_t st) {
@@ -351,15 +439,43 @@ int check_shape(int32_t dtype, int64_t rows, int32_t d_model, int32_t d_ff) {
 
 }  // namespace
 
+// products of the backward pass's last launch: dgate_up, dx, ddown
+static Plan backward_plan(int64_t rows, int32_t d_model, int32_t d_ff, bool dgu, bool dx, bool ddn) {
+    int64_t mnk[3][3];
+    int n = 0;
+    if (dx) { mnk[n][0] = rows; mnk[n][1] = d_model; mnk[n++][2] = 2LL * d_ff; }
+    if (dgu) { mnk[n][0] = 2LL * d_ff; mnk[n][1] = d_model; mnk[n++][2] = rows; }
+    if (ddn) { mnk[n][0] = d_model; mnk[n][1] = d_ff; mnk[n++][2] = rows; }
+    return plan(mnk, n);
+}
+
+static Plan forward_plan(int64_t rows, int32_t d_model, int32_t d_ff) {
+    const int64_t mnk[1][3] = {{rows, d_model, d_ff}};
+    return plan(mnk, 1);
+}
+
+extern "C" int64_t mortar_mlp_dense_scratch_floats(int64_t rows, int32_t d_model, int32_t d_ff, int32_t keep_sums) {
+    const int rc = check_shape(MORTAR_BF16, rows, d_model, d_ff);
+    if (rc == MORTAR_OK && rows <= small::kMaxRows && !keep_sums) return 0;
+    return rc != MORTAR_OK ? rc : forward_plan(rows, d_model, d_ff).floats;
+}
+
+extern "C" int64_t mortar_mlp_dense_backward_scratch_floats(int64_t rows, int32_t d_model, int32_t d_ff, int32_t want_dx,
+                                                            int32_t want_dgate_up, int32_t want_ddown) {
+    const int rc = check_shape(MORTAR_BF16, rows, d_model, d_ff);
+    return rc != MORTAR_OK ? rc : backward_plan(rows, d_model, d_ff, want_dgate_up != 0, want_dx != 0, want_ddown != 0).floats;
+}
+
 extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64_t rows, const void *gate_up,
                                 int64_t ld_gate_up, const void *down, int64_t ld_down, int32_t d_model, int32_t d_ff,
-                                void *hidden, void *gate_up_sums, void *y, int64_t ldy, void *stream) {
+                                void *hidden, void *gate_up_sums, void *y, int64_t ldy, float *scratch, int64_t scratch_floats,
+                                void *stream) {
     if (!x || !gate_up || !down || !hidden || !y) return MORTAR_ERR_NULL;
     int rc = check_shape(dtype, rows, d_model, d_ff);
     if (rc != MORTAR_OK) return rc;
     if (ldx < d_model || ld_gate_up < d_model || ld_down < d_ff || ldy < d_model) return MORTAR_ERR_SHAPE;
     if (misaligned(x) || misaligned(gate_up) || misaligned(down) || misaligned(hidden, 32) || misaligned(gate_up_sums, 32) ||
-        misaligned(y, 32) || ldx % 8 || ld_gate_up % 8 || ld_down % 8 || ldy % 16)
+        misaligned(y, 32) || misaligned(scratch, 32) || ldx % 8 || ld_gate_up % 8 || ld_down % 8 || ldy % 16)
         return MORTAR_ERR_ALIGN;
     if (rows == 0) return MORTAR_OK;
     cudaStream_t st = (cudaStream_t)stream;
@@ -378,6 +494,8 @@ extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64
         q.out = y; q.ld_out = ldy; q.after_previous = 1;
         return small::launch(q, sms, st);
     }
+    const Plan parts = forward_plan(rows, d_model, d_ff);
+    if (parts.floats > 0 && (!scratch || scratch_floats < parts.floats)) return MORTAR_ERR_CAPACITY;
     rc = tc::bind_context();
     if (rc != MORTAR_OK) return rc;
     alignas(64) DenseParams p = {};
@@ -391,21 +509,24 @@ extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64
     alignas(64) DenseParams p2 = {};
     p2.half = p.half;
     rc = add_problem(p2, kStore, hidden, d_ff, false, down, ld_down, false, rows, d_model, d_ff, y, ldy);
-    return rc == MORTAR_OK ? launch<kStore>(p2, st) : rc;
+    if (rc != MORTAR_OK) return rc;
+    cut(p2, parts, scratch);
+    rc = launch<kStore>(p2, st);
+    return rc == MORTAR_OK ? join(p2, st) : rc;
 }
 
 extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int32_t dtype,
                                          int64_t rows, const void *gate_up, int64_t ld_gate_up, const void *down,
                                          int64_t ld_down, int32_t d_model, int32_t d_ff, const void *hidden,
                                          const void *gate_up_sums, void *dgate_up_sums, void *dx, void *dgate_up,
-                                         void *ddown, void *stream) {
+                                         void *ddown, float *scratch, int64_t scratch_floats, void *stream) {
     if (!dy || !x || !gate_up || !down || !hidden || !gate_up_sums || !dgate_up_sums) return MORTAR_ERR_NULL;
     int rc = check_shape(dtype, rows, d_model, d_ff);
     if (rc != MORTAR_OK) return rc;
     if (lddy < d_model || ldx < d_model || ld_gate_up < d_model || ld_down < d_ff) return MORTAR_ERR_SHAPE;
     if (misaligned(dy) || misaligned(x) || misaligned(gate_up) || misaligned(down) || misaligned(hidden, 32) ||
         misaligned(gate_up_sums, 32) || misaligned(dgate_up_sums, 32) || misaligned(dx, 32) || misaligned(dgate_up, 32) ||
-        misaligned(ddown, 32) || lddy % 8 || ldx % 8 || ld_gate_up % 8 || ld_down % 8)
+        misaligned(ddown, 32) || misaligned(scratch, 32) || lddy % 8 || ldx % 8 || ld_gate_up % 8 || ld_down % 8)
         return MORTAR_ERR_ALIGN;
     cudaStream_t st = (cudaStream_t)stream;
     if (rows == 0) {
@@ -413,6 +534,8 @@ extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const voi
         if (ddown) MORTAR_CUDA_CHECK(cudaMemsetAsync(ddown, 0, (size_t)2 * d_ff * d_model, st));
         return MORTAR_OK;
     }
+    const Plan parts = backward_plan(rows, d_model, d_ff, dgate_up != nullptr, dx != nullptr, ddown != nullptr);
+    if (parts.floats > 0 && (!scratch || scratch_floats < parts.floats)) return MORTAR_ERR_CAPACITY;
     rc = tc::bind_context();
     if (rc != MORTAR_OK) return rc;
     const int64_t f2 = 2LL * d_ff;
@@ -428,14 +551,16 @@ extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const voi
     }
     alignas(64) DenseParams p = {};
     p.half = dtype == MORTAR_F16;
-    if (dgate_up)
+    // the longest reduction first
+    if (dx) rc = add_problem(p, kStore, dgate_up_sums, f2, false, gate_up, ld_gate_up, true, rows, d_model, f2, dx, d_model);
+    if (rc == MORTAR_OK && dgate_up)
         rc = add_problem(p, kStore, dgate_up_sums, f2, true, x, ldx, true, f2, d_model, rows, dgate_up, d_model);
-    if (rc == MORTAR_OK && dx)
-        rc = add_problem(p, kStore, dgate_up_sums, f2, false, gate_up, ld_gate_up, true, rows, d_model, f2, dx, d_model);
     if (rc == MORTAR_OK && ddown)
         rc = add_problem(p, kStore, dy, lddy, true, hidden, d_ff, true, d_model, d_ff, rows, ddown, d_ff);
     if (rc != MORTAR_OK || p.n_problems == 0) return rc;
-    return launch<kStore>(p, st);
+    cut(p, parts, scratch);
+    rc = launch<kStore>(p, st);
+    return rc == MORTAR_OK ? join(p, st) : rc;
 }
 
 extern "C" int mortar_dense_error(int32_t *code, int32_t reset) {

@@ -1172,9 +1172,12 @@ def mlp_dense_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor
     sums = x.new_empty((rows, 2 * d_ff)) if want_saved else None
     if rows == 0:
         return y, hidden, sums
+    n = _lib.lib().mortar_mlp_dense_scratch_floats(rows, d_model, d_ff, want_saved)
+    scratch = x.new_empty((n,), dtype=torch.float32) if n > 0 else None
     _launch("mortar_mlp_dense", x, x2.data_ptr(), x2.stride(0), _CODE[x.dtype], rows, gu.data_ptr(), gu.stride(0),
-            dn.data_ptr(), dn.stride(0), d_model, d_ff, hidden.data_ptr(), _at(sums), y.data_ptr(), d_model)
-    _count("dense", 2)
+            dn.data_ptr(), dn.stride(0), d_model, d_ff, hidden.data_ptr(), _at(sums), y.data_ptr(), d_model,
+            _at(scratch), n)
+    _count("dense", 3 if n else 2)
     return y, hidden, sums
 
 
@@ -1202,9 +1205,11 @@ def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor,
     if rows == 0:
         return dx, None if dgu is None else dgu.zero_(), None if ddn is None else ddn.zero_()
     dsums = torch.empty_like(sums)
+    n = _lib.lib().mortar_mlp_dense_backward_scratch_floats(rows, d_model, d_ff, want_dx, want_dgate_up, want_ddown)
+    scratch = x.new_empty((n,), dtype=torch.float32) if n > 0 else None
     _launch("mortar_mlp_dense_backward", x, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), _CODE[dt], rows,
             gu.data_ptr(), gu.stride(0), dn.data_ptr(), dn.stride(0), d_model, d_ff, hidden.data_ptr(), sums.data_ptr(),
-            dsums.data_ptr(), _at(dx), _at(dgu), _at(ddn))
+            dsums.data_ptr(), _at(dx), _at(dgu), _at(ddn), _at(scratch), n)
     _count("dense_backward", (1 if want_dx or want_dgate_up else 0) + 1)
     return dx, dgu, ddn
 

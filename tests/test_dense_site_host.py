@@ -50,7 +50,7 @@ def test_layer_norm_entry_points_validate():
 def test_mlp_dense_entry_points_validate():
     keep, p = _buf()
     f = L.mortar_mlp_dense
-    ok = [p, 64, BF16, 4, p, 64, p, 128, 64, 128, p, p, p, 64, None]
+    ok = [p, 64, BF16, 4, p, 64, p, 128, 64, 128, p, p, p, 64, p, 1 << 20, None]
 
     def call(fn, base, **at):
         args = list(base)
@@ -68,8 +68,14 @@ def test_mlp_dense_entry_points_validate():
     assert call(f, ok, a0=_off(p, 2)) == ALIGN and call(f, ok, a1=68) == ALIGN
     assert call(f, ok, a3=1 << 31) == CAP
     assert call(f, ok, a3=0) == 0
+    need = L.mortar_mlp_dense_scratch_floats(200, 64, 4096, 0)                   # few tiles, a long reduction: it is cut
+    assert need > 0 and L.mortar_mlp_dense_scratch_floats(1 << 16, 2048, 5632, 1) == 0
+    long = dict(a3=200, a7=4096, a9=4096)
+    assert call(f, ok, a14=None, **long) == CAP and call(f, ok, a15=need - 1, **long) == CAP
+    assert L.mortar_mlp_dense_scratch_floats(4, 60, 64, 0) == SHAPE
+    assert L.mortar_mlp_dense_backward_scratch_floats(4, 64, 60, 1, 1, 1) == SHAPE
     b = L.mortar_mlp_dense_backward
-    okb = [p, 64, p, 64, BF16, 4, p, 64, p, 128, 64, 128, p, p, p, p, p, p, None]
+    okb = [p, 64, p, 64, BF16, 4, p, 64, p, 128, 64, 128, p, p, p, p, p, p, p, 1 << 20, None]
     for i in (0, 2, 6, 8, 12, 13, 14):
         assert call(b, okb, **{f"a{i}": None}) == NULL
     assert call(b, okb, a10=60) == SHAPE and call(b, okb, a1=32) == SHAPE
