@@ -334,10 +334,21 @@ dense_reduce_kernel(const float *__restrict__ partial, int splits, long long m, 
     const int col = (int)(at - row * (n / 8)) * 8;
     const float4 *src = reinterpret_cast<const float4 *>(partial + row * n + col);
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s, src += m * n / 4) {
-        const float4 a = __ldg(src), b = __ldg(src + 1);
-        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    // eight parts' loads are in flight together: one at a time the kernel waits for memory once a part
+    const long long step = m * n / 4;
+    for (int s0 = 0; s0 < splits; s0 += 8) {
+        float4 a[8], b[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const bool in = s0 + s < splits;
+            a[s] = in ? __ldg(src + (s0 + s) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+            b[s] = in ? __ldg(src + (s0 + s) * step + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            v[0] += a[s].x; v[1] += a[s].y; v[2] += a[s].z; v[3] += a[s].w;
+            v[4] += b[s].x; v[5] += b[s].y; v[6] += b[s].z; v[7] += b[s].w;
+        }
     }
     *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(out) + row * ld_out + col) =
         make_uint4(tc::pack16(v[0], v[1], half), tc::pack16(v[2], v[3], half), tc::pack16(v[4], v[5], half), tc::pack16(v[6], v[7], half));

@@ -30,7 +30,9 @@ constexpr int kStage = kStageA + kStageB;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpiWarps;   // warps 0..3: copies, MMAs, two that only lend their registers
 constexpr int kTmemCols = 512;
-constexpr int kSmem = kStages * kStage + (2 * kStages + 2) * 8 + 1024;
+constexpr int kTurn = 32 * 33;                   // floats a warp turns a 32 x 32 piece of the result in
+constexpr int kSmem = kStages * kStage + (2 * kStages + 2) * 8 + kEpiWarps * kTurn * 4 + 1024;
+static_assert(kSmem + 64 <= 227 * 1024, "shared memory budget");
 
 __device__ int g_fp8_error;
 
@@ -55,40 +57,49 @@ struct Fp8Params {
 // epilogue of a 256 x 256 tile three times what its 16 blocks of MMAs take (631 against 420 us at 8192 x 2048 -> 11264)
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
-// 32 values of one row from column `col` on; 32 bytes at a time where the row is aligned
-__device__ __forceinline__ void store_row32(const Fp8Params &p, long long row, int col, const float (&v)[32]) {
-    const int left = p.n - col;
-    if (row >= p.rows || left <= 0) return;
-    const long long idx = row * p.ld_out + col;
-    if (p.out_dtype == MORTAR_F32) {
-        float *o = reinterpret_cast<float *>(p.out) + idx;
+// A warp's 32 rows x 32 columns from (row0, col) on; v = this lane's row.  Rows that start on 32 bytes are stored 32
+// bytes at a time, each lane its own.  Others are turned in shared memory, so that the lanes of a store lie side by side
+// in a row (stored value by value from each lane's own row, a ragged tile took three times as long).
+__device__ __forceinline__ void store_32x32(const Fp8Params &p, long long row0, int col, const float (&v)[32], float *turn) {
+    const int left = p.n - col, lane = threadIdx.x & 31;
+    if (left <= 0) return;
+    const long long row = row0 + lane;
+    if (p.vec && left >= 32) {
+        if (row >= p.rows) return;
+        if (p.out_dtype == MORTAR_F32) {
+            float *o = reinterpret_cast<float *>(p.out) + row * p.ld_out + col;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (p.vec && 8 * j + 8 <= left) {
+            for (int j = 0; j < 4; ++j) {
                 uint32_t w[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * j + i]);
                 tc::store_v8(o + 8 * j, w);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (8 * j + i < left) o[8 * j + i] = v[8 * j + i];
             }
+            return;
+        }
+        uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + row * p.ld_out + col;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = tc::pack16(v[16 * j + 2 * i], v[16 * j + 2 * i + 1], p.out_dtype == MORTAR_F16);
+            tc::store_v8(o + 16 * j, w);
         }
         return;
     }
-    const bool half = p.out_dtype == MORTAR_F16;
-    uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + idx;
+    __syncwarp();                                                     // the piece before has been read
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = tc::pack16(v[16 * j + 2 * i], v[16 * j + 2 * i + 1], half);
-        if (p.vec && 16 * j + 16 <= left) tc::store_v8(o + 16 * j, w);
-        else
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (16 * j + i < left) o[16 * j + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    for (int i = 0; i < 32; ++i) turn[lane * 33 + i] = v[i];
+    __syncwarp();
+    if (lane >= left) return;
+    const int rows = (int)min(32LL, p.rows - row0);
+    const long long idx = row0 * p.ld_out + col + lane;
+    if (p.out_dtype == MORTAR_F32) {
+        float *o = reinterpret_cast<float *>(p.out) + idx;
+        for (int r = 0; r < rows; ++r) o[r * p.ld_out] = turn[r * 33 + lane];
+    } else {
+        uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + idx;
+        for (int r = 0; r < rows; ++r) o[r * p.ld_out] = (uint16_t)tc::pack16(turn[r * 33 + lane], 0.f, p.out_dtype == MORTAR_F16);
     }
 }
 
@@ -107,6 +118,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
     // its sums are there; acc_empty (CTA 0's): the warps of both have read the sums
     uint64_t *full = reinterpret_cast<uint64_t *>(stages + kStages * kStage), *done = full + kStages;
     uint64_t *acc_empty = done + kStages;
+    float *turns = reinterpret_cast<float *>(acc_empty + 2);
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -238,7 +250,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                     }
                 }
                 const int col = p.up_row ? tn * 128 + side * 64 + j * 32 : tn * 256 + (j >> 1) * 128 + side * 64 + (j & 1) * 32;
-                store_row32(p, row, col, v);
+                store_32x32(p, row - lane, col, v, turns + (warp - 4) * kTurn);
             }
         }
     }

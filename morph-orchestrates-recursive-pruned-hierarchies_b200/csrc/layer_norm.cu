@@ -476,7 +476,8 @@ layer_norm_far_dw_kernel(const T *dy, long long lddy, const T *x, long long ldx,
     partial[(long long)blockIdx.y * 2 * cols + cols + c] = db;
 }
 
-// dw / db [col] = sum of the partials: eight interleaved chains a column, added in a fixed order.
+// dw / db [col] = sum of the partials: eight interleaved chains a column, added in a fixed order; the loads of
+// a chain's next ten parts are in flight together (one at a time it took 10 us, all of it waiting).
 __global__ void __launch_bounds__(kThreads)
 layer_norm_reduce_kernel(const float *__restrict__ partial, int splits, int cols, float *dw, float *db) {
     __shared__ float part[8][33];
@@ -484,7 +485,13 @@ layer_norm_reduce_kernel(const float *__restrict__ partial, int splits, int cols
     const long long c = (long long)blockIdx.x * 32 + lane;
     float s = 0.f;
     if (c < 2LL * cols)
-        for (int i = chain; i < splits; i += 8) s += partial[(long long)i * 2 * cols + c];
+        for (int i0 = chain; i0 < splits; i0 += 80) {
+            float v[10];
+#pragma unroll
+            for (int i = 0; i < 10; ++i) v[i] = i0 + 8 * i < splits ? __ldg(partial + (long long)(i0 + 8 * i) * 2 * cols + c) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 10; ++i) s += v[i];
+        }
     part[chain][lane] = s;
     __syncthreads();
     if (chain == 0 && c < 2LL * cols) {
