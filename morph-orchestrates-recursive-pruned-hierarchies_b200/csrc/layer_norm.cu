@@ -12,7 +12,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <type_traits>
 #include "common.h"
+#include "tc_pair.cuh"
 
 namespace {
 
@@ -406,6 +408,232 @@ layer_norm_backward_kernel(const T *__restrict__ dy, long long lddy, const T *__
     }
 }
 
+// ---- the same for rows that are whole vectors ---------------------------------------------------
+//
+// Where every row starts on 16 bytes and has a multiple of 8 columns, a unit is there or not, loads and
+// stores are single vectors, and the arithmetic runs on pairs of columns (fma.rn.f32x2 and its like):
+// 20 instructions a column become LN_INSTR forward.  A thread takes NE units side by side in its row.
+
+constexpr int kWholeWarps = 16;                          // of a CTA, one CTA an SM: 128 registers a thread
+
+template <class T> struct Packed { uint4 v[sizeof(T) * kUnit / 16]; };
+template <class T> __device__ __forceinline__ void load_packed(Packed<T> &u, const T *p) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) * kUnit / 16); ++i) u.v[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+}
+// four pairs of columns as fp32
+__device__ __forceinline__ void unpack(const Packed<float> &u, uint64_t (&p)[4]) {
+    p[0] = tc::pair_of(u.v[0].x, u.v[0].y); p[1] = tc::pair_of(u.v[0].z, u.v[0].w);
+    p[2] = tc::pair_of(u.v[1].x, u.v[1].y); p[3] = tc::pair_of(u.v[1].z, u.v[1].w);
+}
+__device__ __forceinline__ void unpack(const Packed<__nv_bfloat16> &u, uint64_t (&p)[4]) {
+    const uint32_t w[4] = {u.v[0].x, u.v[0].y, u.v[0].z, u.v[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = tc::pair_of(w[i] << 16, w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack(const Packed<__half> &u, uint64_t (&p)[4]) {
+    const uint32_t w[4] = {u.v[0].x, u.v[0].y, u.v[0].z, u.v[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        p[i] = tc::pair_of(__float_as_uint(f.x), __float_as_uint(f.y));
+    }
+}
+template <class T> __device__ __forceinline__ void store_pairs(T *dst, const uint64_t (&p)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4 *>(dst)[0] = make_float4(tc::low_of(p[0]), tc::high_of(p[0]), tc::low_of(p[1]), tc::high_of(p[1]));
+        reinterpret_cast<float4 *>(dst)[1] = make_float4(tc::low_of(p[2]), tc::high_of(p[2]), tc::low_of(p[3]), tc::high_of(p[3]));
+    } else {
+        constexpr bool kHalf = std::is_same<T, __half>::value;
+        *reinterpret_cast<uint4 *>(dst) =
+            make_uint4(tc::pack16(tc::low_of(p[0]), tc::high_of(p[0]), kHalf), tc::pack16(tc::low_of(p[1]), tc::high_of(p[1]), kHalf),
+                       tc::pack16(tc::low_of(p[2]), tc::high_of(p[2]), kHalf), tc::pack16(tc::low_of(p[3]), tc::high_of(p[3]), kHalf));
+    }
+}
+__device__ __forceinline__ void load_pairs(const float *p, int c, bool in, float fill, uint64_t (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = p && in ? tc::pair_of(__float_as_uint(__ldg(p + c + 2 * i)), __float_as_uint(__ldg(p + c + 2 * i + 1))) : tc::both(fill);
+}
+
+template <class T, int NE>
+__global__ void __launch_bounds__(32 * kWholeWarps, 1)
+layer_norm_whole_kernel(const T *__restrict__ x, long long ldx, long long rows, int cols, const float *__restrict__ w,
+                        const float *__restrict__ b, float eps, T *__restrict__ y, long long ldy, float *__restrict__ stats,
+                        int warps) {
+    __shared__ float2 red[kWholeWarps][2][16];
+    Group g = make_group(warps, red);
+    const int groups = (int)(blockDim.x >> 5) / warps;
+    const float inv = 1.f / cols;
+    const long long stride = (long long)gridDim.x * groups;
+    long long row = (long long)blockIdx.x * groups + g.id;
+    uint64_t wv[NE][4], bv[NE][4];
+    bool in[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const int c = kUnit * (g.thread + 32 * warps * i);
+        in[i] = c < cols;
+        load_pairs(w, c, in[i], 1.f, wv[i]);
+        load_pairs(b, c, in[i], 0.f, bv[i]);
+    }
+    const T *xp = x + row * ldx + kUnit * g.thread;
+    T *yp = y + row * ldy + kUnit * g.thread;
+    Packed<T> next[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+        if (row < rows && in[i]) load_packed(next[i], xp + 32 * kUnit * warps * i);
+    for (; row < rows; row += stride, yp += stride * ldy) {
+        uint64_t v[NE][4];
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            unpack(next[i], v[i]);
+            if (!in[i]) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0ull;
+        }
+        xp += stride * ldx;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)                                                // under this row's sums
+            if (row + stride < rows && in[i]) load_packed(next[i], xp + 32 * kUnit * warps * i);
+        uint64_t s = 0ull;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s = tc::add2(s, v[i][j]);
+        const float mean = group_sum(tc::low_of(s) + tc::high_of(s), 0.f, g).x * inv;
+        const uint64_t minus = tc::both(-mean);
+        s = 0ull;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+            if (in[i]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[i][j] = tc::add2(v[i][j], minus);
+                    s = tc::fma2(v[i][j], v[i][j], s);
+                }
+            }
+        const float rstd = rsqrtf(group_sum(tc::low_of(s) + tc::high_of(s), 0.f, g).x * inv + eps);
+        const uint64_t r2 = tc::both(rstd);
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+            if (in[i]) {
+                uint64_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = tc::fma2(tc::mul2(v[i][j], r2), wv[i][j], bv[i][j]);
+                store_pairs(yp + 32 * kUnit * warps * i, o);
+            }
+        if (stats && g.thread == 0) {
+            stats[row] = mean;
+            stats[rows + row] = rstd;
+        }
+    }
+}
+
+template <class T, int NE>
+__global__ void __launch_bounds__(32 * kWholeWarps, 1)
+layer_norm_whole_backward_kernel(const T *__restrict__ dy, long long lddy, const T *__restrict__ x, long long ldx,
+                                 long long rows, int cols, const float *__restrict__ w, const float *__restrict__ stats,
+                                 T *__restrict__ dx, long long lddx, float *__restrict__ partial, int warps) {
+    constexpr bool kAhead = NE * sizeof(T) <= 4;         // registers for a row on its way: 16-bit rows of two units, fp32 of one
+    __shared__ float2 red[kWholeWarps][2][16];
+    extern __shared__ float fold[];                      // [groups][columns, rounded up to the group's]
+    Group g = make_group(warps, red);
+    const int groups = (int)(blockDim.x >> 5) / warps;
+    const float inv = 1.f / cols;
+    const long long stride = (long long)gridDim.x * groups;
+    long long row = (long long)blockIdx.x * groups + g.id;
+    uint64_t dw[NE][4], db[NE][4], wv[NE][4];
+    bool in[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const int c = kUnit * (g.thread + 32 * warps * i);
+        in[i] = c < cols;
+        load_pairs(w, c, in[i], 1.f, wv[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dw[i][j] = db[i][j] = 0ull;
+    }
+    const int step = 32 * kUnit * warps;
+    const T *xp = x + row * ldx + kUnit * g.thread, *dp = dy + row * lddy + kUnit * g.thread;
+    Packed<T> nx[NE], nd[NE];
+    float next_mean = 0.f, next_rstd = 0.f;
+    auto fetch = [&](long long r) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+            if (in[i]) {
+                load_packed(nx[i], xp + step * i);
+                load_packed(nd[i], dp + step * i);
+            }
+        next_mean = __ldg(stats + r);
+        next_rstd = __ldg(stats + rows + r);
+        xp += stride * ldx;
+        dp += stride * lddy;
+    };
+    if (kAhead && row < rows) fetch(row);
+    for (; row < rows; row += stride) {
+        if (!kAhead) fetch(row);
+        uint64_t xv[NE][4], dv[NE][4];
+        const float mean = next_mean, rstd = next_rstd;
+        const uint64_t minus = tc::both(-mean), r2 = tc::both(rstd);
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            unpack(nx[i], xv[i]);
+            unpack(nd[i], dv[i]);
+        }
+        if (kAhead && row + stride < rows) fetch(row + stride);
+        uint64_t s1 = 0ull, s2 = 0ull;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+            if (in[i]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    xv[i][j] = tc::mul2(tc::add2(xv[i][j], minus), r2);
+                    dw[i][j] = tc::fma2(dv[i][j], xv[i][j], dw[i][j]);
+                    db[i][j] = tc::add2(db[i][j], dv[i][j]);
+                    dv[i][j] = tc::mul2(dv[i][j], wv[i][j]);
+                    s1 = tc::add2(s1, dv[i][j]);
+                    s2 = tc::fma2(dv[i][j], xv[i][j], s2);
+                }
+            }
+        if (dx) {
+            const float2 c = group_sum(tc::low_of(s1) + tc::high_of(s1), tc::low_of(s2) + tc::high_of(s2), g);
+            const uint64_t c1 = tc::both(-c.x * inv), c2 = tc::both(-c.y * inv);
+            T *op = dx + row * lddx + kUnit * g.thread;
+#pragma unroll
+            for (int i = 0; i < NE; ++i)
+                if (in[i]) {
+                    uint64_t o[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j] = tc::mul2(tc::fma2(xv[i][j], c2, tc::add2(dv[i][j], c1)), r2);
+                    store_pairs(op + step * i, o);
+                }
+        }
+    }
+    if (!partial) return;
+    float *dst = partial + (long long)blockIdx.x * 2 * cols;
+    const int width = step * NE;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        if (groups > 1) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            const int c = kUnit * (g.thread + 32 * warps * i);
+            const uint64_t (&v)[4] = which ? db[i] : dw[i];
+            if (groups > 1) store_pairs(fold + g.id * width + c, v);
+            else if (in[i])
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    dst[which * cols + c + 2 * j] = tc::low_of(v[j]);
+                    dst[which * cols + c + 2 * j + 1] = tc::high_of(v[j]);
+                }
+        }
+        if (groups == 1) continue;
+        __syncthreads();
+        for (int c = threadIdx.x; c < cols; c += blockDim.x) {       // the groups' sums, in group order
+            float s = 0.f;
+            for (int r = 0; r < groups; ++r) s += fold[r * width + c];
+            dst[which * cols + c] = s;
+        }
+    }
+}
+
 // ---- any number of columns: the row is read again for each step -------------------------------
 
 template <class T>
@@ -521,11 +749,59 @@ Layout layout_of(int64_t rows, int32_t cols, int most) {
     return l;
 }
 
-// CTAs of the backward pass, one partial sum each: one per SM at most
-int64_t splits_for(int64_t rows, int32_t cols) {
-    if (cols > kFar) return rows < 4 * 148 ? (rows + 3) / 4 + (rows == 0) : 148;
-    const int64_t need = (rows + layout_of(rows, cols, kBackwardWarps).groups - 1) / layout_of(rows, cols, kBackwardWarps).groups;
-    return need < 1 ? 1 : (need < 148 ? need : 148);
+// CTAs of the backward pass, one partial sum each: one per SM at most, whatever kernel runs
+int64_t splits_for(int64_t rows, int32_t) { return rows < 1 ? 1 : (rows < 148 ? rows : 148); }
+
+// The same for rows of whole vectors, 16 warps a CTA: of the units a thread may take, the number that leaves the fewest
+// lanes and warps idle (the larger on a tie: less to do per row).
+Layout whole_layout(int64_t rows, int32_t cols, int most_units) {
+    const int units = cols / kUnit;
+    Layout best = {0, 0, 0};
+    float best_use = 0.f;
+    for (int ne = most_units; ne >= 1; --ne) {
+        const int warps = (units + 32 * ne - 1) / (32 * ne);
+        if (warps > kWholeWarps) continue;
+        int g = kWholeWarps / warps;
+        if (warps > 1 && g > kMaxGroups) g = kMaxGroups;
+        const float use = (float)units * g / (32.f * ne * kWholeWarps);
+        if (use > best_use * 1.0001f) {
+            best = {ne, warps, g};
+            best_use = use;
+        }
+    }
+    const int64_t share = (rows + 147) / 148;
+    if (best.groups > share) best.groups = (int)(share < 1 ? 1 : share);
+    return best;                                         // units 0: the row does not fit
+}
+
+// the rows' types leave registers for so many units
+template <class T> constexpr int kWholeForward = sizeof(T) == 4 ? 2 : 3;
+constexpr int kWholeBackward = 2;
+
+bool whole_rows(const void *p, int64_t ld, size_t elem) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (size_t)ld * elem % 16 == 0;
+}
+
+template <class T, int NE>
+int run_whole_forward(const Layout &l, const void *x, int64_t ldx, int64_t rows, int32_t cols, const float *w, const float *b,
+                      float eps, void *y, int64_t ldy, float *stats, cudaStream_t st) {
+    const int64_t need = (rows + l.groups - 1) / l.groups;
+    layer_norm_whole_kernel<T, NE><<<(unsigned)(need < 148 ? need : 148), 32 * l.warps * l.groups, 0, st>>>(
+        (const T *)x, ldx, rows, cols, w, b, eps, (T *)y, ldy, stats, l.warps);
+    MORTAR_CUDA_CHECK(cudaGetLastError());
+    return MORTAR_OK;
+}
+
+template <class T, int NE>
+int run_whole_backward(const Layout &l, const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t rows, int32_t cols,
+                       const float *w, const float *stats, void *dx, int64_t lddx, float *partial, int64_t splits,
+                       cudaStream_t st) {
+    // the groups' columns: at most 16 warps' of 2 units, 32 KB
+    const int smem = partial && l.groups > 1 ? l.groups * l.warps * 32 * kUnit * NE * (int)sizeof(float) : 0;
+    layer_norm_whole_backward_kernel<T, NE><<<(unsigned)splits, 32 * l.warps * l.groups, smem, st>>>(
+        (const T *)dy, lddy, (const T *)x, ldx, rows, cols, w, stats, (T *)dx, lddx, partial, l.warps);
+    MORTAR_CUDA_CHECK(cudaGetLastError());
+    return MORTAR_OK;
 }
 
 template <class T, int NE>
@@ -552,6 +828,13 @@ int run_backward(const Layout &l, const void *dy, int64_t lddy, const void *x, i
 template <class T>
 int forward(const void *x, int64_t ldx, int64_t rows, int32_t cols, const float *w, const float *b, float eps, void *y,
             int64_t ldy, float *stats, cudaStream_t st) {
+    if (cols % kUnit == 0 && whole_rows(x, ldx, sizeof(T)) && whole_rows(y, ldy, sizeof(T))) {
+        const Layout l = whole_layout(rows, cols, kWholeForward<T>);
+        if (l.units == 1) return run_whole_forward<T, 1>(l, x, ldx, rows, cols, w, b, eps, y, ldy, stats, st);
+        if (l.units == 2) return run_whole_forward<T, 2>(l, x, ldx, rows, cols, w, b, eps, y, ldy, stats, st);
+        if constexpr (kWholeForward<T> > 2)
+            if (l.units == 3) return run_whole_forward<T, 3>(l, x, ldx, rows, cols, w, b, eps, y, ldy, stats, st);
+    }
     if (cols <= kFar) {
         const Layout l = layout_of(rows, cols, kForwardWarps);
         if (l.units == 1) return run_forward<T, 1>(l, x, ldx, rows, cols, w, b, eps, y, ldy, stats, st);
@@ -569,7 +852,15 @@ int backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t r
              const float *stats, void *dx, int64_t lddx, float *dw, float *db, float *scratch, cudaStream_t st) {
     const int64_t splits = splits_for(rows, cols);
     float *partial = dw || db ? scratch : nullptr;
-    if (cols <= kFar) {
+    Layout wl = {0, 0, 0};
+    if (cols % kUnit == 0 && whole_rows(x, ldx, sizeof(T)) && whole_rows(dy, lddy, sizeof(T)) &&
+        (!dx || whole_rows(dx, lddx, sizeof(T))))
+        wl = whole_layout(rows, cols, kWholeBackward);
+    if (wl.units) {
+        const int rc = wl.units == 1 ? run_whole_backward<T, 1>(wl, dy, lddy, x, ldx, rows, cols, w, stats, dx, lddx, partial, splits, st)
+                                     : run_whole_backward<T, 2>(wl, dy, lddy, x, ldx, rows, cols, w, stats, dx, lddx, partial, splits, st);
+        if (rc != MORTAR_OK) return rc;
+    } else if (cols <= kFar) {
         const Layout l = layout_of(rows, cols, kBackwardWarps);
         const int rc = l.units == 1   ? run_backward<T, 1>(l, dy, lddy, x, ldx, rows, cols, w, stats, dx, lddx, partial, st)
                        : l.units == 2 ? run_backward<T, 2>(l, dy, lddy, x, ldx, rows, cols, w, stats, dx, lddx, partial, st)
