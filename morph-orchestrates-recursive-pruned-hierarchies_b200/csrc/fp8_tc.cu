@@ -50,21 +50,21 @@ struct Fp8Params {
     void *out;
     long long ld_out;
     int out_dtype;
-    int vec;                 // 1: rows of out start on 32 bytes
 };
 
 // exp2-based exponential and an approximate quotient, 2^-22 (1 + |g|) at worst: the exact forms cost the
 // epilogue of a 256 x 256 tile three times what its 16 blocks of MMAs take (631 against 420 us at 8192 x 2048 -> 11264)
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
-// A warp's 32 rows x 32 columns from (row0, col) on; v = this lane's row.  Rows that start on 32 bytes are stored 32
-// bytes at a time, each lane its own.  Others are turned in shared memory, so that the lanes of a store lie side by side
+// A warp's 32 rows x 32 columns from (row0, col) on; v = this lane's row.  Rows that start on 32 bytes and end on a
+// multiple of 32 columns are stored 32 bytes at a time, each lane its own.  Others (TURNED) are turned in shared memory, so that the lanes of a store lie side by side
 // in a row (stored value by value from each lane's own row, a ragged tile took three times as long).
+template <bool TURNED>
 __device__ __forceinline__ void store_32x32(const Fp8Params &p, long long row0, int col, const float (&v)[32], float *turn) {
     const int left = p.n - col, lane = threadIdx.x & 31;
     if (left <= 0) return;
     const long long row = row0 + lane;
-    if (p.vec && left >= 32) {
+    if constexpr (!TURNED) {
         if (row >= p.rows) return;
         if (p.out_dtype == MORTAR_F32) {
             float *o = reinterpret_cast<float *>(p.out) + row * p.ld_out + col;
@@ -86,7 +86,7 @@ __device__ __forceinline__ void store_32x32(const Fp8Params &p, long long row0, 
             tc::store_v8(o + 16 * j, w);
         }
         return;
-    }
+    } else {
     __syncwarp();                                                     // the piece before has been read
 #pragma unroll
     for (int i = 0; i < 32; ++i) turn[lane * 33 + i] = v[i];
@@ -101,6 +101,7 @@ __device__ __forceinline__ void store_32x32(const Fp8Params &p, long long row0, 
         uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + idx;
         for (int r = 0; r < rows; ++r) o[r * p.ld_out] = (uint16_t)tc::pack16(turn[r * 33 + lane], 0.f, p.out_dtype == MORTAR_F16);
     }
+    }
 }
 
 __device__ __forceinline__ void tile_of(const Fp8Params &p, int item, int &tm, int &tn) {
@@ -110,6 +111,7 @@ __device__ __forceinline__ void tile_of(const Fp8Params &p, int item, int &tm, i
     tm = band * 8 + r - tn * h;
 }
 
+template <bool TURNED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
     extern __shared__ uint8_t smem_raw[];
@@ -250,7 +252,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                     }
                 }
                 const int col = p.up_row ? tn * 128 + side * 64 + j * 32 : tn * 256 + (j >> 1) * 128 + side * 64 + (j & 1) * 32;
-                store_32x32(p, row - lane, col, v, turns + (warp - 4) * kTurn);
+                store_32x32<TURNED>(p, row - lane, col, v, turns + (warp - 4) * kTurn);
             }
         }
     }
@@ -267,6 +269,17 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
 bool misaligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
 
 std::mutex g_fp8_mutex;
+
+template <bool TURNED>
+int launch(const Fp8Params &p, int sms, cudaStream_t st) {
+    static bool ready[64] = {false};
+    const int rc = tc::allow_smem(fp8_pair_kernel<TURNED>, kSmem, ready, g_fp8_mutex, nullptr);
+    if (rc != MORTAR_OK) return rc;
+    const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
+    fp8_pair_kernel<TURNED><<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
+    MORTAR_CUDA_CHECK(cudaGetLastError());
+    return MORTAR_OK;
+}
 
 }  // namespace
 
@@ -324,15 +337,9 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     p.w_blocks = (out_features + 127) / 128;
     p.types = (x_type == MORTAR_E5M2 ? 1u << 7 : 0u) | (w_type == MORTAR_E5M2 ? 1u << 10 : 0u);
     p.out = out; p.ld_out = ld_out; p.out_dtype = out_dtype;
-    p.vec = !misaligned(out, 32) && (ld_out * e) % 32 == 0;
+    const bool turned = misaligned(out, 32) || (ld_out * e) % 32 || p.n % 32;
 
-    static bool ready[64] = {false};
-    rc = tc::allow_smem(fp8_pair_kernel, kSmem, ready, g_fp8_mutex, nullptr);
-    if (rc != MORTAR_OK) return rc;
-    const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
-    fp8_pair_kernel<<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
-    MORTAR_CUDA_CHECK(cudaGetLastError());
-    return MORTAR_OK;
+    return turned ? launch<true>(p, sms, st) : launch<false>(p, sms, st);
 }
 
 extern "C" int mortar_linear_fp8_error(int32_t *code, int32_t reset) {
