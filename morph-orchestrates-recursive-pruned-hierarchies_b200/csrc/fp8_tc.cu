@@ -199,23 +199,28 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
         uint32_t g = 0, s = 0, parity = 0;
         bool ok = true;
         for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
-            int tm, tn;
-            tile_of(p, item, tm, tn);
-            const long long row = (long long)tm * 256 + (long long)rank * 128 + quarter * 32 + lane;
-            const int wb0 = p.up_row ? tn : 2 * tn, wb1 = p.up_row ? p.up_row / 128 + tn : 2 * tn + 1;
-            const float *xs = p.xs + (row < p.rows ? row : p.rows - 1) * p.ld_xs;
-            const float *ws0 = p.ws + (long long)wb0 * p.ld_ws, *ws1 = p.ws + (long long)min(wb1, p.w_blocks - 1) * p.ld_ws;
+            // positions in the scale arrays: 32 bits, and the tile's place is worked out again for the stores, since the sums
+            // and what is being read leave few registers (229 -> 213 us)
+            uint32_t at_x, at_w0, at_w1;
+            {
+                int tm, tn;
+                tile_of(p, item, tm, tn);
+                const long long row = (long long)tm * 256 + (long long)rank * 128 + quarter * 32 + lane;
+                const int wb0 = p.up_row ? tn : 2 * tn, wb1 = p.up_row ? p.up_row / 128 + tn : 2 * tn + 1;
+                at_x = (uint32_t)((row < p.rows ? row : p.rows - 1) * p.ld_xs);
+                at_w0 = (uint32_t)(wb0 * p.ld_ws);
+                at_w1 = (uint32_t)(min(wb1, p.w_blocks - 1) * p.ld_ws);
+            }
             uint64_t sum[4][16];                                  // columns 32 j + 2 i, + 1
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum[j][i] = 0ull;
-            float sx = __ldg(xs), s0 = __ldg(ws0), s1 = __ldg(ws1);
-            for (int k = 0; k < p.k_blocks; ++k, ++g) {
+            float sx = __ldg(p.xs + at_x), s0 = __ldg(p.ws + at_w0), s1 = __ldg(p.ws + at_w1);
+            for (int k = p.k_blocks; k > 0; --k, ++g) {
                 const uint32_t buf = g & 1, taddr = taddr0 + buf * 256;
-                const uint32_t f0 = __float_as_uint(sx * s0), f1 = __float_as_uint(sx * s1);
-                const uint64_t ff[2] = {tc::pair_of(f0, f0), tc::pair_of(f1, f1)};
-                if (k + 1 < p.k_blocks) { sx = __ldg(xs + k + 1); s0 = __ldg(ws0 + k + 1); s1 = __ldg(ws1 + k + 1); }
+                const float f0 = sx * s0, f1 = sx * s1;
+                if (k > 1) { sx = __ldg(p.xs + ++at_x); s0 = __ldg(p.ws + ++at_w0); s1 = __ldg(p.ws + ++at_w1); }
                 if (!tc::mbar_wait(done0 + 8 * s, parity, abort_flag, &g_fp8_error, 4)) { ok = false; break; }
                 if (++s == kStages) { s = 0; parity ^= 1; }
                 tc::fence_after();
@@ -230,14 +235,18 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                         __syncwarp();
                         if (lane == 0) tc::arrive_relaxed(lead_empty + 8 * buf);
                     }
+                    const uint64_t ff = tc::both(h ? f1 : f0);
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            sum[2 * h + j][i] = tc::fma2(tc::pair_of(r[j][2 * i], r[j][2 * i + 1]), ff[h], sum[2 * h + j][i]);
+                            sum[2 * h + j][i] = tc::fma2(tc::pair_of(r[j][2 * i], r[j][2 * i + 1]), ff, sum[2 * h + j][i]);
                 }
             }
             if (!ok) break;
+            int tm, tn;
+            tile_of(p, item, tm, tn);
+            const long long row0 = (long long)tm * 256 + (long long)rank * 128 + quarter * 32;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (j >= 2 && p.up_row) break;
@@ -252,7 +261,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                     }
                 }
                 const int col = p.up_row ? tn * 128 + side * 64 + j * 32 : tn * 256 + (j >> 1) * 128 + side * 64 + (j & 1) * 32;
-                store_32x32<TURNED>(p, row - lane, col, v, turns + (warp - 4) * kTurn);
+                store_32x32<TURNED>(p, row0, col, v, turns + (warp - 4) * kTurn);
             }
         }
     }
@@ -301,7 +310,9 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     if (misaligned(x, 16) || misaligned(w, 16) || ldx % 16 || ldw % 16 || misaligned(out, e) || misaligned(x_scale, 4) ||
         misaligned(w_scale, 4))
         return MORTAR_ERR_ALIGN;
-    if (rows > 0x7fffff00LL || out_features > 0x7fffff00) return MORTAR_ERR_CAPACITY;
+    if (rows > 0x7fffff00LL || out_features > 0x7fffff00 || rows * ld_x_scale > 0xffffffffLL ||
+        ((int64_t)out_features + 127) / 128 * ld_w_scale > 0xffffffffLL)
+        return MORTAR_ERR_CAPACITY;
     if (rows == 0) return MORTAR_OK;
     cudaStream_t st = (cudaStream_t)stream;
 

@@ -32,6 +32,17 @@ __device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap *map, 
         "[%0], [%1, {%2, %3}], [%4];\n"
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
 }
+// Whether the phase has completed, without waiting for it (try_wait may hold the thread for a while)
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.b32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+
 // one arrival, when the MMAs issued so far have ended, at the barrier of this offset in both CTAs of the pair
 __device__ __forceinline__ void commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
@@ -89,7 +100,7 @@ __device__ __forceinline__ bool poll_mma8_f16(uint32_t bar, uint32_t parity, uin
     uint32_t ready;
     asm volatile(
         "{\n.reg .pred q, p0, p1;\n.reg .b64 x, y, x2, y2;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 q, [%1], %2;\n"
         "setp.ne.b32 p0, %11, 0;\nsetp.eq.u32 p1, 1, 1;\n"
         "tcgen05.mma.cta_group::2.kind::f16 [%3], %4, %5, %10, p0;\n"
         "add.s64 x, %4, %6;\nadd.s64 y, %5, %7;\nadd.s64 x2, %4, %8;\nadd.s64 y2, %5, %9;\n"
@@ -118,7 +129,7 @@ __device__ __forceinline__ bool poll_mma4_f8(uint32_t bar, uint32_t parity, uint
     uint32_t ready;
     asm volatile(
         "{\n.reg .pred q, p0, p1;\n.reg .b64 x, y;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 q, [%1], %2;\n"
         "setp.ne.u32 p0, 1, 1;\nsetp.eq.u32 p1, 1, 1;\n"
         "tcgen05.mma.cta_group::2.kind::f8f6f4 [%3], %4, %5, %6, p0;\n"
         "add.s64 x, %4, 2;\nadd.s64 y, %5, 2;\n"
