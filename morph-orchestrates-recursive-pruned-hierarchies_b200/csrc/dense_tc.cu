@@ -14,7 +14,7 @@
 // One cluster of two CTAs computes a 256 x kBN tile (each CTA 128 rows; the B operand is split between
 // their shared memories): per SM and 64-wide step 16 KB of A and kBN * 64 bytes of B cross from L2,
 // half of what two single CTAs would read, which is what keeps the copies ahead of the MMAs.  Warp 0
-// issues the copies of its CTA, one thread of CTA 0 issues the MMAs of both, warps 2..9 read the
+// issues the copies of its CTA, one thread of CTA 0 issues the MMAs of both, warps 2..17 read the
 // accumulators (two sets, so that a tile's epilogue runs under the next tile's MMAs).
 // Every wait is bounded.
 #include <cuda.h>
@@ -32,7 +32,7 @@ constexpr int kStages = 3;
 constexpr int kStageA = 128 * 256;               // this CTA's 128 rows, 128 elements of 2 bytes each
 constexpr int kStageB = kBN / 2 * 256;
 constexpr int kStage = kStageA + kStageB;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kTmemCols = 2 * kBN;
 constexpr int kSmem = kStages * kStage + (2 * kStages + 4) * 8 + 1024;
@@ -70,48 +70,13 @@ struct DenseParams {
 // exp2-based exponential and an approximate quotient, off by 2^-22 (1 + |g|) at worst; the result is rounded to 16 bits
 __device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
-// 32 accumulator columns -> 32 16-bit values of one row; n_left = columns of the row from there on (a multiple
-// of 16, as every width is), and 32 bytes at a time since every row starts on 32 bytes
-__device__ __forceinline__ void store32(void *base, long long idx, const float (&v)[32], int n_left, bool half) {
-    uint16_t *dst = reinterpret_cast<uint16_t *>(base) + idx;
+// 16 accumulator columns -> 16 16-bit values of one row, 32 bytes at a time: every row starts on 32 bytes and every
+// width is a multiple of 16
+__device__ __forceinline__ void store16(void *base, long long idx, const uint32_t (&v)[16], bool half) {
+    uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        if (16 * j >= n_left) break;
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = tc::pack16(v[16 * j + 2 * i], v[16 * j + 2 * i + 1], half);
-        tc::store_v8(dst + 16 * j, w);
-    }
-}
-
-__device__ __forceinline__ void store32_f32(float *dst, const float (&v)[32], int n_left) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (8 * j >= n_left) break;
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * j + i]);
-        tc::store_v8(dst + 8 * j, w);
-    }
-}
-
-__device__ __forceinline__ void load32(const void *base, long long idx, uint32_t (&w)[16], int n_left) {
-    const uint16_t *src = reinterpret_cast<const uint16_t *>(base) + idx;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        if (16 * j < n_left) tc::load_v8(src + 16 * j, &w[8 * j]);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[8 * j + i] = 0u;
-    }
-}
-
-__device__ __forceinline__ void acc32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    tc::ld32(taddr, r);
-    tc::wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 8; ++i) w[i] = tc::pack16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), half);
+    tc::store_v8(reinterpret_cast<uint16_t *>(base) + idx, w);
 }
 
 struct TileId { int p, tm, tn, split, k_begin, k_end; };
@@ -258,54 +223,70 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
             if (!tc::mbar_wait(tc::smem_u32(&acc_full[buf]), (it >> 1) & 1, abort_flag, &g_dense_error, 4)) break;
             tc::fence_after();
             const uint32_t taddr = tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16);
+            // 16 columns at a time: sixteen warps of 96 registers hide each other's waits for tensor memory, the special
+            // function unit and memory better than eight that take 32 (mlp step at 4093 x 768/2048: EPI_BEFORE -> EPI_AFTER us)
             if (EPI == kStore) {
-                for (int c = side * (kBN / 2); c < (side + 1) * (kBN / 2); c += 32) {
-                    float v[32];
-                    acc32(taddr + c, v);
+#pragma unroll 2
+                for (int c = side * (kBN / 4); c < (side + 1) * (kBN / 4); c += 16) {
+                    uint32_t v[16];
+                    tc::ld16_ahead(taddr + c, v);
+                    tc::wait_ld();
                     const int col = t.tn * kBN + c;
-                    if (row >= q.m) continue;
-                    if (q.splits == 1) store32(q.out, row * q.ld_out + col, v, q.n - col, half);
-                    else store32_f32(q.partial + ((long long)t.split * q.m + row) * q.n + col, v, q.n - col);
+                    if (row >= q.m || col >= q.n) continue;
+                    if (q.splits == 1) store16(q.out, row * q.ld_out + col, v, half);
+                    else {
+                        float *dst = q.partial + ((long long)t.split * q.m + row) * q.n + col;
+                        uint32_t lo[8], hi[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) { lo[i] = v[i]; hi[i] = v[8 + i]; }
+                        tc::store_v8(dst, lo);
+                        tc::store_v8(dst + 8, hi);
+                    }
                 }
             } else if (EPI == kSwiglu) {
-                for (int c = side * (kBN / 4); c < (side + 1) * (kBN / 4); c += 32) {
-                    float g[32], u[32];
-                    acc32(taddr + c, g);
-                    acc32(taddr + kBN / 2 + c, u);
+#pragma unroll 1
+                for (int c = side * (kBN / 8); c < (side + 1) * (kBN / 8); c += 16) {
+                    uint32_t g[16], u[16];
+                    tc::ld16_ahead(taddr + c, g);
+                    tc::ld16_ahead(taddr + kBN / 2 + c, u);
+                    tc::wait_ld();
                     const int col = t.tn * (kBN / 2) + c;
-                    if (row < q.m) {
-                        if (p.gu) {
-                            store32(p.gu, row * p.ld_gu + col, g, q.n - col, half);
-                            store32(p.gu, row * p.ld_gu + p.d_ff + col, u, q.n - col, half);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid(g[i]) * u[i];
-                        store32(q.out, row * q.ld_out + col, g, q.n - col, half);
+                    if (row >= q.m || col >= q.n) continue;
+                    if (p.gu) {
+                        store16(p.gu, row * p.ld_gu + col, g, half);
+                        store16(p.gu, row * p.ld_gu + p.d_ff + col, u, half);
                     }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float gv = __uint_as_float(g[i]);
+                        g[i] = __float_as_uint(gv * sigmoid(gv) * __uint_as_float(u[i]));
+                    }
+                    store16(q.out, row * q.ld_out + col, g, half);
                 }
             } else {
-                for (int c = side * (kBN / 2); c < (side + 1) * (kBN / 2); c += 32) {
+#pragma unroll 1
+                for (int c = side * (kBN / 4); c < (side + 1) * (kBN / 4); c += 16) {
                     const int col = t.tn * kBN + c;
-                    uint32_t gw[16], uw[16];
-                    if (row < q.m) {
-                        load32(p.gu, row * p.ld_gu + col, gw, q.n - col);
-                        load32(p.gu, row * p.ld_gu + p.d_ff + col, uw, q.n - col);
+                    const bool in = row < q.m && col < q.n;
+                    uint32_t gw[8], uw[8], dh[16];
+                    tc::ld16_ahead(taddr + c, dh);
+                    if (in) {
+                        tc::load_v8(reinterpret_cast<const uint16_t *>(p.gu) + row * p.ld_gu + col, gw);
+                        tc::load_v8(reinterpret_cast<const uint16_t *>(p.gu) + row * p.ld_gu + p.d_ff + col, uw);
                     }
-                    float dh[32];
-                    acc32(taddr + c, dh);
-                    if (row < q.m) {
-                        float g[32], u[32];
+                    tc::wait_ld();
+                    if (!in) continue;
+                    uint32_t dg[8], du[8];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float2 g2 = tc::unpack16(gw[i >> 1], half), u2 = tc::unpack16(uw[i >> 1], half);
-                            const float gv = (i & 1) ? g2.y : g2.x, uv = (i & 1) ? u2.y : u2.x;
-                            const float s = sigmoid(gv), a = gv * s, d = dh[i];
-                            g[i] = d * uv * (s + a * (1.f - s));
-                            u[i] = d * a;
-                        }
-                        store32(q.out, row * q.ld_out + col, g, q.n - col, half);
-                        store32(q.out, row * q.ld_out + p.d_ff + col, u, q.n - col, half);
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 g = tc::unpack16(gw[i], half), u = tc::unpack16(uw[i], half);
+                        const float s0 = sigmoid(g.x), a0 = g.x * s0, d0 = __uint_as_float(dh[2 * i]);
+                        const float s1 = sigmoid(g.y), a1 = g.y * s1, d1 = __uint_as_float(dh[2 * i + 1]);
+                        dg[i] = tc::pack16(d0 * u.x * (s0 + a0 * (1.f - s0)), d1 * u.y * (s1 + a1 * (1.f - s1)), half);
+                        du[i] = tc::pack16(d0 * a0, d1 * a1, half);
                     }
+                    tc::store_v8(reinterpret_cast<uint16_t *>(q.out) + row * q.ld_out + col, dg);
+                    tc::store_v8(reinterpret_cast<uint16_t *>(q.out) + row * q.ld_out + p.d_ff + col, du);
                 }
             }
             tc::fence_before();
