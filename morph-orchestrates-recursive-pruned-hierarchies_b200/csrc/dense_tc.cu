@@ -132,6 +132,8 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
     __syncthreads();
     tc::cluster_sync();                                   // barriers of both CTAs are initialised
     tc::fence_after();
+    tc::let_next();
+    tc::after_previous();                                 // returns at once when this launch waits for none
     const uint32_t tmem = tmem_base_s;
     volatile int *abort_flag = &abort_s;
 
@@ -309,6 +311,8 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
 // out[m][n] = the parts of its reduction added in order, 8 columns a thread
 __global__ void __launch_bounds__(256)
 dense_reduce_kernel(const float *__restrict__ partial, int splits, long long m, int n, void *out, long long ld_out, int half) {
+    tc::let_next();
+    tc::after_previous();
     const long long total = m * (n / 8), at = (long long)blockIdx.x * 256 + threadIdx.x;
     if (at >= total) return;
     const long long row = at / (n / 8);
@@ -401,15 +405,16 @@ int join(const DenseParams &p, cudaStream_t st) {
     for (int i = 0; i < p.n_problems; ++i) {
         const Problem &q = p.prob[i];
         if (q.splits == 1) continue;
-        dense_reduce_kernel<<<(unsigned)((q.m * (q.n / 8) + 255) / 256), 256, 0, st>>>(q.partial, q.splits, q.m, q.n, q.out,
-                                                                                      q.ld_out, p.half);
-        MORTAR_CUDA_CHECK(cudaGetLastError());
+        const int rc = tc::launch_after(dense_reduce_kernel, (unsigned)((q.m * (q.n / 8) + 255) / 256), 256u, 0, st,
+                                        (const float *)q.partial, q.splits, q.m, q.n, q.out, q.ld_out, p.half);
+        if (rc != MORTAR_OK) return rc;
     }
     return MORTAR_OK;
 }
 
+// `follows`: the launch reads what the one before it in the call wrote, and may be set up while that one ends
 template <int EPI>
-int launch(const DenseParams &p, cudaStream_t st) {
+int launch(const DenseParams &p, bool follows, cudaStream_t st) {
     static bool ready[64] = {false};
     int sms = 0;
     int rc = tc::allow_smem(dense_pair_kernel<EPI>, kSmem, ready, g_dense_mutex, nullptr);
@@ -417,6 +422,7 @@ int launch(const DenseParams &p, cudaStream_t st) {
     rc = tc::sm_count(&sms);
     if (rc != MORTAR_OK) return rc;
     const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
+    if (follows) return tc::launch_after(dense_pair_kernel<EPI>, (unsigned)(2 * clusters), (unsigned)kThreads, kSmem, st, p);
     dense_pair_kernel<EPI><<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
     MORTAR_CUDA_CHECK(cudaGetLastError());
     return MORTAR_OK;
@@ -496,14 +502,14 @@ extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64
     p.gu = gate_up_sums;
     p.ld_gu = 2LL * d_ff;
     rc = add_problem(p, kSwiglu, x, ldx, false, gate_up, ld_gate_up, false, rows, d_ff, d_model, hidden, d_ff);
-    if (rc == MORTAR_OK) rc = launch<kSwiglu>(p, st);
+    if (rc == MORTAR_OK) rc = launch<kSwiglu>(p, false, st);
     if (rc != MORTAR_OK) return rc;
     alignas(64) DenseParams p2 = {};
     p2.half = p.half;
     rc = add_problem(p2, kStore, hidden, d_ff, false, down, ld_down, false, rows, d_model, d_ff, y, ldy);
     if (rc != MORTAR_OK) return rc;
     cut(p2, parts, scratch);
-    rc = launch<kStore>(p2, st);
+    rc = launch<kStore>(p2, true, st);
     return rc == MORTAR_OK ? join(p2, st) : rc;
 }
 
@@ -538,7 +544,7 @@ extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const voi
         p.gu = const_cast<void *>(gate_up_sums);
         p.ld_gu = f2;
         rc = add_problem(p, kSwigluBackward, dy, lddy, false, down, ld_down, true, rows, d_ff, d_model, dgate_up_sums, f2);
-        if (rc == MORTAR_OK) rc = launch<kSwigluBackward>(p, st);
+        if (rc == MORTAR_OK) rc = launch<kSwigluBackward>(p, false, st);
         if (rc != MORTAR_OK) return rc;
     }
     alignas(64) DenseParams p = {};
@@ -551,7 +557,7 @@ extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const voi
         rc = add_problem(p, kStore, dy, lddy, true, hidden, d_ff, true, d_model, d_ff, rows, ddown, d_ff);
     if (rc != MORTAR_OK || p.n_problems == 0) return rc;
     cut(p, parts, scratch);
-    rc = launch<kStore>(p, st);
+    rc = launch<kStore>(p, dx || dgate_up, st);
     return rc == MORTAR_OK ? join(p, st) : rc;
 }
 

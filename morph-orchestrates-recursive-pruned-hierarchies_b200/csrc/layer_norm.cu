@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(kBackwardThreads<NE>, 1)
 layer_norm_backward_kernel(const T *__restrict__ dy, long long lddy, const T *__restrict__ x, long long ldx, long long rows,
                            int cols, const float *__restrict__ w, const float *__restrict__ stats, T *__restrict__ dx,
                            long long lddx, float *__restrict__ partial, int warps) {
+    tc::let_next();
     __shared__ float2 red[kBackwardWarps][2][16];
     extern __shared__ float fold[];                      // [groups][columns, rounded up to the group's]
     Group g = make_group(warps, red);
@@ -532,6 +533,7 @@ __global__ void __launch_bounds__(32 * kWholeWarps, 1)
 layer_norm_whole_backward_kernel(const T *__restrict__ dy, long long lddy, const T *__restrict__ x, long long ldx,
                                  long long rows, int cols, const float *__restrict__ w, const float *__restrict__ stats,
                                  T *__restrict__ dx, long long lddx, float *__restrict__ partial, int warps) {
+    tc::let_next();
     constexpr bool kAhead = NE * sizeof(T) <= 4;         // registers for a row on its way: 16-bit rows of two units, fp32 of one
     __shared__ float2 red[kWholeWarps][2][16];
     extern __shared__ float fold[];                      // [groups][columns, rounded up to the group's]
@@ -691,6 +693,7 @@ template <class T>
 __global__ void __launch_bounds__(kThreads)
 layer_norm_far_dw_kernel(const T *dy, long long lddy, const T *x, long long ldx, long long rows, int cols,
                      const float *stats, float *partial, long long rows_per_split) {
+    tc::let_next();
     const int c = blockIdx.x * kThreads + threadIdx.x;
     if (c >= cols) return;
     const long long r0 = blockIdx.y * rows_per_split, r1 = min(rows, r0 + rows_per_split);
@@ -709,6 +712,7 @@ layer_norm_far_dw_kernel(const T *dy, long long lddy, const T *x, long long ldx,
 __global__ void __launch_bounds__(kThreads)
 layer_norm_reduce_kernel(const float *__restrict__ partial, int splits, int cols, float *dw, float *db) {
     __shared__ float part[8][33];
+    tc::after_previous();
     const int lane = threadIdx.x & 31, chain = threadIdx.x >> 5;
     const long long c = (long long)blockIdx.x * 32 + lane;
     float s = 0.f;
@@ -881,8 +885,8 @@ int backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t r
         }
     }
     if (partial) {
-        layer_norm_reduce_kernel<<<(unsigned)((2LL * cols + 31) / 32), kThreads, 0, st>>>(partial, (int)splits, cols, dw, db);
-        MORTAR_CUDA_CHECK(cudaGetLastError());
+        return tc::launch_after(layer_norm_reduce_kernel, (unsigned)((2LL * cols + 31) / 32), (unsigned)kThreads, 0, st,
+                                (const float *)partial, (int)splits, (int)cols, dw, db);
     }
     return MORTAR_OK;
 }

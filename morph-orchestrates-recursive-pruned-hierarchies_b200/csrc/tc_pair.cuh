@@ -188,6 +188,28 @@ __device__ __forceinline__ void drain_after_abort() {
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
 }
 
+// A kernel launched with `launch_after` may start while the one before it in the stream still runs; it
+// calls `after_previous` before it touches that kernel's results.  `let_next` in the earlier kernel
+// lets the next one start (its blocks take their places as this one's leave).
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;\n"); }
+
+template <class Kernel, class... Args>
+inline int launch_after(Kernel kernel, unsigned grid, unsigned block, int smem, cudaStream_t st, const Args &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    MORTAR_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return MORTAR_OK;
+}
+
 // [rows][cols] 8-bit row-major with row stride ld as a 2-D map with a [box_rows][128] box and the
 // 128-byte swizzle.
 inline int encode_u8_2d(CUtensorMap *map, const void *base, int64_t cols, int64_t rows, int64_t ld,
