@@ -1,4 +1,4 @@
-// Products for a few tokens (1 to 32 rows): bound by reading the weights once.
+// Products for a few tokens (up to 32 rows of 16-bit operands, 16 of 8-bit ones): bound by reading the weights once.
 //
 // A warp multiplies 16 weight rows by up to 8, 16 or 32 tokens with mma.sync (M = 16 weight rows, N = 8
 // tokens): at these sizes the tensor cores idle either way, and operands that go straight from
@@ -8,9 +8,10 @@
 // bytes is the i-th operand register.  With the gate, a warp's 16 rows are 8 gate rows and the 8 up rows
 // of the same hidden columns: a thread then holds both sums of its outputs.
 //
-// The warps of a CTA take the pieces of k in turn and add their sums through shared memory in warp
-// order; where there are too few row tiles for the SMs, a cluster of CTAs shares a tile's k and adds
-// in rank order.  The order is fixed, so the same call gives the same bits.
+// One CTA of sixteen warps an SM walks the row tiles; its warps take the pieces of k in turn, the next
+// tile's weights are on their way while this one's sums are added through shared memory, in warp order.
+// Where there are too few row tiles for the SMs, a cluster of CTAs shares a tile's k and adds in rank
+// order.  The order is fixed, so the same call gives the same bits.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -21,7 +22,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 
 enum Kind { kBf16 = 0, kF16 = 1, k8 = 2 };
@@ -54,126 +55,151 @@ __device__ __forceinline__ void store(const small::Params &p, long long idx, flo
     else reinterpret_cast<__half *>(p.out)[idx] = __float2half_rn(v);
 }
 
-// NT: groups of 8 tokens.  A piece is 64 bytes of k; `kUnroll` pieces of a warp are in flight together (for 8-bit
-// operands two pieces make a block with its own scales).
+// Weights of one batch: `kUnroll` pieces of two rows, and their block scales.
+template <int N> struct Batch { uint4 a[N], b[N]; float sa, sb; };
+
+// NT: groups of 8 tokens.  A piece is 64 bytes of k, a batch `kUnroll` of them a warp, and `kSlots` batches, of this tile
+// and the next ones, are on their way or at work: about 64 KB an SM in flight (for 8-bit operands a batch is one block
+// with its own scales).
 template <int KIND, int XT, int WT, int NT, bool GATED>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 1)
 small_kernel(const __grid_constant__ small::Params p) {
-    constexpr int kUnroll = 4;
+    constexpr int kUnroll = KIND != k8 && NT == 1 ? 4 : 2;
+    constexpr int kSlots = kUnroll == 4 || NT == 4 ? 2 : 3;
     __shared__ float part[kWarps][16][8 * NT + 1];
-    __shared__ float tile[16][8 * NT];
+    __shared__ float tile_s[16][8 * NT];
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int tile_id = blockIdx.x / ranks, n0 = tile_id * (GATED ? 8 : 16);
-    // rows of w of this thread: accumulator rows g and g + 8
-    const int row_a = n0 + g, row_b = GATED ? p.up_row + n0 + g : n0 + g + 8;
-    const bool in_a = row_a < p.n, in_b = GATED ? in_a : row_b < p.n;
-    const uint8_t *wa = p.w + (long long)row_a * p.ldw + 16 * t, *wb = p.w + (long long)row_b * p.ldw + 16 * t;
-    const int pieces = (p.k_bytes + 63) >> 6;
-    const int step = KIND == k8 ? 2 : 1;                             // pieces that stay with one warp
-    const int slots = kWarps * ranks, slot = rank * kWarps + warp;
+    constexpr int kTileRows = GATED ? 8 : 16;
+    const int tiles = (p.n + kTileRows - 1) / kTileRows, tile_step = (int)gridDim.x / ranks;
+    const int pieces = (p.k_bytes + 63) >> 6, slots = kWarps * ranks, slot = rank * kWarps + warp;
 
+    // the j-th piece of this warp; every warp makes the same number of batches, the last ones empty-handed
+    auto piece_of = [&](int j) { return KIND == k8 ? ((j >> 1) * slots + slot) * 2 + (j & 1) : j * slots + slot; };
+    const int batches = KIND == k8 ? (pieces + 2 * slots - 1) / (2 * slots) : (pieces + kUnroll * slots - 1) / (kUnroll * slots);
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    Batch<kUnroll> w[kSlots];
+    int next_tile = (int)blockIdx.x / ranks, next_batch = 0;             // what is fetched next
+    auto fetch = [&](Batch<kUnroll> &s) {
+        if (next_tile >= tiles) return;
+        // rows of w of this thread: accumulator rows g and g + 8
+        const int row_a = next_tile * kTileRows + g, row_b = GATED ? p.up_row + row_a : row_a + 8;
+        const bool in_a = row_a < p.n, in_b = GATED ? in_a : row_b < p.n;
+        const uint8_t *wa = p.w + (long long)row_a * p.ldw + 16 * t, *wb = p.w + (long long)row_b * p.ldw + 16 * t;
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) {
+            const int at = piece_of(next_batch * kUnroll + j) * 64;
+            const bool in = at + 16 * t < p.k_bytes;
+            s.a[j] = in && in_a ? load_stream(wa + at) : zero;
+            s.b[j] = in && in_b ? load_stream(wb + at) : zero;
+        }
+        if constexpr (KIND == k8) {
+            const int blk = piece_of(next_batch * kUnroll) >> 1;
+            const bool in = 2 * blk < pieces;
+            s.sa = in && in_a ? __ldg(p.ws + (long long)(row_a >> 7) * p.ld_ws + blk) : 0.f;
+            s.sb = in && in_b ? __ldg(p.ws + (long long)(row_b >> 7) * p.ld_ws + blk) : 0.f;
+        }
+        if (++next_batch == batches) {
+            next_batch = 0;
+            next_tile += tile_step;
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) fetch(w[s]);
+    if (p.after_previous) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    else asm volatile("griddepcontrol.launch_dependents;\n");
+
+    uint4 x[NT][kUnroll];
+    float xs[NT][2];
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-
-    // the j-th piece of this warp
-    auto piece_of = [&](int j) { return KIND == k8 ? ((j >> 1) * slots + slot) * 2 + (j & 1) : j * slots + slot; };
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    uint4 a[kUnroll], b[kUnroll];
-    auto fetch = [&](int j0) {
+    int tile = (int)blockIdx.x / ranks, batch = 0;
+    bool have_x = false;                                                 // one batch a tile: its tokens stay
+    while (tile < tiles) {
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) {
-            const int at = piece_of(j0 + j) * 64, in = at + 16 * t < p.k_bytes;
-            a[j] = in && in_a ? load_stream(wa + at) : zero;
-            b[j] = in && in_b ? load_stream(wb + at) : zero;
-        }
-    };
-    fetch(0);
-    if (p.after_previous) asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    else asm volatile("griddepcontrol.launch_dependents;\n");
-    for (int j0 = 0; piece_of(j0) < pieces; j0 += kUnroll) {
-        uint4 x[NT][kUnroll];
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < kUnroll; ++j) {
-                const int at = piece_of(j0 + j) * 64 + 16 * t, m = 8 * i + g;
-                x[i][j] = at < p.k_bytes && m < p.rows ? *reinterpret_cast<const uint4 *>(p.x + m * p.ldx + at) : zero;
-            }
-        uint4 ca[kUnroll], cb[kUnroll];
-#pragma unroll
-        for (int j = 0; j < kUnroll; ++j) { ca[j] = a[j]; cb[j] = b[j]; }
-        fetch(j0 + kUnroll);
-        if constexpr (KIND != k8) {
-#pragma unroll
-            for (int j = 0; j < kUnroll; ++j)
+        for (int s = 0; s < kSlots; ++s) {
+            if (tile >= tiles) break;
+            if (!have_x) {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    mma<KIND, XT, WT>(acc[i], ca[j].x, cb[j].x, ca[j].y, cb[j].y, x[i][j].x, x[i][j].y);
-                    mma<KIND, XT, WT>(acc[i], ca[j].z, cb[j].z, ca[j].w, cb[j].w, x[i][j].z, x[i][j].w);
-                }
-        } else {
 #pragma unroll
-            for (int j = 0; j < kUnroll; j += 2) {
-                const int blk = piece_of(j0 + j) >> 1;
-                if (2 * blk >= pieces) continue;
-                const float sa = in_a ? __ldg(p.ws + (long long)(row_a >> 7) * p.ld_ws + blk) : 0.f;
-                const float sb = in_b ? __ldg(p.ws + (long long)(row_b >> 7) * p.ld_ws + blk) : 0.f;
+                    for (int j = 0; j < kUnroll; ++j) {
+                        const int at = piece_of(batch * kUnroll + j) * 64 + 16 * t, m = 8 * i + g;
+                        x[i][j] = at < p.k_bytes && m < p.rows ? *reinterpret_cast<const uint4 *>(p.x + m * p.ldx + at) : zero;
+                    }
+                    if constexpr (KIND == k8) {
+                        const int blk = piece_of(batch * kUnroll) >> 1, m = 8 * i + 2 * t;
+                        const bool in = 2 * blk < pieces;
+                        xs[i][0] = in && m < p.rows ? p.xs[m * p.ld_xs + blk] : 0.f;
+                        xs[i][1] = in && m + 1 < p.rows ? p.xs[(m + 1) * p.ld_xs + blk] : 0.f;
+                    }
+                }
+                have_x = batches == 1;
+            }
+            Batch<kUnroll> &c = w[s];
+            if constexpr (KIND != k8) {
+#pragma unroll
+                for (int j = 0; j < kUnroll; ++j)
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        mma<KIND, XT, WT>(acc[i], c.a[j].x, c.b[j].x, c.a[j].y, c.b[j].y, x[i][j].x, x[i][j].y);
+                        mma<KIND, XT, WT>(acc[i], c.a[j].z, c.b[j].z, c.a[j].w, c.b[j].w, x[i][j].z, x[i][j].w);
+                    }
+            } else {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        mma<KIND, XT, WT>(d, ca[j + h].x, cb[j + h].x, ca[j + h].y, cb[j + h].y, x[i][j + h].x, x[i][j + h].y);
-                        mma<KIND, XT, WT>(d, ca[j + h].z, cb[j + h].z, ca[j + h].w, cb[j + h].w, x[i][j + h].z, x[i][j + h].w);
+                        mma<KIND, XT, WT>(d, c.a[h].x, c.b[h].x, c.a[h].y, c.b[h].y, x[i][h].x, x[i][h].y);
+                        mma<KIND, XT, WT>(d, c.a[h].z, c.b[h].z, c.a[h].w, c.b[h].w, x[i][h].z, x[i][h].w);
                     }
-                    const int m = 8 * i + 2 * t;
-                    const float x0 = m < p.rows ? p.xs[m * p.ld_xs + blk] : 0.f, x1 = m + 1 < p.rows ? p.xs[(m + 1) * p.ld_xs + blk] : 0.f;
-                    acc[i][0] = fmaf(d[0], sa * x0, acc[i][0]);
-                    acc[i][1] = fmaf(d[1], sa * x1, acc[i][1]);
-                    acc[i][2] = fmaf(d[2], sb * x0, acc[i][2]);
-                    acc[i][3] = fmaf(d[3], sb * x1, acc[i][3]);
+                    acc[i][0] = fmaf(d[0], c.sa * xs[i][0], acc[i][0]);
+                    acc[i][1] = fmaf(d[1], c.sa * xs[i][1], acc[i][1]);
+                    acc[i][2] = fmaf(d[2], c.sb * xs[i][0], acc[i][2]);
+                    acc[i][3] = fmaf(d[3], c.sb * xs[i][1], acc[i][3]);
                 }
             }
-        }
-    }
-    (void)step;
+            fetch(c);
+            if (++batch < batches) continue;
+            batch = 0;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        part[warp][g][8 * i + 2 * t] = acc[i][0];
-        part[warp][g][8 * i + 2 * t + 1] = acc[i][1];
-        part[warp][g + 8][8 * i + 2 * t] = acc[i][2];
-        part[warp][g + 8][8 * i + 2 * t + 1] = acc[i][3];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * 8 * NT; i += kThreads) {
-        const int r = i & 15, m = i >> 4;
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) s += part[w][r][m];
-        tile[r][m] = s;
-    }
-    if (ranks > 1) {
-        cluster.sync();                                              // every rank's sums are there
-        if (rank == 0)
-            for (int i = threadIdx.x; i < 16 * 8 * NT; i += kThreads) {
-                float s = tile[i & 15][i >> 4];
-                for (int r = 1; r < ranks; ++r) s += cluster.map_shared_rank(&tile[0][0], r)[(i & 15) * 8 * NT + (i >> 4)];
-                tile[i & 15][i >> 4] = s;                            // read by this thread's peers after the barrier below
+            for (int i = 0; i < NT; ++i) {
+                part[warp][g][8 * i + 2 * t] = acc[i][0];
+                part[warp][g][8 * i + 2 * t + 1] = acc[i][1];
+                part[warp][g + 8][8 * i + 2 * t] = acc[i][2];
+                part[warp][g + 8][8 * i + 2 * t + 1] = acc[i][3];
+                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
             }
-        cluster.sync();                                              // and no rank leaves before they have been read
-        if (rank) return;
-    } else {
-        __syncthreads();
-    }
-    constexpr int kOut = GATED ? 8 : 16;
-    for (int i = threadIdx.x; i < kOut * 8 * NT; i += kThreads) {
-        const int r = i % kOut, m = i / kOut;
-        if (m < p.rows && n0 + r < p.n) {
-            const float v = GATED ? silu(tile[r][m]) * tile[r + 8][m] : tile[r][m];
-            store(p, m * p.ld_out + n0 + r, v);
+            __syncthreads();
+            for (int i = threadIdx.x; i < 16 * 8 * NT; i += kThreads) {
+                const int r = i & 15, m = i >> 4;
+                float sum = 0.f;
+#pragma unroll
+                for (int v = 0; v < kWarps; ++v) sum += part[v][r][m];
+                tile_s[r][m] = sum;
+            }
+            if (ranks > 1) cluster.sync();                           // every rank's sums are there
+            else __syncthreads();
+            if (rank == 0)
+                for (int i = threadIdx.x; i < kTileRows * 8 * NT; i += kThreads) {
+                    const int r = i % kTileRows, m = i / kTileRows;
+                    if (m >= p.rows || tile * kTileRows + r >= p.n) continue;
+                    float v = tile_s[r][m], u = GATED ? tile_s[r + 8][m] : 0.f;
+                    for (int q = 1; q < ranks; ++q) {
+                        const float *other = cluster.map_shared_rank(&tile_s[0][0], q);
+                        v += other[r * 8 * NT + m];
+                        if (GATED) u += other[(r + 8) * 8 * NT + m];
+                    }
+                    if (GATED) v = silu(v) * u;
+                    store(p, m * p.ld_out + tile * kTileRows + r, v);
+                }
+            // a tile's sums are not written again, and no rank leaves, before they have been read; in one CTA the next
+            // tile's first barrier sees to that
+            if (ranks > 1) cluster.sync();
+            tile += tile_step;
         }
     }
 }
@@ -182,11 +208,12 @@ template <int KIND, int XT, int WT, int NT, bool GATED>
 int run(const small::Params &p, int sms, cudaStream_t st) {
     const int tiles = (p.n + (GATED ? 7 : 15)) / (GATED ? 8 : 16);
     const int pieces = (p.k_bytes + 63) / 64;
-    // four CTAs an SM, as long as a warp keeps two pieces (a whole scaled block) to itself
+    // a CTA an SM, as long as a warp keeps a piece (a whole scaled block) to itself
     int ranks = 1;
-    while (ranks < 8 && tiles * ranks * 2 <= 4 * sms && pieces >= 2 * kWarps * ranks * 2) ranks *= 2;
+    while (ranks < 8 && tiles * ranks * 2 <= sms && pieces >= (KIND == k8 ? 2 : 1) * kWarps * ranks * 2) ranks *= 2;
+    const int at_once = sms / ranks < tiles ? sms / ranks : tiles;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * ranks));
+    cfg.gridDim = dim3((unsigned)(at_once * ranks));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -206,11 +233,13 @@ int pick(const small::Params &p, int sms, cudaStream_t st) {
     if (p.up_row) {
         if (p.rows <= 8) return run<KIND, XT, WT, 1, true>(p, sms, st);
         if (p.rows <= 16) return run<KIND, XT, WT, 2, true>(p, sms, st);
-        return run<KIND, XT, WT, 4, true>(p, sms, st);
+        if constexpr (KIND != k8) return run<KIND, XT, WT, 4, true>(p, sms, st);
+        return MORTAR_ERR_CAPACITY;
     }
     if (p.rows <= 8) return run<KIND, XT, WT, 1, false>(p, sms, st);
     if (p.rows <= 16) return run<KIND, XT, WT, 2, false>(p, sms, st);
-    return run<KIND, XT, WT, 4, false>(p, sms, st);
+    if constexpr (KIND != k8) return run<KIND, XT, WT, 4, false>(p, sms, st);
+    return MORTAR_ERR_CAPACITY;
 }
 
 }  // namespace

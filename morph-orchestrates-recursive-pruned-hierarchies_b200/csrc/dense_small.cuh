@@ -6,7 +6,10 @@
 
 namespace small {
 
-constexpr int kMaxRows = 32;
+// Most rows that these kernels take, against the tensor-memory kernels of dense_tc.cu and fp8_tc.cu with their 256-row
+// tiles (us, L2 flushed, 2048/5632): 16-bit block of 32 rows 39 here, 45 there; 8-bit 2048 -> 11264 of 16 rows 18 here and
+// 21 there, of 32 rows 25 here and 22 there.
+constexpr int kMaxRows = 32, kMaxRows8 = 16;
 
 struct Params {
     const uint8_t *x, *w;            // rows of bytes

@@ -319,7 +319,7 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     int sms = 0;
     int rc = tc::sm_count(&sms);
     if (rc != MORTAR_OK) return rc;
-    if (rows <= small::kMaxRows) {
+    if (rows <= small::kMaxRows8) {
         small::Params q = {};
         q.x = (const uint8_t *)x; q.ldx = ldx; q.w = (const uint8_t *)w; q.ldw = ldw;
         q.rows = (int)rows; q.n = gated ? out_features / 2 : out_features; q.up_row = gated ? out_features / 2 : 0;

@@ -959,21 +959,28 @@ def rmsnorm_rows(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Ten
 
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16,
          torch.float8_e4m3fn: _lib.E4M3, torch.float8_e5m2: _lib.E5M2}
-_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
-_FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
+_FLOAT_CODE = {dt: c for dt, c in _CODE.items() if c <= _lib.F16}
+_FP8_CODE = {dt: c for dt, c in _CODE.items() if c > _lib.F16}
+
+
+_entry: dict = {}                              # entry points looked up so far
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 
 
 def _launch(where: str, t: torch.Tensor, *args) -> None:
     """Calls the library's ``where`` with ``args`` and the current stream of the device of ``t``, on that
     device.  Tensors go in as their addresses: building pointer objects and a Stream object costs
     more than a small kernel runs."""
-    fn = getattr(_lib.lib(), where)
+    fn = _entry.get(where)
+    if fn is None:
+        fn = _entry[where] = getattr(_lib.lib(), where)
     index = t.get_device()
-    if index == torch.cuda.current_device():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            status = fn(*args, _raw_stream(index))
     if status:
         _lib.check(status, where)
 
@@ -1039,15 +1046,15 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Op
     (None unless ``want_stats``)."""
     if not x.is_cuda:
         _require_cuda(x, "x")
-    code = _CODE.get(x.dtype)
-    if code is None or code > _lib.F16 or x.dim() < 1:
+    code = _FLOAT_CODE.get(x.dtype)
+    if code is None or x.dim() < 1:
         raise ValueError(f"x must be a float32, bfloat16 or float16 tensor [..., cols], got {x.dtype}")
     cols = x.shape[-1]
     if cols < 1:
         raise ValueError("the last dimension is empty: a mean of nothing is not defined")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None:
-            if t.dim() != 1 or t.shape[0] != cols or t.dtype not in _FLOATS:
+            if t.dim() != 1 or t.shape[0] != cols or t.dtype not in _FLOAT_CODE:
                 raise ValueError(f"{name} must be a float tensor [{cols}], got {t.dtype} {list(t.shape)}")
             _same_device(x, name, t)
     y = _like(x)
@@ -1069,8 +1076,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     fp32 [cols]; what is not wanted is None."""
     if not x.is_cuda:
         _require_cuda(x, "x")
-    code = _CODE.get(x.dtype)
-    if code is None or code > _lib.F16 or dy.shape != x.shape:
+    code = _FLOAT_CODE.get(x.dtype)
+    if code is None or dy.shape != x.shape:
         raise ValueError(f"dy has shape {list(dy.shape)}, x {list(x.shape)} ({x.dtype})")
     for name, t in (("dy", dy), ("weight", weight), ("stats", stats)):
         _same_device(x, name, t)
@@ -1142,21 +1149,23 @@ def dense_error(reset: bool = True) -> int:
 
 
 def _mlp_dense_args(x, gate_up, down):
-    _require_cuda(x, "x")
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"mlp_dense takes bfloat16 or float16 activations, got {x.dtype}")
+    if not x.is_cuda:
+        _require_cuda(x, "x")
+    dt = x.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise ValueError(f"mlp_dense takes bfloat16 or float16 activations, got {dt}")
     if x.dim() < 1 or gate_up.dim() != 2 or down.dim() != 2:
         raise ValueError("x [..., d_model], gate_up [2 d_ff, d_model] and down [d_model, d_ff] expected")
     d_model, d_ff = down.shape
-    if tuple(gate_up.shape) != (2 * d_ff, d_model) or x.shape[-1] != d_model:
+    if gate_up.shape != (2 * d_ff, d_model) or x.shape[-1] != d_model:
         raise ValueError(f"x {list(x.shape)}, gate_up {list(gate_up.shape)} and down {list(down.shape)} do not fit: "
                          f"x [..., d_model], gate_up [2 d_ff, d_model] and down [d_model, d_ff] expected")
     if d_model < 1 or d_ff < 1 or d_model % TILE or d_ff % TILE:
         raise ValueError(f"d_model and d_ff must be positive multiples of {TILE}, got {d_model} and {d_ff}")
-    for name, t in (("gate_up", gate_up), ("down", down)):
-        if t.dtype != x.dtype:
-            raise ValueError(f"{name} is {t.dtype}, x is {x.dtype}: one type for all")
-        _same_device(x, name, t)
+    if gate_up.dtype is not dt or down.dtype is not dt:
+        raise ValueError(f"gate_up is {gate_up.dtype}, down {down.dtype} and x {dt}: one type for all")
+    _same_device(x, "gate_up", gate_up)
+    _same_device(x, "down", down)
     return d_model, d_ff
 
 
@@ -1248,10 +1257,11 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1, dtype: torch.dtype = t
     value nearest to x / scale, ties to even, for every input type.  A block of zeros has scale 1;
     one that holds an infinity or a NaN has scale NaN and reads back as NaN.  cols is a multiple
     of 16."""
-    _require_cuda(x, "x")
-    if x.dim() != 2 or x.dtype not in _FLOATS:
+    if not x.is_cuda:
+        _require_cuda(x, "x")
+    if x.dim() != 2 or x.dtype not in _FLOAT_CODE:
         raise ValueError(f"quantize_fp8 takes a 2-D float32, bfloat16 or float16 tensor, got {x.dtype} {list(x.shape)}")
-    if dtype not in _FP8:
+    if dtype not in _FP8_CODE:
         raise ValueError(f"dtype must be float8_e4m3fn or float8_e5m2, got {dtype}")
     if block_rows not in (1, 128):
         raise ValueError(f"block_rows must be 1 or 128, got {block_rows}")
@@ -1272,10 +1282,11 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1, dtype: torch.dtype = t
 def dequantize_fp8(q: torch.Tensor, scale: torch.Tensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """q * scale, rounded once to ``out_dtype``, for what ``quantize_fp8`` gives (or another program
     made, with any scales).  One scale row per row of q, or one per 128 rows."""
-    _require_cuda(q, "q")
-    if q.dim() != 2 or q.dtype not in _FP8:
+    if not q.is_cuda:
+        _require_cuda(q, "q")
+    if q.dim() != 2 or q.dtype not in _FP8_CODE:
         raise ValueError(f"q must be a 2-D float8_e4m3fn or float8_e5m2 tensor, got {q.dtype} {list(q.shape)}")
-    if out_dtype not in _FLOATS:
+    if out_dtype not in _FLOAT_CODE:
         raise ValueError(f"unsupported out_dtype {out_dtype}")
     rows, cols = q.shape
     if cols < 1 or cols % TILE:
@@ -1313,39 +1324,43 @@ def linear_fp8(x: torch.Tensor, w: Fp8Matrix, *, x_scale: Optional[torch.Tensor]
     ``out_dtype`` (default: the type of x, bfloat16 for 8-bit x).  The 8-bit floating-point
     counterpart of ``linear_tc_i8``; for serving, not differentiable (inputs that require a
     gradient are refused while gradients are enabled)."""
-    _require_cuda(x, "x")
-    if x.dtype not in _FLOATS + _FP8 or x.dim() < 1:
-        raise ValueError(f"x must be a float or float8 tensor [..., in], got {x.dtype}")
-    if (x_scale is None) != (x.dtype in _FLOATS):
+    if not x.is_cuda:
+        _require_cuda(x, "x")
+    dt, in_features, out_features = x.dtype, w.in_features, w.out_features
+    if dt not in _CODE or x.dim() < 1:
+        raise ValueError(f"x must be a float or float8 tensor [..., in], got {dt}")
+    if (x_scale is None) != (dt in _FLOAT_CODE):
         raise ValueError("x_scale goes with an 8-bit x, and only with one")
-    if x.shape[-1] != w.in_features:
-        raise ValueError(f"x has last dim {x.shape[-1]}, expected {w.in_features}")
+    if x.shape[-1] != in_features:
+        raise ValueError(f"x has last dim {x.shape[-1]}, expected {in_features}")
     if _wants_grad(x, x_scale):
         raise ValueError("linear_fp8 is not differentiable: detach x or call it under torch.no_grad()")
-    if swiglu and w.out_features % 256:
-        raise ValueError(f"swiglu needs out_features to be a multiple of 256, got {w.out_features}")
+    if swiglu and out_features % 256:
+        raise ValueError(f"swiglu needs out_features to be a multiple of 256, got {out_features}")
     if out_dtype is None:
-        out_dtype = x.dtype if x.dtype in _FLOATS else torch.bfloat16
-    if out_dtype not in _FLOATS:
+        out_dtype = dt if dt in _FLOAT_CODE else torch.bfloat16
+    out_code = _FLOAT_CODE.get(out_dtype)
+    if out_code is None:
         raise ValueError(f"unsupported out_dtype {out_dtype}")
-    _same_device(x, "w", w.data)
-    _same_device(x, "x_scale", x_scale)
-    lead, nb = x.shape[:-1], -(-w.in_features // 128)
-    x2 = x if x.dim() == 2 else x.reshape(-1, w.in_features)
+    data, scale = w.data, w.scale
+    _same_device(x, "w", data)
+    x2 = x if x.dim() == 2 else x.reshape(-1, in_features)
     rows = x2.shape[0]
     if x_scale is None:
         x2, s2 = quantize_fp8(x2)
     else:
-        if x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (*lead, nb):
-            raise ValueError(f"x_scale must be float32 {[*lead, nb]}, got {x_scale.dtype} {list(x_scale.shape)}")
+        _same_device(x, "x_scale", x_scale)
+        if x_scale.dtype is not torch.float32 or x_scale.shape != (*x.shape[:-1], -(-in_features // 128)):
+            raise ValueError(f"x_scale must be float32 {[*x.shape[:-1], -(-in_features // 128)]}, got {x_scale.dtype} "
+                             f"{list(x_scale.shape)}")
         x2, s2 = _rows16(x2), _rows_any(x_scale)
-    n_out = w.out_features // 2 if swiglu else w.out_features
-    out = x.new_empty((*lead, n_out), dtype=out_dtype)
+    n_out = out_features // 2 if swiglu else out_features
+    out = x.new_empty((*x.shape[:-1], n_out), dtype=out_dtype)
     if rows == 0:
         return out
     _launch("mortar_linear_fp8", x, x2.data_ptr(), _CODE[x2.dtype], x2.stride(0), s2.data_ptr(), s2.stride(0), rows,
-            w.data.data_ptr(), _CODE[w.data.dtype], w.data.stride(0), w.scale.data_ptr(), w.scale.stride(0),
-            w.out_features, w.in_features, _lib.FLAG_SWIGLU if swiglu else 0, out.data_ptr(), _CODE[out_dtype], n_out)
+            data.data_ptr(), _CODE[data.dtype], data.stride(0), scale.data_ptr(), scale.stride(0), out_features,
+            in_features, _lib.FLAG_SWIGLU if swiglu else 0, out.data_ptr(), out_code, n_out)
     _count("linear_fp8")
     return out
 
@@ -1357,7 +1372,7 @@ def mlp_fp8(x: torch.Tensor, gate_up: Fp8Matrix, down: Fp8Matrix, *,
     16-bit x), quantise the hidden block, down product.  Four launches; for serving."""
     if gate_up.out_features != 2 * down.in_features or gate_up.in_features != down.out_features:
         raise ValueError("gate_up must be [2 d_ff, d_model] and down [d_model, d_ff]")
-    if x.dtype not in _FLOATS:
+    if x.dtype not in _FLOAT_CODE:
         raise ValueError(f"mlp_fp8 takes float32, bfloat16 or float16 activations, got {x.dtype}")
     h = linear_fp8(x, gate_up, swiglu=True, out_dtype=torch.float16 if x.dtype == torch.float16 else torch.bfloat16)
     return linear_fp8(h, down, out_dtype=x.dtype if out_dtype is None else out_dtype)
