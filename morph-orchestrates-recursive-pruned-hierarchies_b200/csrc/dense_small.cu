@@ -217,13 +217,17 @@ int run(const small::Params &p, int sms, cudaStream_t st) {
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = p.after_previous ? 2 : 1;
+    if (ranks > 1) {
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = (unsigned)ranks;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+    }
+    if (p.after_previous) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     MORTAR_CUDA_CHECK(cudaLaunchKernelEx(&cfg, small_kernel<KIND, XT, WT, NT, GATED>, p));
     return MORTAR_OK;
 }

@@ -780,7 +780,8 @@ Layout whole_layout(int64_t rows, int32_t cols, int most_units) {
 
 // the rows' types leave registers for so many units
 template <class T> constexpr int kWholeForward = sizeof(T) == 4 ? 2 : 3;
-constexpr int kWholeBackward = 2;
+template <class T> constexpr int kWholeBackward = sizeof(T) == 4 ? 1 : 2;             // with a row on its way; fp32 rows of more
+                                                                                      // than 4096 columns take 2 without
 
 bool whole_rows(const void *p, int64_t ld, size_t elem) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (size_t)ld * elem % 16 == 0;
@@ -859,7 +860,7 @@ int backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t r
     Layout wl = {0, 0, 0};
     if (cols % kUnit == 0 && whole_rows(x, ldx, sizeof(T)) && whole_rows(dy, lddy, sizeof(T)) &&
         (!dx || whole_rows(dx, lddx, sizeof(T))))
-        wl = whole_layout(rows, cols, kWholeBackward);
+        wl = whole_layout(rows, cols, cols <= 4096 ? kWholeBackward<T> : 2);
     if (wl.units) {
         const int rc = wl.units == 1 ? run_whole_backward<T, 1>(wl, dy, lddy, x, ldx, rows, cols, w, stats, dx, lddx, partial, splits, st)
                                      : run_whole_backward<T, 2>(wl, dy, lddy, x, ldx, rows, cols, w, stats, dx, lddx, partial, splits, st);
