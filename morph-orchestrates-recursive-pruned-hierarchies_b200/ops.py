@@ -6,6 +6,7 @@ morph/sparse/stk/backend/custom_ops.py:35).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
@@ -1088,6 +1089,16 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     rows = x2.shape[0]
     if stats.dtype != torch.float32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
         raise ValueError(f"stats must be contiguous float32 [2, {rows}]")
+    return _layer_norm_grads(d2, x, x2, code, weight, stats, want_dx, want_dweight, want_dbias)
+
+
+@functools.lru_cache(maxsize=256)
+def _layer_norm_scratch(rows: int, cols: int) -> int:
+    return _lib.lib().mortar_layer_norm_scratch_floats(rows, cols)
+
+
+def _layer_norm_grads(d2, x, x2, code, weight, stats, want_dx, want_dweight, want_dbias):
+    rows, cols = x2.shape
     dx = _like(x) if want_dx else None
     dw = x.new_empty((cols,), dtype=torch.float32) if want_dweight else None
     db = x.new_empty((cols,), dtype=torch.float32) if want_dbias else None
@@ -1095,13 +1106,12 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
     if not (want_dx or want_dweight or want_dbias):
         return dx, dw, db
-    w = _f32(weight)
     scratch, n = None, 0
     if want_dweight or want_dbias:
-        n = _lib.lib().mortar_layer_norm_scratch_floats(rows, cols)
+        n = _layer_norm_scratch(rows, cols)
         scratch = x.new_empty((n,), dtype=torch.float32)
     _launch("mortar_layer_norm_backward", x, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), code, rows, cols,
-            _at(w), stats.data_ptr(), _at(dx), cols, _at(dw), _at(db), _at(scratch), n)
+            _at(_f32(weight)), stats.data_ptr(), _at(dx), cols, _at(dw), _at(db), _at(scratch), n)
     _count("layer_norm_backward", 2 if n else 1)
     return dx, dw, db
 
@@ -1117,8 +1127,10 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         _once("layer_norm")
-        x, weight, stats = ctx.saved_tensors
-        dx, dw, db = layer_norm_backward(dy, x, weight, stats, *ctx.needs_input_grad[:3])
+        x, weight, stats = ctx.saved_tensors                # as the forward call checked them
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dx, dw, db = _layer_norm_grads(_rows_any(dy), x, _rows_any(x), _FLOAT_CODE[x.dtype], weight, stats, need_x, need_w,
+                                       need_b)
         if dw is not None and weight.dtype != torch.float32:
             dw = dw.to(weight.dtype)
         if db is not None and ctx.bias_dtype != torch.float32:
