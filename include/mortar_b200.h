@@ -632,11 +632,11 @@ int mortar_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int6
  * strides that are multiples of 8; what is written or kept 32-byte aligned, ldy a multiple of 16.
  *   hidden        device [rows][d_ff], written: the hidden block (scratch, and an input of the
  *                 backward call)
- *   gate_up_sums  device [rows][2 d_ff], written for the backward call, or NULL
+ *   gate_up_sums  device fp32 [rows][2 d_ff], written for the backward call, or NULL
  * Bounded in-kernel waits report through mortar_dense_error. */
 int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64_t rows, const void *gate_up,
                      int64_t ld_gate_up, const void *down, int64_t ld_down, int32_t d_model, int32_t d_ff,
-                     void *hidden, void *gate_up_sums, void *y, int64_t ldy, float *scratch,
+                     void *hidden, float *gate_up_sums, void *y, int64_t ldy, float *scratch,
                      int64_t scratch_floats, void *stream);
 /* fp32 values the call needs as scratch (32-byte aligned; 0 = none, negative = error): the parts of
  * reductions that are cut where there are few tiles, added in order by a launch of their own.
@@ -645,11 +645,12 @@ int64_t mortar_mlp_dense_scratch_floats(int64_t rows, int32_t d_model, int32_t d
 
 /* Gradients of mortar_mlp_dense from dy [rows][d_model], its inputs, `hidden` and `gate_up_sums`:
  * dx [rows][d_model], dgate_up [2 d_ff][d_model], ddown [d_model][d_ff], contiguous, 32-byte aligned, of
- * the same type; each may be NULL.  `dgate_up_sums` [rows][2 d_ff] is scratch of that type. */
+ * the same type; each may be NULL.  `dgate_up_sums` [rows][2 d_ff] is scratch of that type (the gradients of the
+ * sums, rounded for the tensor cores). */
 int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int32_t dtype,
                               int64_t rows, const void *gate_up, int64_t ld_gate_up, const void *down,
                               int64_t ld_down, int32_t d_model, int32_t d_ff, const void *hidden,
-                              const void *gate_up_sums, void *dgate_up_sums, void *dx, void *dgate_up,
+                              const float *gate_up_sums, void *dgate_up_sums, void *dx, void *dgate_up,
                               void *ddown, float *scratch, int64_t scratch_floats, void *stream);
 int64_t mortar_mlp_dense_backward_scratch_floats(int64_t rows, int32_t d_model, int32_t d_ff,
                                                  int32_t want_dx, int32_t want_dgate_up,

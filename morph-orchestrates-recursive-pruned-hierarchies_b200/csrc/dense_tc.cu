@@ -62,7 +62,7 @@ struct DenseParams {
     int n_problems, n_items;
     int half;                // 1: fp16, 0: bf16
     int d_ff;                // kSwiglu / kSwigluBackward: rows between a gate row and its up row
-    void *gu;                // kSwiglu: where gate and up sums are kept ([m][2 d_ff], or NULL); kSwigluBackward: read
+    float *gu;               // kSwiglu: where gate and up sums are kept ([m][2 d_ff], or NULL); kSwigluBackward: read
     void *hidden;            // unused by kStore
     long long ld_gu;
 };
@@ -77,6 +77,15 @@ __device__ __forceinline__ void store16(void *base, long long idx, const uint32_
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = tc::pack16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), half);
     tc::store_v8(reinterpret_cast<uint16_t *>(base) + idx, w);
+}
+
+// 16 accumulator columns as they are
+__device__ __forceinline__ void store16_f32(float *dst, const uint32_t (&v)[16]) {
+    uint32_t lo[8], hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { lo[i] = v[i]; hi[i] = v[8 + i]; }
+    tc::store_v8(dst, lo);
+    tc::store_v8(dst + 8, hi);
 }
 
 struct TileId { int p, tm, tn, split, k_begin, k_end; };
@@ -236,14 +245,7 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
                     const int col = t.tn * kBN + c;
                     if (row >= q.m || col >= q.n) continue;
                     if (q.splits == 1) store16(q.out, row * q.ld_out + col, v, half);
-                    else {
-                        float *dst = q.partial + ((long long)t.split * q.m + row) * q.n + col;
-                        uint32_t lo[8], hi[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) { lo[i] = v[i]; hi[i] = v[8 + i]; }
-                        tc::store_v8(dst, lo);
-                        tc::store_v8(dst + 8, hi);
-                    }
+                    else store16_f32(q.partial + ((long long)t.split * q.m + row) * q.n + col, v);
                 }
             } else if (EPI == kSwiglu) {
 #pragma unroll 1
@@ -255,8 +257,10 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
                     const int col = t.tn * (kBN / 2) + c;
                     if (row >= q.m || col >= q.n) continue;
                     if (p.gu) {
-                        store16(p.gu, row * p.ld_gu + col, g, half);
-                        store16(p.gu, row * p.ld_gu + p.d_ff + col, u, half);
+                        // kept as fp32: rounded to 16 bits they would add a third rounding to the gradients (error
+                        // 0.0030 instead of 0.0024 of the norm in bf16)
+                        store16_f32(p.gu + row * p.ld_gu + col, g);
+                        store16_f32(p.gu + row * p.ld_gu + p.d_ff + col, u);
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -270,22 +274,30 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
                 for (int c = side * (kBN / 4); c < (side + 1) * (kBN / 4); c += 16) {
                     const int col = t.tn * kBN + c;
                     const bool in = row < q.m && col < q.n;
-                    uint32_t gw[8], uw[8], dh[16];
+                    uint32_t gw[16], uw[16], dh[16];
                     tc::ld16_ahead(taddr + c, dh);
                     if (in) {
-                        tc::load_v8(reinterpret_cast<const uint16_t *>(p.gu) + row * p.ld_gu + col, gw);
-                        tc::load_v8(reinterpret_cast<const uint16_t *>(p.gu) + row * p.ld_gu + p.d_ff + col, uw);
+                        const float *gp = p.gu + row * p.ld_gu + col, *up = gp + p.d_ff;
+                        tc::load_v8(gp, gw);
+                        tc::load_v8(gp + 8, gw + 8);
+                        tc::load_v8(up, uw);
+                        tc::load_v8(up + 8, uw + 8);
                     }
                     tc::wait_ld();
                     if (!in) continue;
                     uint32_t dg[8], du[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float2 g = tc::unpack16(gw[i], half), u = tc::unpack16(uw[i], half);
-                        const float s0 = sigmoid(g.x), a0 = g.x * s0, d0 = __uint_as_float(dh[2 * i]);
-                        const float s1 = sigmoid(g.y), a1 = g.y * s1, d1 = __uint_as_float(dh[2 * i + 1]);
-                        dg[i] = tc::pack16(d0 * u.x * (s0 + a0 * (1.f - s0)), d1 * u.y * (s1 + a1 * (1.f - s1)), half);
-                        du[i] = tc::pack16(d0 * a0, d1 * a1, half);
+                        float o[2], v[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float g = __uint_as_float(gw[2 * i + j]), u = __uint_as_float(uw[2 * i + j]);
+                            const float s = sigmoid(g), a = g * s, d = __uint_as_float(dh[2 * i + j]);
+                            o[j] = d * u * (s + a * (1.f - s));
+                            v[j] = d * a;
+                        }
+                        dg[i] = tc::pack16(o[0], o[1], half);
+                        du[i] = tc::pack16(v[0], v[1], half);
                     }
                     tc::store_v8(reinterpret_cast<uint16_t *>(q.out) + row * q.ld_out + col, dg);
                     tc::store_v8(reinterpret_cast<uint16_t *>(q.out) + row * q.ld_out + p.d_ff + col, du);
@@ -466,7 +478,7 @@ extern "C" int64_t mortar_mlp_dense_backward_scratch_floats(int64_t rows, int32_
 
 extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64_t rows, const void *gate_up,
                                 int64_t ld_gate_up, const void *down, int64_t ld_down, int32_t d_model, int32_t d_ff,
-                                void *hidden, void *gate_up_sums, void *y, int64_t ldy, float *scratch, int64_t scratch_floats,
+                                void *hidden, float *gate_up_sums, void *y, int64_t ldy, float *scratch, int64_t scratch_floats,
                                 void *stream) {
     if (!x || !gate_up || !down || !hidden || !y) return MORTAR_ERR_NULL;
     int rc = check_shape(dtype, rows, d_model, d_ff);
@@ -516,7 +528,7 @@ extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64
 extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int32_t dtype,
                                          int64_t rows, const void *gate_up, int64_t ld_gate_up, const void *down,
                                          int64_t ld_down, int32_t d_model, int32_t d_ff, const void *hidden,
-                                         const void *gate_up_sums, void *dgate_up_sums, void *dx, void *dgate_up,
+                                         const float *gate_up_sums, void *dgate_up_sums, void *dx, void *dgate_up,
                                          void *ddown, float *scratch, int64_t scratch_floats, void *stream) {
     if (!dy || !x || !gate_up || !down || !hidden || !gate_up_sums || !dgate_up_sums) return MORTAR_ERR_NULL;
     int rc = check_shape(dtype, rows, d_model, d_ff);
@@ -541,7 +553,7 @@ extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const voi
         alignas(64) DenseParams p = {};
         p.half = dtype == MORTAR_F16;
         p.d_ff = d_ff;
-        p.gu = const_cast<void *>(gate_up_sums);
+        p.gu = const_cast<float *>(gate_up_sums);
         p.ld_gu = f2;
         rc = add_problem(p, kSwigluBackward, dy, lddy, false, down, ld_down, true, rows, d_ff, d_model, dgate_up_sums, f2);
         if (rc == MORTAR_OK) rc = launch<kSwigluBackward>(p, false, st);

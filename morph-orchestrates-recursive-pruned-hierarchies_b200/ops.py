@@ -1183,14 +1183,14 @@ def _mlp_dense_args(x, gate_up, down):
 
 def mlp_dense_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, want_saved: bool):
     """``mlp_dense`` without its gradient: (y, hidden, sums) with hidden [rows, d_ff] and, when
-    ``want_saved``, sums [rows, 2 d_ff] = x gate_up^T for ``mlp_dense_backward`` (else None)."""
+    ``want_saved``, sums fp32 [rows, 2 d_ff] = x gate_up^T for ``mlp_dense_backward`` (else None)."""
     d_model, d_ff = _mlp_dense_args(x, gate_up, down)
     x2 = _rows16(x if x.dim() == 2 else x.reshape(-1, d_model))
     gu, dn = _rows16(gate_up), _rows16(down)
     rows = x2.shape[0]
     y = _like(x)
     hidden = x.new_empty((rows, d_ff))
-    sums = x.new_empty((rows, 2 * d_ff)) if want_saved else None
+    sums = x.new_empty((rows, 2 * d_ff), dtype=torch.float32) if want_saved else None
     if rows == 0:
         return y, hidden, sums
     n = _lib.lib().mortar_mlp_dense_scratch_floats(rows, d_model, d_ff, want_saved)
@@ -1215,9 +1215,9 @@ def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor,
     d2, x2 = _rows16((dy if dy.dtype == dt else dy.to(dt)).reshape(-1, d_model)), _rows16(x.reshape(-1, d_model))
     gu, dn = _rows16(gate_up), _rows16(down)
     rows = x2.shape[0]
-    for name, t, n in (("hidden", hidden, d_ff), ("sums", sums, 2 * d_ff)):
-        if tuple(t.shape) != (rows, n) or t.dtype != dt or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous {dt} [{rows}, {n}]")
+    for name, t, n, want in (("hidden", hidden, d_ff, dt), ("sums", sums, 2 * d_ff, torch.float32)):
+        if tuple(t.shape) != (rows, n) or t.dtype != want or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {want} [{rows}, {n}]")
     dx = _like(x) if want_dx else None
     dgu = x.new_empty((2 * d_ff, d_model)) if want_dgate_up else None
     ddn = x.new_empty((d_model, d_ff)) if want_ddown else None
@@ -1225,7 +1225,7 @@ def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor,
         return dx, dgu, ddn
     if rows == 0:
         return dx, None if dgu is None else dgu.zero_(), None if ddn is None else ddn.zero_()
-    dsums = torch.empty_like(sums)
+    dsums = x.new_empty((rows, 2 * d_ff))
     n = _lib.lib().mortar_mlp_dense_backward_scratch_floats(rows, d_model, d_ff, want_dx, want_dgate_up, want_ddown)
     scratch = x.new_empty((n,), dtype=torch.float32) if n > 0 else None
     _launch("mortar_mlp_dense_backward", x, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), _CODE[dt], rows,
@@ -1253,8 +1253,9 @@ def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor) -> tor
     x [..., d_model], ``gate_up`` = [Wg; Wu] [2 d_ff, d_model] and ``down`` [d_model, d_ff], all
     bfloat16 or all float16; the dense counterpart of ``mlp_prefill_blocks``
     (morph/model/transformer.py:402-431), differentiable in all three.  d_model and d_ff are
-    multiples of 16.  Sums are fp32; the hidden block and the result are rounded once each, and
-    for the backward pass so are the gate and up sums that it keeps and their gradients.  The note on
+    multiples of 16.  Sums are fp32; the hidden block and the result are rounded once each.  For the
+    backward pass x, the hidden block and the gate and up sums (fp32) are kept; the sums' gradients
+    are rounded once, for the tensor cores, and so are the results.  The note on
     captured backward passes in ``layer_norm`` holds here too."""
     if _wants_grad(x, gate_up, down):
         return _MlpDense.apply(x, gate_up, down)

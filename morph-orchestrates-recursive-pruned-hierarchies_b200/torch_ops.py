@@ -303,7 +303,7 @@ def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor,
 @mlp_dense.register_fake
 def _(x, gate_up, down):
     rows, d_ff = x.numel() // x.shape[-1], down.shape[1]
-    return x.new_empty(x.shape), x.new_empty((rows, d_ff)), x.new_empty((rows, 2 * d_ff))
+    return x.new_empty(x.shape), x.new_empty((rows, d_ff)), x.new_empty((rows, 2 * d_ff), dtype=torch.float32)
 
 
 @torch.library.custom_op(f"{_LIB}::mlp_dense_backward", mutates_args=(), device_types="cuda")
