@@ -17,6 +17,13 @@
 // issues the copies of its CTA, one thread of CTA 0 issues the MMAs of both, warps 2..17 read the
 // accumulators (two sets, so that a tile's epilogue runs under the next tile's MMAs).
 // Every wait is bounded.
+//
+// What bounds it: at 8192 x 2048/5632 every launch draws its operands from L2 at 12.2 to 12.4 TB/s (128 KB a
+// 128-wide step and cluster), which is all that L2 gives: gate/up 236 us = 1600 TFLOP/s without and 278 us with
+// the kept sums, down 137 us = 1380, dh 194 us (its epilogue moves 0.7 GB more), the three last products
+// together 594 us = 1590 TFLOP/s with the tensor pipe busy 88% of the time.  A hand-off of 64-wide steps with
+// one wait for four MMAs reached 1200.  Under the power cap of a long run the whole step comes to 1150 of the
+// library product's sustained 1400 TFLOP/s.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cstdint>
@@ -235,7 +242,8 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
             tc::fence_after();
             const uint32_t taddr = tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16);
             // 16 columns at a time: sixteen warps of 96 registers hide each other's waits for tensor memory, the special
-            // function unit and memory better than eight that take 32 (mlp step at 4093 x 768/2048: EPI_BEFORE -> EPI_AFTER us)
+            // function unit and memory better than eight that take 32 (backward at 4093 x 768/2048: 100 -> 89 us).  Turning
+            // the pieces in shared memory so that lanes lie side by side in memory changed nothing: see the header
             if (EPI == kStore) {
 #pragma unroll 2
                 for (int c = side * (kBN / 4); c < (side + 1) * (kBN / 4); c += 16) {

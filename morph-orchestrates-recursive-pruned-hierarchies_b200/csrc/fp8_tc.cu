@@ -10,9 +10,16 @@
 // block's begins: one pipeline stage is one block (128 bytes of k, a swizzle row), its four MMAs
 // (kind::f8f6f4, K = 32) write one of two accumulator sets, and the epilogue warps read the set,
 // multiply by sx * sw (one factor per thread and 128 columns) and add it to fp32 sums in registers
-// while the MMAs fill the other set.  A cluster of two CTAs computes 256 x 256: per SM and block the
-// MMAs take 512 cycles, the tensor-memory reads of 128 x 256 sums about 256 and their multiply-adds
-// 256 issue slots of each scheduler, so the sums keep up with the MMAs.
+// while the MMAs fill the other set.  A cluster of two CTAs computes 256 x 256: every thread of eight
+// epilogue warps keeps 128 sums, for which the launch's registers are dealt out anew.
+//
+// What bounds it, at 8192 x 2048 -> 11264 with the gate (213 to 225 us, 1700 TFLOP/s): the epilogue warps.
+// The same MMAs and copies with one sum per tile instead of one per block take 139 us.  A block's MMAs are
+// 512 cycles; a warp needs about 800 for it: 150 to see that the block is there, twice 75 to read 64 columns
+// and 150 to multiply and add them (3 cycles a packed multiply-add), 75 to hand the set back, the rest to
+// walk on; and 5700 a tile for the gate and the stores.  Tried without gain: four sets of 128 columns (279
+// us), reading 32 columns ahead (238), asking for the next block before the multiply-adds (the register it
+// takes costs more than it hides), arrivals with release at cluster scope (630: they wait for the stores).
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cstdint>
