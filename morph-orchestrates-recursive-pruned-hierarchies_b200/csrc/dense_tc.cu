@@ -248,6 +248,7 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
 #pragma unroll 2
                 for (int c = side * (kBN / 4); c < (side + 1) * (kBN / 4); c += 16) {
                     uint32_t v[16];
+                    __syncwarp();                                     // lanes whose row does not exist are back
                     tc::ld16_ahead(taddr + c, v);
                     tc::wait_ld();
                     const int col = t.tn * kBN + c;
@@ -259,6 +260,7 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
 #pragma unroll 1
                 for (int c = side * (kBN / 8); c < (side + 1) * (kBN / 8); c += 16) {
                     uint32_t g[16], u[16];
+                    __syncwarp();
                     tc::ld16_ahead(taddr + c, g);
                     tc::ld16_ahead(taddr + kBN / 2 + c, u);
                     tc::wait_ld();
@@ -283,6 +285,7 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
                     const int col = t.tn * kBN + c;
                     const bool in = row < q.m && col < q.n;
                     uint32_t gw[16], uw[16], dh[16];
+                    __syncwarp();
                     tc::ld16_ahead(taddr + c, dh);
                     if (in) {
                         const float *gp = p.gu + row * p.ld_gu + col, *up = gp + p.d_ff;
@@ -328,7 +331,8 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// out[m][n] = the parts of its reduction added in order, 8 columns a thread
+// out[m][n] = the parts of its reduction added in order, 8 columns a thread.  The parts are read past L1: the kernel
+// may start before the one that writes them has ended.
 __global__ void __launch_bounds__(256)
 dense_reduce_kernel(const float *__restrict__ partial, int splits, long long m, int n, void *out, long long ld_out, int half) {
     tc::let_next();
@@ -346,8 +350,8 @@ dense_reduce_kernel(const float *__restrict__ partial, int splits, long long m, 
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
             const bool in = s0 + s < splits;
-            a[s] = in ? __ldg(src + (s0 + s) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
-            b[s] = in ? __ldg(src + (s0 + s) * step + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+            a[s] = in ? __ldcg(src + (s0 + s) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+            b[s] = in ? __ldcg(src + (s0 + s) * step + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
         for (int s = 0; s < 8; ++s) {

@@ -230,6 +230,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                 if (k > 1) { sx = __ldg(p.xs + ++at_x); s0 = __ldg(p.ws + ++at_w0); s1 = __ldg(p.ws + ++at_w1); }
                 if (!tc::mbar_wait(done0 + 8 * s, parity, abort_flag, &g_fp8_error, 4)) { ok = false; break; }
                 if (++s == kStages) { s = 0; parity ^= 1; }
+                __syncwarp();
                 tc::fence_after();
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {

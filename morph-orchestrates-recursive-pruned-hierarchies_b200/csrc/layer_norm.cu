@@ -723,7 +723,7 @@ layer_norm_reduce_kernel(const float *__restrict__ partial, int splits, int cols
         for (int i0 = chain; i0 < splits; i0 += 80) {
             float v[10];
 #pragma unroll
-            for (int i = 0; i < 10; ++i) v[i] = i0 + 8 * i < splits ? __ldg(partial + (long long)(i0 + 8 * i) * 2 * cols + c) : 0.f;
+            for (int i = 0; i < 10; ++i) v[i] = i0 + 8 * i < splits ? __ldcg(partial + (long long)(i0 + 8 * i) * 2 * cols + c) : 0.f;
 #pragma unroll
             for (int i = 0; i < 10; ++i) s += v[i];
         }

@@ -677,8 +677,10 @@ class Fp8Matrix:
         if scale.device != data.device:
             raise ValueError(f"data is on {data.device} but scale on {scale.device}")
         if data.stride(1) != 1 or data.stride(0) % 16 or data.stride(0) < in_features or data.data_ptr() % 16:
-            data = data.contiguous()
-        self.data, self.scale = data, scale.contiguous()
+            data = data.clone(memory_format=torch.contiguous_format)
+        if not scale.is_contiguous() or scale.stride(0) < want[1]:
+            scale = scale.clone(memory_format=torch.contiguous_format)
+        self.data, self.scale = data, scale
         self.out_features, self.in_features = int(out_features), int(in_features)
 
     @classmethod

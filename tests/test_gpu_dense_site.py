@@ -599,3 +599,80 @@ def test_streams_and_graphs():
         for o, i in zip(outs, order):
             assert all(torch.equal(p, q) for p, q in zip(o, want[i]))
     errors_are_clear()
+
+
+def test_broadcast_gradients_and_second_derivatives():
+    """A gradient of stride 0 (from a sum) counts like one that is written out; create_graph is refused."""
+    dt = torch.bfloat16
+    x, gu, dn = (rand(40, 64, seed=1, dt=dt).requires_grad_(), rand(96, 64, seed=2, scale=0.2, dt=dt).requires_grad_(),
+                 rand(64, 48, seed=3, scale=0.2, dt=dt).requires_grad_())
+    a = torch.autograd.grad(ops.mlp_dense(x, gu, dn).sum(), (x, gu, dn))
+    b = torch.autograd.grad(ops.mlp_dense(x, gu, dn), (x, gu, dn), torch.ones(40, 64, device=DEV, dtype=dt))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    for f in (lambda: ops.mlp_dense(x, gu, dn), lambda: ops.layer_norm(x)):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(f().sum(), x, create_graph=True)
+
+
+def test_one_row_views_and_misaligned_weights():
+    """Rows whose stride says nothing (one row, expanded or sliced), and 8-bit weights that start off 16 bytes."""
+    dt = torch.bfloat16
+    gu, dn = rand(96, 64, seed=2, scale=0.2, dt=dt), rand(64, 48, seed=3, scale=0.2, dt=dt)
+    row = rand(1, 64, seed=1, dt=dt)
+    want = ops.mlp_dense(row, gu, dn)
+    views = [row[0], row.expand(3, 64), rand(5, 64, seed=1, dt=dt)[::5], torch.as_strided(row, (1, 64), (1, 1))]
+    for v in views:
+        y = ops.mlp_dense(v, gu, dn)
+        assert y.shape == v.shape
+        assert torch.equal(ops.layer_norm(v).reshape(-1, 64)[0], ops.layer_norm(v.contiguous().clone()).reshape(-1, 64)[0])
+    assert torch.equal(ops.mlp_dense(views[0], gu, dn), want[0]) and torch.equal(ops.mlp_dense(views[3], gu, dn), want)
+    flat = torch.zeros(64 * 128 + 16, device=DEV, dtype=torch.uint8)
+    m = mb.Fp8Matrix.from_dense(rand(64, 128, seed=4))
+    off = flat[4:4 + 64 * 128].view(m.data.dtype).reshape(64, 128)
+    off.copy_(m.data)
+    x = rand(7, 128, seed=5, dt=dt)
+    assert off.data_ptr() % 16 == 4
+    assert torch.equal(ops.linear_fp8(x, mb.Fp8Matrix(off, m.scale)), ops.linear_fp8(x, m))
+    q, s = ops.quantize_fp8(x[:1])
+    assert torch.equal(ops.linear_fp8(q[0], m, x_scale=s[0]), ops.linear_fp8(q, m, x_scale=s)[0])
+    wide = torch.as_strided(s, (1, 1), (0, 1))
+    assert torch.equal(ops.linear_fp8(q, m, x_scale=wide), ops.linear_fp8(q, m, x_scale=s))
+
+
+def test_calls_from_a_new_thread():
+    """A thread that has made no CUDA call yet (as autograd's do) can make these."""
+    import threading
+    dt = torch.bfloat16
+    x, gu, dn = rand(200, 64, seed=1, dt=dt), rand(512, 64, seed=2, scale=0.2, dt=dt), rand(64, 256, seed=3, scale=0.2, dt=dt)
+    m = mb.Fp8Matrix.from_dense(gu)
+    q, s = ops.quantize_fp8(x)
+    want = [ops.mlp_dense(x, gu, dn), ops.linear_fp8(q, m, x_scale=s, swiglu=True), ops.layer_norm(x)]
+    got = []
+
+    def work():
+        got.extend([ops.mlp_dense(x, gu, dn), ops.linear_fp8(q, m, x_scale=s, swiglu=True), ops.layer_norm(x)])
+        torch.cuda.current_stream().synchronize()
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert len(got) == 3 and all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("rows,d,f", [(256, 32, 16384), (512, 4096, 64), (8192, 32, 48)])
+def test_mlp_dense_cut_reductions(rows, d, f):
+    """Few tiles and long reductions: the products are cut and joined; the same bits every time."""
+    dt = torch.bfloat16
+    x = rand(rows, d, seed=1, dt=dt).requires_grad_()
+    gu, dn = rand(2 * f, d, seed=2, scale=d ** -0.5, dt=dt).requires_grad_(), rand(d, f, seed=3, scale=f ** -0.5, dt=dt).requires_grad_()
+    dy = rand(rows, d, seed=4, dt=dt)
+    y = ops.mlp_dense(x, gu, dn)
+    got = (y.detach(), *torch.autograd.grad(y, (x, gu, dn), dy))
+    *refs, parts = mlp_grads_ref(dy, x.detach(), gu.detach(), dn.detach())
+    for name, p, ref, bound in zip(("y", "dx", "dgate_up", "ddown"), got, refs, mlp_bounds(dy, x.detach(), gu.detach(), dn.detach(), parts, dt)):
+        within(p, ref, bound, name)
+        close_in_norm(p, ref, dt, 2, name)
+    y = ops.mlp_dense(x, gu, dn)
+    again = (y.detach(), *torch.autograd.grad(y, (x, gu, dn), dy))
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+    errors_are_clear()
