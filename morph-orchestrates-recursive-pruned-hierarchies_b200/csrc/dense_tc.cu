@@ -343,21 +343,23 @@ dense_reduce_kernel(const float *__restrict__ partial, int splits, long long m, 
     const int col = (int)(at - row * (n / 8)) * 8;
     const float4 *src = reinterpret_cast<const float4 *>(partial + row * n + col);
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    // eight parts' loads are in flight together: one at a time the kernel waits for memory once a part
+    // eight parts' loads are in flight together; loads under a condition would wait for one another, so the last part
+    // stands in for those that do not exist
     const long long step = m * n / 4;
     for (int s0 = 0; s0 < splits; s0 += 8) {
         float4 a[8], b[8];
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-            const bool in = s0 + s < splits;
-            a[s] = in ? __ldcg(src + (s0 + s) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
-            b[s] = in ? __ldcg(src + (s0 + s) * step + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 *at_s = src + min(s0 + s, splits - 1) * step;
+            a[s] = __ldcg(at_s);
+            b[s] = __ldcg(at_s + 1);
         }
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            v[0] += a[s].x; v[1] += a[s].y; v[2] += a[s].z; v[3] += a[s].w;
-            v[4] += b[s].x; v[5] += b[s].y; v[6] += b[s].z; v[7] += b[s].w;
-        }
+        for (int s = 0; s < 8; ++s)
+            if (s0 + s < splits) {
+                v[0] += a[s].x; v[1] += a[s].y; v[2] += a[s].z; v[3] += a[s].w;
+                v[4] += b[s].x; v[5] += b[s].y; v[6] += b[s].z; v[7] += b[s].w;
+            }
     }
     *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(out) + row * ld_out + col) =
         make_uint4(tc::pack16(v[0], v[1], half), tc::pack16(v[2], v[3], half), tc::pack16(v[4], v[5], half), tc::pack16(v[6], v[7], half));
@@ -393,7 +395,7 @@ std::mutex g_dense_mutex;
 // 128-wide steps that each of the 74 clusters would take if a launch's work were spread evenly, and the parts that a
 // product's reduction is cut into: more than one only where its tiles would run twice as long as that or longer (few
 // rows, or few columns of a weight gradient)
-int64_t even_share(int64_t total_steps) { return total_steps < 74 ? 1 : total_steps / 74; }
+int64_t even_share(int64_t total_steps) { return total_steps < 74 ? 1 : (total_steps + 73) / 74; }
 int64_t parts_of(int64_t k_steps, int64_t share) { return k_steps >= 2 * share ? k_steps / share : 1; }
 int64_t steps_of(int64_t k) { return (k + 127) / 128; }
 int64_t tiles_of(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256); }

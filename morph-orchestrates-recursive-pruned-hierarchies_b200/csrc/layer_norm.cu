@@ -719,14 +719,14 @@ layer_norm_reduce_kernel(const float *__restrict__ partial, int splits, int cols
     const int lane = threadIdx.x & 31, chain = threadIdx.x >> 5;
     const long long c = (long long)blockIdx.x * 32 + lane;
     float s = 0.f;
-    if (c < 2LL * cols)
-        for (int i0 = chain; i0 < splits; i0 += 80) {
-            float v[10];
+    const float *src = partial + min(c, 2LL * cols - 1);
+    for (int i0 = chain; i0 < splits; i0 += 80) {
+        float v[10];
 #pragma unroll
-            for (int i = 0; i < 10; ++i) v[i] = i0 + 8 * i < splits ? __ldcg(partial + (long long)(i0 + 8 * i) * 2 * cols + c) : 0.f;
+        for (int i = 0; i < 10; ++i) v[i] = __ldcg(src + (long long)min(i0 + 8 * i, splits - 1) * 2 * cols);
 #pragma unroll
-            for (int i = 0; i < 10; ++i) s += v[i];
-        }
+        for (int i = 0; i < 10; ++i) s += i0 + 8 * i < splits ? v[i] : 0.f;
+    }
     part[chain][lane] = s;
     __syncthreads();
     if (chain == 0 && c < 2LL * cols) {
