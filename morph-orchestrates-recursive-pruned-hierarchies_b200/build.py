@@ -1,4 +1,5 @@
-"""Builds libmortar_b200.so in-tree with nvcc for sm_100a (cross-compiles without a GPU).
+"""Builds libmortar_b200.so in-tree with nvcc for sm_100a (cross-compiles without a GPU), and the torch
+binding of the dense site's operators, _mortar_native.so, with the host compiler.
 
     python morph-orchestrates-recursive-pruned-hierarchies_b200/build.py [--force] [--verbose]
 """
@@ -12,6 +13,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libmortar_b200.so")
+BINDING = os.path.join(CSRC, "torch_binding.cpp")
+NATIVE = os.path.join(PKG, "_mortar_native.so")
 SOURCES = ["host_pack.cpp", "prefill_sched.cpp", "stream_kernels.cu", "prefill_tc.cu", "stack_decode.cu",
            "router.cu", "backward.cu", "backward_tc.cu", "gemv_tc.cu", "layer_norm.cu", "dense_tc.cu", "fp8_quant.cu",
            "fp8_tc.cu", "dense_small.cu"]
@@ -61,7 +64,32 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError(f"link failed ({res.returncode}): {' '.join(cmd)}")
+    build_binding(force=force, verbose=verbose)
     return LIB
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """Compiles csrc/torch_binding.cpp against the installed torch and links it to the library beside it."""
+    newest = max(os.path.getmtime(f) for f in (BINDING, os.path.join(ROOT, "include", "mortar_b200.h")))
+    if not force and os.path.exists(NATIVE) and os.path.getmtime(NATIVE) >= newest:
+        return NATIVE
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    include = [f"-isystem{d}" for d in cpp_extension.include_paths()]
+    include += [f"-I{d}" for d in (sysconfig.get_paths()["include"], os.environ.get("CUDA_HOME", "/usr/local/cuda") + "/include",
+                                   os.path.join(ROOT, "include"))]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-DTORCH_EXTENSION_NAME=_mortar_native", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *include, BINDING, "-o", NATIVE, f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+           f"-L{PKG}", "-l:libmortar_b200.so", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}): {' '.join(cmd)}")
+    return NATIVE
 
 
 if __name__ == "__main__":

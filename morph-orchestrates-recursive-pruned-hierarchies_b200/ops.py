@@ -6,12 +6,12 @@ morph/sparse/stk/backend/custom_ops.py:35).
 from __future__ import annotations
 
 import ctypes as C
-import functools
 from typing import Optional
 
 import torch
 
 from . import _lib
+from ._native import native
 from .format import TILE, BlockSched, Fp8Matrix, GemvBlocks, MortarMatrix, SchedMatrix, StreamMatrix, TopologyDev
 
 _launches = 0      # kernels launched by this module (bench.py reports it)
@@ -19,14 +19,14 @@ _kernel_counts: dict = {}   # the same, per kernel family
 
 
 def launch_count() -> int:
-    return _launches
+    return _launches + sum(native.kernel_counts().values())
 
 
 def kernel_counts() -> dict:
     """Launches so far per kernel family: "act_prep", "bcsr_stream" (the streaming linear / SwiGLU
     kernel), "prefill_panel" (tcgen05 / tensor memory), "stack_decode", "route_flags", "router".
     Tests use the deltas to tell which kernel an operator or module forward ran."""
-    return dict(_kernel_counts)
+    return {**_kernel_counts, **native.kernel_counts()}
 
 
 def _count(name: str, n: int = 1) -> None:
@@ -957,186 +957,12 @@ def rmsnorm_rows(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Ten
 
 
 # ---- the dense MLP site: norm, block before carving, 8-bit serving form -----------------
-
-_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16,
-         torch.float8_e4m3fn: _lib.E4M3, torch.float8_e5m2: _lib.E5M2}
-_FLOAT_CODE = {dt: c for dt, c in _CODE.items() if c <= _lib.F16}
-_FP8_CODE = {dt: c for dt, c in _CODE.items() if c > _lib.F16}
-
-
-_entry: dict = {}                              # entry points looked up so far
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch.cuda.current_device
-
-
-def _launch(where: str, t: torch.Tensor, *args) -> None:
-    """Calls the library's ``where`` with ``args`` and the current stream of the device of ``t``, on that
-    device.  Tensors go in as their addresses: building pointer objects and a Stream object costs
-    more than a small kernel runs."""
-    fn = _entry.get(where)
-    if fn is None:
-        fn = _entry[where] = getattr(_lib.lib(), where)
-    index = t.get_device()
-    if index == _current_device():
-        status = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, _raw_stream(index))
-    if status:
-        _lib.check(status, where)
-
-
-def _at(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _same_device(t: torch.Tensor, name: str, o: Optional[torch.Tensor]) -> None:
-    if o is not None and o.device != t.device:
-        raise ValueError(f"{name} is on {o.device}, expected {t.device}")
-
-
-def _like(t: torch.Tensor) -> torch.Tensor:
-    """An uninitialised contiguous tensor of the shape and type of ``t``."""
-    if t.is_contiguous():
-        return torch.empty_like(t)
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
-
-
-def _f32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
-        return t
-    return t.detach().float().contiguous()
-
-
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [rows, cols] itself when its rows are contiguous and start on 16 bytes, else a copy."""
-    per16 = 16 // t.element_size()
-    if t.stride(1) != 1 or t.stride(0) % per16 or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _wants_grad(*tensors) -> bool:
-    if not torch.is_grad_enabled():
-        return False
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            return True
-    return False
-
-
-def _once(name: str) -> None:
-    """Called in a backward pass: with ``create_graph`` it would have to be differentiable itself."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{name} has no second derivative: call backward without create_graph")
-
-
-def _rows_any(t: torch.Tensor) -> torch.Tensor:
-    """[..., cols] -> [rows, cols] with contiguous rows that do not overlap."""
-    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:
-        t2 = t2.contiguous()
-        if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:          # one row or one column: strides are free
-            t2 = t2.clone(memory_format=torch.contiguous_format).view(t2.shape)
-    return t2
-
-
-def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
-                       want_stats: bool):
-    """``layer_norm`` without its gradient: (y, stats) with stats fp32 [2, rows] = mean and 1/std
-    (None unless ``want_stats``)."""
-    if not x.is_cuda:
-        _require_cuda(x, "x")
-    code = _FLOAT_CODE.get(x.dtype)
-    if code is None or x.dim() < 1:
-        raise ValueError(f"x must be a float32, bfloat16 or float16 tensor [..., cols], got {x.dtype}")
-    cols = x.shape[-1]
-    if cols < 1:
-        raise ValueError("the last dimension is empty: a mean of nothing is not defined")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            if t.dim() != 1 or t.shape[0] != cols or t.dtype not in _FLOAT_CODE:
-                raise ValueError(f"{name} must be a float tensor [{cols}], got {t.dtype} {list(t.shape)}")
-            _same_device(x, name, t)
-    y = _like(x)
-    x2 = _rows_any(x)
-    rows = x2.shape[0]
-    stats = x.new_empty((2, rows), dtype=torch.float32) if want_stats else None
-    if rows == 0:
-        return y, stats
-    w, b = _f32(weight), _f32(bias)
-    _launch("mortar_layer_norm", x, x2.data_ptr(), code, x2.stride(0), rows, cols, _at(w), _at(b), eps, y.data_ptr(),
-            cols, _at(stats))
-    _count("layer_norm")
-    return y, stats
-
-
-def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor,
-                        want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
-    """(dx, dweight, dbias) of ``layer_norm`` from the stats its forward kept; dweight and dbias are
-    fp32 [cols]; what is not wanted is None."""
-    if not x.is_cuda:
-        _require_cuda(x, "x")
-    code = _FLOAT_CODE.get(x.dtype)
-    if code is None or dy.shape != x.shape:
-        raise ValueError(f"dy has shape {list(dy.shape)}, x {list(x.shape)} ({x.dtype})")
-    for name, t in (("dy", dy), ("weight", weight), ("stats", stats)):
-        _same_device(x, name, t)
-    cols = x.shape[-1]
-    if weight is not None and tuple(weight.shape) != (cols,):
-        raise ValueError(f"weight must be [{cols}], got {list(weight.shape)}")
-    d2, x2 = _rows_any(dy if dy.dtype == x.dtype else dy.to(x.dtype)), _rows_any(x)
-    rows = x2.shape[0]
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
-        raise ValueError(f"stats must be contiguous float32 [2, {rows}]")
-    return _layer_norm_grads(d2, x, x2, code, weight, stats, want_dx, want_dweight, want_dbias)
-
-
-@functools.lru_cache(maxsize=256)
-def _layer_norm_scratch(rows: int, cols: int) -> int:
-    return _lib.lib().mortar_layer_norm_scratch_floats(rows, cols)
-
-
-def _layer_norm_grads(d2, x, x2, code, weight, stats, want_dx, want_dweight, want_dbias):
-    rows, cols = x2.shape
-    dx = _like(x) if want_dx else None
-    dw = x.new_empty((cols,), dtype=torch.float32) if want_dweight else None
-    db = x.new_empty((cols,), dtype=torch.float32) if want_dbias else None
-    if rows == 0:
-        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-    if not (want_dx or want_dweight or want_dbias):
-        return dx, dw, db
-    scratch, n = None, 0
-    if want_dweight or want_dbias:
-        n = _layer_norm_scratch(rows, cols)
-        scratch = x.new_empty((n,), dtype=torch.float32)
-    _launch("mortar_layer_norm_backward", x, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), code, rows, cols,
-            _at(_f32(weight)), stats.data_ptr(), _at(dx), cols, _at(dw), _at(db), _at(scratch), n)
-    _count("layer_norm_backward", 2 if n else 1)
-    return dx, dw, db
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        _once("layer_norm")
-        x, weight, stats = ctx.saved_tensors                # as the forward call checked them
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dx, dw, db = _layer_norm_grads(_rows_any(dy), x, _rows_any(x), _FLOAT_CODE[x.dtype], weight, stats, need_x, need_w,
-                                       need_b)
-        if dw is not None and weight.dtype != torch.float32:
-            dw = dw.to(weight.dtype)
-        if db is not None and ctx.bias_dtype != torch.float32:
-            db = db.to(ctx.bias_dtype)
-        return dx, dw, db, None
-
+#
+# These go through the compiled binding (csrc/torch_binding.cpp), which checks, allocates, picks the
+# stream and holds the autograd rules.  Wrong arguments raise ValueError, CPU tensors
+# NotImplementedError, CUDA failures RuntimeError.  The launch goes to the device of the first tensor and
+# that device's current stream; a tensor whose rows are not contiguous (or, for the tensor cores, do not
+# start on 16 bytes) is copied first; nothing is kept from one call for the next.
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
@@ -1148,9 +974,21 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     every operator here it can be captured into a CUDA graph.  When a backward pass is captured,
     no eager autograd graph over the same leaves may be alive (a rule of torch's autograd, whose
     gradient accumulators remember the stream they were made on)."""
-    if _wants_grad(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, eps)
-    return layer_norm_forward(x, weight, bias, eps, False)[0]
+    return native.layer_norm(x, weight, bias, eps)
+
+
+def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
+                       want_stats: bool):
+    """``layer_norm`` without its gradient: (y, stats) with stats fp32 [2, rows] = mean and 1/std
+    (None unless ``want_stats``)."""
+    return native.layer_norm_forward(x, weight, bias, eps, want_stats)
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor,
+                        want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
+    """(dx, dweight, dbias) of ``layer_norm`` from the stats its forward kept; dweight and dbias are
+    fp32 [cols]; what is not wanted is None."""
+    return native.layer_norm_backward(dy, x, weight, stats, want_dx, want_dweight, want_dbias)
 
 
 def dense_error(reset: bool = True) -> int:
@@ -1160,94 +998,6 @@ def dense_error(reset: bool = True) -> int:
     return code.value
 
 
-def _mlp_dense_args(x, gate_up, down):
-    if not x.is_cuda:
-        _require_cuda(x, "x")
-    dt = x.dtype
-    if dt is not torch.bfloat16 and dt is not torch.float16:
-        raise ValueError(f"mlp_dense takes bfloat16 or float16 activations, got {dt}")
-    if x.dim() < 1 or gate_up.dim() != 2 or down.dim() != 2:
-        raise ValueError("x [..., d_model], gate_up [2 d_ff, d_model] and down [d_model, d_ff] expected")
-    d_model, d_ff = down.shape
-    if gate_up.shape != (2 * d_ff, d_model) or x.shape[-1] != d_model:
-        raise ValueError(f"x {list(x.shape)}, gate_up {list(gate_up.shape)} and down {list(down.shape)} do not fit: "
-                         f"x [..., d_model], gate_up [2 d_ff, d_model] and down [d_model, d_ff] expected")
-    if d_model < 1 or d_ff < 1 or d_model % TILE or d_ff % TILE:
-        raise ValueError(f"d_model and d_ff must be positive multiples of {TILE}, got {d_model} and {d_ff}")
-    if gate_up.dtype is not dt or down.dtype is not dt:
-        raise ValueError(f"gate_up is {gate_up.dtype}, down {down.dtype} and x {dt}: one type for all")
-    _same_device(x, "gate_up", gate_up)
-    _same_device(x, "down", down)
-    return d_model, d_ff
-
-
-def mlp_dense_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, want_saved: bool):
-    """``mlp_dense`` without its gradient: (y, hidden, sums) with hidden [rows, d_ff] and, when
-    ``want_saved``, sums fp32 [rows, 2 d_ff] = x gate_up^T for ``mlp_dense_backward`` (else None)."""
-    d_model, d_ff = _mlp_dense_args(x, gate_up, down)
-    x2 = _rows16(x if x.dim() == 2 else x.reshape(-1, d_model))
-    gu, dn = _rows16(gate_up), _rows16(down)
-    rows = x2.shape[0]
-    y = _like(x)
-    hidden = x.new_empty((rows, d_ff))
-    sums = x.new_empty((rows, 2 * d_ff), dtype=torch.float32) if want_saved else None
-    if rows == 0:
-        return y, hidden, sums
-    n = _lib.lib().mortar_mlp_dense_scratch_floats(rows, d_model, d_ff, want_saved)
-    scratch = x.new_empty((n,), dtype=torch.float32) if n > 0 else None
-    _launch("mortar_mlp_dense", x, x2.data_ptr(), x2.stride(0), _CODE[x.dtype], rows, gu.data_ptr(), gu.stride(0),
-            dn.data_ptr(), dn.stride(0), d_model, d_ff, hidden.data_ptr(), _at(sums), y.data_ptr(), d_model,
-            _at(scratch), n)
-    _count("dense", 3 if n else 2)
-    return y, hidden, sums
-
-
-def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor,
-                       hidden: torch.Tensor, sums: torch.Tensor, want_dx: bool = True, want_dgate_up: bool = True,
-                       want_ddown: bool = True):
-    """(dx, dgate_up, ddown) of ``mlp_dense`` from what its forward kept; all in the type of x."""
-    d_model, d_ff = _mlp_dense_args(x, gate_up, down)
-    if dy.shape != x.shape:
-        raise ValueError(f"dy has shape {list(dy.shape)}, x {list(x.shape)}")
-    for name, t in (("dy", dy), ("hidden", hidden), ("sums", sums)):
-        _same_device(x, name, t)
-    dt = x.dtype
-    d2, x2 = _rows16((dy if dy.dtype == dt else dy.to(dt)).reshape(-1, d_model)), _rows16(x.reshape(-1, d_model))
-    gu, dn = _rows16(gate_up), _rows16(down)
-    rows = x2.shape[0]
-    for name, t, n, want in (("hidden", hidden, d_ff, dt), ("sums", sums, 2 * d_ff, torch.float32)):
-        if tuple(t.shape) != (rows, n) or t.dtype != want or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous {want} [{rows}, {n}]")
-    dx = _like(x) if want_dx else None
-    dgu = x.new_empty((2 * d_ff, d_model)) if want_dgate_up else None
-    ddn = x.new_empty((d_model, d_ff)) if want_ddown else None
-    if not (want_dx or want_dgate_up or want_ddown):
-        return dx, dgu, ddn
-    if rows == 0:
-        return dx, None if dgu is None else dgu.zero_(), None if ddn is None else ddn.zero_()
-    dsums = x.new_empty((rows, 2 * d_ff))
-    n = _lib.lib().mortar_mlp_dense_backward_scratch_floats(rows, d_model, d_ff, want_dx, want_dgate_up, want_ddown)
-    scratch = x.new_empty((n,), dtype=torch.float32) if n > 0 else None
-    _launch("mortar_mlp_dense_backward", x, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), _CODE[dt], rows,
-            gu.data_ptr(), gu.stride(0), dn.data_ptr(), dn.stride(0), d_model, d_ff, hidden.data_ptr(), sums.data_ptr(),
-            dsums.data_ptr(), _at(dx), _at(dgu), _at(ddn), _at(scratch), n)
-    _count("dense_backward", (1 if want_dx or want_dgate_up else 0) + 1)
-    return dx, dgu, ddn
-
-
-class _MlpDense(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gate_up, down):
-        y, hidden, sums = mlp_dense_forward(x, gate_up, down, True)
-        ctx.save_for_backward(x, gate_up, down, hidden, sums)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        _once("mlp_dense")
-        return mlp_dense_backward(dy, *ctx.saved_tensors, *ctx.needs_input_grad)
-
-
 def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor) -> torch.Tensor:
     """The gated feed-forward block before it is carved: y = (silu(x Wg^T) * (x Wu^T)) Wd^T for
     x [..., d_model], ``gate_up`` = [Wg; Wu] [2 d_ff, d_model] and ``down`` [d_model, d_ff], all
@@ -1255,11 +1005,23 @@ def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor) -> tor
     (morph/model/transformer.py:402-431), differentiable in all three.  d_model and d_ff are
     multiples of 16.  Sums are fp32; the hidden block and the result are rounded once each.  For the
     backward pass x, the hidden block and the gate and up sums (fp32) are kept; the sums' gradients
-    are rounded once, for the tensor cores, and so are the results.  The note on
-    captured backward passes in ``layer_norm`` holds here too."""
-    if _wants_grad(x, gate_up, down):
-        return _MlpDense.apply(x, gate_up, down)
-    return mlp_dense_forward(x, gate_up, down, False)[0]
+    are rounded once, for the tensor cores, and so are the results.  The note on captured backward
+    passes in ``layer_norm`` holds here too."""
+    return native.mlp_dense(x, gate_up, down)
+
+
+def mlp_dense_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, want_saved: bool):
+    """``mlp_dense`` without its gradient: (y, hidden, sums) with hidden [rows, d_ff] and, when
+    ``want_saved``, sums fp32 [rows, 2 d_ff] = x gate_up^T for ``mlp_dense_backward`` (else None)."""
+    return native.mlp_dense_forward(x, gate_up, down, want_saved)
+
+
+def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor,
+                       hidden: torch.Tensor, sums: torch.Tensor, want_dx: bool = True, want_dgate_up: bool = True,
+                       want_ddown: bool = True):
+    """(dx, dgate_up, ddown) of ``mlp_dense`` from what its forward kept; all in the type of x; what is
+    not wanted is None."""
+    return native.mlp_dense_backward(dy, x, gate_up, down, hidden, sums, want_dx, want_dgate_up, want_ddown)
 
 
 def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1, dtype: torch.dtype = torch.float8_e4m3fn):
@@ -1270,54 +1032,13 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1, dtype: torch.dtype = t
     value nearest to x / scale, ties to even, for every input type.  A block of zeros has scale 1;
     one that holds an infinity or a NaN has scale NaN and reads back as NaN.  cols is a multiple
     of 16."""
-    if not x.is_cuda:
-        _require_cuda(x, "x")
-    if x.dim() != 2 or x.dtype not in _FLOAT_CODE:
-        raise ValueError(f"quantize_fp8 takes a 2-D float32, bfloat16 or float16 tensor, got {x.dtype} {list(x.shape)}")
-    if dtype not in _FP8_CODE:
-        raise ValueError(f"dtype must be float8_e4m3fn or float8_e5m2, got {dtype}")
-    if block_rows not in (1, 128):
-        raise ValueError(f"block_rows must be 1 or 128, got {block_rows}")
-    rows, cols = x.shape
-    if cols < 1 or cols % TILE:
-        raise ValueError(f"cols must be a positive multiple of {TILE}, got {cols}")
-    x2 = _rows16(x)
-    q = x.new_empty((rows, cols), dtype=dtype)
-    scale = x.new_empty((-(-rows // block_rows), -(-cols // 128)), dtype=torch.float32)
-    if rows == 0:
-        return q, scale
-    _launch("mortar_quantize_fp8", x, x2.data_ptr(), _CODE[x.dtype], x2.stride(0), rows, cols, block_rows, q.data_ptr(),
-            _CODE[dtype], cols, scale.data_ptr())
-    _count("quantize_fp8")
-    return q, scale
+    return native.quantize_fp8(x, block_rows, dtype)
 
 
 def dequantize_fp8(q: torch.Tensor, scale: torch.Tensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """q * scale, rounded once to ``out_dtype``, for what ``quantize_fp8`` gives (or another program
     made, with any scales).  One scale row per row of q, or one per 128 rows."""
-    if not q.is_cuda:
-        _require_cuda(q, "q")
-    if q.dim() != 2 or q.dtype not in _FP8_CODE:
-        raise ValueError(f"q must be a 2-D float8_e4m3fn or float8_e5m2 tensor, got {q.dtype} {list(q.shape)}")
-    if out_dtype not in _FLOAT_CODE:
-        raise ValueError(f"unsupported out_dtype {out_dtype}")
-    rows, cols = q.shape
-    if cols < 1 or cols % TILE:
-        raise ValueError(f"cols must be a positive multiple of {TILE}, got {cols}")
-    nb = -(-cols // 128)
-    if scale.dtype != torch.float32 or tuple(scale.shape) not in ((rows, nb), (-(-rows // 128), nb)):
-        raise ValueError(f"scale must be float32 [{rows}, {nb}] or [{-(-rows // 128)}, {nb}], got {scale.dtype} "
-                         f"{list(scale.shape)}")
-    _same_device(q, "scale", scale)
-    block_rows = 1 if scale.shape[0] == rows else 128
-    out = q.new_empty((rows, cols), dtype=out_dtype)
-    if rows == 0:
-        return out
-    q2, s2 = _rows16(q), scale.contiguous()
-    _launch("mortar_dequantize_fp8", q, q2.data_ptr(), _CODE[q.dtype], q2.stride(0), s2.data_ptr(), rows, cols, block_rows,
-            out.data_ptr(), _CODE[out_dtype], cols)
-    _count("dequantize_fp8")
-    return out
+    return native.dequantize_fp8(q, scale, out_dtype)
 
 
 def linear_fp8_error(reset: bool = True) -> int:
@@ -1337,45 +1058,7 @@ def linear_fp8(x: torch.Tensor, w: Fp8Matrix, *, x_scale: Optional[torch.Tensor]
     ``out_dtype`` (default: the type of x, bfloat16 for 8-bit x).  The 8-bit floating-point
     counterpart of ``linear_tc_i8``; for serving, not differentiable (inputs that require a
     gradient are refused while gradients are enabled)."""
-    if not x.is_cuda:
-        _require_cuda(x, "x")
-    dt, in_features, out_features = x.dtype, w.in_features, w.out_features
-    if dt not in _CODE or x.dim() < 1:
-        raise ValueError(f"x must be a float or float8 tensor [..., in], got {dt}")
-    if (x_scale is None) != (dt in _FLOAT_CODE):
-        raise ValueError("x_scale goes with an 8-bit x, and only with one")
-    if x.shape[-1] != in_features:
-        raise ValueError(f"x has last dim {x.shape[-1]}, expected {in_features}")
-    if _wants_grad(x, x_scale):
-        raise ValueError("linear_fp8 is not differentiable: detach x or call it under torch.no_grad()")
-    if swiglu and out_features % 256:
-        raise ValueError(f"swiglu needs out_features to be a multiple of 256, got {out_features}")
-    if out_dtype is None:
-        out_dtype = dt if dt in _FLOAT_CODE else torch.bfloat16
-    out_code = _FLOAT_CODE.get(out_dtype)
-    if out_code is None:
-        raise ValueError(f"unsupported out_dtype {out_dtype}")
-    data, scale = w.data, w.scale
-    _same_device(x, "w", data)
-    x2 = x if x.dim() == 2 else x.reshape(-1, in_features)
-    rows = x2.shape[0]
-    if x_scale is None:
-        x2, s2 = quantize_fp8(x2)
-    else:
-        _same_device(x, "x_scale", x_scale)
-        if x_scale.dtype is not torch.float32 or x_scale.shape != (*x.shape[:-1], -(-in_features // 128)):
-            raise ValueError(f"x_scale must be float32 {[*x.shape[:-1], -(-in_features // 128)]}, got {x_scale.dtype} "
-                             f"{list(x_scale.shape)}")
-        x2, s2 = _rows16(x2), _rows_any(x_scale)
-    n_out = out_features // 2 if swiglu else out_features
-    out = x.new_empty((*x.shape[:-1], n_out), dtype=out_dtype)
-    if rows == 0:
-        return out
-    _launch("mortar_linear_fp8", x, x2.data_ptr(), _CODE[x2.dtype], x2.stride(0), s2.data_ptr(), s2.stride(0), rows,
-            data.data_ptr(), _CODE[data.dtype], data.stride(0), scale.data_ptr(), scale.stride(0), out_features,
-            in_features, _lib.FLAG_SWIGLU if swiglu else 0, out.data_ptr(), out_code, n_out)
-    _count("linear_fp8")
-    return out
+    return native.linear_fp8(x, x_scale, w.data, w.scale, swiglu, out_dtype)
 
 
 def mlp_fp8(x: torch.Tensor, gate_up: Fp8Matrix, down: Fp8Matrix, *,
@@ -1385,7 +1068,7 @@ def mlp_fp8(x: torch.Tensor, gate_up: Fp8Matrix, down: Fp8Matrix, *,
     16-bit x), quantise the hidden block, down product.  Four launches; for serving."""
     if gate_up.out_features != 2 * down.in_features or gate_up.in_features != down.out_features:
         raise ValueError("gate_up must be [2 d_ff, d_model] and down [d_model, d_ff]")
-    if x.dtype not in _FLOAT_CODE:
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError(f"mlp_fp8 takes float32, bfloat16 or float16 activations, got {x.dtype}")
     h = linear_fp8(x, gate_up, swiglu=True, out_dtype=torch.float16 if x.dtype == torch.float16 else torch.bfloat16)
     return linear_fp8(h, down, out_dtype=x.dtype if out_dtype is None else out_dtype)
