@@ -12,8 +12,11 @@ MODULE_PATH = os.path.join(_lib.PKG, "_mortar_native.so")
 
 
 class _Native:
+    def loaded(self) -> bool:
+        return "_module" in self.__dict__
+
     def __getattr__(self, name):
-        if "_module" not in self.__dict__:
+        if not self.loaded():
             _lib.lib()                                         # the library it is linked against, and its error if missing
             if not os.path.exists(MODULE_PATH):
                 raise ImportError(f"{MODULE_PATH} is missing: the extension must be built first "

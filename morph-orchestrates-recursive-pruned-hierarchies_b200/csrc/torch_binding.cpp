@@ -3,15 +3,18 @@
 // for a few microseconds on a small batch; the same steps in Python took 10 to 19 us a call and 115 us a
 // training step of the layer norm.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 #include <algorithm>
 #include <atomic>
 #include <optional>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 #include "mortar_b200.h"
 
@@ -81,7 +84,7 @@ Tensor rows2d(const Tensor &t) { return t.dim() == 2 ? t : t.reshape({-1, t.size
 Tensor rows_of(const Tensor &t, bool aligned) {
     const Tensor r = rows2d(t);
     const int64_t per16 = 16 / (int64_t)r.element_size();
-    const bool ok = r.stride(1) == 1 && r.stride(0) >= r.size(1) &&
+    const bool ok = r.stride(1) == 1 && r.stride(0) >= r.size(1) && !r.is_neg() &&
                     (!aligned || (r.stride(0) % per16 == 0 && reinterpret_cast<uintptr_t>(r.const_data_ptr()) % 16 == 0));
     return ok ? r : r.clone(at::MemoryFormat::Contiguous);
 }
@@ -111,11 +114,39 @@ void refuse_second(const char *name) {
     TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivative: call backward without create_graph");
 }
 
+// A leaf's gradient is accumulated on the stream that was current when the oldest living graph took the leaf up.
+// A backward pass that is being captured cannot make the default stream wait for it: the capture fails inside the
+// autograd engine, and the process ends with it.  So a forward call under capture refuses when a leaf above it is so
+// held.  (The walk runs while a graph is captured, never in an eager step.)
+void refuse_capture(const char *name, std::initializer_list<const Tensor *> ts) {
+    using torch::autograd::Node;
+    const c10::cuda::CUDAGuard guard((*ts.begin())->device());
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+    std::vector<std::shared_ptr<Node>> todo;
+    std::unordered_set<Node *> seen;
+    const auto visit = [&](const std::shared_ptr<Node> &node) {
+        if (node && seen.insert(node.get()).second) todo.push_back(node);
+    };
+    for (const Tensor *t : ts)
+        if (t->defined() && t->requires_grad())
+            visit(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!todo.empty()) {
+        const std::shared_ptr<Node> node = todo.back();
+        todo.pop_back();
+        for (const auto &edge : node->next_edges()) visit(edge.function);
+        if (node->num_outputs() != 0) continue;          // not a leaf's accumulator
+        const auto s = node->stream();
+        TORCH_CHECK(!s.has_value() || c10::cuda::CUDAStream(*s).stream() != nullptr, name,
+                    ": a tensor whose gradient a graph from the default stream still holds cannot be part of a captured "
+                    "training step: drop that graph's outputs first, or detach them");
+    }
+}
+
 // ---- layer norm -------------------------------------------------------------------------------
 
 Tensor as_f32(const Tensor &t) {
-    if (!t.defined() || (t.scalar_type() == at::kFloat && t.is_contiguous())) return t;
-    return t.detach().to(at::kFloat).contiguous();
+    if (!t.defined() || (t.scalar_type() == at::kFloat && t.is_contiguous() && !t.is_neg())) return t;
+    return t.detach().to(at::kFloat).contiguous().resolve_neg();
 }
 
 void check_columns(const Tensor &x, const char *name, const Tensor &t) {
@@ -208,7 +239,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps) {
     const Tensor w = or_none(weight), b = or_none(bias);
-    if (wants_grad({&x, &w, &b})) return LayerNorm::apply(x, weight, bias, eps);
+    if (wants_grad({&x, &w, &b})) {
+        need_cuda(x, "x");
+        refuse_capture("layer_norm", {&x, &w, &b});
+        return LayerNorm::apply(x, weight, bias, eps);
+    }
     return std::get<0>(layer_norm_forward(x, w, b, eps, false));
 }
 
@@ -307,7 +342,11 @@ struct MlpDense : torch::autograd::Function<MlpDense> {
 };
 
 Tensor mlp_dense(const Tensor &x, const Tensor &gate_up, const Tensor &down) {
-    if (wants_grad({&x, &gate_up, &down})) return MlpDense::apply(x, gate_up, down);
+    if (wants_grad({&x, &gate_up, &down})) {
+        need_cuda(x, "x");
+        refuse_capture("mlp_dense", {&x, &gate_up, &down});
+        return MlpDense::apply(x, gate_up, down);
+    }
     return std::get<0>(mlp_dense_forward(x, gate_up, down, false));
 }
 
@@ -347,7 +386,7 @@ Tensor dequantize_fp8(const Tensor &q, const Tensor &scale, at::ScalarType out_d
     const Launch on(q);
     const Tensor y = at::empty({rows, cols}, q.options().dtype(out_dtype));
     if (rows == 0) return y;
-    const Tensor r = rows_of(q, true), s = scale.contiguous();
+    const Tensor r = rows_of(q, true), s = scale.contiguous().resolve_neg();
     check(mortar_dequantize_fp8(in(r), q_code, ld(r), in_f32(s), rows, (int32_t)cols, scale.size(0) == rows ? 1 : 128, out(y),
                                 code, cols, on.stream), "mortar_dequantize_fp8");
     count(kDequantize, 1);
@@ -360,7 +399,12 @@ Tensor linear_fp8(const Tensor &x, const OptTensor &x_scale, const Tensor &data,
     const int code = code_of(x.scalar_type());
     TORCH_CHECK_VALUE(code >= 0 && x.dim() >= 1, "x must be a float or float8 tensor [..., in], got ", x.scalar_type());
     TORCH_CHECK_VALUE(x_scale.has_value() == is_fp8(code), "x_scale goes with an 8-bit x, and only with one");
+    TORCH_CHECK_VALUE(data.dim() == 2 && is_fp8(code_of(data.scalar_type())), "w.data must be a float8 matrix, got ",
+                      data.scalar_type(), " ", data.sizes());
     const int64_t n = data.size(0), k = data.size(1), nb = (k + 127) / 128;
+    TORCH_CHECK_VALUE(data.stride(1) == 1 && scale.scalar_type() == at::kFloat && scale.dim() == 2 &&
+                          scale.size(0) == (n + 127) / 128 && scale.size(1) == nb && scale.stride(1) == 1,
+                      "w.scale must be float32 [", (n + 127) / 128, ", ", nb, "], got ", scale.scalar_type(), " ", scale.sizes());
     TORCH_CHECK_VALUE(x.size(-1) == k, "x has last dim ", x.size(-1), ", expected ", k);
     TORCH_CHECK_VALUE(n <= INT32_MAX && k <= INT32_MAX, "a matrix [", n, ", ", k, "] is too large");
     const Tensor given = or_none(x_scale);
@@ -371,6 +415,7 @@ Tensor linear_fp8(const Tensor &x, const OptTensor &x_scale, const Tensor &data,
     const int y_code = code_of(y_type);
     TORCH_CHECK_VALUE(is_float(y_code), "unsupported out_dtype ", y_type);
     same_device(x, "w", data);
+    same_device(x, "w.scale", scale);
     if (given.defined()) {
         same_device(x, "x_scale", given);
         bool fits = given.scalar_type() == at::kFloat && given.dim() == x.dim() && given.size(-1) == nb;
@@ -403,18 +448,21 @@ Tensor linear_fp8(const Tensor &x, const OptTensor &x_scale, const Tensor &data,
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     namespace py = pybind11;
-    m.def("layer_norm", &layer_norm);
+    // no call touches a Python object: other threads run meanwhile, as with torch's own operators
+    const py::call_guard<py::gil_scoped_release> no_gil;
+    m.def("layer_norm", &layer_norm, no_gil);
     m.def("layer_norm_forward", [](const Tensor &x, const OptTensor &w, const OptTensor &b, double eps, bool stats) {
         return layer_norm_forward(x, or_none(w), or_none(b), eps, stats);
-    });
+    }, no_gil);
     m.def("layer_norm_backward", [](const Tensor &dy, const Tensor &x, const OptTensor &w, const Tensor &stats, bool dx,
-                                    bool dw, bool db) { return layer_norm_backward(dy, x, or_none(w), stats, dx, dw, db); });
-    m.def("mlp_dense", &mlp_dense);
-    m.def("mlp_dense_forward", &mlp_dense_forward);
-    m.def("mlp_dense_backward", &mlp_dense_backward);
-    m.def("quantize_fp8", &quantize_fp8);
-    m.def("dequantize_fp8", &dequantize_fp8);
-    m.def("linear_fp8", &linear_fp8);
+                                    bool dw, bool db) { return layer_norm_backward(dy, x, or_none(w), stats, dx, dw, db); },
+          no_gil);
+    m.def("mlp_dense", &mlp_dense, no_gil);
+    m.def("mlp_dense_forward", &mlp_dense_forward, no_gil);
+    m.def("mlp_dense_backward", &mlp_dense_backward, no_gil);
+    m.def("quantize_fp8", &quantize_fp8, no_gil);
+    m.def("dequantize_fp8", &dequantize_fp8, no_gil);
+    m.def("linear_fp8", &linear_fp8, no_gil);
     m.def("kernel_counts", [] {
         py::dict d;
         for (int i = 0; i < kFamilies; ++i)

@@ -18,15 +18,19 @@ _launches = 0      # kernels launched by this module (bench.py reports it)
 _kernel_counts: dict = {}   # the same, per kernel family
 
 
+def _native_counts() -> dict:
+    return native.kernel_counts() if native.loaded() else {}
+
+
 def launch_count() -> int:
-    return _launches + sum(native.kernel_counts().values())
+    return _launches + sum(_native_counts().values())
 
 
 def kernel_counts() -> dict:
     """Launches so far per kernel family: "act_prep", "bcsr_stream" (the streaming linear / SwiGLU
     kernel), "prefill_panel" (tcgen05 / tensor memory), "stack_decode", "route_flags", "router".
     Tests use the deltas to tell which kernel an operator or module forward ran."""
-    return {**_kernel_counts, **native.kernel_counts()}
+    return {**_kernel_counts, **_native_counts()}
 
 
 def _count(name: str, n: int = 1) -> None:

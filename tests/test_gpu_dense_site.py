@@ -676,3 +676,127 @@ def test_mlp_dense_cut_reductions(rows, d, f):
     again = (y.detach(), *torch.autograd.grad(y, (x, gu, dn), dy))
     assert all(torch.equal(p, q) for p, q in zip(got, again))
     errors_are_clear()
+
+
+def test_calls_from_many_threads_at_once():
+    """Threads on streams of their own call every operator at the same time, forward and backward."""
+    import threading
+    dt = torch.bfloat16
+    gu, dn = rand(512, 128, seed=2, scale=0.2, dt=dt), rand(128, 256, seed=3, scale=0.2, dt=dt)
+    w, b = rand(128, seed=4), rand(128, seed=5)
+    m = mb.Fp8Matrix.from_dense(gu)
+    xs = [rand(rows, 128, seed=rows, dt=dt) for rows in (1, 37, 300, 1111)]
+
+    def step(x):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, gu, dn)]
+        n = ops.layer_norm(*leaves[:3])
+        y = ops.mlp_dense(n, *leaves[3:])
+        return [y.detach(), ops.linear_fp8(n.detach(), m, swiglu=True), *torch.autograd.grad(y.square().sum(), leaves)]
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    wrong, ran = [], []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = step(xs[i])
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(k for k, (p, q) in enumerate(zip(got, want[i])) if not torch.equal(p, q))
+        ran.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert sorted(ran) == list(range(len(xs))) and not wrong
+    errors_are_clear()
+
+
+def test_captured_training_step_beside_an_eager_graph():
+    """A training step cannot be captured while a graph of the default stream holds the gradients of the same
+    leaves (it is refused before anything is captured); a served step can, and so can the training step once
+    that graph is gone."""
+    dt = torch.bfloat16
+    site = mb.modules.SwiGLUDense(64, 128, device=DEV, dtype=dt)
+    x = rand(40, 64, seed=1, dt=dt)
+    dy = rand(40, 64, seed=2, dt=dt)
+    held = site(x)
+    params = list(site.parameters())
+    want = [held.detach().clone(), *torch.autograd.grad(held, params, dy, retain_graph=True)]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(graph):
+            site(x)
+    gu = site.gate_up.weight
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.mlp_dense(x, gu, site.down.weight.detach())
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        y = site(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[0])
+    del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = site(x)
+        got = torch.autograd.grad(y, params, dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip((y.detach(), *got), want))
+    errors_are_clear()
+
+
+def test_negated_views():
+    """Views that stand for the negative of what memory holds (the imaginary part of a conjugate)."""
+    z = torch.complex(rand(9, 64, seed=1), rand(9, 64, seed=2))
+    x = z.conj().imag
+    assert x.is_neg()
+    plain = (-z.imag).contiguous()
+    assert torch.equal(ops.layer_norm(x), ops.layer_norm(plain))
+    assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(ops.quantize_fp8(x), ops.quantize_fp8(plain)))
+    w = z[0].conj().imag
+    assert torch.equal(ops.layer_norm(plain, w, w), ops.layer_norm(plain, plain[0], plain[0]))
+    one = torch._neg_view(rand(64, seed=3))
+    assert torch.equal(ops.layer_norm(plain, one), ops.layer_norm(plain, one.resolve_neg()))
+    packed = torch._neg_view(plain)
+    assert packed.is_contiguous() and torch.equal(ops.layer_norm(packed), ops.layer_norm(packed.resolve_neg()))
+
+
+def test_replaced_parts_of_a_matrix_are_refused():
+    m = mb.Fp8Matrix.from_dense(rand(256, 256, seed=1))
+    x = rand(5, 256, seed=2, dt=torch.bfloat16)
+    for part, value in (("scale", m.scale[:1]), ("scale", m.scale.double()), ("scale", m.scale.cpu()), ("data", m.data[0]),
+                        ("data", m.data.view(torch.uint8)), ("data", m.data.t())):
+        keep = getattr(m, part)
+        setattr(m, part, value)
+        with pytest.raises(ValueError):
+            ops.linear_fp8(x, m)
+        setattr(m, part, keep)
+    ops.linear_fp8(x, m)
+
+
+def test_captured_step_of_cast_weights_beside_an_eager_graph():
+    """The same where the operator does not see the leaf itself: fp32 weights that are cast on the way."""
+    site = mb.modules.SwiGLUDense(64, 128, norm=True, device=DEV)
+    x = rand(40, 64, seed=1, dt=torch.bfloat16)
+    held = site(x)
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            site(x)
+    weights = [p.detach().requires_grad_() for p in (site.gate_up.weight, site.down.weight)]
+    cast = [w.to(torch.bfloat16) for w in weights]
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.mlp_dense(x, *cast)
+    del held, cast
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(site(x).square().sum(), list(site.parameters()))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, torch.autograd.grad(site(x).square().sum(), list(site.parameters()))))
+    errors_are_clear()
