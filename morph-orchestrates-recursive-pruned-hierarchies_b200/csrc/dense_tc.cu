@@ -11,15 +11,15 @@
 // accumulator tile, so the gate is applied where the sums are read, and the backward of the gate is
 // the epilogue of dh.
 //
-// One cluster of two CTAs computes a 256 x kBN tile (each CTA 128 rows; the B operand is split between
-// their shared memories): per SM and 64-wide step 16 KB of A and kBN * 64 bytes of B cross from L2,
+// One cluster of two CTAs computes a tile of 256 rows and 256 or 128 columns (each CTA 128 rows; the B operand is
+// split between their shared memories): per SM and 64-wide step 16 KB of A and 64 bytes a column of B cross from L2,
 // half of what two single CTAs would read, which is what keeps the copies ahead of the MMAs.  Warp 0
 // issues the copies of its CTA, one thread of CTA 0 issues the MMAs of both, warps 2..17 read the
 // accumulators (two sets, so that a tile's epilogue runs under the next tile's MMAs).
 // Every wait is bounded.
 //
 // What bounds it: at 8192 x 2048/5632 every launch draws its operands from L2 at 12.2 to 12.4 TB/s (128 KB a
-// 128-wide step and cluster), which is all that L2 gives: gate/up 236 us = 1600 TFLOP/s without and 278 us with
+// 128-wide step and cluster of 256 columns), which is all that L2 gives: gate/up 236 us = 1600 TFLOP/s without and 278 us with
 // the kept sums, down 137 us = 1380, dh 194 us (its epilogue moves 0.7 GB more), the three last products
 // together 594 us = 1590 TFLOP/s with the tensor pipe busy 88% of the time.  A hand-off of 64-wide steps with
 // one wait for four MMAs reached 1200.  Under the power cap of a long run the whole step comes to 1150 of the
@@ -34,17 +34,20 @@
 
 namespace {
 
-constexpr int kBN = 256;                         // accumulator columns of a tile
-constexpr int kStages = 3;
 constexpr int kStageA = 128 * 256;               // this CTA's 128 rows, 128 elements of 2 bytes each
-constexpr int kStageB = kBN / 2 * 256;
-constexpr int kStage = kStageA + kStageB;
 constexpr int kEpiWarps = 16;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
-constexpr int kTmemCols = 2 * kBN;
-constexpr int kSmem = kStages * kStage + (2 * kStages + 4) * 8 + 1024;
 constexpr int kMaxProblems = 3;
-static_assert(kSmem <= 227 * 1024, "shared memory budget");
+constexpr int kClusters = 74;                    // CTA pairs that run at once
+
+// BN: accumulator columns of a tile, 256 or 128
+template <int BN> struct Shape {
+    static constexpr int kStages = BN == 256 ? 3 : 4;
+    static constexpr int kStageB = BN / 2 * 256;
+    static constexpr int kStage = kStageA + kStageB;
+    static constexpr int kSmem = kStages * kStage + (2 * kStages + 4) * 8 + 1024;
+    static_assert(kSmem <= 227 * 1024, "shared memory budget");
+};
 
 __device__ int g_dense_error;
 
@@ -120,9 +123,10 @@ __device__ __forceinline__ TileId tile_of(const DenseParams &p, int item) {
     return t;
 }
 
-template <int EPI>
+template <int EPI, int kBN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 dense_pair_kernel(const __grid_constant__ DenseParams p) {
+    constexpr int kStages = Shape<kBN>::kStages, kStageB = Shape<kBN>::kStageB, kStage = Shape<kBN>::kStage, kTmemCols = 2 * kBN;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *full = reinterpret_cast<uint64_t *>(stages + kStages * kStage), *empty = full + kStages;
@@ -369,16 +373,16 @@ bool misaligned(const void *p, size_t a = 16) { return reinterpret_cast<uintptr_
 
 // Adds C[m][n] = sum_k A[m][k] B[n][k] to a launch.  `a` is [m][k] (row stride lda) or, with a_mn, [k][m];
 // `b` is [n][k] or, with b_mn, [k][n].  For kSwiglu n counts hidden columns and b has 2 n rows.
-int add_problem(DenseParams &p, int epi, const void *a, int64_t lda, bool a_mn, const void *b, int64_t ldb, bool b_mn,
+int add_problem(DenseParams &p, int epi, int bn, const void *a, int64_t lda, bool a_mn, const void *b, int64_t ldb, bool b_mn,
                 int64_t m, int64_t n, int64_t k, void *out, int64_t ld_out) {
     const int i = p.n_problems;
     Problem &q = p.prob[i];
-    const int64_t b_rows = epi == kSwiglu ? 2 * n : n, tile_n = epi == kSwiglu ? kBN / 2 : kBN;
+    const int64_t b_rows = epi == kSwiglu ? 2 * n : n, tile_n = epi == kSwiglu ? bn / 2 : bn;
     int rc = a_mn ? tc::encode_bf16_2d(&p.map_a[i], a, m, k, lda, 64, 128)
                   : tc::encode_bf16_2d(&p.map_a[i], a, k, m, lda, 64, 128);
     if (rc != MORTAR_OK) return rc;
     rc = b_mn ? tc::encode_bf16_2d(&p.map_b[i], b, b_rows, k, ldb, 64, 128)
-              : tc::encode_bf16_2d(&p.map_b[i], b, k, b_rows, ldb, 64, kBN / 2);
+              : tc::encode_bf16_2d(&p.map_b[i], b, k, b_rows, ldb, 64, (uint32_t)(bn / 2));
     if (rc != MORTAR_OK) return rc;
     const int64_t tm = (m + 255) / 256, tn = (n + tile_n - 1) / tile_n;
     if (tm * tn + p.n_items > 0x3fffffff) return MORTAR_ERR_CAPACITY;
@@ -392,23 +396,37 @@ int add_problem(DenseParams &p, int epi, const void *a, int64_t lda, bool a_mn, 
 
 std::mutex g_dense_mutex;
 
-// 128-wide steps that each of the 74 clusters would take if a launch's work were spread evenly, and the parts that a
-// product's reduction is cut into: more than one only where its tiles would run twice as long as that or longer (few
-// rows, or few columns of a weight gradient)
-int64_t even_share(int64_t total_steps) { return total_steps < 74 ? 1 : (total_steps + 73) / 74; }
-int64_t parts_of(int64_t k_steps, int64_t share) { return k_steps >= 2 * share ? k_steps / share : 1; }
 int64_t steps_of(int64_t k) { return (k + 127) / 128; }
-int64_t tiles_of(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256); }
+int64_t tiles_of(int64_t m, int64_t n, int bn) { return ((m + 255) / 256) * ((n + bn - 1) / bn); }
 
-struct Plan { int64_t parts[kMaxProblems], floats; };
+// Tiles of 128 columns where all of a launch's run at once, else of 256: half the tile takes half the time, but reads three
+// quarters of the memory.  Forward and backward of 333 x 768/2048 29.0 + 39.2 -> 24.8 + 33.1 us, 2048 x 512/512 30.9 + 41.1
+// -> 26.7 + 26.9; with 128 columns also where three rounds of them replace two of 256: 2048 x 768/1536 56.0 -> 58.8 backward,
+// 4096 x 2048/1280 74.3 + 132.5 -> 81.8 + 157.3.
+int width_of(int64_t tiles_256) { return 2 * tiles_256 <= kClusters ? 128 : 256; }
+
+// The parts that a reduction of `k_steps` 128-wide steps is cut into, where a launch takes `total` steps over all its
+// tiles: more than one where a tile would run for twice the even share of a cluster or longer (few rows, or few columns
+// of a weight gradient), no more than leave all parts of the launch running at once, and no more than the longest part
+// needs.
+int64_t parts_of(int64_t k_steps, int64_t total) {
+    const int64_t most = total < kClusters ? k_steps : k_steps * kClusters / total;
+    if (most < 2) return 1;
+    const int64_t longest = (k_steps + most - 1) / most;
+    return (k_steps + longest - 1) / longest;
+}
+
+struct Plan { int bn; int64_t parts[kMaxProblems], floats; };
 
 // of up to three products m x n over k in one launch
 Plan plan(const int64_t (*mnk)[3], int count) {
     Plan r = {};
-    int64_t total = 0;
-    for (int i = 0; i < count; ++i) total += tiles_of(mnk[i][0], mnk[i][1]) * steps_of(mnk[i][2]);
+    int64_t total = 0, tiles = 0;
+    for (int i = 0; i < count; ++i) tiles += tiles_of(mnk[i][0], mnk[i][1], 256);
+    r.bn = width_of(tiles);
+    for (int i = 0; i < count; ++i) total += tiles_of(mnk[i][0], mnk[i][1], r.bn) * steps_of(mnk[i][2]);
     for (int i = 0; i < count; ++i) {
-        r.parts[i] = parts_of(steps_of(mnk[i][2]), even_share(total));
+        r.parts[i] = parts_of(steps_of(mnk[i][2]), total);
         if (r.parts[i] > 1) r.floats += r.parts[i] * mnk[i][0] * mnk[i][1];
     }
     return r;
@@ -438,20 +456,26 @@ int join(const DenseParams &p, cudaStream_t st) {
     return MORTAR_OK;
 }
 
-// `follows`: the launch reads what the one before it in the call wrote, and may be set up while that one ends
-template <int EPI>
-int launch(const DenseParams &p, bool follows, cudaStream_t st) {
+template <int EPI, int BN>
+int launch_width(const DenseParams &p, bool follows, cudaStream_t st) {
     static bool ready[64] = {false};
+    constexpr int kSmem = Shape<BN>::kSmem;
     int sms = 0;
-    int rc = tc::allow_smem(dense_pair_kernel<EPI>, kSmem, ready, g_dense_mutex, nullptr);
+    int rc = tc::allow_smem(dense_pair_kernel<EPI, BN>, kSmem, ready, g_dense_mutex, nullptr);
     if (rc != MORTAR_OK) return rc;
     rc = tc::sm_count(&sms);
     if (rc != MORTAR_OK) return rc;
     const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
-    if (follows) return tc::launch_after(dense_pair_kernel<EPI>, (unsigned)(2 * clusters), (unsigned)kThreads, kSmem, st, p);
-    dense_pair_kernel<EPI><<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
+    if (follows) return tc::launch_after(dense_pair_kernel<EPI, BN>, (unsigned)(2 * clusters), (unsigned)kThreads, kSmem, st, p);
+    dense_pair_kernel<EPI, BN><<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
     MORTAR_CUDA_CHECK(cudaGetLastError());
     return MORTAR_OK;
+}
+
+// `follows`: the launch reads what the one before it in the call wrote, and may be set up while that one ends
+template <int EPI>
+int launch(const DenseParams &p, int bn, bool follows, cudaStream_t st) {
+    return bn == 128 ? launch_width<EPI, 128>(p, follows, st) : launch_width<EPI, 256>(p, follows, st);
 }
 
 int check_shape(int32_t dtype, int64_t rows, int32_t d_model, int32_t d_ff) {
@@ -527,15 +551,16 @@ extern "C" int mortar_mlp_dense(const void *x, int64_t ldx, int32_t dtype, int64
     p.d_ff = d_ff;
     p.gu = gate_up_sums;
     p.ld_gu = 2LL * d_ff;
-    rc = add_problem(p, kSwiglu, x, ldx, false, gate_up, ld_gate_up, false, rows, d_ff, d_model, hidden, d_ff);
-    if (rc == MORTAR_OK) rc = launch<kSwiglu>(p, false, st);
+    const int bn = width_of(tiles_of(rows, 2LL * d_ff, 256));
+    rc = add_problem(p, kSwiglu, bn, x, ldx, false, gate_up, ld_gate_up, false, rows, d_ff, d_model, hidden, d_ff);
+    if (rc == MORTAR_OK) rc = launch<kSwiglu>(p, bn, false, st);
     if (rc != MORTAR_OK) return rc;
     alignas(64) DenseParams p2 = {};
     p2.half = p.half;
-    rc = add_problem(p2, kStore, hidden, d_ff, false, down, ld_down, false, rows, d_model, d_ff, y, ldy);
+    rc = add_problem(p2, kStore, parts.bn, hidden, d_ff, false, down, ld_down, false, rows, d_model, d_ff, y, ldy);
     if (rc != MORTAR_OK) return rc;
     cut(p2, parts, scratch);
-    rc = launch<kStore>(p2, true, st);
+    rc = launch<kStore>(p2, parts.bn, true, st);
     return rc == MORTAR_OK ? join(p2, st) : rc;
 }
 
@@ -569,21 +594,22 @@ extern "C" int mortar_mlp_dense_backward(const void *dy, int64_t lddy, const voi
         p.d_ff = d_ff;
         p.gu = const_cast<float *>(gate_up_sums);
         p.ld_gu = f2;
-        rc = add_problem(p, kSwigluBackward, dy, lddy, false, down, ld_down, true, rows, d_ff, d_model, dgate_up_sums, f2);
-        if (rc == MORTAR_OK) rc = launch<kSwigluBackward>(p, false, st);
+        const int bn = width_of(tiles_of(rows, d_ff, 256));
+        rc = add_problem(p, kSwigluBackward, bn, dy, lddy, false, down, ld_down, true, rows, d_ff, d_model, dgate_up_sums, f2);
+        if (rc == MORTAR_OK) rc = launch<kSwigluBackward>(p, bn, false, st);
         if (rc != MORTAR_OK) return rc;
     }
     alignas(64) DenseParams p = {};
     p.half = dtype == MORTAR_F16;
     // the longest reduction first
-    if (dx) rc = add_problem(p, kStore, dgate_up_sums, f2, false, gate_up, ld_gate_up, true, rows, d_model, f2, dx, d_model);
+    if (dx) rc = add_problem(p, kStore, parts.bn, dgate_up_sums, f2, false, gate_up, ld_gate_up, true, rows, d_model, f2, dx, d_model);
     if (rc == MORTAR_OK && dgate_up)
-        rc = add_problem(p, kStore, dgate_up_sums, f2, true, x, ldx, true, f2, d_model, rows, dgate_up, d_model);
+        rc = add_problem(p, kStore, parts.bn, dgate_up_sums, f2, true, x, ldx, true, f2, d_model, rows, dgate_up, d_model);
     if (rc == MORTAR_OK && ddown)
-        rc = add_problem(p, kStore, dy, lddy, true, hidden, d_ff, true, d_model, d_ff, rows, ddown, d_ff);
+        rc = add_problem(p, kStore, parts.bn, dy, lddy, true, hidden, d_ff, true, d_model, d_ff, rows, ddown, d_ff);
     if (rc != MORTAR_OK || p.n_problems == 0) return rc;
     cut(p, parts, scratch);
-    rc = launch<kStore>(p, dx || dgate_up, st);
+    rc = launch<kStore>(p, parts.bn, dx || dgate_up, st);
     return rc == MORTAR_OK ? join(p, st) : rc;
 }
 

@@ -821,3 +821,10 @@ def test_linear_fp8_rounds_of_whole_and_half_tiles(rows, out, cols):
 @pytest.mark.parametrize("d_ff", [128 * 40, 128 * 75])
 def test_linear_fp8_gate_of_whole_and_half_tiles(d_ff):
     test_linear_fp8_with_the_gate(300, d_ff, 400, torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("rows,d,f", [(2100, 528, 2064), (5000, 1040, 400), (1030, 2576, 1296)])
+def test_mlp_dense_tiles_of_both_widths(rows, d, f):
+    """Launches whose tiles fill the machine and launches whose do not, ragged in every direction: of the first shape
+    gate/up, dh and the gradients run on tiles of 256 columns and down on 128, of the second only dh on 128."""
+    test_mlp_dense_cut_reductions(rows, d, f)
