@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <mutex>
 #include <type_traits>
 #include "common.h"
 #include "tc_pair.cuh"
@@ -411,19 +412,29 @@ layer_norm_backward_kernel(const T *__restrict__ dy, long long lddy, const T *__
 
 // ---- the same for rows that are whole vectors ---------------------------------------------------
 //
-// Where every row starts on 16 bytes and has a multiple of 8 columns, a unit is there or not, loads and
-// stores are single vectors, and the arithmetic runs on pairs of columns (fma.rn.f32x2 and its like): 16 to
-// 18 instructions a column forward and 29 backward, against 20 and 34 above.  A thread takes NE units of its
-// row.  [16384][2048] fp32: forward 57 us = 4.7 TB/s, backward 73 us = 5.5 TB/s (a copy reaches 5.9 here);
-// [65536][2048] bf16: 117 us = 4.6 TB/s and 161 us = 5.0 TB/s (the kernels above: 180 and 207 us).  What is left
-// is the two sums that a row waits for.
+// Where every row starts on 16 bytes (fp32: 32) and has a multiple of 8 columns, a unit is there or not, loads
+// and stores are single vectors of a unit's size, and the arithmetic runs on pairs of columns (fma.rn.f32x2 and its
+// like): 16 to 18 instructions a column forward and 29 backward, against 20 and 34 above.  A thread takes NE units
+// of its row.  The next row is on its way meanwhile, forward in registers, backward two or three rows in shared
+// memory (forward too that takes longer: bf16 39 instead of 35 us).  [16384][2048] fp32: forward 48 us = 5.5 TB/s (57
+// with a unit in two 16-byte vectors), backward 73 us = 5.5 TB/s (a copy reaches 5.9 here); [65536][2048] bf16: 115 us =
+// 4.7 TB/s and 140 us = 5.7 TB/s (the kernels above: 180 and 207 us); [8192][5632] fp32 backward 131 us (192 without rows
+// on their way, which fp32 rows of two units have no registers for).  What is left forward is the two sums that a row
+// waits for.
 
 constexpr int kWholeWarps = 16;                          // of a CTA, one CTA an SM: 128 registers a thread
 
-template <class T> struct Packed { uint4 v[sizeof(T) * kUnit / 16]; };
+template <class T> constexpr int kVecs = sizeof(T) * kUnit / 16;                     // 16-byte vectors of a unit
+template <class T> struct Packed { uint4 v[kVecs<T>]; };
 template <class T> __device__ __forceinline__ void load_packed(Packed<T> &u, const T *p) {
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) * kUnit / 16); ++i) u.v[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    if constexpr (sizeof(T) == 4) {
+        uint32_t r[8];
+        tc::load_v8(reinterpret_cast<const float *>(p), r);
+        u.v[0] = make_uint4(r[0], r[1], r[2], r[3]);
+        u.v[1] = make_uint4(r[4], r[5], r[6], r[7]);
+    } else {
+        u.v[0] = __ldg(reinterpret_cast<const uint4 *>(p));
+    }
 }
 // four pairs of columns as fp32
 __device__ __forceinline__ void unpack(const Packed<float> &u, uint64_t (&p)[4]) {
@@ -445,8 +456,10 @@ __device__ __forceinline__ void unpack(const Packed<__half> &u, uint64_t (&p)[4]
 }
 template <class T> __device__ __forceinline__ void store_pairs(T *dst, const uint64_t (&p)[4]) {
     if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4 *>(dst)[0] = make_float4(tc::low_of(p[0]), tc::high_of(p[0]), tc::low_of(p[1]), tc::high_of(p[1]));
-        reinterpret_cast<float4 *>(dst)[1] = make_float4(tc::low_of(p[2]), tc::high_of(p[2]), tc::low_of(p[3]), tc::high_of(p[3]));
+        uint32_t r[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { r[2 * i] = __float_as_uint(tc::low_of(p[i])); r[2 * i + 1] = __float_as_uint(tc::high_of(p[i])); }
+        tc::store_v8(dst, r);
     } else {
         constexpr bool kHalf = std::is_same<T, __half>::value;
         *reinterpret_cast<uint4 *>(dst) =
@@ -531,58 +544,116 @@ layer_norm_whole_kernel(const T *__restrict__ x, long long ldx, long long rows, 
     }
 }
 
+// Rows on their way in shared memory, so that they hold no registers: a thread copies the vectors of its own units
+// where a unit is one vector, and of fp32 units, two vectors, a warp's lanes copy vectors that lie side by side (each its
+// own they would ask for half a sector at a time: 111 instead of 78 us at [16384][2048]).  `kSlots` rows of R operands, one
+// of them at work; a slot is filled again a row after it was read.
+template <class T, int NE, int R> struct Ring {
+    static constexpr int kV = kVecs<T>, kRow = R * NE * kV;                           // vectors of a thread and a row
+    static constexpr int kSlots = 4 * kRow * 16 * 32 * kWholeWarps <= 200 * 1024 ? 4 : 3;
+    static constexpr int kBytes = kSlots * kRow * 16;                                 // of a thread
+    uint4 *mine;
+    bool there[NE][kV];
+    int get_slot = 0, put_slot = 0;
+    // `col`: the first column of this thread's unit 0, `step`: columns from unit to unit
+    __device__ __forceinline__ Ring(uint4 *shared, int col, int step, int cols)
+        : mine(shared + (threadIdx.x >> 5) * kSlots * kRow * 32 + (threadIdx.x & 31)) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+#pragma unroll
+            for (int v = 0; v < kV; ++v) there[i][v] = first(col) + 128 * v + step * i < cols;
+    }
+    static __device__ __forceinline__ int first(int col) { return kV == 1 ? col : col - 4 * (int)(threadIdx.x & 31); }
+    __device__ __forceinline__ uint4 *at(int slot, int r, int i) { return mine + ((slot * R + r) * NE + i) * kV * 32; }
+    // `row`: column `first(col)` of the row
+    __device__ __forceinline__ void put(int r, const T *row, int step) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+#pragma unroll
+            for (int v = 0; v < kV; ++v)
+                if (there[i][v])
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(tc::smem_u32(at(put_slot, r, i) + 32 * v)),
+                                 "l"(row + step * i + 128 * v) : "memory");
+    }
+    __device__ __forceinline__ void end_row() {                                       // also where no row is left
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        if (++put_slot == kSlots) put_slot = 0;
+    }
+    __device__ __forceinline__ void wait_row() {
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(kSlots - 2) : "memory");
+        if (kV > 1) __syncwarp();
+    }
+    __device__ __forceinline__ void get(int r, int i, Packed<T> &u) {
+#pragma unroll
+        for (int v = 0; v < kV; ++v) u.v[v] = at(get_slot, r, i)[(int)(threadIdx.x & 31) * (kV - 1) + v];
+    }
+    __device__ __forceinline__ void end_read() {
+        if (kV > 1) __syncwarp();
+        if (++get_slot == kSlots) get_slot = 0;
+    }
+};
+
 template <class T, int NE>
 __global__ void __launch_bounds__(32 * kWholeWarps, 1)
 layer_norm_whole_backward_kernel(const T *__restrict__ dy, long long lddy, const T *__restrict__ x, long long ldx,
                                  long long rows, int cols, const float *__restrict__ w, const float *__restrict__ stats,
                                  T *__restrict__ dx, long long lddx, float *__restrict__ partial, int warps) {
     tc::let_next();
-    constexpr bool kAhead = NE * sizeof(T) <= 4;         // registers for a row on its way: 16-bit rows of two units, fp32 of one
     __shared__ float2 red[kWholeWarps][2][16];
-    extern __shared__ float fold[];                      // [groups][columns, rounded up to the group's]
+    extern __shared__ uint4 ring_s[];
+    float *fold = reinterpret_cast<float *>(ring_s);     // at the end: [groups][columns, rounded up to the group's]
     Group g = make_group(warps, red);
     const int groups = (int)(blockDim.x >> 5) / warps;
     const float inv = 1.f / cols;
     const long long stride = (long long)gridDim.x * groups;
     long long row = (long long)blockIdx.x * groups + g.id;
-    uint64_t dw[NE][4], db[NE][4], wv[NE][4];
+    const int step = 32 * kUnit * warps;
+    Ring<T, NE, 2> ring(ring_s, kUnit * g.thread, step, cols);
+    const T *xp = x + row * ldx + ring.first(kUnit * g.thread), *dp = dy + row * lddy + ring.first(kUnit * g.thread);
     bool in[NE];
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-        const int c = kUnit * (g.thread + 32 * warps * i);
-        in[i] = c < cols;
-        load_pairs(w, c, in[i], 1.f, wv[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dw[i][j] = db[i][j] = 0ull;
-    }
-    const int step = 32 * kUnit * warps;
-    const T *xp = x + row * ldx + kUnit * g.thread, *dp = dy + row * lddy + kUnit * g.thread;
-    Packed<T> nx[NE], nd[NE];
-    float next_mean = 0.f, next_rstd = 0.f;
-    auto fetch = [&](long long r) {
-#pragma unroll
-        for (int i = 0; i < NE; ++i)
-            if (in[i]) {
-                load_packed(nx[i], xp + step * i);
-                load_packed(nd[i], dp + step * i);
-            }
-        next_mean = __ldg(stats + r);
-        next_rstd = __ldg(stats + rows + r);
+    for (int i = 0; i < NE; ++i) in[i] = kUnit * (g.thread + 32 * warps * i) < cols;
+    long long ahead = row;
+    auto fetch = [&] {
+        if (ahead < rows) {
+            ring.put(0, xp, step);
+            ring.put(1, dp, step);
+        }
+        ring.end_row();
+        ahead += stride;
         xp += stride * ldx;
         dp += stride * lddy;
     };
-    if (kAhead && row < rows) fetch(row);
+#pragma unroll
+    for (int k = 1; k < ring.kSlots; ++k) fetch();
+    uint64_t dw[NE][4], db[NE][4], wv[NE][4];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        load_pairs(w, kUnit * (g.thread + 32 * warps * i), in[i], 1.f, wv[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dw[i][j] = db[i][j] = 0ull;
+    }
+    float next_mean = row < rows ? __ldg(stats + row) : 0.f, next_rstd = row < rows ? __ldg(stats + rows + row) : 0.f;
     for (; row < rows; row += stride) {
-        if (!kAhead) fetch(row);
         uint64_t xv[NE][4], dv[NE][4];
         const float mean = next_mean, rstd = next_rstd;
         const uint64_t minus = tc::both(-mean), r2 = tc::both(rstd);
+        ring.wait_row();
 #pragma unroll
-        for (int i = 0; i < NE; ++i) {
-            unpack(nx[i], xv[i]);
-            unpack(nd[i], dv[i]);
+        for (int i = 0; i < NE; ++i)
+            if (in[i]) {
+                Packed<T> ux, ud;
+                ring.get(0, i, ux);
+                ring.get(1, i, ud);
+                unpack(ux, xv[i]);
+                unpack(ud, dv[i]);
+            }
+        ring.end_read();
+        fetch();
+        if (row + stride < rows) {
+            next_mean = __ldg(stats + row + stride);
+            next_rstd = __ldg(stats + rows + row + stride);
         }
-        if (kAhead && row + stride < rows) fetch(row + stride);
         uint64_t s1 = 0ull, s2 = 0ull;
 #pragma unroll
         for (int i = 0; i < NE; ++i)
@@ -621,7 +692,11 @@ layer_norm_whole_backward_kernel(const T *__restrict__ dy, long long lddy, const
         for (int i = 0; i < NE; ++i) {
             const int c = kUnit * (g.thread + 32 * warps * i);
             const uint64_t (&v)[4] = which ? db[i] : dw[i];
-            if (groups > 1) store_pairs(fold + g.id * width + c, v);
+            if (groups > 1) {
+                float4 *f = reinterpret_cast<float4 *>(fold + g.id * width + c);
+                f[0] = make_float4(tc::low_of(v[0]), tc::high_of(v[0]), tc::low_of(v[1]), tc::high_of(v[1]));
+                f[1] = make_float4(tc::low_of(v[2]), tc::high_of(v[2]), tc::low_of(v[3]), tc::high_of(v[3]));
+            }
             else if (in[i])
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -783,11 +858,13 @@ Layout whole_layout(int64_t rows, int32_t cols, int most_units) {
 
 // the rows' types leave registers for so many units
 template <class T> constexpr int kWholeForward = sizeof(T) == 4 ? 2 : 3;
-template <class T> constexpr int kWholeBackward = sizeof(T) == 4 ? 1 : 2;             // with a row on its way; fp32 rows of more
-                                                                                      // than 4096 columns take 2 without
+template <class T> constexpr int kWholeBackward = sizeof(T) == 4 ? 1 : 2;             // fp32 rows of more than 4096 columns take 2
+                                                                                      // (at 2048 columns: 82 instead of 77 us)
+
+std::mutex g_norm_mutex;
 
 bool whole_rows(const void *p, int64_t ld, size_t elem) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (size_t)ld * elem % 16 == 0;
+    return reinterpret_cast<uintptr_t>(p) % (kUnit * elem) == 0 && ld % kUnit == 0;
 }
 
 template <class T, int NE>
@@ -804,9 +881,13 @@ template <class T, int NE>
 int run_whole_backward(const Layout &l, const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t rows, int32_t cols,
                        const float *w, const float *stats, void *dx, int64_t lddx, float *partial, int64_t splits,
                        cudaStream_t st) {
-    // the groups' columns: at most 16 warps' of 2 units, 32 KB
-    const int smem = partial && l.groups > 1 ? l.groups * l.warps * 32 * kUnit * NE * (int)sizeof(float) : 0;
-    layer_norm_whole_backward_kernel<T, NE><<<(unsigned)splits, 32 * l.warps * l.groups, smem, st>>>(
+    static bool ready[64] = {false};
+    const int threads = 32 * l.warps * l.groups;
+    static_assert(Ring<T, NE, 2>::kBytes >= kUnit * NE * (int)sizeof(float), "the groups' sums fit where the rows were");
+    const int rc = tc::allow_smem(layer_norm_whole_backward_kernel<T, NE>, Ring<T, NE, 2>::kBytes * 32 * kWholeWarps, ready,
+                                  g_norm_mutex, nullptr);
+    if (rc != MORTAR_OK) return rc;
+    layer_norm_whole_backward_kernel<T, NE><<<(unsigned)splits, threads, Ring<T, NE, 2>::kBytes * threads, st>>>(
         (const T *)dy, lddy, (const T *)x, ldx, rows, cols, w, stats, (T *)dx, lddx, partial, l.warps);
     MORTAR_CUDA_CHECK(cudaGetLastError());
     return MORTAR_OK;
