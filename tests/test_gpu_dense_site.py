@@ -828,3 +828,42 @@ def test_mlp_dense_tiles_of_both_widths(rows, d, f):
     """Launches whose tiles fill the machine and launches whose do not, ragged in every direction: of the first shape
     gate/up, dh and the gradients run on tiles of 256 columns and down on 128, of the second only dh on 128."""
     test_mlp_dense_cut_reductions(rows, d, f)
+
+
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_fp8_rows_off_32_bytes(dt, block_rows):
+    """Rows that start on 16 but not on 32 bytes, read and written."""
+    e = dt.itemsize
+    x = rand(130, 416, seed=1, dt=dt)[:, :400].contiguous()
+    per16 = 16 // e
+    wide = torch.zeros(130, 400 + per16, device=DEV, dtype=dt)
+    views = [wide[:, :400], wide[:, per16:]]
+    want = ops.quantize_fp8(x, block_rows=block_rows)
+    for v in views:
+        v.copy_(x)
+        got = ops.quantize_fp8(v, block_rows=block_rows)
+        assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))
+    back = ops.dequantize_fp8(*want, out_dtype=dt)
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dt]
+    wide.fill_(7.0)
+    rc = mb._lib.lib().mortar_dequantize_fp8(want[0].data_ptr(), 3, 400, want[1].data_ptr(), 130, 400, block_rows,
+                                             wide[:, per16:].data_ptr(), code, 400 + per16, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(wide[:, per16:], back) and bool((wide[:, :per16] == 7.0).all())
+
+
+@pytest.mark.parametrize("off,ld", [(4, 72), (0, 68), (8, 72), (4, 68)])
+def test_layer_norm_fp32_rows_off_32_bytes(off, ld):
+    """fp32 rows whose 8-column units start on 16 bytes only take the kernel for any alignment: the results are as close."""
+    flat = torch.zeros(33 * 72 + 16, device=DEV)
+    x = torch.as_strided(flat, (33, 64), (ld, 1), off)
+    x.copy_(rand(33, 64, seed=1) + 0.5)
+    w, b, dy = rand(64, seed=2), rand(64, seed=3), rand(33, 64, seed=4)
+    y, stats = ops.layer_norm_forward(x, w, b, 1e-5, True)
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, stats)
+    ry, xh, rstd, mean, rdx, rdw, rdb = ln_ref(x, w, b, 1e-5, dy)
+    # 64 terms in sums of depth <= 16, a few operations each: 64 f of the largest magnitudes that meet
+    within(y, ry, 64 * F * (1 + ry.abs().max()), "y")
+    within(dx, rdx, 64 * F * (1 + rdx.abs().max()) * (1 + xh.abs().max()) ** 2, "dx")
+    within(dw, rdw.sum(0), 64 * F * (dy.double() * xh).abs().sum(0), "dw")
+    within(db, rdb.sum(0), 64 * F * dy.double().abs().sum(0), "db")
