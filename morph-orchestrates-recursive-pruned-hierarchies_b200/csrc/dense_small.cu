@@ -13,7 +13,7 @@
 // Where there are too few row tiles for the SMs, a cluster of CTAs shares a tile's k and adds in rank
 // order.  The order is fixed, so the same call gives the same bits.
 //
-// One token, 2048/5632: gate/up (46 MB) 13.7 us = 3.4 TB/s, down (23 MB) 11.1 us, 19.4 us together since the second
+// One token, 2048/5632: gate/up (46 MB) 13.7 us = 3.4 TB/s, down (23 MB) 11.1 us, 18.3 us together since the second
 // fetches weights while the first ends.  4 tokens against the 8-bit 2048 -> 11264 matrix (23 MB): 11.6 us.  With
 // several microseconds of launch and first access in each, a longer queue of weights (64 KB an SM here) has
 // nothing left to hide; CTAs of one tile each instead of a queue across tiles took 24.6 us for the block.

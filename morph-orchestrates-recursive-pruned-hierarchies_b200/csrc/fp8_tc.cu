@@ -13,11 +13,12 @@
 // while the MMAs fill the other set.  A cluster of two CTAs computes 256 x 256: every thread of eight
 // epilogue warps keeps 128 sums, for which the launch's registers are dealt out anew.
 //
-// What bounds it, at 8192 x 2048 -> 11264 with the gate (213 to 225 us, 1700 TFLOP/s): the epilogue warps.
+// What bounds it, at 8192 x 2048 -> 11264 with the gate (206 to 220 us, 1720 to 1830 TFLOP/s, 233 in a long
+// run under the power cap): the epilogue warps.
 // The same MMAs and copies with one sum per tile instead of one per block take 139 us.  A block's MMAs are
 // 512 cycles; a warp needs about 800 for it: 150 to see that the block is there, twice 75 to read 64 columns
 // and 150 to multiply and add them (3 cycles a packed multiply-add), 75 to hand the set back, the rest to
-// walk on; and 5700 a tile for the gate and the stores.  Tried without gain: four sets of 128 columns (279
+// walk on; and 4700 a tile for the gate and the stores (193 us without the gate).  Tried without gain: four sets of 128 columns (279
 // us), reading 32 columns ahead (238), asking for the next block before the multiply-adds (the register it
 // takes costs more than it hides), arrivals with release at cluster scope (630: they wait for the stores).
 #include <cuda.h>
@@ -61,9 +62,19 @@ struct Fp8Params {
     int out_dtype;
 };
 
-// exp2-based exponential and an approximate quotient, 2^-22 (1 + |g|) at worst: the exact forms cost the
-// epilogue of a 256 x 256 tile three times what its 16 blocks of MMAs take (631 against 420 us at 8192 x 2048 -> 11264)
-__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
+__device__ __forceinline__ float exp2_of(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float inverse_of(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+// silu(g) u of two columns, from the approximate power and inverse: off by 2^-22 (1 + |g|) of the result at worst.  A
+// tile's 16384 a CTA keep the special function unit busy for 2000 of 19000 cycles; with __expf and __fdividef, which
+// handle more than is needed here, the product of the header took 216 where it takes 206 us, with expf and a division 631.
+__device__ __forceinline__ uint64_t gated(uint64_t g, uint64_t u) {
+    const uint64_t t = tc::mul2(g, tc::both(-1.4426950408889634f));       // exp(-g) = 2^t
+    const uint64_t d = tc::add2(tc::pair_of(__float_as_uint(exp2_of(tc::low_of(t))), __float_as_uint(exp2_of(tc::high_of(t)))),
+                                tc::both(1.f));
+    const uint64_t r = tc::pair_of(__float_as_uint(inverse_of(tc::low_of(d))), __float_as_uint(inverse_of(tc::high_of(d))));
+    return tc::mul2(tc::mul2(g, r), u);
+}
 
 // A warp's 32 rows x 32 columns from (row0, col) on; v = this lane's row.  Rows that start on 32 bytes and end on a
 // multiple of 32 columns are stored 32 bytes at a time, each lane its own.  Others (TURNED) are turned in shared memory, so that the lanes of a store lie side by side
@@ -282,12 +293,9 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                 float v[32];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    v[2 * i] = tc::low_of(sum[j][i]);
-                    v[2 * i + 1] = tc::high_of(sum[j][i]);
-                    if (p.up_row) {
-                        v[2 * i] = silu(v[2 * i]) * tc::low_of(sum[(j + kPer) % (2 * kPer)][i]);
-                        v[2 * i + 1] = silu(v[2 * i + 1]) * tc::high_of(sum[(j + kPer) % (2 * kPer)][i]);
-                    }
+                    const uint64_t y = p.up_row ? gated(sum[j][i], sum[(j + kPer) % (2 * kPer)][i]) : sum[j][i];
+                    v[2 * i] = tc::low_of(y);
+                    v[2 * i + 1] = tc::high_of(y);
                 }
                 int col;
                 if constexpr (HALF) col = p.up_row ? tn * 128 + part * 64 + side * 32 : tn * 256 + part * 128 + j * 64 + side * 32;
