@@ -335,13 +335,28 @@ dense_pair_kernel(const __grid_constant__ DenseParams p) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// out[m][n] = the parts of its reduction added in order, 8 columns a thread.  The parts are read past L1: the kernel
-// may start before the one that writes them has ended.
+struct Join {
+    const float *partial;    // [splits][m][n]
+    void *out;               // 16-bit [m][n]
+    long long m, ld_out;
+    int n, splits;
+    unsigned first_block;
+};
+struct Joins { Join part[kMaxProblems]; int count, half; };
+
+// out[m][n] = the parts of its reduction added in order, 8 columns a thread, for all cut products of a launch.  The parts
+// are read past L1: the kernel may start before the one that writes them has ended.
 __global__ void __launch_bounds__(256)
-dense_reduce_kernel(const float *__restrict__ partial, int splits, long long m, int n, void *out, long long ld_out, int half) {
+dense_reduce_kernel(const __grid_constant__ Joins joins) {
     tc::let_next();
     tc::after_previous();
-    const long long total = m * (n / 8), at = (long long)blockIdx.x * 256 + threadIdx.x;
+    int p = 0;
+    while (p + 1 < joins.count && blockIdx.x >= joins.part[p + 1].first_block) ++p;
+    const Join &q = joins.part[p];
+    const float *partial = q.partial;
+    const long long m = q.m;
+    const int n = q.n, splits = q.splits, half = joins.half;
+    const long long total = m * (n / 8), at = (long long)(blockIdx.x - q.first_block) * 256 + threadIdx.x;
     if (at >= total) return;
     const long long row = at / (n / 8);
     const int col = (int)(at - row * (n / 8)) * 8;
@@ -365,7 +380,7 @@ dense_reduce_kernel(const float *__restrict__ partial, int splits, long long m, 
                 v[4] += b[s].x; v[5] += b[s].y; v[6] += b[s].z; v[7] += b[s].w;
             }
     }
-    *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(out) + row * ld_out + col) =
+    *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(q.out) + row * q.ld_out + col) =
         make_uint4(tc::pack16(v[0], v[1], half), tc::pack16(v[2], v[3], half), tc::pack16(v[4], v[5], half), tc::pack16(v[6], v[7], half));
 }
 
@@ -446,14 +461,18 @@ void cut(DenseParams &p, const Plan &plan, float *scratch) {
 }
 
 int join(const DenseParams &p, cudaStream_t st) {
+    Joins j = {};
+    int64_t blocks = 0;
     for (int i = 0; i < p.n_problems; ++i) {
         const Problem &q = p.prob[i];
         if (q.splits == 1) continue;
-        const int rc = tc::launch_after(dense_reduce_kernel, (unsigned)((q.m * (q.n / 8) + 255) / 256), 256u, 0, st,
-                                        (const float *)q.partial, q.splits, q.m, q.n, q.out, q.ld_out, p.half);
-        if (rc != MORTAR_OK) return rc;
+        j.part[j.count++] = {q.partial, q.out, q.m, q.ld_out, q.n, q.splits, (unsigned)blocks};
+        blocks += (q.m * (q.n / 8) + 255) / 256;
     }
-    return MORTAR_OK;
+    if (j.count == 0) return MORTAR_OK;
+    if (blocks > 0x7fffffffLL) return MORTAR_ERR_CAPACITY;
+    j.half = p.half;
+    return tc::launch_after(dense_reduce_kernel, (unsigned)blocks, 256u, 0, st, j);
 }
 
 template <int EPI, int BN>
