@@ -321,6 +321,187 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
+// ---- up to 32 rows: the operands change places -------------------------------------------------
+//
+// With a few tokens most of a 256 x 256 tile's rows do not exist, but its epilogue takes as long.  Here the weights are
+// the 256 rows of a tile and 32 tokens its columns: a thread holds 16 sums of one output column, and the tokens'
+// scales come from a table in shared memory.  With the gate, a CTA's 128 rows are groups of 16 gate rows and the 16 up rows
+// of the same hidden columns, so that lanes l and l + 16 of a warp hold the two sums of an output and exchange them at
+// the end.
+//
+// 32 x 2048 -> 11264 with the gate 13.1 us (L2 flushed 17.3) against 16.6 (21.5) on the tiles above, 32 x 768 -> 4096 9.0
+// against 10.4, 17 x 5632 -> 2048 the same 24.7: a block's way from copy to sums.  With 64 or 128 tokens reading the table for
+// every block takes longer than the larger tile's epilogue (64 x 2048 -> 11264 14.6 against 16.6, 64 x 5632 -> 2048
+// 28.9 against 24.8; 128 rows 20.7 and 38.6 against 16.6 and 25.8); four accumulator sets instead of two changed nothing.
+constexpr int kFewRows = 32;
+constexpr int kFewStages = 6;
+constexpr int kFewB = kFewRows / 2 * 128;                        // this CTA's half of the tokens, one block
+constexpr int kFewStage = kStageA + kFewB;
+constexpr int kFewFixed = kFewStages * kFewStage + (2 * kFewStages + 2) * 8 + 1024;
+constexpr int kFewBlocks = (226 * 1024 - kFewFixed) / (4 * kFewRows);      // that the table has room for
+constexpr int few_smem(int k_blocks) { return kFewFixed + 4 * kFewRows * k_blocks; }
+
+__device__ __forceinline__ void store_one(const Fp8Params &p, int m, int col, float v) {
+    if (m >= p.rows || col >= p.n) return;
+    const long long idx = m * p.ld_out + col;
+    if (p.out_dtype == MORTAR_F32) reinterpret_cast<float *>(p.out)[idx] = v;
+    else reinterpret_cast<uint16_t *>(p.out)[idx] = (uint16_t)tc::pack16(v, 0.f, p.out_dtype == MORTAR_F16);
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+fp8_few_kernel(const __grid_constant__ Fp8Params p) {
+    constexpr int kHeld = kFewRows / 2;                             // sums of a thread
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t *>(stages + kFewStages * kFewStage), *done = full + kFewStages;
+    uint64_t *acc_empty = done + kFewStages;
+    float *table = reinterpret_cast<float *>(acc_empty + 2);     // [block][token]
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int abort_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = tc::cluster_rank();
+    const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        abort_s = 0;
+        for (int s = 0; s < kFewStages; ++s) { tc::mbar_init(tc::smem_u32(&full[s]), 1); tc::mbar_init(tc::smem_u32(&done[s]), 1); }
+        for (int s = 0; s < 2; ++s) tc::mbar_init(tc::smem_u32(&acc_empty[s]), 2 * kEpiWarps);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                     ::"r"(tc::smem_u32(&tmem_base_s)), "r"(2 * kFewRows) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();
+    tc::fence_after();
+    const uint32_t tmem = tmem_base_s;
+    volatile int *abort_flag = &abort_s;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint32_t full_lead = tc::cluster_addr(tc::smem_u32(full), 0);
+            const uint32_t done0 = tc::smem_u32(done), stage0 = tc::smem_u32(stages);
+            uint32_t s = 0, parity = 1;
+            bool ok = true;
+            for (int tile = cluster_id; tile < p.n_items && ok; tile += n_clusters)
+                for (int k = 0; k < p.k_blocks; ++k) {
+                    if (!tc::mbar_wait(done0 + 8 * s, parity, abort_flag, &g_fp8_error, 1)) { ok = false; break; }
+                    const uint32_t bar = full_lead + 8 * s, dst = stage0 + s * kFewStage;
+                    if (rank == 0) tc::mbar_arrive_expect_tx(tc::smem_u32(&full[s]), 2 * kFewStage);
+                    if (p.up_row) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            tc::load_pair_3d(dst + 4096 * i, &p.map_w, k * 128, tile * 128 + (int)rank * 64 + 16 * i, 0, bar);
+                    } else {
+                        tc::load_pair(dst, &p.map_w, k * 128, tile * 256 + (int)rank * 128, bar);
+                    }
+                    tc::load_pair(dst + kStageA, &p.map_x, k * 128, (int)rank * kHeld, bar);
+                    if (++s == kFewStages) { s = 0; parity ^= 1; }
+                }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && lane == 0) {
+            const uint32_t idesc = (1u << 4) | p.types | ((uint32_t)(kFewRows >> 3) << 17) | ((256u >> 4) << 24);
+            const uint32_t full0 = tc::smem_u32(full), done0 = tc::smem_u32(done), acc_empty0 = tc::smem_u32(acc_empty);
+            const uint64_t da = tc::make_smem_desc(tc::smem_u32(stages), 16, 1024, 2);
+            const uint64_t db = tc::make_smem_desc(tc::smem_u32(stages) + kStageA, 16, 1024, 2);
+            uint32_t s = 0, parity = 0, g = 0;
+            bool ok = true, ready = tc::mbar_try_wait(full0, 0);
+            for (int tile = cluster_id; tile < p.n_items && ok; tile += n_clusters)
+                for (int k = 0; k < p.k_blocks; ++k, ++g) {
+                    const uint32_t buf = g & 1;
+                    if ((!ready && !tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_fp8_error, 3)) ||
+                        !tc::mbar_wait(acc_empty0 + 8 * buf, ((g >> 1) & 1) ^ 1u, abort_flag, &g_fp8_error, 2)) { ok = false; break; }
+                    tc::fence_after();
+                    const uint64_t at = (uint64_t)(s * (kFewStage >> 4));
+                    const uint32_t bar = done0 + 8 * s;
+                    if (++s == kFewStages) { s = 0; parity ^= 1; }
+                    ready = tc::poll_mma4_f8(full0 + 8 * s, parity, tmem + buf * kFewRows, da + at, db + at, idesc);
+                    tc::commit_both(bar);
+                }
+        }
+    } else if (warp >= 4) {
+        // warp w: weight rows 32 (w % 4) .. +31 of the CTA's, tokens kHeld side .. +kHeld - 1
+        const int quarter = warp & 3, side = (warp - 4) >> 2, tid = (int)threadIdx.x - 128;
+#pragma unroll 4
+        for (int i = tid; i < kFewRows * p.k_blocks; i += 32 * kEpiWarps) {
+            const int m = i / p.k_blocks, b = i - m * p.k_blocks;
+            table[b * kFewRows + m] = m < p.rows ? __ldg(p.xs + m * p.ld_xs + b) : 0.f;
+        }
+        asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kEpiWarps) : "memory");       // before any of them can give up
+        const uint32_t done0 = tc::smem_u32(done), lead_empty = tc::cluster_addr(tc::smem_u32(acc_empty), 0);
+        const uint32_t taddr0 = tmem + ((uint32_t)(quarter * 32) << 16) + side * kHeld;
+        const bool upper = lane >= 16;
+        uint32_t g = 0, s = 0, parity = 0;
+        bool ok = true;
+        for (int tile = cluster_id; tile < p.n_items && ok; tile += n_clusters) {
+            const int block = p.up_row ? tile + (upper ? p.up_row / 128 : 0) : min(2 * tile + (int)rank, p.w_blocks - 1);
+            uint32_t at_w = (uint32_t)(block * p.ld_ws);
+            float next = __ldg(p.ws + at_w);
+            uint64_t sum[kHeld / 2];
+#pragma unroll
+            for (int i = 0; i < kHeld / 2; ++i) sum[i] = 0ull;
+            for (int k = 0; k < p.k_blocks; ++k, ++g) {
+                const uint32_t buf = g & 1;
+                const uint64_t sw2 = tc::both(next);
+                if (k + 1 < p.k_blocks) next = __ldg(p.ws + ++at_w);
+                const float4 *sx = reinterpret_cast<const float4 *>(table + k * kFewRows + side * kHeld);
+                if (!tc::mbar_wait(done0 + 8 * s, parity, abort_flag, &g_fp8_error, 4)) { ok = false; break; }
+                if (++s == kFewStages) { s = 0; parity ^= 1; }
+                __syncwarp();
+                tc::fence_after();
+                uint32_t r[kHeld];
+#pragma unroll
+                for (int c = 0; c < kHeld; c += 16) tc::ld16_ahead(taddr0 + buf * kFewRows + c, *reinterpret_cast<uint32_t (*)[16]>(r + c));
+                tc::wait_ld();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::arrive_relaxed(lead_empty + 8 * buf);
+#pragma unroll
+                for (int i = 0; i < kHeld / 4; ++i) {
+                    const float4 f = sx[i];
+                    sum[2 * i] = tc::fma2(tc::pair_of(r[4 * i], r[4 * i + 1]),
+                                          tc::mul2(tc::pair_of(__float_as_uint(f.x), __float_as_uint(f.y)), sw2), sum[2 * i]);
+                    sum[2 * i + 1] = tc::fma2(tc::pair_of(r[4 * i + 2], r[4 * i + 3]),
+                                              tc::mul2(tc::pair_of(__float_as_uint(f.z), __float_as_uint(f.w)), sw2), sum[2 * i + 1]);
+                }
+            }
+            if (!ok) break;
+            // with the gate lanes below 16 finish the first half of the tokens, the others the second half
+            const int col = p.up_row ? tile * 128 + (int)rank * 64 + quarter * 16 + (lane & 15)
+                                     : tile * 256 + (int)rank * 128 + quarter * 32 + lane;
+            if (p.up_row) {
+#pragma unroll
+                for (int i = 0; i < kHeld / 4; ++i) {
+                    const uint64_t mine = upper ? sum[kHeld / 4 + i] : sum[i];
+                    const uint64_t other = __shfl_xor_sync(0xffffffffu, upper ? sum[i] : sum[kHeld / 4 + i], 16);
+                    const uint64_t y = upper ? gated(other, mine) : gated(mine, other);
+                    const int m = side * kHeld + (upper ? kHeld / 2 : 0) + 2 * i;
+                    store_one(p, m, col, tc::low_of(y));
+                    store_one(p, m + 1, col, tc::high_of(y));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kHeld / 2; ++i) {
+                    store_one(p, side * kHeld + 2 * i, col, tc::low_of(sum[i]));
+                    store_one(p, side * kHeld + 2 * i + 1, col, tc::high_of(sum[i]));
+                }
+            }
+        }
+    }
+
+    __syncwarp();
+    if (*abort_flag) tc::drain_after_abort();
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(2 * kFewRows) : "memory");
+}
+
 bool misaligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
 
 std::mutex g_fp8_mutex;
@@ -332,6 +513,24 @@ int launch(const Fp8Params &p, int sms, cudaStream_t st) {
     if (rc != MORTAR_OK) return rc;
     const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
     fp8_pair_kernel<TURNED, HALVES><<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
+    MORTAR_CUDA_CHECK(cudaGetLastError());
+    return MORTAR_OK;
+}
+
+// `p` without its maps
+int launch_few(Fp8Params &p, const void *x, int64_t ldx, const void *w, int64_t ldw, int in_features, int out_features, int sms,
+               cudaStream_t st) {
+    static bool ready[64] = {false};
+    int rc = tc::allow_smem(fp8_few_kernel, few_smem(kFewBlocks), ready, g_fp8_mutex, nullptr);
+    if (rc != MORTAR_OK) return rc;
+    rc = tc::encode_u8_2d(&p.map_x, x, in_features, p.rows, ldx, kFewRows / 2);
+    if (rc != MORTAR_OK) return rc;
+    rc = p.up_row ? tc::encode_u8_3d(&p.map_w, w, in_features, p.up_row, ldw, 16)
+                  : tc::encode_u8_2d(&p.map_w, w, in_features, out_features, ldw, 128);
+    if (rc != MORTAR_OK) return rc;
+    p.n_items = (out_features + 255) / 256;
+    const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
+    fp8_few_kernel<<<(unsigned)(2 * clusters), kThreads, few_smem(p.k_blocks), st>>>(p);
     MORTAR_CUDA_CHECK(cudaGetLastError());
     return MORTAR_OK;
 }
@@ -377,14 +576,22 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     rc = tc::bind_context();
     if (rc != MORTAR_OK) return rc;
     alignas(64) Fp8Params p = {};
-    rc = tc::encode_u8_2d(&p.map_x, x, in_features, rows, ldx, 128);
-    if (rc != MORTAR_OK) return rc;
-    rc = tc::encode_u8_2d(&p.map_w, w, in_features, out_features, ldw, 128);
-    if (rc != MORTAR_OK) return rc;
     p.xs = x_scale; p.ws = w_scale; p.ld_xs = ld_x_scale; p.ld_ws = ld_w_scale;
     p.rows = rows;
     p.n = gated ? out_features / 2 : out_features;
     p.up_row = gated ? out_features / 2 : 0;
+    p.k_blocks = (int)k_blocks;
+    p.w_blocks = (out_features + 127) / 128;
+    p.out = out; p.ld_out = ld_out; p.out_dtype = out_dtype;
+    if (rows <= kFewRows && k_blocks <= kFewBlocks) {
+        p.types = (w_type == MORTAR_E5M2 ? 1u << 7 : 0u) | (x_type == MORTAR_E5M2 ? 1u << 10 : 0u);
+        return launch_few(p, x, ldx, w, ldw, in_features, out_features, sms, st);
+    }
+    p.types = (x_type == MORTAR_E5M2 ? 1u << 7 : 0u) | (w_type == MORTAR_E5M2 ? 1u << 10 : 0u);
+    rc = tc::encode_u8_2d(&p.map_x, x, in_features, rows, ldx, 128);
+    if (rc != MORTAR_OK) return rc;
+    rc = tc::encode_u8_2d(&p.map_w, w, in_features, out_features, ldw, 128);
+    if (rc != MORTAR_OK) return rc;
     const int tile_n = gated ? 128 : 256;
     p.tiles_m = (int)((rows + 255) / 256);
     p.tiles_n = (p.n + tile_n - 1) / tile_n;
@@ -399,10 +606,6 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
         rc = tc::encode_u8_2d(&p.map_w_half, w, in_features, out_features, ldw, 64);
         if (rc != MORTAR_OK) return rc;
     }
-    p.k_blocks = (int)k_blocks;
-    p.w_blocks = (out_features + 127) / 128;
-    p.types = (x_type == MORTAR_E5M2 ? 1u << 7 : 0u) | (w_type == MORTAR_E5M2 ? 1u << 10 : 0u);
-    p.out = out; p.ld_out = ld_out; p.out_dtype = out_dtype;
     const bool turned = misaligned(out, 32) || (ld_out * e) % 32 || p.n % 32;
 
     if (p.whole < tiles) return turned ? launch<true, true>(p, sms, st) : launch<false, true>(p, sms, st);

@@ -32,6 +32,12 @@ __device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap *map, 
         "[%0], [%1, {%2, %3}], [%4];\n"
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
 }
+__device__ __forceinline__ void load_pair_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t cluster_bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];\n"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(cluster_bar) : "memory");
+}
 // Whether the phase has completed, without waiting for it (try_wait may hold the thread for a while)
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -222,6 +228,25 @@ inline int encode_u8_2d(CUtensorMap *map, const void *base, int64_t cols, int64_
     const cuuint32_t box[2] = {128, box_rows};
     const cuuint32_t estride[2] = {1, 1};
     const CUresult cr = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), gdim, gstride, box,
+                               estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) {
+        mortar_set_cuda_error("cuTensorMapEncodeTiled", "failed to encode a tensor map");
+        return MORTAR_ERR_CUDA;
+    }
+    return MORTAR_OK;
+}
+
+// The same matrix seen as its two halves of `rows` rows each: a box is the same [box_rows] rows of both.
+inline int encode_u8_3d(CUtensorMap *map, const void *base, int64_t cols, int64_t rows, int64_t ld, uint32_t box_rows) {
+    EncodeTiledFn encode;
+    const int rc = get_encode_fn(&encode);
+    if (rc != MORTAR_OK) return rc;
+    const cuuint64_t gdim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 2};
+    const cuuint64_t gstride[2] = {(cuuint64_t)ld, (cuuint64_t)ld * (cuuint64_t)rows};
+    const cuuint32_t box[3] = {128, box_rows, 2};
+    const cuuint32_t estride[3] = {1, 1, 1};
+    const CUresult cr = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), gdim, gstride, box,
                                estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (cr != CUDA_SUCCESS) {

@@ -867,3 +867,34 @@ def test_layer_norm_fp32_rows_off_32_bytes(off, ld):
     within(dx, rdx, 64 * F * (1 + rdx.abs().max()) * (1 + xh.abs().max()) ** 2, "dx")
     within(dw, rdw.sum(0), 64 * F * (dy.double() * xh).abs().sum(0), "dw")
     within(db, rdb.sum(0), 64 * F * dy.double().abs().sum(0), "db")
+
+
+@pytest.mark.parametrize("rows,out,cols", [(17, 128, 128), (32, 3333, 272), (33, 20000, 144), (64, 1000, 400), (65, 129, 2000),
+                                           (100, 16, 16), (127, 20736, 96), (128, 515, 656), (18, 16, 16), (31, 20736, 96),
+                                           (32, 20000, 656), (19, 129, 2000)])
+def test_linear_fp8_few_rows(rows, out, cols):
+    """17 to 32 rows, where the operands change places, and a few more: one tile and more than run at once, ragged widths."""
+    test_linear_fp8(rows, out, cols, torch.float8_e5m2, torch.float8_e4m3fn)
+    test_linear_fp8(rows, out, cols, torch.float8_e4m3fn, torch.float8_e5m2)
+
+
+@pytest.mark.parametrize("rows,d_ff,cols", [(17, 128, 16), (31, 1280, 272), (40, 128 * 76, 144), (64, 384, 2000), (128, 640, 400),
+                                            (32, 128 * 76, 144), (20, 384, 2000)])
+def test_linear_fp8_few_rows_with_the_gate(rows, d_ff, cols):
+    test_linear_fp8_with_the_gate(rows, d_ff, cols, torch.float8_e4m3fn)
+    test_linear_fp8_with_the_gate(rows, d_ff, cols, torch.float8_e5m2)
+
+
+def test_linear_fp8_few_rows_write_their_rows_only():
+    """The C entry with rows of the output further apart than they are wide, and a wide reduction that the few rows'
+    table has no room for."""
+    for rows, out, cols in ((33, 300, 272), (100, 64, 128 * 170), (19, 300, 272), (30, 64, 128 * 1000)):
+        x, xs, w, ws = fp8_operands(rows, out, cols, torch.float8_e4m3fn, torch.float8_e4m3fn)
+        y = torch.full((rows + 3, out + 5), 7.0, device=DEV)
+        rc = mb._lib.lib().mortar_linear_fp8(x.data_ptr(), 3, cols, xs.data_ptr(), xs.shape[1], rows, w.data_ptr(), 3, cols, ws.data_ptr(),
+                                             ws.shape[1], out, cols, 0, y.data_ptr(), 0, out + 5, torch.cuda.current_stream().cuda_stream)
+        ref, mag = fp8_linear_ref(x, xs, w, ws)
+        assert rc == 0
+        within(y[:rows, :out], ref, fp8_bound(ref, mag, cols, torch.float32))
+        assert bool((y[rows:] == 7).all()) and bool((y[:, out:] == 7).all())
+    errors_are_clear()
