@@ -1,4 +1,4 @@
-// Products for a few tokens (up to 32 rows of 16-bit operands, 16 of 8-bit ones): bound by reading the weights once.
+// Products for a few tokens (up to 32 rows; 8-bit operands of more than 16 only where the weight is narrow): bound by reading the weights once.
 //
 // A warp multiplies 16 weight rows by up to 8, 16 or 32 tokens with mma.sync (M = 16 weight rows, N = 8
 // tokens): at these sizes the tensor cores idle either way, and operands that go straight from
@@ -242,13 +242,11 @@ int pick(const small::Params &p, int sms, cudaStream_t st) {
     if (p.up_row) {
         if (p.rows <= 8) return run<KIND, XT, WT, 1, true>(p, sms, st);
         if (p.rows <= 16) return run<KIND, XT, WT, 2, true>(p, sms, st);
-        if constexpr (KIND != k8) return run<KIND, XT, WT, 4, true>(p, sms, st);
-        return MORTAR_ERR_CAPACITY;
+        return run<KIND, XT, WT, 4, true>(p, sms, st);
     }
     if (p.rows <= 8) return run<KIND, XT, WT, 1, false>(p, sms, st);
     if (p.rows <= 16) return run<KIND, XT, WT, 2, false>(p, sms, st);
-    if constexpr (KIND != k8) return run<KIND, XT, WT, 4, false>(p, sms, st);
-    return MORTAR_ERR_CAPACITY;
+    return run<KIND, XT, WT, 4, false>(p, sms, st);
 }
 
 }  // namespace

@@ -6,10 +6,10 @@
 
 namespace small {
 
-// Most rows that these kernels take, against the tensor-memory kernels of dense_tc.cu and fp8_tc.cu with their 256-row
-// tiles (us, L2 flushed, 2048/5632): 16-bit block of 32 rows 39 here, 45 there; 8-bit 2048 -> 11264 of 16 rows 18 here and
-// 21 there, of 32 rows 25 here and 22 there.
-constexpr int kMaxRows = 32, kMaxRows8 = 16;
+// Most rows that these kernels take.  Against the tensor-memory kernels (us, L2 flushed): 16-bit block 2048/5632 of 32 rows
+// 39 here, 45 in dense_tc.cu with its 256-row tiles; 8-bit operands of 17 to 32 rows only where the weight is narrow, as
+// fp8_tc.cu says.
+constexpr int kMaxRows = 32;
 
 struct Params {
     const uint8_t *x, *w;            // rows of bytes

@@ -23,6 +23,7 @@
 // takes costs more than it hides), arrivals with release at cluster scope (630: they wait for the stores).
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <algorithm>
 #include <cstdint>
 #include <mutex>
 #include <type_traits>
@@ -330,7 +331,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
 // the end.
 //
 // 32 x 2048 -> 11264 with the gate 13.1 us (L2 flushed 17.3) against 16.6 (21.5) on the tiles above, 32 x 768 -> 4096 9.0
-// against 10.4, 17 x 5632 -> 2048 the same 24.7: a block's way from copy to sums.  With 64 or 128 tokens reading the table for
+// against 10.4: a block's way from copy to sums.  With 64 or 128 tokens reading the table for
 // every block takes longer than the larger tile's epilogue (64 x 2048 -> 11264 14.6 against 16.6, 64 x 5632 -> 2048
 // 28.9 against 24.8; 128 rows 20.7 and 38.6 against 16.6 and 25.8); four accumulator sets instead of two changed nothing.
 constexpr int kFewRows = 32;
@@ -564,7 +565,11 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     int sms = 0;
     int rc = tc::sm_count(&sms);
     if (rc != MORTAR_OK) return rc;
-    if (rows <= small::kMaxRows8) {
+    // Up to 16 rows the small kernel wins everywhere, up to 32 where its CTAs share the reduction of few output columns: 32 x
+    // 5632 -> 2048 12.9 against 24.8 us below, 32 x 2048 -> 2048 8.3 against 12.6, 32 x 768 -> 2304 7.2 against 9.0,
+    // 32 x 4096 -> 4096 16.7 against 20.0; but 32 x 2048 -> 5632 14.4 against 12.9, 32 x 768 -> 4096 10.4 against 9.1
+    const int64_t row_tiles = ((int64_t)out_features + 255) / 256;
+    if (rows <= 16 || (rows <= small::kMaxRows && row_tiles <= std::max<int64_t>(k_blocks, 12))) {
         small::Params q = {};
         q.x = (const uint8_t *)x; q.ldx = ldx; q.w = (const uint8_t *)w; q.ldw = ldw;
         q.rows = (int)rows; q.n = gated ? out_features / 2 : out_features; q.up_row = gated ? out_features / 2 : 0;

@@ -898,3 +898,12 @@ def test_linear_fp8_few_rows_write_their_rows_only():
         within(y[:rows, :out], ref, fp8_bound(ref, mag, cols, torch.float32))
         assert bool((y[rows:] == 7).all()) and bool((y[:, out:] == 7).all())
     errors_are_clear()
+
+
+@pytest.mark.parametrize("rows,out,cols", [(17, 300, 400), (24, 515, 2000), (32, 3070, 144), (32, 4096, 2064), (31, 16, 16)])
+def test_linear_fp8_few_rows_of_narrow_weights(rows, out, cols):
+    """17 to 32 rows and few output columns: the reduction is shared instead."""
+    test_linear_fp8(rows, out, cols, torch.float8_e4m3fn, torch.float8_e4m3fn)
+    test_linear_fp8(rows, out, cols, torch.float8_e5m2, torch.float8_e5m2)
+    if out == 4096:
+        test_linear_fp8_with_the_gate(rows, out // 2, cols, torch.float8_e4m3fn)
