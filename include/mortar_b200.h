@@ -687,6 +687,15 @@ int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, const float *x
                       int64_t rows, const void *w, int32_t w_type, int64_t ldw, const float *w_scale,
                       int64_t ld_w_scale, int32_t out_features, int32_t in_features, int32_t flags,
                       void *out, int32_t out_dtype, int64_t ld_out, void *stream);
+/* The same with room to cut a long reduction over few tiles: scratch is a device array of
+ * mortar_linear_fp8_scratch_floats(...) floats on 32 bytes (0: none is needed, scratch may be NULL, and
+ * NULL is always allowed: nothing is cut then).  The parts are added in order. */
+int mortar_linear_fp8_cut(const void *x, int32_t x_type, int64_t ldx, const float *x_scale, int64_t ld_x_scale,
+                          int64_t rows, const void *w, int32_t w_type, int64_t ldw, const float *w_scale,
+                          int64_t ld_w_scale, int32_t out_features, int32_t in_features, int32_t flags,
+                          void *out, int32_t out_dtype, int64_t ld_out, float *scratch, int64_t scratch_floats,
+                          void *stream);
+int64_t mortar_linear_fp8_scratch_floats(int64_t rows, int32_t out_features, int32_t in_features, int32_t flags);
 int mortar_linear_fp8_error(int32_t *code, int32_t reset);
 
 #ifdef __cplusplus

@@ -55,6 +55,8 @@ struct Fp8Params {
     int tiles_m, tiles_n;
     int whole, n_items;      // items: the first `whole` tiles, then the others' left and right halves
     int k_blocks;
+    int parts;               // of the reduction, an item each (all tiles are halves then); more than one: `out` holds fp32
+    long long part_step;     // [parts][rows][ld_out], `part_step` elements from part to part
     int up_row;              // 0, or the first up row of w (gate applied)
     int w_blocks;            // rows of ws
     uint32_t types;          // operand type bits of the instruction descriptor
@@ -81,14 +83,14 @@ __device__ __forceinline__ uint64_t gated(uint64_t g, uint64_t u) {
 // multiple of 32 columns are stored 32 bytes at a time, each lane its own.  Others (TURNED) are turned in shared memory, so that the lanes of a store lie side by side
 // in a row (stored value by value from each lane's own row, a ragged tile took three times as long).
 template <bool TURNED>
-__device__ __forceinline__ void store_32x32(const Fp8Params &p, long long row0, int col, const float (&v)[32], float *turn) {
+__device__ __forceinline__ void store_32x32(const Fp8Params &p, void *out, long long row0, int col, const float (&v)[32], float *turn) {
     const int left = p.n - col, lane = threadIdx.x & 31;
     if (left <= 0) return;
     const long long row = row0 + lane;
     if constexpr (!TURNED) {
         if (row >= p.rows) return;
         if (p.out_dtype == MORTAR_F32) {
-            float *o = reinterpret_cast<float *>(p.out) + row * p.ld_out + col;
+            float *o = reinterpret_cast<float *>(out) + row * p.ld_out + col;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t w[8];
@@ -98,7 +100,7 @@ __device__ __forceinline__ void store_32x32(const Fp8Params &p, long long row0, 
             }
             return;
         }
-        uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + row * p.ld_out + col;
+        uint16_t *o = reinterpret_cast<uint16_t *>(out) + row * p.ld_out + col;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             uint32_t w[8];
@@ -116,10 +118,10 @@ __device__ __forceinline__ void store_32x32(const Fp8Params &p, long long row0, 
     const int rows = (int)min(32LL, p.rows - row0);
     const long long idx = row0 * p.ld_out + col + lane;
     if (p.out_dtype == MORTAR_F32) {
-        float *o = reinterpret_cast<float *>(p.out) + idx;
+        float *o = reinterpret_cast<float *>(out) + idx;
         for (int r = 0; r < rows; ++r) o[r * p.ld_out] = turn[r * 33 + lane];
     } else {
-        uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + idx;
+        uint16_t *o = reinterpret_cast<uint16_t *>(out) + idx;
         for (int r = 0; r < rows; ++r) o[r * p.ld_out] = (uint16_t)tc::pack16(turn[r * 33 + lane], 0.f, p.out_dtype == MORTAR_F16);
     }
     }
@@ -131,13 +133,24 @@ __device__ __forceinline__ void tile_at(const Fp8Params &p, int i, int &tm, int 
     tn = r / h;
     tm = band * 8 + r - tn * h;
 }
+// What a launch cuts: nothing, the tiles of its last round in two, or (all tiles being halves) their reductions too.
+enum Cut { kWhole = 0, kHalves = 1, kParts = 2 };
 // The tile of an item of halves; returns which half of its columns.
+template <int CUT>
 __device__ __forceinline__ int half_at(const Fp8Params &p, int item, int &tm, int &tn) {
-    tile_at(p, p.whole + ((item - p.whole) >> 1), tm, tn);
-    return (item - p.whole) & 1;
+    const int over = CUT == kParts ? item / p.parts : item - p.whole;
+    tile_at(p, CUT == kParts ? over >> 1 : p.whole + (over >> 1), tm, tn);
+    return over & 1;
+}
+// The blocks of an item: all, or its part of them.
+template <int CUT> __device__ __forceinline__ int first_block(const Fp8Params &p, int item) {
+    return CUT == kParts ? (int)((long long)p.k_blocks * (item % p.parts) / p.parts) : 0;
+}
+template <int CUT> __device__ __forceinline__ int end_block(const Fp8Params &p, int item) {
+    return CUT == kParts ? (int)((long long)p.k_blocks * (item % p.parts + 1) / p.parts) : p.k_blocks;
 }
 
-template <bool TURNED, bool HALVES>
+template <bool TURNED, int CUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
     extern __shared__ uint8_t smem_raw[];
@@ -168,6 +181,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
     __syncthreads();
     tc::cluster_sync();
     tc::fence_after();
+    if constexpr (CUT == kParts) tc::let_next();
     const uint32_t tmem = tmem_base_s;
     volatile int *abort_flag = &abort_s;
 
@@ -183,13 +197,14 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
             for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
                 int tm, tn;
                 int part = -1;
-                if (!HALVES || item < p.whole) tile_at(p, item, tm, tn);
-                else part = half_at(p, item, tm, tn);
+                if (CUT == kWhole || (CUT == kHalves && item < p.whole)) tile_at(p, item, tm, tn);
+                else part = half_at<CUT>(p, item, tm, tn);
+                const int end = end_block<CUT>(p, item);
                 const int row0 = tm * 256 + (int)rank * 128;
                 const int wide = part < 0 ? 128 : 64;                 // this CTA's columns
                 const int col0 = (p.up_row ? tn * 128 + (rank ? p.up_row : 0) + (part > 0 ? 64 : 0)
                                            : tn * 256 + (part > 0 ? 128 : 0) + (int)rank * wide);
-                for (int k = 0; k < p.k_blocks; ++k) {
+                for (int k = first_block<CUT>(p, item); k < end; ++k) {
                     if (!tc::mbar_wait(done0 + 8 * s, parity, abort_flag, &g_fp8_error, 1)) { ok = false; break; }
                     const uint32_t bar = full_lead + 8 * s, dst = stage0 + s * kStage;
                     if (rank == 0) tc::mbar_arrive_expect_tx(tc::smem_u32(&full[s]), 2 * (kStageA + wide * 128));
@@ -207,8 +222,9 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
             uint32_t s = 0, parity = 0, g = 0;
             bool ok = true, ready = tc::mbar_try_wait(full0, 0);
             for (int item = cluster_id; item < p.n_items && ok; item += n_clusters) {
-                const uint32_t idesc = !HALVES || item < p.whole ? idesc_256 : idesc_128;
-                for (int k = 0; k < p.k_blocks; ++k, ++g) {
+                const uint32_t idesc = CUT == kWhole || (CUT == kHalves && item < p.whole) ? idesc_256 : idesc_128;
+                const int blocks = end_block<CUT>(p, item) - first_block<CUT>(p, item);
+                for (int k = 0; k < blocks; ++k, ++g) {
                     const uint32_t buf = g & 1;
                     if ((!ready && !tc::mbar_wait(full0 + 8 * s, parity, abort_flag, &g_fp8_error, 3)) ||
                         !tc::mbar_wait(acc_empty0 + 8 * buf, ((g >> 1) & 1) ^ 1u, abort_flag, &g_fp8_error, 2)) { ok = false; break; }
@@ -240,7 +256,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
             {
                 int tm, tn;
                 int part = 0;
-                if constexpr (HALF) part = half_at(p, item, tm, tn);
+                if constexpr (HALF) part = half_at<CUT>(p, item, tm, tn);
                 else tile_at(p, item, tm, tn);
                 const long long row = (long long)tm * 256 + (long long)rank * 128 + quarter * 32 + lane;
                 const int wb0 = p.up_row ? tn : HALF ? min(2 * tn + part, p.w_blocks - 1) : 2 * tn;
@@ -248,6 +264,10 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                 at_x = (uint32_t)((row < p.rows ? row : p.rows - 1) * p.ld_xs);
                 at_w0 = (uint32_t)(wb0 * p.ld_ws);
                 at_w1 = (uint32_t)(min(wb1, p.w_blocks - 1) * p.ld_ws);
+                if constexpr (CUT == kParts) {
+                    const uint32_t first = (uint32_t)first_block<CUT>(p, item);
+                    at_x += first; at_w0 += first; at_w1 += first;
+                }
             }
             uint64_t sum[2 * kPer][16];                           // columns 32 j + 2 i, + 1
 #pragma unroll
@@ -255,7 +275,7 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum[j][i] = 0ull;
             float sx = __ldg(p.xs + at_x), s0 = __ldg(p.ws + at_w0), s1 = __ldg(p.ws + at_w1);
-            for (int k = p.k_blocks; k > 0; --k, ++g) {
+            for (int k = end_block<CUT>(p, item) - first_block<CUT>(p, item); k > 0; --k, ++g) {
                 const uint32_t buf = g & 1, taddr = taddr0 + buf * 256 - (HALF ? side * 32 : 0);
                 const float f0 = sx * s0, f1 = sx * s1;
                 if (k > 1) { sx = __ldg(p.xs + ++at_x); s0 = __ldg(p.ws + ++at_w0); s1 = __ldg(p.ws + ++at_w1); }
@@ -285,8 +305,10 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
             }
             int tm, tn;
             int part = 0;
-            if constexpr (HALF) part = half_at(p, item, tm, tn);
+            if constexpr (HALF) part = half_at<CUT>(p, item, tm, tn);
             else tile_at(p, item, tm, tn);
+            void *out = p.out;
+            if constexpr (CUT == kParts) out = reinterpret_cast<float *>(p.out) + item % p.parts * p.part_step;
             const long long row0 = (long long)tm * 256 + (long long)rank * 128 + quarter * 32;
 #pragma unroll
             for (int j = 0; j < 2 * kPer; ++j) {
@@ -301,14 +323,15 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
                 int col;
                 if constexpr (HALF) col = p.up_row ? tn * 128 + part * 64 + side * 32 : tn * 256 + part * 128 + j * 64 + side * 32;
                 else col = p.up_row ? tn * 128 + side * 64 + j * 32 : tn * 256 + (j >> 1) * 128 + side * 64 + (j & 1) * 32;
-                store_32x32<TURNED>(p, row0, col, v, turns + (warp - 4) * kTurn);
+                store_32x32<TURNED>(p, out, row0, col, v, turns + (warp - 4) * kTurn);
             }
             return true;
         };
         int item = cluster_id;
         bool ok = true;
-        for (; ok && item < p.whole; item += n_clusters) ok = finish(item, std::false_type());
-        if constexpr (HALVES) {                                   // one round at most
+        if constexpr (CUT != kParts)
+            for (; ok && item < p.whole; item += n_clusters) ok = finish(item, std::false_type());
+        if constexpr (CUT != kWhole) {                            // one round at most
             if (ok && item < p.n_items) finish(item, std::true_type());
         }
     }
@@ -320,6 +343,36 @@ fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
     tc::cluster_sync();
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// out = the parts of a reduction, fp32 [parts][rows][ld], added in order; four columns a thread.  They are read past L1:
+// the kernel may start before the one that writes them has ended.
+__global__ void __launch_bounds__(256)
+fp8_join_kernel(const float *partial, int parts, long long part_step, long long ld, long long rows, int n, void *out,
+                long long ld_out, int out_dtype) {
+    tc::after_previous();
+    const long long quads = ld / 4, at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= rows * quads) return;
+    const long long row = at / quads;
+    const int col = (int)(at - row * quads) * 4;
+    const float *src = partial + row * ld + col;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < parts; i0 += 4) {
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __ldcg(reinterpret_cast<const float4 *>(src + min(i0 + i, parts - 1) * part_step));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i0 + i < parts) { s.x += v[i].x; s.y += v[i].y; s.z += v[i].z; s.w += v[i].w; }
+    }
+    const float r[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (col + i >= n) continue;
+        const long long idx = row * ld_out + col + i;
+        if (out_dtype == MORTAR_F32) reinterpret_cast<float *>(out)[idx] = r[i];
+        else reinterpret_cast<uint16_t *>(out)[idx] = (uint16_t)tc::pack16(r[i], 0.f, out_dtype == MORTAR_F16);
+    }
 }
 
 // ---- up to 32 rows: the operands change places -------------------------------------------------
@@ -507,13 +560,13 @@ bool misaligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p)
 
 std::mutex g_fp8_mutex;
 
-template <bool TURNED, bool HALVES>
+template <bool TURNED, int CUT>
 int launch(const Fp8Params &p, int sms, cudaStream_t st) {
     static bool ready[64] = {false};
-    const int rc = tc::allow_smem(fp8_pair_kernel<TURNED, HALVES>, kSmem, ready, g_fp8_mutex, nullptr);
+    const int rc = tc::allow_smem(fp8_pair_kernel<TURNED, CUT>, kSmem, ready, g_fp8_mutex, nullptr);
     if (rc != MORTAR_OK) return rc;
     const int clusters = p.n_items < sms / 2 ? p.n_items : sms / 2;
-    fp8_pair_kernel<TURNED, HALVES><<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
+    fp8_pair_kernel<TURNED, CUT><<<(unsigned)(2 * clusters), kThreads, kSmem, st>>>(p);
     MORTAR_CUDA_CHECK(cudaGetLastError());
     return MORTAR_OK;
 }
@@ -536,12 +589,41 @@ int launch_few(Fp8Params &p, const void *x, int64_t ldx, const void *w, int64_t 
     return MORTAR_OK;
 }
 
+// Parts that the reduction of a product without the gate is cut into: where the half tiles fill no more than half of the
+// machine and enough blocks are saved to pay for the join (3 to 4 us; a block of a half tile takes 0.3).  64 x 5632 -> 2048
+// 25.2 -> 15 us, 333 x 5632 -> 2048 26.7 -> 22, 64 x 2048 -> 768 13.4 -> 10.4, 333 x 2048 -> 768 (13 blocks saved) the
+// same 14.5.
+constexpr int64_t kLeastSaved = 12, kClusters = 74;              // blocks; CTA pairs that run at once
+int64_t parts_of(int64_t rows, int64_t out_features, int64_t k_blocks, bool gated) {
+    if (gated || rows <= small::kMaxRows) return 1;
+    const int64_t halves = 2 * ((rows + 255) / 256) * ((out_features + 255) / 256), most = std::min(kClusters / halves, k_blocks);
+    if (most < 2) return 1;
+    const int64_t longest = (k_blocks + most - 1) / most;
+    return k_blocks - longest >= kLeastSaved ? (k_blocks + longest - 1) / longest : 1;
+}
+int64_t padded(int64_t n) { return (n + 31) / 32 * 32; }
+
 }  // namespace
+
+extern "C" int64_t mortar_linear_fp8_scratch_floats(int64_t rows, int32_t out_features, int32_t in_features, int32_t flags) {
+    if (rows < 0 || out_features <= 0 || in_features <= 0 || in_features % 16) return MORTAR_ERR_SHAPE;
+    if (flags & ~MORTAR_FLAG_SWIGLU) return MORTAR_ERR_DTYPE;
+    const int64_t parts = parts_of(rows, out_features, ((int64_t)in_features + 127) / 128, (flags & MORTAR_FLAG_SWIGLU) != 0);
+    return parts > 1 ? parts * rows * padded(out_features) : 0;
+}
 
 extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, const float *x_scale, int64_t ld_x_scale,
                                  int64_t rows, const void *w, int32_t w_type, int64_t ldw, const float *w_scale,
                                  int64_t ld_w_scale, int32_t out_features, int32_t in_features, int32_t flags, void *out,
                                  int32_t out_dtype, int64_t ld_out, void *stream) {
+    return mortar_linear_fp8_cut(x, x_type, ldx, x_scale, ld_x_scale, rows, w, w_type, ldw, w_scale, ld_w_scale, out_features,
+                                 in_features, flags, out, out_dtype, ld_out, nullptr, 0, stream);
+}
+
+extern "C" int mortar_linear_fp8_cut(const void *x, int32_t x_type, int64_t ldx, const float *x_scale, int64_t ld_x_scale,
+                                     int64_t rows, const void *w, int32_t w_type, int64_t ldw, const float *w_scale,
+                                     int64_t ld_w_scale, int32_t out_features, int32_t in_features, int32_t flags, void *out,
+                                     int32_t out_dtype, int64_t ld_out, float *scratch, int64_t scratch_floats, void *stream) {
     if (!x || !x_scale || !w || !w_scale || !out) return MORTAR_ERR_NULL;
     const bool gated = (flags & MORTAR_FLAG_SWIGLU) != 0;
     const int64_t k_blocks = ((int64_t)in_features + 127) / 128;
@@ -554,7 +636,7 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
         return MORTAR_ERR_DTYPE;
     const size_t e = out_dtype == MORTAR_F32 ? 4 : 2;
     if (misaligned(x, 16) || misaligned(w, 16) || ldx % 16 || ldw % 16 || misaligned(out, e) || misaligned(x_scale, 4) ||
-        misaligned(w_scale, 4))
+        misaligned(w_scale, 4) || misaligned(scratch, 32))
         return MORTAR_ERR_ALIGN;
     if (rows > 0x7fffff00LL || out_features > 0x7fffff00 || rows * ld_x_scale > 0xffffffffLL ||
         ((int64_t)out_features + 127) / 128 * ld_w_scale > 0xffffffffLL)
@@ -605,16 +687,32 @@ extern "C" int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, con
     // The tiles of a round that is at most half full are cut in two.  Behind no, one, two and four full rounds that takes
     // 12.4 -> 10.4, 20.6 -> 18.6, 38.8 -> 37.2 and 60.8 -> 59.8 us; behind six it changes nothing, and behind more the
     // kernel that can do both is the slower one (nineteen: 216.6 -> 220.7).
+    p.parts = 1;
     p.whole = 2 * rest <= clusters && tiles < 5 * clusters ? tiles - rest : tiles;
     p.n_items = 2 * tiles - p.whole;
     if (p.whole < tiles) {
         rc = tc::encode_u8_2d(&p.map_w_half, w, in_features, out_features, ldw, 64);
         if (rc != MORTAR_OK) return rc;
     }
+    const int64_t parts = scratch ? parts_of(rows, out_features, k_blocks, gated) : 1;
+    if (parts > 1) {
+        const int64_t ld = padded(out_features);
+        if (scratch_floats < parts * rows * ld) return MORTAR_ERR_CAPACITY;
+        const int64_t blocks = (rows * (ld / 4) + 255) / 256;
+        if (blocks > 0x7fffffffLL) return MORTAR_ERR_CAPACITY;
+        p.parts = (int)parts;
+        p.part_step = rows * ld;
+        p.n_items = 2 * tiles * p.parts;
+        p.out = scratch; p.ld_out = ld; p.out_dtype = MORTAR_F32;
+        rc = launch<false, kParts>(p, sms, st);
+        if (rc != MORTAR_OK) return rc;
+        return tc::launch_after(fp8_join_kernel, (unsigned)blocks, 256u, 0, st, (const float *)scratch, (int)parts, (long long)p.part_step,
+                                (long long)ld, (long long)rows, (int)out_features, out, (long long)ld_out, (int)out_dtype);
+    }
     const bool turned = misaligned(out, 32) || (ld_out * e) % 32 || p.n % 32;
 
-    if (p.whole < tiles) return turned ? launch<true, true>(p, sms, st) : launch<false, true>(p, sms, st);
-    return turned ? launch<true, false>(p, sms, st) : launch<false, false>(p, sms, st);
+    if (p.whole < tiles) return turned ? launch<true, kHalves>(p, sms, st) : launch<false, kHalves>(p, sms, st);
+    return turned ? launch<true, kWhole>(p, sms, st) : launch<false, kWhole>(p, sms, st);
 }
 
 extern "C" int mortar_linear_fp8_error(int32_t *code, int32_t reset) {

@@ -437,10 +437,15 @@ Tensor linear_fp8(const Tensor &x, const OptTensor &x_scale, const Tensor &data,
     } else {
         std::tie(r, s) = quantize_fp8(r, 1, at::kFloat8_e4m3fn);
     }
-    check(mortar_linear_fp8(in(r), code_of(r.scalar_type()), ld(r), in_f32(s), ld(s), rows, in(data),
-                            code_of(data.scalar_type()), ld(data), in_f32(scale), ld(scale), (int32_t)n, (int32_t)k,
-                            swiglu ? MORTAR_FLAG_SWIGLU : 0, out(y), y_code, n_out, on.stream), "mortar_linear_fp8");
-    count(kLinearFp8, 1);
+    const int32_t flags = swiglu ? MORTAR_FLAG_SWIGLU : 0;
+    const int64_t scratch_floats = mortar_linear_fp8_scratch_floats(rows, (int32_t)n, (int32_t)k, flags);
+    check(scratch_floats, "mortar_linear_fp8_scratch_floats");
+    Tensor scratch;
+    if (scratch_floats) scratch = floats({scratch_floats}, x);
+    check(mortar_linear_fp8_cut(in(r), code_of(r.scalar_type()), ld(r), in_f32(s), ld(s), rows, in(data),
+                                code_of(data.scalar_type()), ld(data), in_f32(scale), ld(scale), (int32_t)n, (int32_t)k, flags,
+                                out(y), y_code, n_out, out_f32(scratch), scratch_floats, on.stream), "mortar_linear_fp8");
+    count(kLinearFp8, scratch_floats ? 2 : 1);
     return y;
 }
 

@@ -209,3 +209,16 @@ def test_modules_hold_their_parameters():
         mb.SwiGLUFp8(q(192, 64), q(64, 96))                          # 96 hidden columns: no multiple of 128
     with pytest.raises(ValueError):
         mb.SwiGLUFp8(q(256, 64), q(128, 128))
+
+
+def test_linear_fp8_scratch():
+    n = L.mortar_linear_fp8_scratch_floats
+    assert n(64, 2048, 5632, 0) > 0 and n(64, 2048, 5632, 1) == 0
+    assert n(4, 2048, 5632, 0) == 0 and n(8192, 2048, 5632, 0) == 0 and n(64, 2048, 256, 0) == 0 and n(0, 2048, 5632, 0) == 0
+    assert n(64, 2048, 5630, 0) == SHAPE and n(64, 0, 5632, 0) == SHAPE and n(-1, 64, 64, 0) == SHAPE and n(64, 64, 64, 2) == DTYPE
+    keep, p = _buf()
+    ok = [p, E4M3, 5632, p, 44, 64, p, E4M3, 5632, p, 44, 2048, 5632, 0, p, BF16, 2048]
+    f = L.mortar_linear_fp8_cut
+    assert f(*ok[:5], 0, *ok[6:], None, 0, None) == 0
+    assert f(None, *ok[1:], None, 0, None) == NULL
+    assert f(*ok, _off(p, 16), 1 << 30, None) == ALIGN

@@ -907,3 +907,26 @@ def test_linear_fp8_few_rows_of_narrow_weights(rows, out, cols):
     test_linear_fp8(rows, out, cols, torch.float8_e5m2, torch.float8_e5m2)
     if out == 4096:
         test_linear_fp8_with_the_gate(rows, out // 2, cols, torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("rows,out,cols", [(33, 2048, 5632), (64, 300, 128 * 40 + 16), (128, 515, 4096), (333, 768, 128 * 23), (600, 300, 3200)])
+def test_linear_fp8_cut_reductions(rows, out, cols):
+    """Few tiles and long reductions: the parts are joined in order, the same bits every time (the called test compares
+    two calls), any output type, width and stride."""
+    assert mb._lib.lib().mortar_linear_fp8_scratch_floats(rows, out, cols, 0) > 0
+    test_linear_fp8(rows, out, cols, torch.float8_e4m3fn, torch.float8_e4m3fn)
+    x, xs, w, ws = fp8_operands(rows, out, cols, torch.float8_e5m2, torch.float8_e4m3fn)
+    whole, cut = (torch.full((rows + 2, out + 3), 7.0, device=DEV) for _ in range(2))
+    lib, st = mb._lib.lib(), torch.cuda.current_stream().cuda_stream
+    n = lib.mortar_linear_fp8_scratch_floats(rows, out, cols, 0)
+    scratch = torch.empty(n, device=DEV)
+    args = lambda y: (x.data_ptr(), 4, cols, xs.data_ptr(), xs.shape[1], rows, w.data_ptr(), 3, cols, ws.data_ptr(), ws.shape[1], out, cols, 0,
+                      y.data_ptr(), 0, out + 3)
+    assert lib.mortar_linear_fp8(*args(whole), st) == 0
+    assert lib.mortar_linear_fp8_cut(*args(cut), scratch.data_ptr(), n, st) == 0
+    assert lib.mortar_linear_fp8_cut(*args(cut), scratch.data_ptr(), n - 1, st) == -8
+    ref, mag = fp8_linear_ref(x, xs, w, ws)
+    for y in (whole, cut):
+        within(y[:rows, :out], ref, fp8_bound(ref, mag, cols, torch.float32))
+        assert bool((y[rows:] == 7).all()) and bool((y[:, out:] == 7).all())
+    errors_are_clear()
