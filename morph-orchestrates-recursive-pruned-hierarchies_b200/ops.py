@@ -1069,7 +1069,8 @@ def mlp_fp8(x: torch.Tensor, gate_up: Fp8Matrix, down: Fp8Matrix, *,
             out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """The gated feed-forward block in 8-bit floating point, the form ``mlp_prefill_tc_i8`` has in
     int8: quantise x, gate/up product with the gate applied (hidden block bfloat16, or the type of a
-    16-bit x), quantise the hidden block, down product.  Four launches; for serving."""
+    16-bit x), quantise the hidden block, down product.  Four launches, five where the down
+    product is cut; for serving."""
     if gate_up.out_features != 2 * down.in_features or gate_up.in_features != down.out_features:
         raise ValueError("gate_up must be [2 d_ff, d_model] and down [d_model, d_ff]")
     if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
