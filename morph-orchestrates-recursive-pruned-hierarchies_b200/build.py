@@ -83,7 +83,10 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            "-DTORCH_EXTENSION_NAME=_mortar_native", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *include, BINDING, "-o", NATIVE, f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
-           f"-L{PKG}", "-l:libmortar_b200.so", "-Wl,-rpath,$ORIGIN"]
+           f"-L{PKG}", "-l:libmortar_b200.so", "-Wl,-rpath,$ORIGIN",
+           # the C++ runtime and the unwinder that torch runs on, whatever the compiler links by default: with copies of its own
+           # (a compiler that has only the static ones) the binding's exceptions end the process
+           "-nostdlib++", "-l:libstdc++.so.6", "-shared-libgcc", "-l:libgcc_s.so.1"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
