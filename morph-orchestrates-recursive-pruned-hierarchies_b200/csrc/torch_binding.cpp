@@ -91,6 +91,9 @@ Tensor rows_of(const Tensor &t, bool aligned) {
 // elements from row to row (a copy of one row may keep a stride that says nothing)
 int64_t ld(const Tensor &rows) { return std::max(rows.stride(0), rows.size(1)); }
 
+// Rows that the kernels may walk at `ld(t)` as they are: none lies over the next.
+bool apart(const Tensor &t) { return t.size(0) < 2 || t.stride(0) >= t.size(1); }
+
 Tensor like(const Tensor &t) { return t.is_contiguous() ? at::empty_like(t) : at::empty(t.sizes(), t.options()); }
 Tensor floats(at::IntArrayRef shape, const Tensor &on) { return at::empty(shape, on.options().dtype(at::kFloat)); }
 const void *in(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
@@ -405,6 +408,8 @@ Tensor linear_fp8(const Tensor &x, const OptTensor &x_scale, const Tensor &data,
     TORCH_CHECK_VALUE(data.stride(1) == 1 && scale.scalar_type() == at::kFloat && scale.dim() == 2 &&
                           scale.size(0) == (n + 127) / 128 && scale.size(1) == nb && scale.stride(1) == 1,
                       "w.scale must be float32 [", (n + 127) / 128, ", ", nb, "], got ", scale.scalar_type(), " ", scale.sizes());
+    TORCH_CHECK_VALUE(apart(data) && apart(scale), "the rows of w.data or w.scale overlap (strides ", data.strides(), " and ",
+                      scale.strides(), "): pass a contiguous copy");
     TORCH_CHECK_VALUE(x.size(-1) == k, "x has last dim ", x.size(-1), ", expected ", k);
     TORCH_CHECK_VALUE(n <= INT32_MAX && k <= INT32_MAX, "a matrix [", n, ", ", k, "] is too large");
     const Tensor given = or_none(x_scale);

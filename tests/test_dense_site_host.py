@@ -222,3 +222,25 @@ def test_linear_fp8_scratch():
     assert f(*ok[:5], 0, *ok[6:], None, 0, None) == 0
     assert f(None, *ok[1:], None, 0, None) == NULL
     assert f(*ok, _off(p, 16), 1 << 30, None) == ALIGN
+
+
+def fake_matrix(data, scale):
+    """A matrix whose parts were put in place one by one (fake tensors have no address for the constructor)."""
+    w = mb.Fp8Matrix.__new__(mb.Fp8Matrix)
+    w.data, w.scale = data, scale
+    w.out_features, w.in_features = data.shape
+    return w
+
+
+def test_parts_of_a_matrix_whose_rows_overlap_are_refused():
+    """Replaced parts whose rows lie over one another (expanded, or a window that moves by less than a row): the kernels
+    walk rows of the full width and would read past the end."""
+    with FakeTensorMode():
+        data, scale = (torch.empty(256, 256, device="cuda", dtype=torch.float8_e4m3fn),
+                       torch.empty(2, 2, device="cuda", dtype=torch.float32))
+        x = torch.empty(4, 256, device="cuda", dtype=torch.float8_e4m3fn)
+        xs = torch.empty(4, 2, device="cuda", dtype=torch.float32)
+        for d, s in ((data[:1].expand(256, 256), scale), (data.as_strided((256, 256), (16, 1)), scale),
+                     (data, scale[:1].expand(2, 2)), (data, scale.as_strided((2, 2), (1, 1)))):
+            with pytest.raises(ValueError, match="overlap"):
+                mb.ops.linear_fp8(x, fake_matrix(d, s), x_scale=xs)
