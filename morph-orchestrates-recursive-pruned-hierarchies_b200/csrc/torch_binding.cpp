@@ -408,6 +408,7 @@ Tensor linear_fp8(const Tensor &x, const OptTensor &x_scale, const Tensor &data,
     TORCH_CHECK_VALUE(data.stride(1) == 1 && scale.scalar_type() == at::kFloat && scale.dim() == 2 &&
                           scale.size(0) == (n + 127) / 128 && scale.size(1) == nb && scale.stride(1) == 1,
                       "w.scale must be float32 [", (n + 127) / 128, ", ", nb, "], got ", scale.scalar_type(), " ", scale.sizes());
+    TORCH_CHECK_VALUE(!data.is_neg() && !scale.is_neg(), "w.data or w.scale is a view of negative values: pass a copy");
     TORCH_CHECK_VALUE(apart(data) && apart(scale), "the rows of w.data or w.scale overlap (strides ", data.strides(), " and ",
                       scale.strides(), "): pass a contiguous copy");
     TORCH_CHECK_VALUE(x.size(-1) == k, "x has last dim ", x.size(-1), ", expected ", k);

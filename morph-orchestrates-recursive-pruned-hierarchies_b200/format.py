@@ -678,7 +678,7 @@ class Fp8Matrix:
             raise ValueError(f"data is on {data.device} but scale on {scale.device}")
         if data.stride(1) != 1 or data.stride(0) % 16 or data.stride(0) < in_features or data.data_ptr() % 16:
             data = data.clone(memory_format=torch.contiguous_format)
-        if not scale.is_contiguous() or scale.stride(0) < want[1]:
+        if scale.stride() != (want[1], 1) or scale.is_neg():                # also where a dimension of 1 hides a stride
             scale = scale.clone(memory_format=torch.contiguous_format)
         self.data, self.scale = data, scale
         self.out_features, self.in_features = int(out_features), int(in_features)

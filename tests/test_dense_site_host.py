@@ -244,3 +244,23 @@ def test_parts_of_a_matrix_whose_rows_overlap_are_refused():
                      (data, scale[:1].expand(2, 2)), (data, scale.as_strided((2, 2), (1, 1)))):
             with pytest.raises(ValueError, match="overlap"):
                 mb.ops.linear_fp8(x, fake_matrix(d, s), x_scale=xs)
+
+
+def test_matrix_lays_its_scales_out():
+    """One column of scales in any stride (a transposed row), and views that stand for the negative of what memory holds."""
+    data = torch.zeros(300, 64, dtype=torch.float8_e4m3fn)
+    row = torch.tensor([[1.0, 2.0, 3.0]])
+    m = mb.Fp8Matrix(data, row.t())
+    assert m.scale.stride() == (1, 1) and torch.equal(m.scale, row.t())
+    one = torch.as_strided(row, (1, 1), (7, 7))
+    assert mb.Fp8Matrix(data[:100], one).scale.stride() == (1, 1)
+    m = mb.Fp8Matrix(data, torch._neg_view(row.t().contiguous()))
+    assert not m.scale.is_neg() and torch.equal(m.scale, -row.t())
+    kept = torch.tensor([[1.0], [2.0], [3.0]])
+    assert mb.Fp8Matrix(data, kept).scale is kept                        # nothing is copied without need
+    with FakeTensorMode():
+        x = torch.empty(4, 64, device="cuda", dtype=torch.float8_e4m3fn)
+        xs = torch.empty(4, 1, device="cuda", dtype=torch.float32)
+        d, s = torch.empty(300, 64, device="cuda", dtype=torch.float8_e4m3fn), torch.empty(3, 1, device="cuda")
+        with pytest.raises(ValueError, match="negative"):
+            mb.ops.linear_fp8(x, fake_matrix(d, torch._neg_view(s)), x_scale=xs)
