@@ -91,6 +91,9 @@ Tensor rows_of(const Tensor &t, bool aligned) {
 // elements from row to row (a copy of one row may keep a stride that says nothing)
 int64_t ld(const Tensor &rows) { return std::max(rows.stride(0), rows.size(1)); }
 
+// memory holds the values themselves, one after the other
+bool plain(const Tensor &t) { return t.is_contiguous() && !t.is_neg(); }
+
 // Rows that the kernels may walk at `ld(t)` as they are: none lies over the next.
 bool apart(const Tensor &t) { return t.size(0) < 2 || t.stride(0) >= t.size(1); }
 
@@ -195,7 +198,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor &dy, const T
     check_columns(x, "weight", weight);
     const int64_t cols = x.size(-1), rows = x.numel() / cols;
     TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat && stats.dim() == 2 && stats.size(0) == 2 && stats.size(1) == rows &&
-                          stats.is_contiguous(), "stats must be contiguous float32 [2, ", rows, "]");
+                          plain(stats), "stats must be contiguous float32 [2, ", rows, "]");
     const Launch on(x);
     Tensor dx, dw, db, scratch;
     if (want_dx) dx = like(x);
@@ -305,9 +308,9 @@ std::tuple<Tensor, Tensor, Tensor> mlp_dense_backward(const Tensor &dy, const Te
     const auto dt = x.scalar_type();
     const int64_t rows = x.numel() / s.d_model;
     TORCH_CHECK_VALUE(hidden.dim() == 2 && hidden.size(0) == rows && hidden.size(1) == s.d_ff && hidden.scalar_type() == dt &&
-                          hidden.is_contiguous(), "hidden must be contiguous ", dt, " [", rows, ", ", s.d_ff, "]");
+                          plain(hidden), "hidden must be contiguous ", dt, " [", rows, ", ", s.d_ff, "]");
     TORCH_CHECK_VALUE(sums.dim() == 2 && sums.size(0) == rows && sums.size(1) == 2 * s.d_ff && sums.scalar_type() == at::kFloat &&
-                          sums.is_contiguous(), "sums must be contiguous float32 [", rows, ", ", 2 * s.d_ff, "]");
+                          plain(sums), "sums must be contiguous float32 [", rows, ", ", 2 * s.d_ff, "]");
     const Launch on(x);
     Tensor dx, dgu, ddn, scratch;
     if (want_dx) dx = like(x);

@@ -264,3 +264,16 @@ def test_matrix_lays_its_scales_out():
         d, s = torch.empty(300, 64, device="cuda", dtype=torch.float8_e4m3fn), torch.empty(3, 1, device="cuda")
         with pytest.raises(ValueError, match="negative"):
             mb.ops.linear_fp8(x, fake_matrix(d, torch._neg_view(s)), x_scale=xs)
+
+
+def test_negated_views_of_what_a_forward_call_kept_are_refused():
+    with FakeTensorMode():
+        def z(*shape, dt=torch.bfloat16):
+            return torch.empty(*shape, device="cuda", dtype=dt)
+        x, gu, dn, hidden, sums = z(4, 64), z(64, 64), z(64, 32), z(4, 32), z(4, 64, dt=torch.float32)
+        neg = torch._neg_view
+        for f in (lambda: mb.ops.layer_norm_backward(x, x, None, neg(z(2, 4, dt=torch.float32))),
+                  lambda: mb.ops.mlp_dense_backward(x, x, gu, dn, neg(hidden), sums),
+                  lambda: mb.ops.mlp_dense_backward(x, x, gu, dn, hidden, neg(sums))):
+            with pytest.raises(ValueError, match="must be contiguous"):
+                f()
