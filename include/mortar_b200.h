@@ -663,8 +663,8 @@ int mortar_dense_error(int32_t *code, int32_t reset);
  * scale per block of block_rows x 128, scale [ceil(rows / block_rows)][ceil(cols / 128)];
  * block_rows is 1 (activations) or 128 (weights).  A block's scale is the smallest power of two that
  * brings it into the type's range, and q the value nearest to x / scale, ties to even; zeros have
- * scale 1, a block with an infinity or a NaN scale NaN.  cols a multiple of 16, pointers and row
- * strides 16-byte aligned. */
+ * scale 1, a block with an infinity or a NaN scale NaN.  cols a multiple of 16 up to 2^30, pointers and
+ * row strides 16-byte aligned. */
 int mortar_quantize_fp8(const void *x, int32_t dtype, int64_t ldx, int64_t rows, int32_t cols,
                         int32_t block_rows, void *q, int32_t q_dtype, int64_t ldq, float *scale,
                         void *stream);
@@ -682,7 +682,7 @@ int mortar_dequantize_fp8(const void *q, int32_t q_dtype, int64_t ldq, const flo
  *   flags      0 or MORTAR_FLAG_SWIGLU: y = silu(first half) * second half of the output columns;
  *              out_features a multiple of 256 then
  *   out        fp32, bf16 or fp16, sums in fp32, rounded once
- * in_features is a multiple of 16.  Bounded in-kernel waits report through mortar_linear_fp8_error. */
+ * in_features is a multiple of 16 up to 2^30.  Bounded in-kernel waits report through mortar_linear_fp8_error. */
 int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, const float *x_scale, int64_t ld_x_scale,
                       int64_t rows, const void *w, int32_t w_type, int64_t ldw, const float *w_scale,
                       int64_t ld_w_scale, int32_t out_features, int32_t in_features, int32_t flags,

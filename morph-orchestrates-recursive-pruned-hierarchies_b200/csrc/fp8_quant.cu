@@ -23,6 +23,7 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int32_t kMaxCols = 1 << 30;                    // columns are counted in 32 bits
 
 // 16 neighbouring values of a row as 32-bit words.  WIDE: the row's pieces of 32 bytes start on 32 bytes and are
 // moved whole (in two halves, lanes that lie 32 bytes apart ask for half a sector at a time).
@@ -257,6 +258,7 @@ int check(const void *x, int64_t ldx, int x_dtype, int64_t rows, int32_t cols, i
     if ((x_dtype != MORTAR_F32 && x_dtype != MORTAR_BF16 && x_dtype != MORTAR_F16) ||
         (q_dtype != MORTAR_E4M3 && q_dtype != MORTAR_E5M2))
         return MORTAR_ERR_DTYPE;
+    if (cols > kMaxCols) return MORTAR_ERR_CAPACITY;
     const size_t e = x_dtype == MORTAR_F32 ? 4 : 2;
     if (misaligned(x, 16) || (ldx * e) % 16 || misaligned(q, 16) || ldq % 16 || misaligned(scale, 4))
         return MORTAR_ERR_ALIGN;

@@ -560,6 +560,8 @@ bool misaligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p)
 
 std::mutex g_fp8_mutex;
 
+constexpr int32_t kMaxIn = 1 << 30;              // bytes of a row are counted in 32 bits
+
 template <bool TURNED, int CUT>
 int launch(const Fp8Params &p, int sms, cudaStream_t st) {
     static bool ready[64] = {false};
@@ -608,6 +610,7 @@ int64_t padded(int64_t n) { return (n + 31) / 32 * 32; }
 extern "C" int64_t mortar_linear_fp8_scratch_floats(int64_t rows, int32_t out_features, int32_t in_features, int32_t flags) {
     if (rows < 0 || out_features <= 0 || in_features <= 0 || in_features % 16) return MORTAR_ERR_SHAPE;
     if (flags & ~MORTAR_FLAG_SWIGLU) return MORTAR_ERR_DTYPE;
+    if (in_features > kMaxIn) return MORTAR_ERR_CAPACITY;
     const int64_t parts = parts_of(rows, out_features, ((int64_t)in_features + 127) / 128, (flags & MORTAR_FLAG_SWIGLU) != 0);
     return parts > 1 ? parts * rows * padded(out_features) : 0;
 }
@@ -638,7 +641,7 @@ extern "C" int mortar_linear_fp8_cut(const void *x, int32_t x_type, int64_t ldx,
     if (misaligned(x, 16) || misaligned(w, 16) || ldx % 16 || ldw % 16 || misaligned(out, e) || misaligned(x_scale, 4) ||
         misaligned(w_scale, 4) || misaligned(scratch, 32))
         return MORTAR_ERR_ALIGN;
-    if (rows > 0x7fffff00LL || out_features > 0x7fffff00 || rows * ld_x_scale > 0xffffffffLL ||
+    if (in_features > kMaxIn || rows > 0x7fffff00LL || out_features > 0x7fffff00 || rows * ld_x_scale > 0xffffffffLL ||
         ((int64_t)out_features + 127) / 128 * ld_w_scale > 0xffffffffLL)
         return MORTAR_ERR_CAPACITY;
     if (rows == 0) return MORTAR_OK;

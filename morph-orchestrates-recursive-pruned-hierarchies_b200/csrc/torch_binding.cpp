@@ -366,7 +366,7 @@ std::tuple<Tensor, Tensor> quantize_fp8(const Tensor &x, int64_t block_rows, at:
     TORCH_CHECK_VALUE(is_fp8(q_code), "dtype must be float8_e4m3fn or float8_e5m2, got ", dtype);
     TORCH_CHECK_VALUE(block_rows == 1 || block_rows == 128, "block_rows must be 1 or 128, got ", block_rows);
     const int64_t rows = x.size(0), cols = x.size(1);
-    TORCH_CHECK_VALUE(cols >= 1 && cols % 16 == 0 && cols <= INT32_MAX, "cols must be a positive multiple of 16, got ", cols);
+    TORCH_CHECK_VALUE(cols >= 1 && cols % 16 == 0 && cols <= (1 << 30), "cols must be a positive multiple of 16 up to 2^30, got ", cols);
     const Launch on(x);
     const Tensor r = rows_of(x, true), q = at::empty({rows, cols}, x.options().dtype(dtype));
     const Tensor scale = floats({(rows + block_rows - 1) / block_rows, (cols + 127) / 128}, x);
@@ -384,7 +384,7 @@ Tensor dequantize_fp8(const Tensor &q, const Tensor &scale, at::ScalarType out_d
                       q.scalar_type(), " ", q.sizes());
     TORCH_CHECK_VALUE(is_float(code), "unsupported out_dtype ", out_dtype);
     const int64_t rows = q.size(0), cols = q.size(1), nb = (cols + 127) / 128, rb = (rows + 127) / 128;
-    TORCH_CHECK_VALUE(cols >= 1 && cols % 16 == 0 && cols <= INT32_MAX, "cols must be a positive multiple of 16, got ", cols);
+    TORCH_CHECK_VALUE(cols >= 1 && cols % 16 == 0 && cols <= (1 << 30), "cols must be a positive multiple of 16 up to 2^30, got ", cols);
     TORCH_CHECK_VALUE(scale.scalar_type() == at::kFloat && scale.dim() == 2 && scale.size(1) == nb &&
                           (scale.size(0) == rows || scale.size(0) == rb), "scale must be float32 [", rows, ", ", nb, "] or [",
                       rb, ", ", nb, "], got ", scale.scalar_type(), " ", scale.sizes());

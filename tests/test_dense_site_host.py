@@ -277,3 +277,25 @@ def test_negated_views_of_what_a_forward_call_kept_are_refused():
                   lambda: mb.ops.mlp_dense_backward(x, x, gu, dn, hidden, neg(sums))):
             with pytest.raises(ValueError, match="must be contiguous"):
                 f()
+
+
+def test_fp8_widths_end_at_2_to_the_30():
+    """Wider rows would leave 32 bits where blocks and bytes of a row are counted."""
+    keep, p = _buf()
+    over = (1 << 30) + 16
+    for wide in (over, (1 << 31) - 16):
+        for block_rows in (1, 128):
+            assert L.mortar_quantize_fp8(p, BF16, wide, 1, wide, block_rows, p, E4M3, wide, p, None) == CAP
+            assert L.mortar_dequantize_fp8(p, E4M3, wide, p, 1, wide, block_rows, p, BF16, wide, None) == CAP
+        for rows in (1, 20, 200):
+            args = [p, E4M3, wide, p, wide // 128 + 1, rows, p, E4M3, wide, p, wide // 128 + 1, 64, wide, 0, p, BF16, 64]
+            assert L.mortar_linear_fp8(*args, None) == CAP
+            assert L.mortar_linear_fp8_cut(*args, p, 1 << 40, None) == CAP
+            assert L.mortar_linear_fp8_scratch_floats(rows, 64, wide, 0) == CAP
+    assert L.mortar_quantize_fp8(p, BF16, 1 << 30, 0, 1 << 30, 1, p, E4M3, 1 << 30, p, None) == 0
+    assert L.mortar_linear_fp8_scratch_floats(4, 64, 1 << 30, 0) == 0
+    with FakeTensorMode():
+        x = torch.empty(1, over, device="cuda", dtype=torch.bfloat16)
+        for f in (lambda: mb.ops.quantize_fp8(x), lambda: mb.ops.dequantize_fp8(x.to(torch.float8_e4m3fn), x.new_empty(1, (over + 127) // 128, dtype=torch.float32))):
+            with pytest.raises(ValueError, match="cols"):
+                f()
