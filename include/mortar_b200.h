@@ -696,6 +696,8 @@ int mortar_linear_fp8_cut(const void *x, int32_t x_type, int64_t ldx, const floa
                           void *out, int32_t out_dtype, int64_t ld_out, float *scratch, int64_t scratch_floats,
                           void *stream);
 int64_t mortar_linear_fp8_scratch_floats(int64_t rows, int32_t out_features, int32_t in_features, int32_t flags);
+/* The parts that it cuts the reduction into on a device of `sms` SMs (1 = it is not cut). */
+int64_t mortar_linear_fp8_parts(int64_t rows, int32_t out_features, int32_t in_features, int32_t flags, int32_t sms);
 int mortar_linear_fp8_error(int32_t *code, int32_t reset);
 
 #ifdef __cplusplus

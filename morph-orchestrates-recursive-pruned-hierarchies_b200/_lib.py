@@ -141,6 +141,7 @@ _SIGNATURES = {
     "mortar_linear_fp8_cut": (C.c_int, [_vp, _i32, _i64, _vp, _i64, _i64, _vp, _i32, _i64, _vp, _i64, _i32, _i32, _i32,
                                     _vp, _i32, _i64, _vp, _i64, _vp]),
     "mortar_linear_fp8_scratch_floats": (_i64, [_i64, _i32, _i32, _i32]),
+    "mortar_linear_fp8_parts": (_i64, [_i64, _i32, _i32, _i32, _i32]),
     "mortar_linear_fp8_error": (C.c_int, [_vp, _i32]),
 }
 

@@ -595,10 +595,13 @@ int launch_few(Fp8Params &p, const void *x, int64_t ldx, const void *w, int64_t 
 // machine and enough blocks are saved to pay for the join (3 to 4 us; a block of a half tile takes 0.3).  64 x 5632 -> 2048
 // 25.2 -> 15 us, 333 x 5632 -> 2048 26.7 -> 22, 64 x 2048 -> 768 13.4 -> 10.4, 333 x 2048 -> 768 (13 blocks saved) the
 // same 14.5.
-constexpr int64_t kLeastSaved = 12, kClusters = 74;              // blocks; CTA pairs that run at once
-int64_t parts_of(int64_t rows, int64_t out_features, int64_t k_blocks, bool gated) {
+// The kernel gives a cluster one part at most, so the clusters are those of the device that it runs on; scratch is asked
+// for as if there were kMostClusters (fewer clusters never take more parts).
+constexpr int64_t kLeastSaved = 12, kMostClusters = 74;          // blocks; CTA pairs that run at once
+int64_t parts_of(int64_t rows, int64_t out_features, int64_t k_blocks, bool gated, int64_t clusters) {
     if (gated || rows <= small::kMaxRows) return 1;
-    const int64_t halves = 2 * ((rows + 255) / 256) * ((out_features + 255) / 256), most = std::min(kClusters / halves, k_blocks);
+    const int64_t halves = 2 * ((rows + 255) / 256) * ((out_features + 255) / 256);
+    const int64_t most = std::min(std::min(clusters, kMostClusters) / halves, k_blocks);
     if (most < 2) return 1;
     const int64_t longest = (k_blocks + most - 1) / most;
     return k_blocks - longest >= kLeastSaved ? (k_blocks + longest - 1) / longest : 1;
@@ -607,11 +610,16 @@ int64_t padded(int64_t n) { return (n + 31) / 32 * 32; }
 
 }  // namespace
 
-extern "C" int64_t mortar_linear_fp8_scratch_floats(int64_t rows, int32_t out_features, int32_t in_features, int32_t flags) {
-    if (rows < 0 || out_features <= 0 || in_features <= 0 || in_features % 16) return MORTAR_ERR_SHAPE;
+extern "C" int64_t mortar_linear_fp8_parts(int64_t rows, int32_t out_features, int32_t in_features, int32_t flags, int32_t sms) {
+    if (rows < 0 || out_features <= 0 || in_features <= 0 || in_features % 16 || sms < 2) return MORTAR_ERR_SHAPE;
     if (flags & ~MORTAR_FLAG_SWIGLU) return MORTAR_ERR_DTYPE;
     if (in_features > kMaxIn) return MORTAR_ERR_CAPACITY;
-    const int64_t parts = parts_of(rows, out_features, ((int64_t)in_features + 127) / 128, (flags & MORTAR_FLAG_SWIGLU) != 0);
+    return parts_of(rows, out_features, ((int64_t)in_features + 127) / 128, (flags & MORTAR_FLAG_SWIGLU) != 0, sms / 2);
+}
+
+extern "C" int64_t mortar_linear_fp8_scratch_floats(int64_t rows, int32_t out_features, int32_t in_features, int32_t flags) {
+    const int64_t parts = mortar_linear_fp8_parts(rows, out_features, in_features, flags, 2 * kMostClusters);
+    if (parts < 0) return parts;
     return parts > 1 ? parts * rows * padded(out_features) : 0;
 }
 
@@ -693,11 +701,11 @@ extern "C" int mortar_linear_fp8_cut(const void *x, int32_t x_type, int64_t ldx,
     p.parts = 1;
     p.whole = 2 * rest <= clusters && tiles < 5 * clusters ? tiles - rest : tiles;
     p.n_items = 2 * tiles - p.whole;
-    if (p.whole < tiles) {
+    const int64_t parts = scratch ? parts_of(rows, out_features, k_blocks, gated, clusters) : 1;
+    if (p.whole < tiles || parts > 1) {
         rc = tc::encode_u8_2d(&p.map_w_half, w, in_features, out_features, ldw, 64);
         if (rc != MORTAR_OK) return rc;
     }
-    const int64_t parts = scratch ? parts_of(rows, out_features, k_blocks, gated) : 1;
     if (parts > 1) {
         const int64_t ld = padded(out_features);
         if (scratch_floats < parts * rows * ld) return MORTAR_ERR_CAPACITY;

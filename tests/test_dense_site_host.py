@@ -211,6 +211,29 @@ def test_modules_hold_their_parameters():
         mb.SwiGLUFp8(q(256, 64), q(128, 128))
 
 
+def test_linear_fp8_parts_run_at_once_on_any_device():
+    """The kernel that cuts a reduction gives a cluster of two SMs one part of one half tile at most, whatever the number of
+    SMs, and the parts fit the scratch that was asked for."""
+    n = L.mortar_linear_fp8_parts
+    cut = 0
+    for rows in (33, 64, 333, 512, 1000, 4000):
+        for out in (64, 768, 2048, 2304, 4096):
+            for k in (128, 2048, 5632, 16384):
+                halves = 2 * -(-rows // 256) * -(-out // 256)
+                assert n(rows, out, k, 1, 148) == 1 or out % 256
+                for sms in (2, 16, 40, 70, 108, 132, 146, 148, 160):
+                    parts = n(rows, out, k, 0, sms)
+                    assert 1 <= parts <= -(-k // 128) and (parts == 1 or halves * parts <= sms // 2)
+                    need = parts * rows * (-(-out // 32) * 32) if parts > 1 else 0
+                    assert need <= L.mortar_linear_fp8_scratch_floats(rows, out, k, 0)
+                    cut += parts > 1
+                parts = n(rows, out, k, 0, 148)
+                assert L.mortar_linear_fp8_scratch_floats(rows, out, k, 0) == (parts * rows * (-(-out // 32) * 32) if parts > 1 else 0)
+    assert cut > 100
+    assert n(64, 2048, 5632, 0, 148) == 4 and n(512, 2304, 5632, 0, 148) == 2 and n(512, 2304, 5632, 0, 132) == 1
+    assert n(64, 2048, 5632, 0, 0) == SHAPE and n(-1, 64, 64, 0, 148) == SHAPE
+
+
 def test_linear_fp8_scratch():
     n = L.mortar_linear_fp8_scratch_floats
     assert n(64, 2048, 5632, 0) > 0 and n(64, 2048, 5632, 1) == 0
