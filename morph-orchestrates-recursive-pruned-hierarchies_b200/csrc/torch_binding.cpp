@@ -74,6 +74,14 @@ bool wants_grad(std::initializer_list<const Tensor *> ts) {
     return false;
 }
 
+// No operator here has a forward-mode derivative.  A tangent is no gradient that is required (and stays on where none are
+// recorded), so it is asked for by itself: without this the kernels would drop it in silence.
+void refuse_tangents(const char *name, std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        TORCH_CHECK_VALUE(!t->defined() || !t->unsafeGetTensorImpl()->_fw_grad(0, *t).defined(), name,
+                          " has no forward-mode derivative: give it the primal of a dual tensor");
+}
+
 // ---- layouts ----------------------------------------------------------------------------------
 
 // [..., cols] -> [rows, cols]
@@ -165,6 +173,7 @@ void check_columns(const Tensor &x, const char *name, const Tensor &t) {
 std::tuple<Tensor, Tensor> layer_norm_forward(const Tensor &x, const Tensor &weight, const Tensor &bias, double eps,
                                               bool want_stats) {
     need_cuda(x, "x");
+    refuse_tangents("layer_norm", {&x, &weight, &bias});
     const int code = code_of(x.scalar_type());
     TORCH_CHECK_VALUE(is_float(code) && x.dim() >= 1, "x must be a float32, bfloat16 or float16 tensor [..., cols], got ",
                       x.scalar_type());
@@ -190,6 +199,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor &dy, const T
                                                        const Tensor &stats, bool want_dx, bool want_dweight,
                                                        bool want_dbias) {
     need_cuda(x, "x");
+    refuse_tangents("layer_norm_backward", {&dy, &x, &weight});
     const int code = code_of(x.scalar_type());
     TORCH_CHECK_VALUE(is_float(code) && x.dim() >= 1 && x.size(-1) >= 1 && dy.sizes() == x.sizes(), "dy has shape ",
                       dy.sizes(), ", x ", x.sizes(), " (", x.scalar_type(), ")");
@@ -247,6 +257,7 @@ Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bia
     const Tensor w = or_none(weight), b = or_none(bias);
     if (wants_grad({&x, &w, &b})) {
         need_cuda(x, "x");
+        refuse_tangents("layer_norm", {&x, &w, &b});        // inside `apply` forward mode is off
         refuse_capture("layer_norm", {&x, &w, &b});
         return LayerNorm::apply(x, weight, bias, eps);
     }
@@ -280,6 +291,7 @@ MlpShape check_mlp(const Tensor &x, const Tensor &gate_up, const Tensor &down) {
 std::tuple<Tensor, Tensor, Tensor> mlp_dense_forward(const Tensor &x, const Tensor &gate_up, const Tensor &down,
                                                      bool want_saved) {
     const MlpShape s = check_mlp(x, gate_up, down);
+    refuse_tangents("mlp_dense", {&x, &gate_up, &down});
     const Launch on(x);
     const Tensor r = rows_of(x, true), gu = rows_of(gate_up, true), dn = rows_of(down, true);
     const int64_t rows = r.size(0);
@@ -301,6 +313,7 @@ std::tuple<Tensor, Tensor, Tensor> mlp_dense_backward(const Tensor &dy, const Te
                                                       const Tensor &down, const Tensor &hidden, const Tensor &sums,
                                                       bool want_dx, bool want_dgate_up, bool want_ddown) {
     const MlpShape s = check_mlp(x, gate_up, down);
+    refuse_tangents("mlp_dense_backward", {&dy, &x, &gate_up, &down});
     TORCH_CHECK_VALUE(dy.sizes() == x.sizes(), "dy has shape ", dy.sizes(), ", x ", x.sizes());
     same_device(x, "dy", dy);
     same_device(x, "hidden", hidden);
@@ -350,6 +363,7 @@ struct MlpDense : torch::autograd::Function<MlpDense> {
 Tensor mlp_dense(const Tensor &x, const Tensor &gate_up, const Tensor &down) {
     if (wants_grad({&x, &gate_up, &down})) {
         need_cuda(x, "x");
+        refuse_tangents("mlp_dense", {&x, &gate_up, &down});
         refuse_capture("mlp_dense", {&x, &gate_up, &down});
         return MlpDense::apply(x, gate_up, down);
     }
@@ -360,6 +374,7 @@ Tensor mlp_dense(const Tensor &x, const Tensor &gate_up, const Tensor &down) {
 
 std::tuple<Tensor, Tensor> quantize_fp8(const Tensor &x, int64_t block_rows, at::ScalarType dtype) {
     need_cuda(x, "x");
+    refuse_tangents("quantize_fp8", {&x});
     const int code = code_of(x.scalar_type()), q_code = code_of(dtype);
     TORCH_CHECK_VALUE(x.dim() == 2 && is_float(code), "quantize_fp8 takes a 2-D float32, bfloat16 or float16 tensor, got ",
                       x.scalar_type(), " ", x.sizes());
@@ -379,6 +394,7 @@ std::tuple<Tensor, Tensor> quantize_fp8(const Tensor &x, int64_t block_rows, at:
 
 Tensor dequantize_fp8(const Tensor &q, const Tensor &scale, at::ScalarType out_dtype) {
     need_cuda(q, "q");
+    refuse_tangents("dequantize_fp8", {&q, &scale});
     const int q_code = code_of(q.scalar_type()), code = code_of(out_dtype);
     TORCH_CHECK_VALUE(q.dim() == 2 && is_fp8(q_code), "q must be a 2-D float8_e4m3fn or float8_e5m2 tensor, got ",
                       q.scalar_type(), " ", q.sizes());
@@ -417,6 +433,7 @@ Tensor linear_fp8(const Tensor &x, const OptTensor &x_scale, const Tensor &data,
     TORCH_CHECK_VALUE(x.size(-1) == k, "x has last dim ", x.size(-1), ", expected ", k);
     TORCH_CHECK_VALUE(n <= INT32_MAX && k <= INT32_MAX, "a matrix [", n, ", ", k, "] is too large");
     const Tensor given = or_none(x_scale);
+    refuse_tangents("linear_fp8", {&x, &given, &data, &scale});
     TORCH_CHECK_VALUE(!wants_grad({&x, &given}),
                       "linear_fp8 is not differentiable: detach x or call it under torch.no_grad()");
     TORCH_CHECK_VALUE(!swiglu || n % 256 == 0, "swiglu needs out_features to be a multiple of 256, got ", n);

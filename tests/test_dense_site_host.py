@@ -322,3 +322,44 @@ def test_fp8_widths_end_at_2_to_the_30():
         for f in (lambda: mb.ops.quantize_fp8(x), lambda: mb.ops.dequantize_fp8(x.to(torch.float8_e4m3fn), x.new_empty(1, (over + 127) // 128, dtype=torch.float32))):
             with pytest.raises(ValueError, match="cols"):
                 f()
+
+
+def test_tangents_are_refused():
+    """Forward mode: no operator of the site has such a derivative, and none may drop a tangent in silence, without gradients
+    (forward mode stays on under no_grad) or with them."""
+    import torch.autograd.forward_ad as fwd
+    with FakeTensorMode(), fwd.dual_level():
+        def z(*shape, dt=torch.bfloat16, dual=False, grad=False):
+            t = torch.empty(*shape, device="cuda", dtype=dt).requires_grad_(grad)
+            return fwd.make_dual(t, torch.empty_like(t)) if dual else t
+        f32 = dict(dt=torch.float32)
+        stats, hidden, sums = z(2, 4, **f32), z(4, 32), z(4, 64, **f32)
+        calls = [
+            lambda **d: mb.ops.layer_norm(z(4, 64, **d)),
+            lambda **d: mb.ops.layer_norm(z(4, 64), z(64, **d)),
+            lambda **d: mb.ops.layer_norm(z(4, 64), None, z(64, **d)),
+            lambda **d: mb.ops.layer_norm_forward(z(4, 64, **d), None, None, 1e-5, True),
+            lambda **d: mb.ops.layer_norm_backward(z(4, 64, **d), z(4, 64), None, stats),
+            lambda **d: mb.ops.layer_norm_backward(z(4, 64), z(4, 64), z(64, **d), stats),
+            lambda **d: mb.ops.mlp_dense(z(4, 64, **d), z(64, 64), z(64, 32)),
+            lambda **d: mb.ops.mlp_dense(z(4, 64), z(64, 64, **d), z(64, 32)),
+            lambda **d: mb.ops.mlp_dense(z(4, 64), z(64, 64), z(64, 32, **d)),
+            lambda **d: mb.ops.mlp_dense_forward(z(4, 64, **d), z(64, 64), z(64, 32), False),
+            lambda **d: mb.ops.mlp_dense_backward(z(4, 64, **d), z(4, 64), z(64, 64), z(64, 32), hidden, sums),
+            lambda **d: mb.ops.quantize_fp8(z(4, 64, **d)),
+            lambda **d: mb.ops.dequantize_fp8(z(4, 64, dt=torch.float8_e4m3fn), z(4, 1, **f32, **d)),
+            lambda **d: mb.ops.linear_fp8(z(4, 64, **d), fake_matrix(z(64, 64, dt=torch.float8_e4m3fn), z(1, 1, **f32))),
+            lambda **d: mb.ops.linear_fp8(z(4, 64, dt=torch.float8_e4m3fn), fake_matrix(z(64, 64, dt=torch.float8_e4m3fn), z(1, 1, **f32)),
+                                          x_scale=z(4, 1, **f32, **d)),
+            lambda **d: mb.ops.linear_fp8(z(4, 64), fake_matrix(z(64, 64, dt=torch.float8_e4m3fn), z(1, 1, **f32, **d))),
+            lambda **d: mb.ops.mlp_fp8(z(4, 64, **d), fake_matrix(z(256, 64, dt=torch.float8_e4m3fn), z(2, 1, **f32)),
+                                       fake_matrix(z(64, 128, dt=torch.float8_e4m3fn), z(1, 1, **f32))),
+        ]
+        for i, call in enumerate(calls):
+            for mode in (torch.no_grad, torch.enable_grad):
+                with mode(), pytest.raises(ValueError, match="forward-mode"):
+                    call(dual=True)
+                    pytest.fail(f"call {i} was not refused")
+        for call in (calls[0], calls[6]):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(dual=True, grad=True)
