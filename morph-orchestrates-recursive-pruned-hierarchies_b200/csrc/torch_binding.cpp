@@ -82,6 +82,11 @@ void refuse_tangents(const char *name, std::initializer_list<const Tensor *> ts)
                           " has no forward-mode derivative: give it the primal of a dual tensor");
 }
 
+// The 8-bit operators record no gradient.
+void refuse_gradients(const char *name, std::initializer_list<const Tensor *> ts) {
+    TORCH_CHECK_VALUE(!wants_grad(ts), name, " is not differentiable: detach its inputs or call it under torch.no_grad()");
+}
+
 // ---- layouts ----------------------------------------------------------------------------------
 
 // [..., cols] -> [rows, cols]
@@ -375,6 +380,7 @@ Tensor mlp_dense(const Tensor &x, const Tensor &gate_up, const Tensor &down) {
 std::tuple<Tensor, Tensor> quantize_fp8(const Tensor &x, int64_t block_rows, at::ScalarType dtype) {
     need_cuda(x, "x");
     refuse_tangents("quantize_fp8", {&x});
+    refuse_gradients("quantize_fp8", {&x});
     const int code = code_of(x.scalar_type()), q_code = code_of(dtype);
     TORCH_CHECK_VALUE(x.dim() == 2 && is_float(code), "quantize_fp8 takes a 2-D float32, bfloat16 or float16 tensor, got ",
                       x.scalar_type(), " ", x.sizes());
@@ -395,6 +401,7 @@ std::tuple<Tensor, Tensor> quantize_fp8(const Tensor &x, int64_t block_rows, at:
 Tensor dequantize_fp8(const Tensor &q, const Tensor &scale, at::ScalarType out_dtype) {
     need_cuda(q, "q");
     refuse_tangents("dequantize_fp8", {&q, &scale});
+    refuse_gradients("dequantize_fp8", {&q, &scale});
     const int q_code = code_of(q.scalar_type()), code = code_of(out_dtype);
     TORCH_CHECK_VALUE(q.dim() == 2 && is_fp8(q_code), "q must be a 2-D float8_e4m3fn or float8_e5m2 tensor, got ",
                       q.scalar_type(), " ", q.sizes());
@@ -434,8 +441,7 @@ Tensor linear_fp8(const Tensor &x, const OptTensor &x_scale, const Tensor &data,
     TORCH_CHECK_VALUE(n <= INT32_MAX && k <= INT32_MAX, "a matrix [", n, ", ", k, "] is too large");
     const Tensor given = or_none(x_scale);
     refuse_tangents("linear_fp8", {&x, &given, &data, &scale});
-    TORCH_CHECK_VALUE(!wants_grad({&x, &given}),
-                      "linear_fp8 is not differentiable: detach x or call it under torch.no_grad()");
+    refuse_gradients("linear_fp8", {&x, &given, &data, &scale});
     TORCH_CHECK_VALUE(!swiglu || n % 256 == 0, "swiglu needs out_features to be a multiple of 256, got ", n);
     const at::ScalarType y_type = out_dtype.value_or(is_float(code) ? x.scalar_type() : at::kBFloat16);
     const int y_code = code_of(y_type);

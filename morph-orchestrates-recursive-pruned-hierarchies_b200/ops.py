@@ -1035,7 +1035,8 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1, dtype: torch.dtype = t
     scale is the smallest power of two that brings its block into the type's range, so q is the
     value nearest to x / scale, ties to even, for every input type.  A block of zeros has scale 1;
     one that holds an infinity or a NaN has scale NaN and reads back as NaN.  cols is a multiple
-    of 16."""
+    of 16, up to 2^30.  Like the other 8-bit operators not differentiable: an input that requires a
+    gradient is refused while gradients are enabled."""
     return native.quantize_fp8(x, block_rows, dtype)
 
 
@@ -1060,8 +1061,8 @@ def linear_fp8(x: torch.Tensor, w: Fp8Matrix, *, x_scale: Optional[torch.Tensor]
     [..., ceil(in / 128)] as ``quantize_fp8`` gives, or fp32 / bf16 / fp16 and then quantised to e4m3
     first.  Every block's sum is scaled in fp32 and added in fp32; the result is rounded once to
     ``out_dtype`` (default: the type of x, bfloat16 for 8-bit x).  The 8-bit floating-point
-    counterpart of ``linear_tc_i8``; for serving, not differentiable (inputs that require a
-    gradient are refused while gradients are enabled)."""
+    counterpart of ``linear_tc_i8``; for serving, not differentiable (inputs and scales that require
+    a gradient are refused while gradients are enabled)."""
     return native.linear_fp8(x, x_scale, w.data, w.scale, swiglu, out_dtype)
 
 

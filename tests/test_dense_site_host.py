@@ -363,3 +363,27 @@ def test_tangents_are_refused():
         for call in (calls[0], calls[6]):
             with pytest.raises(ValueError, match="forward-mode"):
                 call(dual=True, grad=True)
+
+
+def test_8_bit_operators_refuse_what_requires_a_gradient():
+    """One rule for all of them: none records a gradient, so none takes an input that asks for one while they are recorded.
+    Under no_grad the call goes on (as far as fake tensors let it: there is no device to launch on)."""
+    with FakeTensorMode():
+        def z(*shape, dt=torch.float32, grad=False):
+            return torch.empty(*shape, device="cuda", dtype=dt).requires_grad_(grad)
+        q8 = torch.float8_e4m3fn
+        calls = [
+            lambda g: mb.ops.quantize_fp8(z(4, 64, grad=g)),
+            lambda g: mb.ops.dequantize_fp8(z(4, 64, dt=q8), z(4, 1, grad=g)),
+            lambda g: mb.ops.linear_fp8(z(4, 64, grad=g), fake_matrix(z(64, 64, dt=q8), z(1, 1))),
+            lambda g: mb.ops.linear_fp8(z(4, 64, dt=q8), fake_matrix(z(64, 64, dt=q8), z(1, 1)), x_scale=z(4, 1, grad=g)),
+            lambda g: mb.ops.linear_fp8(z(4, 64), fake_matrix(z(64, 64, dt=q8), z(1, 1, grad=g))),
+        ]
+        for i, call in enumerate(calls):
+            with pytest.raises(ValueError, match="not differentiable"):
+                call(True)
+                pytest.fail(f"call {i} was not refused")
+            if not torch.cuda.is_available():
+                with torch.no_grad(), pytest.raises(RuntimeError) as e:
+                    call(True)
+                assert "not differentiable" not in str(e.value)
