@@ -930,3 +930,108 @@ def test_linear_fp8_cut_reductions(rows, out, cols):
         within(y[:rows, :out], ref, fp8_bound(ref, mag, cols, torch.float32))
         assert bool((y[rows:] == 7).all()) and bool((y[:, out:] == 7).all())
     errors_are_clear()
+
+
+# ---- many rows, tiles and units for each worker ------------------------------------------------
+
+LN_MANY_ROWS = [(12007, 768), (6001, 1536), (5003, 2048), (1501, 4096), (1703, 5632), (1103, 8192), (14503, 136), (1003, 12000),
+                (1002, 16384), (5003, 1001), (3001, 2047), (1005, 8191), (905, 16383), (20011, 7), (1502, 20011)]
+
+
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("rows,cols", LN_MANY_ROWS)
+def test_layer_norm_many_rows_a_group(rows, cols, dt):
+    """Each group of warps takes three to twenty rows, the last of them not in all groups: the row that is on its way, slots
+    that are filled again, sums that take turns, and column sums that are carried from row to row, for every number of units
+    a thread takes (8 to 32 columns), rows of whole vectors and others, and rows that are read again."""
+    test_layer_norm_and_its_gradients(rows, cols, dt)
+    x, dy = (rand(rows, cols, seed=1, scale=2.0) + 0.5).to(dt), rand(rows, cols, seed=4, dt=dt)
+    w = 1 + rand(cols, seed=2, scale=0.2)
+    _, stats = ops.layer_norm_forward(x, w, None, 1e-5, True)
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, stats)
+    # one gradient without the others has the same bits
+    assert torch.equal(ops.layer_norm_backward(dy, x, w, stats, True, False, False)[0], dx)
+    got = ops.layer_norm_backward(dy, x, w, stats, False, True, True)
+    assert got[0] is None and torch.equal(got[1], dw) and torch.equal(got[2], db)
+
+
+@pytest.mark.parametrize("dt", FLOATS)
+def test_layer_norm_many_rows_of_a_wider_tensor(dt):
+    """The same for rows that start anywhere and end inside a wider tensor, whose other values are NaN."""
+    wide = torch.full((3001, 520), float("nan"), device=DEV, dtype=dt)
+    x, dy, w = rand(3001, 512, seed=1, dt=dt), rand(3001, 512, seed=2, dt=dt), 1 + rand(512, seed=3, scale=0.2)
+    y, stats = ops.layer_norm_forward(x, w, None, 1e-5, True)
+    want = ops.layer_norm_backward(dy, x, w, stats)
+    ry, xh, rstd, _, rdx, tw, tb = ln_ref(x, w, None, 1e-5, dy)
+    by, bdx = ln_bounds(x, w, None, ry, xh, rstd, rdx, dy, dt)
+    for off in (1, 3, 8):
+        v = wide[:, off:off + 512]
+        v.copy_(x)
+        got, st = ops.layer_norm_forward(v, w, None, 1e-5, True)
+        dx, dw, db = ops.layer_norm_backward(dy, v, w, st)
+        within(got, ry, by, f"y at {off}")
+        within(dx, rdx, bdx, f"dx at {off}")
+        # two sums in another order: each off by its bound
+        n = 3001 / 8 + 320
+        assert bool(((dw - want[1]).double().abs() <= 2 * F * (n * tw.abs() + (512 / 16 + 48) * (tw.abs() + dy.double().abs() * rstd * x.double().abs().mean(-1, keepdim=True))).sum(0)).all())
+        assert bool(((db - want[2]).double().abs() <= 2 * F * n * tb.abs().sum(0)).all())
+        wide.fill_(float("nan"))
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("rows,cols,block_rows", [(6007, 2064, 1), (40009, 144, 1), (6007, 2064, 128)])
+def test_quantize_fp8_many_units_a_warp(rows, cols, block_rows, dt, dtype):
+    """More blocks than the grid's warps take at once, written and read back."""
+    test_quantize_fp8_is_exact(rows, cols, block_rows, dt, dtype)
+
+
+@pytest.mark.parametrize("rows,d,f", [(8200, 1040, 2576), (8200, 2064, 528)])
+def test_mlp_dense_many_tiles_a_cluster(rows, d, f):
+    """Four and more tiles a cluster in every launch: both accumulators in turn, more than once."""
+    test_mlp_dense_cut_reductions(rows, d, f)
+
+
+@pytest.mark.parametrize("rows,out,cols", [(5000, 6500, 144), (5000, 6656, 400), (20, 60000, 272), (32, 40960, 400), (5, 30000, 272), (12, 30720, 656)])
+def test_linear_fp8_many_tiles_a_cluster(rows, out, cols):
+    """The same for the 8-bit product: whole tiles alone (seven rounds), few rows on either kind of kernel."""
+    test_linear_fp8(rows, out, cols, torch.float8_e4m3fn, torch.float8_e4m3fn)
+    if out % 256 == 0:
+        test_linear_fp8_with_the_gate(rows, out // 2, cols, torch.float8_e5m2)
+
+
+# ---- derivatives that do not exist -------------------------------------------------------------
+
+def test_no_derivative_vanishes():
+    """Tangents and required gradients where an operator has no rule: refused, not dropped."""
+    import torch.autograd.forward_ad as fwd
+    x, w = rand(5, 64, seed=1), rand(64, 64, seed=2)
+    xb, gu, dn = (rand(5, 64, seed=3, dt=torch.bfloat16), rand(64, 64, seed=4, dt=torch.bfloat16), rand(64, 32, seed=5, dt=torch.bfloat16))
+    m = mb.Fp8Matrix.from_dense(w)
+    q, s = ops.quantize_fp8(x)
+    with fwd.dual_level(), torch.no_grad():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for f in (lambda: ops.layer_norm(dual), lambda: ops.quantize_fp8(dual), lambda: ops.linear_fp8(dual, m),
+                  lambda: ops.mlp_dense(fwd.make_dual(xb, xb), gu, dn), lambda: ops.mlp_fp8(dual, m, m),
+                  lambda: torch.ops.mortar_b200.layer_norm(dual, None, None, 1e-5),
+                  lambda: torch.ops.mortar_b200.mlp_dense(fwd.make_dual(xb, xb), gu, dn)):
+            with pytest.raises(ValueError):
+                f()
+        primal, _ = fwd.unpack_dual(dual)
+        assert torch.equal(ops.layer_norm(primal), ops.layer_norm(x))
+    leaf = x.clone().requires_grad_()
+    for f in (lambda: ops.quantize_fp8(leaf), lambda: ops.dequantize_fp8(q, s.clone().requires_grad_()), lambda: ops.linear_fp8(leaf, m),
+              lambda: ops.linear_fp8(q, mb.Fp8Matrix(m.data, m.scale.clone().requires_grad_()), x_scale=s)):
+        with pytest.raises(ValueError, match="not differentiable"):
+            f()
+        with torch.no_grad():
+            f()
+
+
+def test_linear_fp8_takes_scales_of_any_stride():
+    """One column of scales that is a transposed row, and scales that are the negative of what memory holds."""
+    x, xs, w, ws = fp8_operands(40, 300, 64, torch.float8_e4m3fn, torch.float8_e4m3fn)
+    want = ops.linear_fp8(x, mb.Fp8Matrix(w, ws), x_scale=xs)
+    assert torch.equal(ops.linear_fp8(x, mb.Fp8Matrix(w, ws.reshape(1, 3).clone().t()), x_scale=xs), want)
+    assert torch.equal(ops.linear_fp8(x, mb.Fp8Matrix(w, torch._neg_view(-ws)), x_scale=xs), want)
+    assert torch.equal(torch.ops.mortar_b200.linear_fp8(x, xs, w, ws.reshape(1, 3).clone().t(), False, want.dtype), want)
