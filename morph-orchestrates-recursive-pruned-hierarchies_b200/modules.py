@@ -400,7 +400,8 @@ class SwiGLUDense(nn.Module):
 
 class SwiGLUFp8(nn.Module):
     """The MLP site served in 8-bit floating point (``ops.mlp_fp8``), with the layer norm of the
-    ``SwiGLUDense`` it was made from: ``norm`` = (weight, bias, eps) or None."""
+    ``SwiGLUDense`` it was made from: ``norm`` = (weight, bias, eps) or None.  Casts of the module
+    leave its matrices in 8 bits and their scales in fp32."""
 
     def __init__(self, gate_up: Fp8Matrix, down: Fp8Matrix, norm=None):
         super().__init__()
@@ -415,6 +416,16 @@ class SwiGLUFp8(nn.Module):
         self.register_buffer("norm_bias", None if norm is None else norm[1])
         self.eps = None if norm is None else float(norm[2])
         self.d_model, self.d_ff = down.out_features, down.in_features
+
+    def _apply(self, fn, recurse=True):
+        # casts of a model (.bfloat16(), .to(dtype)) count 8-bit floating point among the types they change; the matrices
+        # follow a move to another device but keep their types
+        held = [self.gate_up_data, self.gate_up_scale, self.down_data, self.down_scale]
+
+        def keep(t):
+            out = fn(t)
+            return t.to(out.device) if out.dtype != t.dtype and any(t is h for h in held) else out
+        return super()._apply(keep, recurse)
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor) -> torch.Tensor:

@@ -387,3 +387,23 @@ def test_8_bit_operators_refuse_what_requires_a_gradient():
                 with torch.no_grad(), pytest.raises(RuntimeError) as e:
                     call(True)
                 assert "not differentiable" not in str(e.value)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.float(), lambda m: m.double(),
+                                  lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu", torch.float16)])
+def test_a_cast_of_the_model_leaves_the_8_bit_form(cast):
+    gen = torch.Generator().manual_seed(0)
+    def matrix(o, i):
+        return mb.Fp8Matrix(torch.randn(o, i, generator=gen).to(torch.float8_e4m3fn),
+                            torch.rand(-(-o // 128), -(-i // 128), generator=gen) + 1.0 / 3)
+    site = mb.SwiGLUFp8(matrix(256, 64), matrix(64, 128), (torch.ones(64), torch.zeros(64), 1e-5))
+    before = {k: v.clone() for k, v in site.state_dict().items()}
+    model = cast(torch.nn.Sequential(torch.nn.Linear(64, 64), site))
+    for k, v in site.state_dict().items():
+        if k.startswith("norm"):                                     # the norm follows the model
+            assert v.dtype == model[0].weight.dtype
+        else:
+            assert v.dtype == before[k].dtype and torch.equal(v.view(torch.uint8), before[k].view(torch.uint8)), k
+    mb.Fp8Matrix(site.gate_up_data, site.gate_up_scale)
+    moved = site.to("meta")
+    assert moved.down_data.is_meta and moved.down_data.dtype == torch.float8_e4m3fn
