@@ -15,7 +15,7 @@ shape and dtype.  There is no CPU implementation: calling an op with CPU tensors
     mortar_b200::mlp_prefill_tc(x, <gate_up sched>, <down sched>, gates?, n_clusters) -> y
     mortar_b200::stack_decode(x!, blobs, table, app_layer, status!, ...) -> ()   (in place)
     mortar_b200::layer_norm(x, weight?, bias?, eps) -> (y, stats)            (differentiable in y)
-    mortar_b200::mlp_dense(x, gate_up, down) -> (y, hidden, sums)            (differentiable in y)
+    mortar_b200::mlp_dense(x, gate_up, down, want_saved=True) -> (y, hidden, sums)   (differentiable in y)
     mortar_b200::quantize_fp8(x, block_rows, e5m2) -> (q, scale);  dequantize_fp8(q, scale, out_dtype) -> x
     mortar_b200::linear_fp8(x, x_scale?, w, w_scale, swiglu, out_dtype) -> y
     <stream> = grp_ptr, grp_cols, grp_codes, scale, out_features, in_features, n_groups
@@ -263,16 +263,24 @@ def _(x, weight, bias, eps):
     return x.new_empty(x.shape), x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32)
 
 
+def _some(t: Optional[torch.Tensor], like: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """A registered operator returns tensors only: what is not wanted is an empty one."""
+    return like.new_empty(0, dtype=dtype) if t is None else t
+
+
 @torch.library.custom_op(f"{_LIB}::layer_norm_backward", mutates_args=(), device_types="cuda")
-def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor],
-                        stats: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return ops.layer_norm_backward(dy, x, weight, stats)
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor,
+                        want_dx: bool = True, want_dweight: bool = True,
+                        want_dbias: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    dx, dw, db = ops.layer_norm_backward(dy, x, weight, stats, want_dx, want_dweight, want_dbias)
+    return _some(dx, x), _some(dw, stats), _some(db, stats)
 
 
 @layer_norm_backward.register_fake
-def _(dy, x, weight, stats):
-    col = x.new_empty((x.shape[-1],), dtype=torch.float32)
-    return x.new_empty(x.shape), col, torch.empty_like(col)
+def _(dy, x, weight, stats, want_dx=True, want_dweight=True, want_dbias=True):
+    cols = x.shape[-1]
+    return (x.new_empty(x.shape if want_dx else 0), stats.new_empty(cols if want_dweight else 0),
+            stats.new_empty(cols if want_dbias else 0))
 
 
 def _layer_norm_setup(ctx, inputs, output):
@@ -284,47 +292,60 @@ def _layer_norm_setup(ctx, inputs, output):
 
 def _layer_norm_grad(ctx, dy, _dstats):
     x, weight, stats = ctx.saved_tensors
-    dx, dw, db = torch.ops.mortar_b200.layer_norm_backward(dy, x, weight, stats)
-    return (dx, None if weight is None else dw.to(weight.dtype),
-            None if ctx.bias_dtype is None else db.to(ctx.bias_dtype), None)
+    want = [bool(w) for w in ctx.needs_input_grad[:3]]
+    dx, dw, db = torch.ops.mortar_b200.layer_norm_backward(dy, x, weight, stats, *want)
+    return (dx if want[0] else None, dw.to(weight.dtype) if want[1] else None,
+            db.to(ctx.bias_dtype) if want[2] else None, None)
 
 
 layer_norm.register_autograd(_layer_norm_grad, setup_context=_layer_norm_setup)
 
 
 @torch.library.custom_op(f"{_LIB}::mlp_dense", mutates_args=(), device_types="cuda")
-def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor,
-              down: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor,
+              want_saved: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``ops.mlp_dense`` and what its gradient needs (hidden block, gate and up sums); differentiable
-    in the first result."""
-    return ops.mlp_dense_forward(x, gate_up, down, True)
+    in the first result.  With ``want_saved`` false nothing is kept (both are empty) and there is no
+    gradient: the form for serving, which runs what ``ops.mlp_dense`` runs without gradients."""
+    y, hidden, sums = ops.mlp_dense_forward(x, gate_up, down, want_saved)
+    if not want_saved:
+        hidden = None                                      # scratch of the call
+    return y, _some(hidden, x), _some(sums, x, torch.float32)
 
 
 @mlp_dense.register_fake
-def _(x, gate_up, down):
+def _(x, gate_up, down, want_saved=True):
     rows, d_ff = x.numel() // x.shape[-1], down.shape[1]
+    if not want_saved:
+        return x.new_empty(x.shape), x.new_empty(0), x.new_empty(0, dtype=torch.float32)
     return x.new_empty(x.shape), x.new_empty((rows, d_ff)), x.new_empty((rows, 2 * d_ff), dtype=torch.float32)
 
 
 @torch.library.custom_op(f"{_LIB}::mlp_dense_backward", mutates_args=(), device_types="cuda")
 def mlp_dense_backward(dy: torch.Tensor, x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor,
-                       hidden: torch.Tensor,
-                       sums: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return ops.mlp_dense_backward(dy, x, gate_up, down, hidden, sums)
+                       hidden: torch.Tensor, sums: torch.Tensor, want_dx: bool = True, want_dgate_up: bool = True,
+                       want_ddown: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    dx, dgu, ddn = ops.mlp_dense_backward(dy, x, gate_up, down, hidden, sums, want_dx, want_dgate_up, want_ddown)
+    return _some(dx, x), _some(dgu, x), _some(ddn, x)
 
 
 @mlp_dense_backward.register_fake
-def _(dy, x, gate_up, down, hidden, sums):
-    return x.new_empty(x.shape), x.new_empty(gate_up.shape), x.new_empty(down.shape)
+def _(dy, x, gate_up, down, hidden, sums, want_dx=True, want_dgate_up=True, want_ddown=True):
+    return (x.new_empty(x.shape if want_dx else 0), x.new_empty(gate_up.shape if want_dgate_up else 0),
+            x.new_empty(down.shape if want_ddown else 0))
 
 
 def _mlp_dense_setup(ctx, inputs, output):
-    ctx.save_for_backward(*inputs, output[1], output[2])
+    if not inputs[3]:
+        raise ValueError("mlp_dense: an input requires a gradient, but want_saved is false and nothing was kept for it")
+    ctx.save_for_backward(*inputs[:3], output[1], output[2])
     ctx.mark_non_differentiable(output[1], output[2])
 
 
 def _mlp_dense_grad(ctx, dy, _dhidden, _dsums):
-    return torch.ops.mortar_b200.mlp_dense_backward(dy, *ctx.saved_tensors)
+    want = [bool(w) for w in ctx.needs_input_grad[:3]]
+    grads = torch.ops.mortar_b200.mlp_dense_backward(dy, *ctx.saved_tensors, *want)
+    return (*(g if w else None for g, w in zip(grads, want)), None)
 
 
 mlp_dense.register_autograd(_mlp_dense_grad, setup_context=_mlp_dense_setup)

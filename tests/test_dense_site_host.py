@@ -407,3 +407,25 @@ def test_a_cast_of_the_model_leaves_the_8_bit_form(cast):
     mb.Fp8Matrix(site.gate_up_data, site.gate_up_scale)
     moved = site.to("meta")
     assert moved.down_data.is_meta and moved.down_data.dtype == torch.float8_e4m3fn
+
+
+def test_registered_operators_make_what_is_wanted():
+    """The registered block has a form that keeps nothing (served tokens write no sums and take the kernels for few rows), and
+    both registered backward operators leave out what is not asked for."""
+    ns = torch.ops.mortar_b200
+    with FakeTensorMode():
+        def z(*shape, dt=torch.bfloat16, grad=False):
+            return torch.empty(*shape, device="cuda", dtype=dt).requires_grad_(grad)
+        x, gu, dn, col = z(1, 64), z(256, 64), z(64, 128), z(64)
+        y, hidden, sums = ns.mlp_dense(x, gu, dn, False)
+        assert y.shape == (1, 64) and hidden.numel() == 0 and sums.numel() == 0
+        assert hidden.dtype == torch.bfloat16 and sums.dtype == torch.float32
+        with pytest.raises(ValueError, match="want_saved"):
+            ns.mlp_dense(z(1, 64, grad=True), gu, dn, False)
+        _, hidden, sums = ns.mlp_dense(x, gu, dn)
+        stats = z(2, 1, dt=torch.float32)
+        for want in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (True, True, True)):
+            got = ns.mlp_dense_backward(x, x, gu, dn, hidden, sums, *want)
+            assert [g.shape for g in got] == [t.shape if w else (0,) for t, w in zip((x, gu, dn), want)]
+            got = ns.layer_norm_backward(x, x, col, stats, *want)
+            assert [g.shape for g in got] == [t.shape if w else (0,) for t, w in zip((x, col, col), want)]

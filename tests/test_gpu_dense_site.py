@@ -1035,3 +1035,42 @@ def test_linear_fp8_takes_scales_of_any_stride():
     assert torch.equal(ops.linear_fp8(x, mb.Fp8Matrix(w, ws.reshape(1, 3).clone().t()), x_scale=xs), want)
     assert torch.equal(ops.linear_fp8(x, mb.Fp8Matrix(w, torch._neg_view(-ws)), x_scale=xs), want)
     assert torch.equal(torch.ops.mortar_b200.linear_fp8(x, xs, w, ws.reshape(1, 3).clone().t(), False, want.dtype), want)
+
+
+# ---- the registered operators ------------------------------------------------------------------
+
+def test_registered_block_without_gradients_is_the_served_one():
+    """``want_saved=False``: the kernels and the bits of the call without gradients, at one token and at many."""
+    dt = torch.bfloat16
+    gu, dn = rand(512, 128, seed=1, scale=0.1, dt=dt), rand(128, 256, seed=2, scale=0.1, dt=dt)
+    for rows in (1, 32, 33, 300):
+        x = rand(rows, 128, seed=3, dt=dt)
+        before = ops.kernel_counts().get("dense", 0)
+        y, hidden, sums = torch.ops.mortar_b200.mlp_dense(x, gu, dn, False)
+        between = ops.kernel_counts()["dense"]
+        assert torch.equal(y, ops.mlp_dense(x, gu, dn)) and hidden.numel() == 0 and sums.numel() == 0
+        assert between - before == ops.kernel_counts()["dense"] - between
+    errors_are_clear()
+
+
+@pytest.mark.parametrize("wanted", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 1, 1)])
+def test_registered_rules_compute_the_wanted_gradients(wanted, monkeypatch):
+    asked = []
+    for name in ("mlp_dense_backward", "layer_norm_backward"):
+        def recorded(*args, real=getattr(ops, name)):
+            asked.append([bool(w) for w in args[-3:]])
+            return real(*args)
+        monkeypatch.setattr(ops, name, recorded)
+    ns, dt = torch.ops.mortar_b200, torch.bfloat16
+    for call, parts in ((ns.mlp_dense, (rand(40, 64, seed=1, dt=dt), rand(256, 64, seed=2, scale=0.1, dt=dt), rand(64, 128, seed=3, scale=0.1, dt=dt))),
+                        (lambda *a: ns.layer_norm(*a, 1e-5), (rand(40, 64, seed=1, dt=dt), rand(64, seed=2), rand(64, seed=3, dt=dt)))):
+        plain = ops.mlp_dense if call is ns.mlp_dense else ops.layer_norm
+        leaves = [t.requires_grad_(bool(w)) for t, w in zip(parts, wanted)]
+        chosen = [t for t in leaves if t.requires_grad]
+        dy = rand(40, 64, seed=4, dt=dt)
+        asked.clear()
+        got = torch.autograd.grad(call(*leaves)[0], chosen, dy)
+        assert asked == [[bool(w) for w in wanted]]
+        want = torch.autograd.grad(plain(*leaves), chosen, dy)
+        assert all(torch.equal(p, q) and p.dtype == q.dtype for p, q in zip(got, want))
+    errors_are_clear()
