@@ -137,9 +137,9 @@ void refuse_second(const char *name) {
 // A backward pass that is being captured cannot make the default stream wait for it: the capture fails inside the
 // autograd engine, and the process ends with it.  So a forward call under capture refuses when a leaf above it is so
 // held.  (The walk runs while a graph is captured, never in an eager step.)
-void refuse_capture(const char *name, std::initializer_list<const Tensor *> ts) {
+void refuse_capture(const char *name, at::ArrayRef<const Tensor *> ts) {
     using torch::autograd::Node;
-    const c10::cuda::CUDAGuard guard((*ts.begin())->device());
+    const c10::cuda::CUDAGuard guard(ts.front()->device());
     if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
     std::vector<std::shared_ptr<Node>> todo;
     std::unordered_set<Node *> seen;
@@ -487,6 +487,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     namespace py = pybind11;
     // no call touches a Python object: other threads run meanwhile, as with torch's own operators
     const py::call_guard<py::gil_scoped_release> no_gil;
+    m.def("refuse_capture", [](const std::string &name, const std::vector<OptTensor> &ts) {
+        std::vector<Tensor> held;
+        std::vector<const Tensor *> at;
+        for (const OptTensor &t : ts) held.push_back(or_none(t));
+        for (const Tensor &t : held) at.push_back(&t);
+        refuse_capture(name.c_str(), at);
+    }, no_gil);
     m.def("layer_norm", &layer_norm, no_gil);
     m.def("layer_norm_forward", [](const Tensor &x, const OptTensor &w, const OptTensor &b, double eps, bool stats) {
         return layer_norm_forward(x, or_none(w), or_none(b), eps, stats);

@@ -41,6 +41,7 @@ import numpy as np
 import torch
 
 from . import ops
+from ._native import native
 from .format import (BlockSched, Fp8Matrix, MortarMatrix, SchedMatrix, StreamMatrix, TopologyDev, matrix_from_stream, pack_codes_2bit,
                      wants_block_path)
 
@@ -283,7 +284,17 @@ def _(dy, x, weight, stats, want_dx=True, want_dweight=True, want_dbias=True):
             stats.new_empty(cols if want_dbias else 0))
 
 
+def _refuse_capture(name, tensors):
+    """What ``ops.layer_norm`` and ``ops.mlp_dense`` refuse in their forward call: a captured training step whose leaves a graph
+    of the default stream still holds (its backward pass would end the process)."""
+    if torch.cuda.is_initialized() and not torch.compiler.is_compiling():
+        with torch.cuda.device(tensors[0].device):
+            if torch.cuda.is_current_stream_capturing():
+                native.refuse_capture(name, tensors)
+
+
 def _layer_norm_setup(ctx, inputs, output):
+    _refuse_capture("layer_norm", inputs[:3])
     x, weight, bias, _ = inputs
     ctx.save_for_backward(x, weight, output[1])
     ctx.mark_non_differentiable(output[1])
@@ -338,6 +349,7 @@ def _(dy, x, gate_up, down, hidden, sums, want_dx=True, want_dgate_up=True, want
 def _mlp_dense_setup(ctx, inputs, output):
     if not inputs[3]:
         raise ValueError("mlp_dense: an input requires a gradient, but want_saved is false and nothing was kept for it")
+    _refuse_capture("mlp_dense", inputs[:3])
     ctx.save_for_backward(*inputs[:3], output[1], output[2])
     ctx.mark_non_differentiable(output[1], output[2])
 

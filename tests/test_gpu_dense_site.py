@@ -1074,3 +1074,38 @@ def test_registered_rules_compute_the_wanted_gradients(wanted, monkeypatch):
         want = torch.autograd.grad(plain(*leaves), chosen, dy)
         assert all(torch.equal(p, q) and p.dtype == q.dtype for p, q in zip(got, want))
     errors_are_clear()
+
+
+def test_captured_registered_step_beside_an_eager_graph():
+    """The registered operators refuse the captured training step that ``ops`` refuses, and take it once the graph that holds
+    the leaves is gone."""
+    ns, dt = torch.ops.mortar_b200, torch.bfloat16
+    x, dy = rand(40, 64, seed=1, dt=dt), rand(40, 64, seed=2, dt=dt)
+    leaves = [rand(64, seed=3).requires_grad_(), rand(64, seed=4).requires_grad_(),
+              rand(256, 64, seed=5, scale=0.1, dt=dt).requires_grad_(), rand(64, 128, seed=6, scale=0.1, dt=dt).requires_grad_()]
+
+    def step():
+        n = ns.layer_norm(x, *leaves[:2], 1e-5)[0]
+        return ns.mlp_dense(n, *leaves[2:])[0]
+
+    held = step()
+    want = [held.detach().clone(), *torch.autograd.grad(held, leaves, dy, retain_graph=True)]
+    for call in (lambda: ns.layer_norm(x, *leaves[:2], 1e-5), lambda: ns.mlp_dense(x, *leaves[2:]), step):
+        with pytest.raises(RuntimeError, match="default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        y = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[0])
+    del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+        got = torch.autograd.grad(y, leaves, dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip((y.detach(), *got), want))
+    errors_are_clear()
