@@ -676,9 +676,11 @@ class Fp8Matrix:
             raise ValueError(f"scale must be float32 {list(want)}, got {scale.dtype} {list(scale.shape)}")
         if scale.device != data.device:
             raise ValueError(f"data is on {data.device} but scale on {scale.device}")
-        if data.stride(1) != 1 or data.stride(0) % 16 or data.stride(0) < in_features or data.data_ptr() % 16:
+        # torch.compile knows neither addresses nor the sign of a view; the registered operator makes the matrix again, with both
+        known = not torch.compiler.is_compiling()
+        if data.stride(1) != 1 or data.stride(0) % 16 or data.stride(0) < in_features or (known and data.data_ptr() % 16):
             data = data.clone(memory_format=torch.contiguous_format)
-        if scale.stride() != (want[1], 1) or scale.is_neg():                # also where a dimension of 1 hides a stride
+        if scale.stride() != (want[1], 1) or (known and scale.is_neg()):                # also where a dimension of 1 hides a stride
             scale = scale.clone(memory_format=torch.contiguous_format)
         self.data, self.scale = data, scale
         self.out_features, self.in_features = int(out_features), int(in_features)

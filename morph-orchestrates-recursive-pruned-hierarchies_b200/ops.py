@@ -966,7 +966,12 @@ def rmsnorm_rows(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Ten
 # stream and holds the autograd rules.  Wrong arguments raise ValueError, CPU tensors
 # NotImplementedError, CUDA failures RuntimeError.  The launch goes to the device of the first tensor and
 # that device's current stream; a tensor whose rows are not contiguous (or, for the tensor cores, do not
-# start on 16 bytes) is copied first; nothing is kept from one call for the next.
+# start on 16 bytes) is copied first; nothing is kept from one call for the next.  Inside torch.compile, which cannot
+# look into a compiled function, the same names go through the registered operators (torch_ops.py).
+
+_registered = torch.ops.mortar_b200
+_compiling = torch.compiler.is_compiling
+
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
@@ -978,6 +983,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     every operator here it can be captured into a CUDA graph.  When a backward pass is captured,
     no eager autograd graph over the same leaves may be alive (a rule of torch's autograd, whose
     gradient accumulators remember the stream they were made on)."""
+    if _compiling():
+        return _registered.layer_norm(x, weight, bias, eps)[0]
     return native.layer_norm(x, weight, bias, eps)
 
 
@@ -1011,6 +1018,9 @@ def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor) -> tor
     backward pass x, the hidden block and the gate and up sums (fp32) are kept; the sums' gradients
     are rounded once, for the tensor cores, and so are the results.  The note on captured backward
     passes in ``layer_norm`` holds here too."""
+    if _compiling():
+        grads = torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad)
+        return _registered.mlp_dense(x, gate_up, down, grads)[0]
     return native.mlp_dense(x, gate_up, down)
 
 
@@ -1037,12 +1047,18 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1, dtype: torch.dtype = t
     one that holds an infinity or a NaN has scale NaN and reads back as NaN.  cols is a multiple
     of 16, up to 2^30.  Like the other 8-bit operators not differentiable: an input that requires a
     gradient is refused while gradients are enabled."""
+    if _compiling():
+        if dtype not in (torch.float8_e4m3fn, torch.float8_e5m2):
+            raise ValueError(f"dtype must be float8_e4m3fn or float8_e5m2, got {dtype}")
+        return _registered.quantize_fp8(x, block_rows, dtype == torch.float8_e5m2)
     return native.quantize_fp8(x, block_rows, dtype)
 
 
 def dequantize_fp8(q: torch.Tensor, scale: torch.Tensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """q * scale, rounded once to ``out_dtype``, for what ``quantize_fp8`` gives (or another program
     made, with any scales).  One scale row per row of q, or one per 128 rows."""
+    if _compiling():
+        return _registered.dequantize_fp8(q, scale, out_dtype)
     return native.dequantize_fp8(q, scale, out_dtype)
 
 
@@ -1063,6 +1079,10 @@ def linear_fp8(x: torch.Tensor, w: Fp8Matrix, *, x_scale: Optional[torch.Tensor]
     ``out_dtype`` (default: the type of x, bfloat16 for 8-bit x).  The 8-bit floating-point
     counterpart of ``linear_tc_i8``; for serving, not differentiable (inputs and scales that require
     a gradient are refused while gradients are enabled)."""
+    if _compiling():
+        if out_dtype is None:
+            out_dtype = x.dtype if x_scale is None else torch.bfloat16
+        return _registered.linear_fp8(x, x_scale, w.data, w.scale, swiglu, out_dtype)
     return native.linear_fp8(x, x_scale, w.data, w.scale, swiglu, out_dtype)
 
 

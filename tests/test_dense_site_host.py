@@ -429,3 +429,44 @@ def test_registered_operators_make_what_is_wanted():
             assert [g.shape for g in got] == [t.shape if w else (0,) for t, w in zip((x, gu, dn), want)]
             got = ns.layer_norm_backward(x, x, col, stats, *want)
             assert [g.shape for g in got] == [t.shape if w else (0,) for t, w in zip((x, col, col), want)]
+
+
+def test_the_site_compiles_into_one_graph():
+    """torch.compile(fullgraph=True) of the modules and the operators traces to the registered operators: with the sums kept
+    where a gradient is wanted, without them where none is."""
+    graphs = []
+
+    def backend(module, _):
+        graphs.append([n for n in module.graph.nodes if str(n.target).startswith("mortar_b200.")])
+        return module.forward
+
+    def traced(f, *args):
+        torch._dynamo.reset()
+        graphs.clear()
+        y = torch.compile(f, backend=backend, fullgraph=True)(*args)
+        assert len(graphs) == 1
+        return y, [str(n.target).split(".")[1] for n in graphs[0]]
+
+    with FakeTensorMode():
+        def z(*shape, dt=torch.bfloat16):
+            return torch.empty(*shape, device="cuda", dtype=dt)
+        def matrix(o, i):
+            return fake_matrix(z(o, i, dt=torch.float8_e4m3fn), z(-(-o // 128), -(-i // 128), dt=torch.float32))
+        site, x = mb.SwiGLUDense(64, 128, norm=True, device="cuda", dtype=torch.bfloat16), z(4, 64)
+        y, names = traced(site, x)
+        assert names == ["layer_norm", "mlp_dense"] and graphs[0][1].args[3] is True and y.requires_grad and y.shape == x.shape
+        y, names = traced(torch.no_grad()(site.forward), x)
+        assert names == ["layer_norm", "mlp_dense"] and graphs[0][1].args[3] is False and not y.requires_grad
+        gate_up, down = matrix(256, 64), matrix(64, 128)
+        served = mb.SwiGLUFp8(gate_up, down, (z(64), z(64), 1e-5))
+        y, names = traced(served, x)
+        assert names == ["layer_norm", "linear_fp8", "linear_fp8"] and y.shape == x.shape and y.dtype == x.dtype
+        y, names = traced(lambda t: mb.ops.mlp_fp8(t, gate_up, down, out_dtype=torch.float32), x)
+        assert names == ["linear_fp8", "linear_fp8"] and y.dtype == torch.float32
+        def quantised(t):
+            q, s = mb.ops.quantize_fp8(t, block_rows=1, dtype=torch.float8_e5m2)
+            return mb.ops.linear_fp8(q, gate_up, x_scale=s, swiglu=True), mb.ops.dequantize_fp8(q, s, out_dtype=torch.float16)
+        (y, back), names = traced(quantised, x)
+        assert sorted(names) == ["dequantize_fp8", "linear_fp8", "quantize_fp8"]
+        assert y.shape == (4, 128) and y.dtype == torch.bfloat16 and back.dtype == torch.float16
+    torch._dynamo.reset()

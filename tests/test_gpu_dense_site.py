@@ -1109,3 +1109,27 @@ def test_captured_registered_step_beside_an_eager_graph():
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip((y.detach(), *got), want))
     errors_are_clear()
+
+
+def test_compiled_site_is_the_eager_one():
+    """The site compiled into one graph (captured ahead of time, run as it is): the bits of the eager calls, trained and
+    served, and the same kernels for a served token."""
+    torch.manual_seed(0)
+    site = mb.SwiGLUDense(64, 128, norm=True, device=DEV, dtype=torch.bfloat16)
+    params = list(site.parameters())
+    compiled = torch.compile(site, backend="aot_eager", fullgraph=True)
+    for rows in (40, 1):
+        x, dy = rand(rows, 64, seed=rows, dt=torch.bfloat16).requires_grad_(), rand(rows, 64, seed=3, dt=torch.bfloat16)
+        y, want = compiled(x), site(x)
+        assert torch.equal(y, want)
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, *params), dy), torch.autograd.grad(want, (x, *params), dy)))
+        with torch.no_grad():
+            first = ops.kernel_counts()["dense"]
+            want = site(x)
+            second = ops.kernel_counts()["dense"]
+            assert torch.equal(compiled(x), want) and ops.kernel_counts()["dense"] - second == second - first
+    served = site.to_fp8()
+    x = rand(40, 64, seed=7, dt=torch.bfloat16)
+    assert torch.equal(torch.compile(served, backend="aot_eager", fullgraph=True)(x), served(x))
+    torch._dynamo.reset()
+    errors_are_clear()
