@@ -68,30 +68,57 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
-def build_binding(force: bool = False, verbose: bool = False) -> str:
-    """Compiles csrc/torch_binding.cpp against the installed torch and links it to the library beside it."""
-    newest = max(os.path.getmtime(f) for f in (BINDING, os.path.join(ROOT, "include", "mortar_b200.h")))
-    if not force and os.path.exists(NATIVE) and os.path.getmtime(NATIVE) >= newest:
-        return NATIVE
+BINDING_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_mortar_native"]
+# The C++ runtime and the unwinder that torch runs on, whatever the compiler links by default: with copies of its own (a
+# compiler that has only the static ones) the binding's exceptions end the process.  Compilers that do not know the first flag
+# (g++ before 13) look into the shared library first all the same, since it comes before the one that they add.
+NO_OWN_RUNTIME = "-nostdlib++"
+RUNTIME = ["-l:libstdc++.so.6", "-shared-libgcc", "-l:libgcc_s.so.1"]
+
+
+def build_binding(force: bool = False, verbose: bool = False):
+    """Compiles csrc/torch_binding.cpp against the installed torch and links it to the library beside it;
+    returns its path.  It is built again when a source is newer, or when the command, torch or Python
+    are not those that it was built with.  Without torch or Python's headers it is left out (None): the library
+    and its C entry points need neither."""
     import sysconfig
-    import torch
-    from torch.utils import cpp_extension
+    python_include = sysconfig.get_paths()["include"]
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:
+        missing = "torch is not installed"
+    else:
+        missing = None if os.path.exists(os.path.join(python_include, "Python.h")) else f"there is no Python.h in {python_include}"
+    if missing:
+        sys.stderr.write(f"{missing}: the torch binding of the dense site is not built, the C library is complete\n")
+        return None
+    cxx = os.environ.get("CXX", "g++")
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     include = [f"-isystem{d}" for d in cpp_extension.include_paths()]
-    include += [f"-I{d}" for d in (sysconfig.get_paths()["include"], os.environ.get("CUDA_HOME", "/usr/local/cuda") + "/include",
+    include += [f"-I{d}" for d in (python_include, os.environ.get("CUDA_HOME", "/usr/local/cuda") + "/include",
                                    os.path.join(ROOT, "include"))]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-DTORCH_EXTENSION_NAME=_mortar_native", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+    knows = subprocess.run([cxx, NO_OWN_RUNTIME, "-E", "-x", "c++", os.devnull], capture_output=True).returncode == 0
+    cmd = [cxx, *BINDING_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *include, BINDING, "-o", NATIVE, f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
-           f"-L{PKG}", "-l:libmortar_b200.so", "-Wl,-rpath,$ORIGIN",
-           # the C++ runtime and the unwinder that torch runs on, whatever the compiler links by default: with copies of its own
-           # (a compiler that has only the static ones) the binding's exceptions end the process
-           "-nostdlib++", "-l:libstdc++.so.6", "-shared-libgcc", "-l:libgcc_s.so.1"]
+           f"-L{PKG}", "-l:libmortar_b200.so", "-Wl,-rpath,$ORIGIN", *([NO_OWN_RUNTIME] if knows else []), *RUNTIME]
+    made_with = "\n".join([*cmd, torch.__version__, str(sysconfig.get_config_var("SOABI"))])
+    record = os.path.join(OBJ, "_mortar_native.built_with")
+    newest = max(os.path.getmtime(f) for f in (BINDING, os.path.join(ROOT, "include", "mortar_b200.h")))
+    if not force and os.path.exists(NATIVE) and os.path.getmtime(NATIVE) >= newest and os.path.exists(record):
+        with open(record) as f:
+            if f.read() == made_with:
+                return NATIVE
+    if os.path.exists(record):
+        os.remove(record)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed ({res.returncode}): {' '.join(cmd)}")
+    os.makedirs(OBJ, exist_ok=True)
+    with open(record, "w") as f:
+        f.write(made_with)
     return NATIVE
 
 
