@@ -628,7 +628,8 @@ int mortar_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int6
 /* The gated feed-forward block before it is carved (morph/model/transformer.py:402-431):
  *   y = (silu(x Wg^T) * (x Wu^T)) Wd^T,  gate_up = [Wg; Wu] [2 d_ff][d_model], down [d_model][d_ff]
  * x, weights and results are bf16 or fp16 (dtype, one for all); sums are fp32; the hidden block and y
- * are rounded once each.  d_model and d_ff are multiples of 16; x and the weights 16-byte aligned with row
+ * are rounded once each (the gate's exponential and quotient are the approximate ones, off by 2^-22 (1 + |g|)
+ * of the value at most).  d_model and d_ff are multiples of 16; x and the weights 16-byte aligned with row
  * strides that are multiples of 8; what is written or kept 32-byte aligned, ldy a multiple of 16.
  *   hidden        device [rows][d_ff], written: the hidden block (scratch, and an input of the
  *                 backward call)
@@ -668,7 +669,7 @@ int mortar_dense_error(int32_t *code, int32_t reset);
 int mortar_quantize_fp8(const void *x, int32_t dtype, int64_t ldx, int64_t rows, int32_t cols,
                         int32_t block_rows, void *q, int32_t q_dtype, int64_t ldq, float *scale,
                         void *stream);
-/* out = q * scale, rounded once. */
+/* out = q * scale in fp32 (exact for powers of two), rounded to the type of out. */
 int mortar_dequantize_fp8(const void *q, int32_t q_dtype, int64_t ldq, const float *scale, int64_t rows,
                           int32_t cols, int32_t block_rows, void *out, int32_t out_dtype,
                           int64_t ld_out, void *stream);
@@ -678,10 +679,11 @@ int mortar_dequantize_fp8(const void *q, int32_t q_dtype, int64_t ldq, const flo
  *   x, w       device [rows][in_features] / [out_features][in_features], MORTAR_E4M3 or MORTAR_E5M2
  *              each, 16-byte aligned, row strides multiples of 16
  *   x_scale, w_scale   device fp32, row strides ld_x_scale / ld_w_scale; any finite values whose
- *              products are finite
+ *              products are finite and no subnormal numbers (such a product has fewer bits)
  *   flags      0 or MORTAR_FLAG_SWIGLU: y = silu(first half) * second half of the output columns;
  *              out_features a multiple of 256 then
- *   out        fp32, bf16 or fp16, sums in fp32, rounded once
+ *   out        fp32, bf16 or fp16, sums in fp32, rounded once; the gate's exponential and quotient are
+ *              approximate, off by 2^-22 (1 + |g|) of the value at most, several roundings of an fp32 result
  * in_features is a multiple of 16 up to 2^30.  Bounded in-kernel waits report through mortar_linear_fp8_error. */
 int mortar_linear_fp8(const void *x, int32_t x_type, int64_t ldx, const float *x_scale, int64_t ld_x_scale,
                       int64_t rows, const void *w, int32_t w_type, int64_t ldw, const float *w_scale,

@@ -692,7 +692,7 @@ class Fp8Matrix:
         return cls(*ops.quantize_fp8(weight.detach(), block_rows=cls.BLOCK, dtype=dtype))
 
     def to_dense(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """data * scale, rounded once to ``dtype``."""
+        """data * scale in fp32 (exact for powers of two), rounded to ``dtype``."""
         from . import ops
         return ops.dequantize_fp8(self.data, self.scale, out_dtype=dtype)
 

@@ -28,7 +28,8 @@ def launch_count() -> int:
 
 def kernel_counts() -> dict:
     """Launches so far per kernel family: "act_prep", "bcsr_stream" (the streaming linear / SwiGLU
-    kernel), "prefill_panel" (tcgen05 / tensor memory), "stack_decode", "route_flags", "router".
+    kernel), "prefill_panel" (tcgen05 / tensor memory), "stack_decode", "route_flags", "router"; of the
+    dense site "layer_norm", "layer_norm_backward", "dense", "dense_backward", "quantize_fp8", "dequantize_fp8", "linear_fp8".
     Tests use the deltas to tell which kernel an operator or module forward ran."""
     return {**_kernel_counts, **_native_counts()}
 
@@ -1014,8 +1015,8 @@ def mlp_dense(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor) -> tor
     x [..., d_model], ``gate_up`` = [Wg; Wu] [2 d_ff, d_model] and ``down`` [d_model, d_ff], all
     bfloat16 or all float16; the dense counterpart of ``mlp_prefill_blocks``
     (morph/model/transformer.py:402-431), differentiable in all three.  d_model and d_ff are
-    multiples of 16.  Sums are fp32; the hidden block and the result are rounded once each.  For the
-    backward pass x, the hidden block and the gate and up sums (fp32) are kept; the sums' gradients
+    multiples of 16.  Sums are fp32; the hidden block and the result are rounded once each, and the gate is
+    computed to 2^-22 (1 + |g|) of its value.  For the backward pass x, the hidden block and the gate and up sums (fp32) are kept; the sums' gradients
     are rounded once, for the tensor cores, and so are the results.  The note on captured backward
     passes in ``layer_norm`` holds here too."""
     if _compiling():
@@ -1055,7 +1056,7 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1, dtype: torch.dtype = t
 
 
 def dequantize_fp8(q: torch.Tensor, scale: torch.Tensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """q * scale, rounded once to ``out_dtype``, for what ``quantize_fp8`` gives (or another program
+    """q * scale in fp32 (exact for powers of two), rounded to ``out_dtype``, for what ``quantize_fp8`` gives (or another program
     made, with any scales).  One scale row per row of q, or one per 128 rows."""
     if _compiling():
         return _registered.dequantize_fp8(q, scale, out_dtype)
@@ -1076,7 +1077,8 @@ def linear_fp8(x: torch.Tensor, w: Fp8Matrix, *, x_scale: Optional[torch.Tensor]
     (out a multiple of 256 then).  x is either 8-bit already, with ``x_scale``
     [..., ceil(in / 128)] as ``quantize_fp8`` gives, or fp32 / bf16 / fp16 and then quantised to e4m3
     first.  Every block's sum is scaled in fp32 and added in fp32; the result is rounded once to
-    ``out_dtype`` (default: the type of x, bfloat16 for 8-bit x).  The 8-bit floating-point
+    ``out_dtype`` (default: the type of x, bfloat16 for 8-bit x); with ``swiglu`` the gate is computed to
+    2^-22 (1 + |g|) of its value.  The 8-bit floating-point
     counterpart of ``linear_tc_i8``; for serving, not differentiable (inputs and scales that require
     a gradient are refused while gradients are enabled)."""
     if _compiling():
