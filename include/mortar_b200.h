@@ -679,7 +679,8 @@ int mortar_dequantize_fp8(const void *q, int32_t q_dtype, int64_t ldq, const flo
  *   x, w       device [rows][in_features] / [out_features][in_features], MORTAR_E4M3 or MORTAR_E5M2
  *              each, 16-byte aligned, row strides multiples of 16
  *   x_scale, w_scale   device fp32, row strides ld_x_scale / ld_w_scale; any finite values whose
- *              products are finite and no subnormal numbers (such a product has fewer bits)
+ *              products are finite and no subnormal numbers (such a product has fewer bits);
+ *              rows * ld_x_scale and ceil(out_features / 128) * ld_w_scale below 2^32
  *   flags      0 or MORTAR_FLAG_SWIGLU: y = silu(first half) * second half of the output columns;
  *              out_features a multiple of 256 then
  *   out        fp32, bf16 or fp16, sums in fp32, rounded once; the gate's exponential and quotient are

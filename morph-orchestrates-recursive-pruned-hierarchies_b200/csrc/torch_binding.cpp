@@ -466,6 +466,7 @@ Tensor linear_fp8(const Tensor &x, const OptTensor &x_scale, const Tensor &data,
     if (given.defined()) {
         r = rows_of(x, true);
         s = rows_of(given, false);
+        if (ld(s) > UINT32_MAX / rows) s = s.clone(at::MemoryFormat::Contiguous);     // the kernels keep 32-bit positions of scales
     } else {
         std::tie(r, s) = quantize_fp8(r, 1, at::kFloat8_e4m3fn);
     }

@@ -1133,3 +1133,18 @@ def test_compiled_site_is_the_eager_one():
     assert torch.equal(torch.compile(served, backend="aot_eager", fullgraph=True)(x), served(x))
     torch._dynamo.reset()
     errors_are_clear()
+
+
+def test_linear_fp8_takes_scales_that_lie_far_apart():
+    """Rows of scales whose positions pass 32 bits (a column of a very wide table) are copied, as other strides are."""
+    for rows in (2, 40):
+        x, xs, w, ws = fp8_operands(rows, 300, 272, torch.float8_e4m3fn, torch.float8_e4m3fn)
+        m = mb.Fp8Matrix(w, ws)
+        step = (1 << 32) // (rows - 1) + 8
+        table = torch.empty((rows - 1) * step + 3, device=DEV)       # 17 GB, of which the rows of scales are written
+        far = table.as_strided((rows, 3), (step, 1))
+        far.copy_(xs)
+        assert torch.equal(ops.linear_fp8(x, m, x_scale=far), ops.linear_fp8(x, m, x_scale=xs))
+        del far, table
+        torch.cuda.empty_cache()
+    errors_are_clear()
