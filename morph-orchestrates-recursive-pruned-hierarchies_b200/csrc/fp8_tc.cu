@@ -13,7 +13,7 @@
 // while the MMAs fill the other set.  A cluster of two CTAs computes 256 x 256: every thread of eight
 // epilogue warps keeps 128 sums, for which the launch's registers are dealt out anew.
 //
-// What bounds it, at 8192 x 2048 -> 11264 with the gate (206 to 220 us, 1720 to 1830 TFLOP/s, 233 to 246 in
+// What bounds it, at 8192 x 2048 -> 11264 with the gate (206 to 220 us, 1720 to 1830 TFLOP/s, 233 to 248 in
 // a long run under the power cap): the epilogue warps.
 // The same MMAs and copies with one sum per tile instead of one per block take 139 us.  A block's MMAs are
 // 512 cycles; a warp needs about 800 for it: 150 to see that the block is there, twice 75 to read 64 columns
